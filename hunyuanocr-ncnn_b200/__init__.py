@@ -52,6 +52,7 @@ EXPORTED_SYMBOLS = (
     "hy_ctx_set_token_callback", "hy_debug_wait_stats", "hy_ctx_last_timing", "hy_ctx_last_dflash_timing",
     "hy_ctx_set_wait_limit", "hy_debug_wait_probe", "hy_ctx_create_from_package", "hy_draft_load_package",
     "hy_package_inspect", "hy_package_read_tensor", "hy_debug_step_trace",
+    "hy_paged_kv_write", "hy_paged_kv_read", "hy_paged_attention", "hy_paged_attention_workspace",
 )
 TOKEN_CALLBACK = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.c_void_p)
 DFLASH_MASK_TOKEN = 120817

@@ -19,11 +19,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libhy_decode.so")
 RECORD = os.path.join(HERE, "libhy_decode.build.json")   # what the last in-tree build compiled, and how
-SOURCES = [os.path.join(HERE, "csrc", "hy_capi.cu"), os.path.join(HERE, "csrc", "hy_package.cpp")]
+SOURCES = [os.path.join(HERE, "csrc", "hy_capi.cu"), os.path.join(HERE, "csrc", "hy_paged.cu"),
+           os.path.join(HERE, "csrc", "hy_package.cpp")]
 DEPS = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))] + [
-    os.path.join(REPO, "include", "hy_decode.h")]
+    os.path.join(REPO, "include", "hy_decode.h"), os.path.join(REPO, "include", "hy_paged.h")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+FLAGS = ["--threads", "0", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "-shared", "-I" + os.path.join(REPO, "include")]
 
 
@@ -74,7 +75,7 @@ def build_shim_test(force: bool = False) -> str:
     """Compile the C++17 layer's test program (tests/cpp/test_shim.cpp, over
     include/hunyuan_ocr_cuda.h) against the in-tree library."""
     deps = [SHIM_TEST_SRC, LIB, os.path.join(REPO, "include", "hunyuan_ocr_cuda.h"),
-            os.path.join(REPO, "include", "hy_decode.h")]
+            os.path.join(REPO, "include", "hy_decode.h"), os.path.join(REPO, "include", "hy_paged.h")]
     if not force and os.path.exists(SHIM_TEST_BIN) and all(
             os.path.getmtime(d) <= os.path.getmtime(SHIM_TEST_BIN) for d in deps):
         return SHIM_TEST_BIN

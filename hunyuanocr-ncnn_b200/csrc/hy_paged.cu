@@ -1,0 +1,271 @@
+// C ABI of the paged KV cache (include/hy_paged.h): checks of arguments, the
+// choice of kernels, launches. Every check that needs no device comes before
+// the first CUDA call.
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <climits>
+#include <string>
+#include <type_traits>
+
+#include "hy_paged.cuh"
+#include "hy_paged_attn.cuh"
+#include "hy_paged.h"
+
+namespace hy_internal {
+void set_last_error(const std::string& msg);
+}
+
+using namespace hy;
+
+namespace {
+
+int fail(int code, const char* msg) noexcept
+{
+    try
+    {
+        hy_internal::set_last_error(msg);
+    }
+    catch (...)   // no memory for the message: the status still tells
+    {
+    }
+    return code;
+}
+
+int cuda_fail(const char* what, cudaError_t e) noexcept
+{
+    char msg[256];
+    snprintf(msg, sizeof msg, "%s: %s", what, cudaGetErrorString(e));
+    return fail(e == cudaErrorMemoryAllocation ? HY_ERR_OUT_OF_MEMORY : HY_ERR_CUDA, msg);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int elem_size(int dtype) { return dtype == HY_DTYPE_F32 ? 4 : dtype == HY_DTYPE_BF16 ? 2 : 1; }
+
+int check_cache(const hy_paged_cache* c)
+{
+    if (!c) return fail(HY_ERR_INVALID_ARGUMENT, "cache is null");
+    if (c->dtype < HY_DTYPE_F32 || c->dtype > HY_DTYPE_INT8)
+        return fail(HY_ERR_INVALID_ARGUMENT, "cache dtype must be F32, BF16, E4M3 or INT8");
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(HY_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (c->num_pages < 1 || c->page_size < 1 || c->num_kv_heads < 1)
+        return fail(HY_ERR_INVALID_ARGUMENT, "num_pages, page_size and num_kv_heads must be positive");
+    if (c->num_kv_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "num_kv_heads must be at most 1024");
+    if (!c->k_dev || !c->v_dev) return fail(HY_ERR_INVALID_ARGUMENT, "cache memory is null");
+    const int e = elem_size(c->dtype);
+    if (!aligned16(c->k_dev) || !aligned16(c->v_dev) || c->page_stride * e % 16 || c->head_stride * e % 16 ||
+        c->row_stride * e % 16)
+        return fail(HY_ERR_INVALID_ARGUMENT, "cache rows must start on 16 bytes");
+    if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->scale_page_stride < 0 ||
+        c->scale_head_stride < 0 || c->scale_row_stride < 0)
+        return fail(HY_ERR_INVALID_ARGUMENT, "cache strides must not be negative");
+    const bool codes = e == 1;
+    if (codes && (!c->k_scale_dev || !c->v_scale_dev))
+        return fail(HY_ERR_INVALID_ARGUMENT, "an 8-bit cache needs k and v scales");
+    if (!codes && (c->k_scale_dev || c->v_scale_dev))
+        return fail(HY_ERR_INVALID_ARGUMENT, "scales belong to 8-bit caches only");
+    if (c->device < 0) return fail(HY_ERR_INVALID_ARGUMENT, "device must not be negative");
+    return HY_OK;
+}
+
+int check_batch(const hy_paged_batch* b, const hy_paged_cache* c)
+{
+    if (!b) return fail(HY_ERR_INVALID_ARGUMENT, "batch is null");
+    if (b->num_seqs < 0 || b->num_seqs > 65535) return fail(HY_ERR_INVALID_ARGUMENT, "num_seqs must be in 0..65535");
+    if (b->max_rows < 0) return fail(HY_ERR_INVALID_ARGUMENT, "max_rows must not be negative");
+    if (b->num_seqs == 0) return HY_OK;
+    if (b->table_width < 0 || b->table_stride < 0)
+        return fail(HY_ERR_INVALID_ARGUMENT, "table_width and table_stride must not be negative");
+    if (static_cast<long long>(b->table_width) * c->page_size > INT_MAX / 2)
+        return fail(HY_ERR_CAPACITY, "table_width * page_size must be below 2^30");
+    if (!b->q_start_dev || !b->kv_len_dev || (b->table_width > 0 && !b->block_table_dev))
+        return fail(HY_ERR_INVALID_ARGUMENT, "batch arrays are null");
+    return HY_OK;
+}
+
+int check_rows(const char* name, const void* p, long long row_stride, long long head_stride, int dtype)
+{
+    char msg[96];
+    const int e = elem_size(dtype);
+    const char* what = !p                                                                      ? "%s is null"
+                       : row_stride < 0 || head_stride < 0                                     ? "%s strides must not be negative"
+                       : !aligned16(p) || row_stride * e % 16 || head_stride * e % 16          ? "%s rows must start on 16 bytes"
+                                                                                               : nullptr;
+    if (!what) return HY_OK;
+    snprintf(msg, sizeof msg, what, name);
+    return fail(HY_ERR_INVALID_ARGUMENT, msg);
+}
+
+int check_dtype(int rows, int dtype)
+{
+    if (rows < 0) return fail(HY_ERR_INVALID_ARGUMENT, "rows must not be negative");
+    if (dtype != HY_DTYPE_F32 && dtype != HY_DTYPE_BF16)
+        return fail(HY_ERR_INVALID_ARGUMENT, "row dtype must be F32 or BF16");
+    return HY_OK;
+}
+
+// The cache's device for the length of a call.
+class DeviceGuard {
+public:
+    explicit DeviceGuard(int device)
+    {
+        error_ = cudaGetDevice(&before_);
+        if (error_ == cudaSuccess && before_ != device)
+        {
+            error_ = cudaSetDevice(device);
+            restore_ = error_ == cudaSuccess;
+        }
+    }
+    ~DeviceGuard()
+    {
+        if (restore_) cudaSetDevice(before_);
+    }
+    cudaError_t error() const { return error_; }
+
+private:
+    int before_ = 0;
+    bool restore_ = false;
+    cudaError_t error_;
+};
+
+PagedCache device_cache(const hy_paged_cache* c)
+{
+    return {c->k_dev, c->v_dev, c->k_scale_dev, c->v_scale_dev, c->page_stride, c->head_stride, c->row_stride,
+            c->scale_page_stride, c->scale_head_stride, c->scale_row_stride, c->num_pages, c->page_size,
+            c->num_kv_heads, c->status_dev};
+}
+
+PagedBatch device_batch(const hy_paged_batch* b, int rows)
+{
+    return {b->q_start_dev, b->kv_len_dev, b->block_table_dev, b->table_stride, b->table_width, b->num_seqs, rows};
+}
+
+template <typename T>
+struct Tag {
+    using type = T;
+};
+
+// f(row type, cache type, head_dim) with the run-time types as types.
+template <typename F>
+auto with_types(int row_dtype, int cache_dtype, int head_dim, F&& f)
+{
+    auto dim = [&](auto rt, auto ct) {
+        return head_dim == 64 ? f(rt, ct, std::integral_constant<int, 64>{})
+                              : f(rt, ct, std::integral_constant<int, 128>{});
+    };
+    auto cache = [&](auto rt) {
+        switch (cache_dtype)
+        {
+        case HY_DTYPE_F32: return dim(rt, Tag<float>{});
+        case HY_DTYPE_BF16: return dim(rt, Tag<__nv_bfloat16>{});
+        case HY_DTYPE_E4M3: return dim(rt, Tag<E4M3>{});
+        default: return dim(rt, Tag<Int8>{});
+        }
+    };
+    return row_dtype == HY_DTYPE_F32 ? cache(Tag<float>{}) : cache(Tag<__nv_bfloat16>{});
+}
+
+int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int dtype, void* k,
+               long long krs, long long khs, void* v, long long vrs, long long vhs, void* stream)
+{
+    int rc = check_cache(cache);
+    if (!rc) rc = check_batch(batch, cache);
+    if (!rc) rc = check_dtype(rows, dtype);
+    if (rc) return rc;
+    if (rows == 0 || batch->num_seqs == 0) return HY_OK;
+    rc = check_rows("k", k, krs, khs, dtype);
+    if (!rc) rc = check_rows("v", v, vrs, vhs, dtype);
+    if (rc) return rc;
+    DeviceGuard guard(cache->device);
+    if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
+    const PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, krs, khs, vrs, vhs};
+    with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
+        using RT = typename decltype(rt)::type;
+        using CT = typename decltype(ct)::type;
+        const dim3 grid(rows), block(kRowWarps * 32);
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (write) paged_write_kernel<RT, CT, decltype(d)::value><<<grid, block, 0, s>>>(a);
+        else paged_read_kernel<RT, CT, decltype(d)::value><<<grid, block, 0, s>>>(a);
+    });
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? HY_OK : cuda_fail(write ? "paged write" : "paged read", e);
+}
+
+int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype)
+{
+    int rc = check_cache(cache);
+    if (!rc) rc = check_batch(batch, cache);
+    if (!rc) rc = check_dtype(rows, dtype);
+    if (rc) return rc;
+    if (q_heads < 1 || q_heads % cache->num_kv_heads)
+        return fail(HY_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of num_kv_heads");
+    if (q_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "q_heads must be at most 1024");
+    return HY_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hy_paged_kv_write(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int dtype, const void* k_dev,
+                      int64_t k_row_stride, int64_t k_head_stride, const void* v_dev, int64_t v_row_stride,
+                      int64_t v_head_stride, void* stream)
+{
+    return paged_rows(true, cache, batch, rows, dtype, const_cast<void*>(k_dev), k_row_stride, k_head_stride,
+                      const_cast<void*>(v_dev), v_row_stride, v_head_stride, stream);
+}
+
+int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int dtype, void* k_dev,
+                     int64_t k_row_stride, int64_t k_head_stride, void* v_dev, int64_t v_row_stride,
+                     int64_t v_head_stride, void* stream)
+{
+    return paged_rows(false, cache, batch, rows, dtype, k_dev, k_row_stride, k_head_stride, v_dev, v_row_stride,
+                      v_head_stride, stream);
+}
+
+int hy_paged_attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads,
+                                 int dtype, size_t* bytes)
+{
+    const int rc = check_attention(cache, batch, rows, q_heads, dtype);
+    if (rc) return rc;
+    if (!bytes) return fail(HY_ERR_INVALID_ARGUMENT, "bytes is null");
+    *bytes = 0;
+    return HY_OK;
+}
+
+int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
+                       const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, void* out_dev,
+                       int64_t out_row_stride, int64_t out_head_stride, float scale, int causal, int window, int sinks,
+                       void* workspace_dev, size_t workspace_bytes, void* stream)
+{
+    int rc = check_attention(cache, batch, rows, q_heads, dtype);
+    if (rc) return rc;
+    if (window < 0 || sinks < 0) return fail(HY_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
+    if (!causal && window > 0) return fail(HY_ERR_UNSUPPORTED, "a window needs causal attention");
+    if (!(scale == scale) || scale - scale != 0.f) return fail(HY_ERR_INVALID_ARGUMENT, "scale must be finite");
+    if (rows == 0 || batch->num_seqs == 0) return HY_OK;
+    rc = check_rows("q", q_dev, q_row_stride, q_head_stride, dtype);
+    if (!rc) rc = check_rows("out", out_dev, out_row_stride, out_head_stride, dtype);
+    if (rc) return rc;
+    if (q_dev == out_dev) return fail(HY_ERR_INVALID_ARGUMENT, "q and out must not overlap");
+    (void)workspace_dev;
+    (void)workspace_bytes;
+    DeviceGuard guard(cache->device);
+    if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
+    const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
+                          out_row_stride, out_head_stride, q_heads, q_heads / cache->num_kv_heads, causal != 0, window,
+                          window > 0 ? sinks : 0, scale * 1.4426950408889634f};
+    with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
+        using RT = typename decltype(rt)::type;
+        using CT = typename decltype(ct)::type;
+        const long long items = static_cast<long long>(rows) * q_heads;
+        paged_attn_rows_kernel<RT, CT, decltype(d)::value>
+            <<<static_cast<unsigned>((items + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    });
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? HY_OK : cuda_fail("paged attention", e);
+}
+
+}  // extern "C"

@@ -1,0 +1,416 @@
+// Paged KV cache: rows written into pages (quantised as they are written) and
+// read back. The attention over the pages is in hy_paged_attn.cuh.
+//
+// A batch names its sequences by device arrays: the row range q_start[s] ..
+// q_start[s + 1], the cache length kv_len[s] (the new rows included) and a row
+// of page numbers; every kernel checks what it reads from them and skips what
+// does not hold, setting a bit of the status word.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "hy_device.cuh"
+
+namespace hy {
+
+// Status bits (enum hy_paged_status).
+constexpr int kPagedBadPage = 1;
+constexpr int kPagedBadLength = 2;
+constexpr int kPagedBadRows = 4;
+constexpr int kPagedTimeout = 8;
+
+struct PagedCache {
+    void* k;
+    void* v;
+    float* k_scale;   // 8-bit caches
+    float* v_scale;
+    long long page_stride, head_stride, row_stride;      // elements
+    long long s_page_stride, s_head_stride, s_row_stride;
+    int num_pages, page_size, kv_heads;
+    int* status;
+};
+
+struct PagedBatch {
+    const int* q_start;
+    const int* kv_len;
+    const int* table;
+    long long table_stride;
+    int table_width, num_seqs, rows;
+};
+
+__device__ __forceinline__ void paged_status(int* status, int bit)
+{
+    if (status) atomicOr(status, bit);
+}
+
+// Rows and cache length of sequence s; false (and a status bit) when they do not hold.
+struct PagedSeq {
+    int row0, n, kv;
+};
+__device__ __forceinline__ bool paged_seq(const PagedBatch& b, int s, int page_size, int* status, PagedSeq& o)
+{
+    const int r0 = __ldg(b.q_start + s), r1 = __ldg(b.q_start + s + 1), kv = __ldg(b.kv_len + s);
+    o.row0 = r0;
+    o.n = r1 - r0;
+    o.kv = kv;
+    if (r0 < 0 || r1 < r0 || r1 > b.rows)
+    {
+        paged_status(status, kPagedBadRows);
+        return false;
+    }
+    if (kv < 0 || kv > static_cast<long long>(b.table_width) * page_size)
+    {
+        paged_status(status, kPagedBadLength);
+        return false;
+    }
+    return true;
+}
+
+// The sequence that holds row r (the last one whose q_start is <= r), by the
+// whole warp: 32 starts per round, counted by a ballot. -1: no sequence does.
+__device__ __forceinline__ int paged_find_seq(const PagedBatch& b, int r, int lane)
+{
+    int below = 0;
+    for (int s0 = 0; s0 <= b.num_seqs; s0 += 32)
+    {
+        const int s = s0 + lane;
+        const bool le = s <= b.num_seqs && __ldg(b.q_start + s) <= r;
+        const int c = __popc(__ballot_sync(0xffffffffu, le));
+        below += c;
+        if (c < 32) break;
+    }
+    return (below == 0 || below > b.num_seqs) ? -1 : below - 1;
+}
+
+// ---------------------------------------------------------------------------
+// Element types of the cache.
+// ---------------------------------------------------------------------------
+struct E4M3 {
+    uint8_t c;
+};
+struct Int8 {
+    uint8_t c;
+};
+template <typename CT>
+constexpr bool kCodes = (sizeof(CT) == 1);   // codes with a scale
+
+// x / s rounded to int8, ties to even, for |x| <= 127 s (1 + 2^-23). inv = 1 / s.
+// x * inv is off by a few ulp, so only a quotient that close to a tie needs the
+// exact sign of x - (n + 1/2) s, which the fused multiply-add gives.
+__device__ __forceinline__ uint32_t quant_int8(float x, float s, float inv)
+{
+    const float q = x * inv;
+    float r = rintf(q);
+    if (fabsf(q - r) > 0.4999f)
+    {
+        const float lo = floorf(q);
+        const float d = fmaf(-(lo + 0.5f), s, x);
+        const bool odd = (static_cast<int>(lo) & 1) != 0;
+        r = (d > 0.f || (d == 0.f && odd)) ? lo + 1.f : lo;
+    }
+    r = fminf(fmaxf(r, -127.f), 127.f);
+    return static_cast<uint32_t>(static_cast<int>(r)) & 0xffu;
+}
+
+// x / s rounded to E4M3 (4 exponent bits, bias 7; 3 fraction bits), ties to
+// even, at most 448: as above, the hardware's rounding of x * inv except near a
+// tie and among the subnormals (|q| < 2^-6), where the sign of a - mid s decides.
+__device__ __forceinline__ uint32_t quant_e4m3(float x, float s, float inv)
+{
+    const float q = x * inv;
+    const uint32_t b = __float_as_uint(q) & 0x7fffffffu;
+    const int off = static_cast<int>(b & 0xFFFFFu) - 0x80000;
+    const bool sub = b < 0x3C800000u;   // 2^-6
+    if ((sub && b != 0) || (off >= -8 && off <= 8))
+    {
+        const float a = fabsf(x), aq = __uint_as_float(b);
+        int lo;
+        float mid;
+        if (sub)
+        {
+            lo = static_cast<int>(aq * 512.f);
+            mid = (static_cast<float>(lo) + 0.5f) * (1.f / 512.f);
+        }
+        else
+        {
+            lo = static_cast<int>(b >> 20) - (120 << 3);
+            mid = __uint_as_float((b & 0xFFF00000u) | 0x80000u);
+        }
+        const float d = fmaf(-mid, s, a);
+        if (d > 0.f || (d == 0.f && (lo & 1))) ++lo;
+        return static_cast<uint32_t>(min(lo, 0x7E)) | ((__float_as_uint(x) >> 24) & 0x80u);
+    }
+    return __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+}
+
+template <typename CT>
+__device__ __forceinline__ uint32_t quant(float x, float s, float inv)
+{
+    if constexpr (std::is_same_v<CT, E4M3>) return quant_e4m3(x, s, inv);
+    else return quant_int8(x, s, inv);
+}
+template <typename CT>
+constexpr float kCodeMax = std::is_same_v<CT, E4M3> ? 448.f : 127.f;
+
+// Four codes of a word as fp32.
+template <typename CT>
+__device__ __forceinline__ void decode4(uint32_t w, float* o)
+{
+    if constexpr (std::is_same_v<CT, E4M3>)
+    {
+        const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(w & 0xffffu, __NV_E4M3)));
+        const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(w >> 16, __NV_E4M3)));
+        o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+    }
+}
+
+// E consecutive elements (E = 4 or 8) at p as fp32, by the widest loads; stores likewise.
+template <typename T, int E>
+__device__ __forceinline__ void load_row(const void* base, long long off, float* x)
+{
+    if constexpr (sizeof(T) == 4)
+    {
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+        {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off + i));
+            x[i] = f.x; x[i + 1] = f.y; x[i + 2] = f.z; x[i + 3] = f.w;
+        }
+    }
+    else if constexpr (sizeof(T) == 2)
+    {
+        uint32_t w[E / 2];
+        const uint16_t* p = static_cast<const uint16_t*>(base) + off;
+        if constexpr (E == 8)
+        {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+        }
+        else
+        {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            w[0] = u.x; w[1] = u.y;
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i)
+        {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    else
+    {
+        const uint8_t* p = static_cast<const uint8_t*>(base) + off;
+        if constexpr (E == 8)
+        {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            decode4<T>(u.x, x);
+            decode4<T>(u.y, x + 4);
+        }
+        else
+        {
+            decode4<T>(__ldg(reinterpret_cast<const uint32_t*>(p)), x);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int E>   // fp32 or bf16
+__device__ __forceinline__ void store_row(void* base, long long off, const float* x)
+{
+    if constexpr (sizeof(T) == 4)
+    {
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+            *reinterpret_cast<float4*>(static_cast<float*>(base) + off + i) =
+                make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    }
+    else
+    {
+        uint16_t* p = static_cast<uint16_t*>(base) + off;
+        if constexpr (E == 8)
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
+                                                      pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        else
+            *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Write and read back. One CTA (4 warps) per row; the row's 2 x kv_heads
+// vectors (k, then v) are shared out to groups of lanes that hold 16 bytes of
+// the row tensor each, so that a row's loads are all wide and all in flight at
+// once; the maximum of a vector is taken in registers and its codes leave in
+// the same pass. Bound by memory: each byte moves once.
+// ---------------------------------------------------------------------------
+constexpr int kRowWarps = 4;
+
+struct PagedRowArgs {
+    PagedCache c;
+    PagedBatch b;
+    void* k;   // row tensors
+    void* v;
+    long long k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+};
+
+// Where row r belongs: its page's and row's offsets. False: nowhere.
+__device__ __forceinline__ bool paged_place(const PagedCache& c, const PagedBatch& b, int r, int lane, long long& off,
+                                            long long& s_off)
+{
+    const int s = paged_find_seq(b, r, lane);
+    if (s < 0) return false;
+    PagedSeq q;
+    if (!paged_seq(b, s, c.page_size, c.status, q)) return false;
+    if (r < q.row0 || r >= q.row0 + q.n)   // q_start is not ascending
+    {
+        paged_status(c.status, kPagedBadRows);
+        return false;
+    }
+    const int p = q.kv - q.n + (r - q.row0);
+    if (p < 0) return false;
+    const int pg = __ldg(b.table + s * b.table_stride + p / c.page_size);
+    const int in = p % c.page_size;
+    if (pg < 0 || pg >= c.num_pages)
+    {
+        paged_status(c.status, kPagedBadPage);
+        return false;
+    }
+    off = pg * c.page_stride + in * c.row_stride;
+    s_off = pg * c.s_page_stride + in * c.s_row_stride;
+    return true;
+}
+
+template <typename RT, typename CT, int D>
+__global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const PagedRowArgs a)
+{
+    constexpr int E = 16 / static_cast<int>(sizeof(RT));   // elements per lane
+    constexpr int LPV = D / E;                             // lanes per vector: 8, 16 or 32
+    constexpr int VPW = 32 / LPV;                          // vectors per warp and step
+    constexpr int U = 4;                                   // steps in flight
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = blockIdx.x;
+    const int nv = 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+
+    auto load = [&](int v0, float (&x)[U][E]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
+            if (vec >= nv) continue;
+            const bool isv = vec >= a.c.kv_heads;
+            const int h = isv ? vec - a.c.kv_heads : vec;
+            load_row<RT, E>(isv ? a.v : a.k,
+                            isv ? r * a.v_row_stride + h * a.v_head_stride + d
+                                : r * a.k_row_stride + h * a.k_head_stride + d,
+                            x[u]);
+        }
+    };
+    float x[U][E];
+    load(0, x);   // ahead of the look-up of the row's place: a row's values do not depend on it
+    long long off, s_off;
+    if (!paged_place(a.c, a.b, r, lane, off, s_off)) return;
+    for (int v0 = 0; v0 < nv; v0 += U * kRowWarps * VPW)
+    {
+        if (v0) load(v0, x);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
+            const bool live = vec < nv;
+            const bool isv = vec >= a.c.kv_heads;
+            const int h = isv ? vec - a.c.kv_heads : vec;
+            const long long at = off + h * a.c.head_stride + d;
+            void* const pool = isv ? a.c.v : a.c.k;
+            if constexpr (kCodes<CT>)
+            {
+                // The largest magnitude by its bits: an infinity or a NaN comes out on top.
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (live) m = max(m, __float_as_uint(x[u][i]) & 0x7fffffffu);
+#pragma unroll
+                for (int o = LPV / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const bool finite = m < 0x7f800000u;
+                const float scale =
+                    finite ? fmaxf(__fdiv_rn(__uint_as_float(m), kCodeMax<CT>), 1.17549435e-38f) : __int_as_float(0x7fffffff);
+                if (!live) continue;
+                const float inv = __fdiv_rn(1.f, scale);
+                uint32_t w[E / 4];
+#pragma unroll
+                for (int i = 0; i < E / 4; ++i)
+                {
+                    w[i] = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (finite) w[i] |= quant<CT>(x[u][4 * i + e], scale, inv) << (8 * e);
+                }
+                uint8_t* p = static_cast<uint8_t*>(pool) + at;
+                if constexpr (E == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(p) = w[0];
+                if (lane % LPV == 0) (isv ? a.c.v_scale : a.c.k_scale)[s_off + h * a.c.s_head_stride] = scale;
+            }
+            else
+            {
+                if (live) store_row<CT, E>(pool, at, x[u]);
+            }
+        }
+    }
+}
+
+template <typename RT, typename CT, int D>
+__global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedRowArgs a)
+{
+    constexpr int E = 16 / static_cast<int>(sizeof(RT));
+    constexpr int LPV = D / E;
+    constexpr int VPW = 32 / LPV;
+    constexpr int U = 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = blockIdx.x;
+    const int nv = 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+    long long off, s_off;
+    if (!paged_place(a.c, a.b, r, lane, off, s_off)) return;
+    for (int v0 = 0; v0 < nv; v0 += U * kRowWarps * VPW)
+    {
+        float x[U][E], scale[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
+            if (vec >= nv) continue;
+            const bool isv = vec >= a.c.kv_heads;
+            const int h = isv ? vec - a.c.kv_heads : vec;
+            load_row<CT, E>(isv ? a.c.v : a.c.k, off + h * a.c.head_stride + d, x[u]);
+            if constexpr (kCodes<CT>) scale[u] = __ldg((isv ? a.c.v_scale : a.c.k_scale) + s_off + h * a.c.s_head_stride);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
+            if (vec >= nv) continue;
+            const bool isv = vec >= a.c.kv_heads;
+            const int h = isv ? vec - a.c.kv_heads : vec;
+            if constexpr (kCodes<CT>)
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[u][i] *= scale[u];
+            store_row<RT, E>(isv ? a.v : a.k,
+                             isv ? r * a.v_row_stride + h * a.v_head_stride + d
+                                 : r * a.k_row_stride + h * a.k_head_stride + d,
+                             x[u]);
+        }
+    }
+}
+
+}  // namespace hy
