@@ -193,6 +193,48 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     return e == cudaSuccess ? HY_OK : cuda_fail(write ? "paged write" : "paged read", e);
 }
 
+// Lets Kernel have `smem` bytes of dynamic shared memory; set once per device.
+template <auto Kernel>
+cudaError_t allow_smem(int smem, int device)
+{
+    static std::atomic<unsigned long long> done{0};
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    const cudaError_t e =
+        cudaFuncSetAttribute(reinterpret_cast<const void*>(Kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+// Columns of a tile in units of 8 (see paged_split_kernel): as many as a sequence's rows need, up to 32.
+int split_tiles_n(int max_rows, int group)
+{
+    const long long cols = static_cast<long long>(max_rows) * group;
+    return cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+}
+
+template <typename QT, typename CT, int D, int NT>
+cudaError_t launch_split(const PagedAttnArgs& a, int device, cudaStream_t s)
+{
+    using Sh = SplitShape<QT, CT, D, NT>;
+    cudaError_t e = allow_smem<paged_split_kernel<QT, CT, D, NT>>(Sh::SMEM, device);
+    if (e != cudaSuccess) return e;
+    paged_split_kernel<QT, CT, D, NT><<<Sh::GRID, kSplitThreads, Sh::SMEM, s>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // The join may start while the split kernel runs; it waits for its end.
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(Sh::GRID);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_join_kernel<QT, Sh::F16, D, NT>, a);
+}
+
 int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype)
 {
     int rc = check_cache(cache);
@@ -202,7 +244,16 @@ int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, in
     if (q_heads < 1 || q_heads % cache->num_kv_heads)
         return fail(HY_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of num_kv_heads");
     if (q_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "q_heads must be at most 1024");
+    if (static_cast<long long>(rows) * q_heads > INT_MAX)
+        return fail(HY_ERR_CAPACITY, "rows * q_heads must be below 2^31");
     return HY_OK;
+}
+
+// Descriptions and two parts for every CTA.
+size_t attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int q_heads)
+{
+    const int cols = 8 * split_tiles_n(batch->max_rows, q_heads / cache->num_kv_heads);
+    return kSplitDescBytes + static_cast<size_t>(2 * kSplitMaxCtas) * cols * (cache->head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -231,7 +282,7 @@ int hy_paged_attention_workspace(const hy_paged_cache* cache, const hy_paged_bat
     const int rc = check_attention(cache, batch, rows, q_heads, dtype);
     if (rc) return rc;
     if (!bytes) return fail(HY_ERR_INVALID_ARGUMENT, "bytes is null");
-    *bytes = 0;
+    *bytes = attention_workspace(cache, batch, q_heads);
     return HY_OK;
 }
 
@@ -250,21 +301,26 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     if (!rc) rc = check_rows("out", out_dev, out_row_stride, out_head_stride, dtype);
     if (rc) return rc;
     if (q_dev == out_dev) return fail(HY_ERR_INVALID_ARGUMENT, "q and out must not overlap");
-    (void)workspace_dev;
-    (void)workspace_bytes;
+    if (!workspace_dev || !aligned16(workspace_dev))
+        return fail(HY_ERR_INVALID_ARGUMENT, "the workspace is null or not on 16 bytes");
+    if (workspace_bytes < attention_workspace(cache, batch, q_heads))
+        return fail(HY_ERR_CAPACITY, "the workspace is too small");
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
+    const int group = q_heads / cache->num_kv_heads;
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
-                          out_row_stride, out_head_stride, q_heads, q_heads / cache->num_kv_heads, causal != 0, window,
-                          window > 0 ? sinks : 0, scale * 1.4426950408889634f};
-    with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
+                          out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
+                          scale * 1.4426950408889634f, workspace_dev};
+    const int nt = split_tiles_n(batch->max_rows, group);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
         using RT = typename decltype(rt)::type;
         using CT = typename decltype(ct)::type;
-        const long long items = static_cast<long long>(rows) * q_heads;
-        paged_attn_rows_kernel<RT, CT, decltype(d)::value>
-            <<<static_cast<unsigned>((items + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
+        constexpr int D = decltype(d)::value;
+        return nt == 1   ? launch_split<RT, CT, D, 1>(a, cache->device, s)
+               : nt == 2 ? launch_split<RT, CT, D, 2>(a, cache->device, s)
+                         : launch_split<RT, CT, D, 4>(a, cache->device, s);
     });
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? HY_OK : cuda_fail("paged attention", e);
 }
 
