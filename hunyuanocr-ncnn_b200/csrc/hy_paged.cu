@@ -41,6 +41,15 @@ int cuda_fail(const char* what, cudaError_t e) noexcept
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// log2 of n where it is one, else -1.
+int power_of_two(int n)
+{
+    if (n & (n - 1)) return -1;
+    int s = 0;
+    while ((1 << s) < n) ++s;
+    return s;
+}
+
 int elem_size(int dtype) { return dtype == HY_DTYPE_F32 ? 4 : dtype == HY_DTYPE_BF16 ? 2 : 1; }
 
 int check_cache(const hy_paged_cache* c)
@@ -310,7 +319,7 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     const int group = q_heads / cache->num_kv_heads;
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
-                          scale * 1.4426950408889634f, workspace_dev};
+                          power_of_two(cache->page_size), scale * 1.4426950408889634f, workspace_dev};
     const int nt = split_tiles_n(batch->max_rows, group);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {

@@ -22,6 +22,7 @@ struct PagedAttnArgs {
     long long q_row_stride, q_head_stride, o_row_stride, o_head_stride;
     int q_heads, group;   // group = q_heads / kv_heads
     int causal, window, sinks;
+    int page_shift;       // log2(page_size), or -1
     float scale_log2;     // scale * log2(e)
     void* work;           // workspace
 };
@@ -177,12 +178,12 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x)
 // Few rows per sequence: the keys are split over the GPU.
 //
 // The work is the list of (sequence, tile of 8 NT columns, KV head) items, each
-// of ceil(keys / 64) tiles (at least one); CTA i of G takes the tiles [T i / G, T (i + 1) / G)
-// of the whole list, whatever items they belong to, so every CTA streams the same
-// number of keys however ragged the lengths are. Memory bounds it (a key is
-// used by the group's heads only), so all that matters is that loads never pause: every
-// warp owns 16 of a tile's 64 keys and a cp.async ring of its own, and the warps
-// meet only at the end of an item.
+// of ceil(keys / TILE) tiles (at least one), T in all; CTA i of G takes the next
+// ceil(T / G) tiles of the whole list, whatever items they belong to, so every CTA
+// streams the same number of keys however ragged the lengths are. Memory bounds it
+// (a key is used by the group's heads only), so all that matters is that loads
+// never pause: every warp owns a quarter of a tile's keys and a cp.async ring of its
+// own, and the warps meet only at the end of an item.
 //
 // The products are taken transposed, S^T[key x column] = K Q^T and O^T[dim x
 // column] = V^T P^T: with the columns in the 8-wide dimension a decode step of
@@ -203,8 +204,7 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x)
 // ---------------------------------------------------------------------------
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
-constexpr int kSplitKeys = 16 * kSplitWarps;   // keys of a tile
-constexpr int kSplitMaxCtas = 2 * 148;         // two CTAs per SM
+constexpr int kSplitMaxCtas = 3 * 148;   // three CTAs per SM
 
 struct PagedJoin {   // description of an item whose parts are joined; count 0: none
     int count, first_slot, first_cta, row0, col0, cols, head, pad;
@@ -217,8 +217,12 @@ struct SplitShape {
     static constexpr int NK = std::is_same_v<CT, float> ? 3 : 1;               // terms of k and v
     static constexpr int COLS = 8 * NT;
     static constexpr int RB = D * static_cast<int>(sizeof(CT));                // bytes of a row
-    static constexpr int STAGE = 2 * 16 * RB;                                  // a warp's 16 keys and values
-    static constexpr int SCALES = F16 ? 128 : 0;
+    // Keys of a warp's step: 32 where that is 8 KB or less (the work that a step
+    // costs whatever its keys - addresses, maxima, shuffles - is halved), else 16.
+    static constexpr int KEYS = RB <= 128 ? 32 : 16;
+    static constexpr int TILE = kSplitWarps * KEYS;
+    static constexpr int STAGE = 2 * KEYS * RB;                                // a warp's keys and values
+    static constexpr int SCALES = F16 ? 2 * KEYS * 4 : 0;
     static constexpr int QB = (D / 16) * NT * NQ * 256;
     static constexpr int FIX = QB + 2 * COLS * 4 + kSplitWarps * COLS * 8 + 64;
     static constexpr int fit(int kb, int most)
@@ -226,13 +230,13 @@ struct SplitShape {
         const int n = (kb * 1024 - FIX) / (kSplitWarps * (STAGE + SCALES + 16));
         return n < most ? n : most;
     }
-    static constexpr int OCC = fit(112, 6) >= 2 ? 2 : 1;
-    static constexpr int S = OCC == 2 ? fit(112, 6) : fit(224, 6);
+    static constexpr int OCC = (NT == 1 && fit(74, 4) >= 2) ? 3 : fit(112, 4) >= 2 ? 2 : 1;
+    static constexpr int S = OCC == 3 ? fit(74, 4) : OCC == 2 ? fit(112, 4) : fit(224, 4);
     static constexpr int RING = kSplitWarps * S * STAGE;
     static constexpr int MERGE = kSplitWarps * COLS * (D + 4) * 4;   // the warps' sums, over the drained ring
     static constexpr int BODY = RING > MERGE ? RING : MERGE;
     static constexpr int SC_OFF = BODY;
-    static constexpr int MASK_OFF = SC_OFF + kSplitWarps * S * SCALES;
+    static constexpr int MASK_OFF = SC_OFF + kSplitWarps * S * SCALES;   // a bit for every key that is there
     static constexpr int Q_OFF = (MASK_OFF + kSplitWarps * S * 4 + 127) / 128 * 128;
     static constexpr int QS_OFF = Q_OFF + QB;                        // [COLS] 2^-k of a column's q
     static constexpr int ML_OFF = QS_OFF + COLS * 4;                 // [warps][COLS] (m, l)
@@ -274,7 +278,7 @@ __device__ __forceinline__ int split_v_at(int r, int c)
     else
     {
         // 64-byte rows: even rows first, so that rows 0, 2, 4, 6 span both halves of the banks.
-        const int pos = (r & 8) | ((r & 1) << 2) | ((r & 6) >> 1);
+        const int pos = (r & ~7) | ((r & 1) << 2) | ((r & 6) >> 1);
         return pos * RB + ((c ^ (pos & 2)) << 4);
     }
 }
@@ -290,17 +294,18 @@ __device__ __forceinline__ int split_row_tiles(const PagedAttnArgs& a, int n)
 {
     return (n * a.group + COLS - 1) / COLS;
 }
-__device__ __forceinline__ int split_tiles(int keys) { return max(1, (keys + kSplitKeys - 1) / kSplitKeys); }
+template <int TILE>
+__device__ __forceinline__ int split_tiles(int keys) { return max(1, (keys + TILE - 1) / TILE); }
 
 // Tiles of sequence s, all its items.
-template <int COLS>
+template <int COLS, int TILE>
 __device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
 {
     PagedSeq q;
     if (s >= a.b.num_seqs || !paged_seq(a.b, s, a.c.page_size, a.c.status, q)) return 0;
     long long c = 0;
     const int rt = split_row_tiles<COLS>(a, q.n);
-    for (int t = 0; t < rt; ++t) c += split_tiles(paged_span(a, q, t * COLS, COLS).n);
+    for (int t = 0; t < rt; ++t) c += split_tiles<TILE>(paged_span(a, q, t * COLS, COLS).n);
     return c * a.c.kv_heads;
 }
 
@@ -309,9 +314,10 @@ __device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
 struct SplitStart {
     long long x0, x1, total;   // the CTA's tiles; of all
     long long in_seq;          // x0 counted from its sequence's first tile
-    int seq, ctas;             // CTAs that the work is given to: no more than tiles
+    long long share;           // tiles per CTA
+    int seq;
 };
-template <int COLS>
+template <int COLS, int TILE>
 __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long long* scan)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -320,24 +326,23 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     o.total = 0;
     const int rounds = (a.b.num_seqs + kSplitThreads - 1) / kSplitThreads;
     long long mine = 0;
-    for (int r = 0; r < rounds; ++r) mine = split_cost<COLS>(a, r * kSplitThreads + tid), o.total += mine;
+    for (int r = 0; r < rounds; ++r) mine = split_cost<COLS, TILE>(a, r * kSplitThreads + tid), o.total += mine;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) o.total += __shfl_xor_sync(0xffffffffu, o.total, d);
     if (lane == 0) scan[warp] = o.total;
     __syncthreads();
     o.total = 0;
     for (int w = 0; w < kSplitWarps; ++w) o.total += scan[w];
-    o.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), o.total));
+    o.share = max(1ll, (o.total + gridDim.x - 1) / gridDim.x);
+    o.x0 = min(o.total, o.share * blockIdx.x);
+    o.x1 = min(o.total, o.x0 + o.share);
     o.seq = 0;
     o.in_seq = 0;
-    o.x0 = o.x1 = 0;
-    if (static_cast<int>(blockIdx.x) >= o.ctas) return o;
-    o.x0 = o.total * blockIdx.x / o.ctas;
-    o.x1 = o.total * (blockIdx.x + 1) / o.ctas;
+    if (o.x0 >= o.x1) return o;
     long long base = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        if (rounds > 1) mine = split_cost<COLS>(a, r * kSplitThreads + tid);
+        if (rounds > 1) mine = split_cost<COLS, TILE>(a, r * kSplitThreads + tid);
         long long inc = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1)
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
     using Sh = SplitShape<QT, CT, D, NT>;
     constexpr bool F16 = Sh::F16;
     constexpr int NQ = Sh::NQ, NK = Sh::NK, COLS = Sh::COLS, S = Sh::S, RB = Sh::RB, CPR = RB / 16;
-    constexpr int KS = D / 16, MTS = D / 16;
+    constexpr int KS = D / 16, MTS = D / 16, KEYS = Sh::KEYS, TILE = Sh::TILE, HV = KEYS / 16;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan[6];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
     PagedJoin* const desc = static_cast<PagedJoin*>(a.work) + blockIdx.x;
     float* const parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.work) + kSplitDescBytes);
 
-    const SplitStart st = split_start<COLS>(a, scan);
+    const SplitStart st = split_start<COLS, Sh::TILE>(a, scan);
     if (st.x0 >= st.x1)
     {
         if (tid == 0) desc->count = 0;
@@ -395,7 +400,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
     for (it.tile = 0;; ++it.tile)
     {
         it.w = paged_span(a, it.q, it.tile * COLS, COLS);
-        it.tiles = split_tiles(it.w.n);
+        it.tiles = split_tiles<Sh::TILE>(it.w.n);
         if (in < static_cast<long long>(it.tiles) * a.c.kv_heads) break;
         if ((it.tile + 1) * COLS >= it.q.n * a.group) return;   // (the arrays changed under the call)
         in -= static_cast<long long>(it.tiles) * a.c.kv_heads;
@@ -419,43 +424,47 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
         const int cols = min(COLS, it.q.n * a.group - it.tile * COLS);
         const int* const table = a.b.table + it.seq * a.b.table_stride;
 
-        // ---- loads: this warp's 16 keys of tile tile0 + i into slot i % S ----
-        const int kr = lane & 15;
+        // ---- loads: this warp's keys of tile tile0 + i into slot i % S ----
+        const int kr = lane % KEYS;
         auto key_of = [&](int u) { return u < it.w.sinks ? u : it.w.lo + u - it.w.sinks; };
-        auto page_of = [&](int i) {   // -1: no key
-            const int u = (tile0 + i) * kSplitKeys + warp * 16 + kr;
-            return (i < n_tiles && u < it.w.n) ? __ldg(table + key_of(u) / a.c.page_size) : -1;
+        // Page and row in it of this lane's key of a tile, looked up a step ahead of the load.
+        int pg_next = 0, in_next = 0;
+        auto look_up = [&](int i) {
+            const int u = (tile0 + i) * TILE + warp * KEYS + kr;
+            if (i >= n_tiles || u >= it.w.n) return;
+            const int j = key_of(u), pg = a.page_shift >= 0 ? j >> a.page_shift : j / a.c.page_size;
+            in_next = j - pg * a.c.page_size;
+            pg_next = __ldg(table + pg);
         };
-        int pg_next = page_of(0);
+        look_up(0);
         auto load = [&](int i) {
             if (i < n_tiles)
             {
                 const int slot = i % S;
-                const int u = (tile0 + i) * kSplitKeys + warp * 16 + kr;
-                const int pg = pg_next;
-                const bool live = u < it.w.n;
-                const bool ok = live && pg >= 0 && pg < a.c.num_pages;
+                const bool live = (tile0 + i) * TILE + warp * KEYS + kr < it.w.n;
+                const bool ok = live && pg_next >= 0 && pg_next < a.c.num_pages;
                 if (live && !ok) paged_status(a.c.status, kPagedBadPage);
-                const int in_page = live ? key_of(u) % a.c.page_size : 0;
-                const long long off = ok ? pg * a.c.page_stride + in_page * a.c.row_stride + it.head * a.c.head_stride : 0;
-                const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+                const long long off = ok ? pg_next * a.c.page_stride + in_next * a.c.row_stride + it.head * a.c.head_stride : 0;
+                const uint32_t mask = __ballot_sync(0xffffffffu, ok);
                 if (lane == 0) masks[slot] = mask;
                 const uint32_t base = ring_u + slot * Sh::STAGE;
 #pragma unroll
-                for (int x = 0; x < 16 * CPR / 32; ++x)
+                for (int x = 0; x < KEYS * CPR / 32; ++x)
                 {
                     const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
                     const long long o = __shfl_sync(0xffffffffu, off, r) + c * (16 / static_cast<int>(sizeof(CT)));
                     const bool pr = (mask >> r) & 1u;
                     cp_async16_zfill(base + split_k_at<CT, D>(r, c), static_cast<const CT*>(a.c.k) + o, pr);
-                    cp_async16_zfill(base + 16 * RB + split_v_at<CT, D>(r, c), static_cast<const CT*>(a.c.v) + o, pr);
+                    cp_async16_zfill(base + KEYS * RB + split_v_at<CT, D>(r, c), static_cast<const CT*>(a.c.v) + o, pr);
                 }
                 if constexpr (F16)
                 {
-                    const long long so = ok ? pg * a.c.s_page_stride + in_page * a.c.s_row_stride + it.head * a.c.s_head_stride : 0;
-                    cp_async4_zfill(sc_u + slot * Sh::SCALES + lane * 4, (lane < 16 ? a.c.k_scale : a.c.v_scale) + so, ok);
+                    const long long so = ok ? pg_next * a.c.s_page_stride + in_next * a.c.s_row_stride + it.head * a.c.s_head_stride : 0;
+                    const uint32_t dst = sc_u + slot * Sh::SCALES + kr * 4;
+                    cp_async4_zfill(dst, a.c.k_scale + so, ok);
+                    cp_async4_zfill(dst + KEYS * 4, a.c.v_scale + so, ok);
                 }
-                pg_next = page_of(i + 1);
+                look_up(i + 1);
             }
             cp_commit();
         };
@@ -556,116 +565,119 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
             cp_wait<S - 2>();
             __syncwarp();
             load(i + S - 1);
-            const int u0 = (tile0 + i) * kSplitKeys + warp * 16;
+            const int u0 = (tile0 + i) * TILE + warp * KEYS;
             if (u0 >= it.w.n) continue;   // nothing for this warp in the item's last tile
             const int slot = i % S;
-            const uint32_t kb = ring_u + slot * Sh::STAGE, vb = kb + 16 * RB;
+            const uint32_t kb = ring_u + slot * Sh::STAGE, vb = kb + KEYS * RB;
             const uint32_t live = masks[slot];
 
-            float sc[NT][4];
+            // Scores of the step's keys: sc[hv][nt] holds keys 16 hv + g and + 8.
+            float sc[HV][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-            uint4 w0, w1;   // 8-bit keys: 64 dimensions of rows g and g + 8
+            for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+                for (int nt = 0; nt < NT; ++nt) sc[hv][nt][0] = sc[hv][nt][1] = sc[hv][nt][2] = sc[hv][nt][3] = 0.f;
+#pragma unroll
+            for (int hv = 0; hv < HV; ++hv)
             {
-                uint32_t ka[NK][4];
-                if constexpr (sizeof(CT) == 2)
+                uint4 w0, w1;   // 8-bit keys: 64 dimensions of rows g and g + 8
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
                 {
-                    ldmatrix4(ka[0], kb + split_k_at<CT, D>(lane & 15, 2 * ks + (lane >> 4)));
-                }
-                else if constexpr (sizeof(CT) == 4)
-                {
-                    const uint4 x = lds128(kb + split_k_at<CT, D>(g, 4 * ks + t)), y = lds128(kb + split_k_at<CT, D>(g + 8, 4 * ks + t));
-                    uint32_t p[NK];
-                    split_pair<false, NK>(__uint_as_float(x.x), __uint_as_float(x.y), p);
-#pragma unroll
-                    for (int n = 0; n < NK; ++n) ka[n][0] = p[n];
-                    split_pair<false, NK>(__uint_as_float(y.x), __uint_as_float(y.y), p);
-#pragma unroll
-                    for (int n = 0; n < NK; ++n) ka[n][1] = p[n];
-                    split_pair<false, NK>(__uint_as_float(x.z), __uint_as_float(x.w), p);
-#pragma unroll
-                    for (int n = 0; n < NK; ++n) ka[n][2] = p[n];
-                    split_pair<false, NK>(__uint_as_float(y.z), __uint_as_float(y.w), p);
-#pragma unroll
-                    for (int n = 0; n < NK; ++n) ka[n][3] = p[n];
-                }
-                else
-                {
-                    if (ks % 4 == 0)
+                    uint32_t ka[NK][4];
+                    if constexpr (sizeof(CT) == 2)
                     {
-                        w0 = lds128(kb + split_k_at<CT, D>(g, ks + t));
-                        w1 = lds128(kb + split_k_at<CT, D>(g + 8, ks + t));
+                        ldmatrix4(ka[0], kb + split_k_at<CT, D>(16 * hv + (lane & 15), 2 * ks + (lane >> 4)));
                     }
-                    const uint32_t x = ks % 4 == 0 ? w0.x : ks % 4 == 1 ? w0.y : ks % 4 == 2 ? w0.z : w0.w;
-                    const uint32_t y = ks % 4 == 0 ? w1.x : ks % 4 == 1 ? w1.y : ks % 4 == 2 ? w1.z : w1.w;
-                    ka[0][0] = codes_f16<CT>(x);
-                    ka[0][1] = codes_f16<CT>(y);
-                    ka[0][2] = codes_f16<CT>(x >> 16);
-                    ka[0][3] = codes_f16<CT>(y >> 16);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = NQ - 1; j >= 0; --j)
+                    else if constexpr (sizeof(CT) == 4)
                     {
-                        const uint2 b = q_frag(j, ks, nt);
+                        const uint4 x = lds128(kb + split_k_at<CT, D>(16 * hv + g, 4 * ks + t)),
+                                    y = lds128(kb + split_k_at<CT, D>(16 * hv + g + 8, 4 * ks + t));
+                        uint32_t p[NK];
+                        auto put = [&](int at, uint32_t lo, uint32_t hi) {
+                            split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
 #pragma unroll
-                        for (int n = NK - 1; n >= 0; --n)
-                            if (n + j <= 2) mma16816<F16>(sc[nt], ka[n], b.x, b.y);
+                            for (int n = 0; n < NK; ++n) ka[n][at] = p[n];
+                        };
+                        put(0, x.x, x.y);
+                        put(1, y.x, y.y);
+                        put(2, x.z, x.w);
+                        put(3, y.z, y.w);
                     }
+                    else
+                    {
+                        if (ks % 4 == 0)
+                        {
+                            w0 = lds128(kb + split_k_at<CT, D>(16 * hv + g, ks + t));
+                            w1 = lds128(kb + split_k_at<CT, D>(16 * hv + g + 8, ks + t));
+                        }
+                        const uint32_t x = ks % 4 == 0 ? w0.x : ks % 4 == 1 ? w0.y : ks % 4 == 2 ? w0.z : w0.w;
+                        const uint32_t y = ks % 4 == 0 ? w1.x : ks % 4 == 1 ? w1.y : ks % 4 == 2 ? w1.z : w1.w;
+                        ka[0][0] = codes_f16<CT>(x);
+                        ka[0][1] = codes_f16<CT>(y);
+                        ka[0][2] = codes_f16<CT>(x >> 16);
+                        ka[0][3] = codes_f16<CT>(y >> 16);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = NQ - 1; j >= 0; --j)
+                        {
+                            const uint2 b = q_frag(j, ks, nt);
+#pragma unroll
+                            for (int n = NK - 1; n >= 0; --n)
+                                if (n + j <= 2) mma16816<F16>(sc[hv][nt], ka[n], b.x, b.y);
+                        }
+                }
             }
 
-            // Scores in units of log 2, masks, the weights' exponents.
-            float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f, ev0 = 0.f, ev1 = 0.f;
-            if constexpr (F16)
-            {
-                const uint32_t s = sc_u + slot * Sh::SCALES;
-                ks0 = lds_f32(s + g * 4);
-                ks1 = lds_f32(s + (g + 8) * 4);
-                vs0 = lds_f32(s + 64 + g * 4);
-                vs1 = lds_f32(s + 64 + (g + 8) * 4);
-                // The maximum is taken over the score plus the exponent of the value's scale, so that
-                // a weight times its scale is below 2 and fits f16 (times 2^14).
-                ev0 = fminf(fmaxf(static_cast<float>(static_cast<int>(__float_as_uint(vs0) >> 23) - 127), -100.f), 100.f);
-                ev1 = fminf(fmaxf(static_cast<float>(static_cast<int>(__float_as_uint(vs1) >> 23) - 127), -100.f), 100.f);
-                vs0 *= 16384.f;
-                vs1 *= 16384.f;
-            }
-            const int j_first = key_of(u0), j_last = key_of(min(u0 + 15, it.w.n - 1));
-            const bool whole = live == 0xffffu &&
+            // Scores in units of log 2, masks, the weights' exponents. Index [hv][r]: key 16 hv + 8 r + g.
+            float vs[HV][2], ev[HV][2], kf[HV][2];
+#pragma unroll
+            for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                {
+                    kf[hv][r] = vs[hv][r] = 1.f;
+                    ev[hv][r] = 0.f;
+                    if constexpr (F16)
+                    {
+                        const uint32_t at = sc_u + slot * Sh::SCALES + (16 * hv + 8 * r + g) * 4;
+                        kf[hv][r] = lds_f32(at);
+                        const float v = lds_f32(at + KEYS * 4);
+                        // The maximum is taken over the score plus the exponent of the value's scale, so that
+                        // a weight times its scale is below 2 and fits f16 (times 2^14).
+                        ev[hv][r] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(v) >> 23) - 127, -100), 100));
+                        vs[hv][r] = v * 16384.f;
+                    }
+                }
+            const int j_first = key_of(u0), j_last = key_of(min(u0 + KEYS - 1, it.w.n - 1));
+            const bool whole = live == (KEYS == 32 ? 0xffffffffu : 0xffffu) &&
                                (!a.causal || (j_last <= it.w.p_first &&
                                               (a.window == 0 || j_first > it.w.p_last - a.window || j_last < a.sinks))) &&
                                it.w.p_first >= 0;
-            bool hidden = false;   // some column does not see a key that was loaded
+            uint32_t seen = 0xffffffffu;   // bit ((hv * 2 + r) * NT + nt) * 2 + e: the column sees the key
+            bool hidden = false;           // some column does not see a key that was loaded
             if (!whole)
             {
-                const int j0 = key_of(u0 + g), j1 = key_of(u0 + g + 8);
-                const bool l0 = (live >> g) & 1u, l1 = (live >> (g + 8)) & 1u;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+                    for (int r = 0; r < 2; ++r)
                     {
-                        const bool v0 = l0 && paged_sees(a, pos[nt][e], j0), v1 = l1 && paged_sees(a, pos[nt][e], j1);
-                        hidden |= (l0 && !v0) || (l1 && !v1);
-                        sc[nt][e] = v0 ? sc[nt][e] * (fac[nt][e] * ks0) : -INFINITY;
-                        sc[nt][2 + e] = v1 ? sc[nt][2 + e] * (fac[nt][e] * ks1) : -INFINITY;
+                        const int in16 = 16 * hv + 8 * r + g, j = key_of(u0 + in16);
+                        const bool there = (live >> in16) & 1u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                            {
+                                const bool v = there && paged_sees(a, pos[nt][e], j);
+                                hidden |= there && !v;
+                                if (!v) seen &= ~(1u << (((hv * 2 + r) * NT + nt) * 2 + e));
+                            }
                     }
             }
-            else
-            {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                    {
-                        sc[nt][e] *= fac[nt][e] * ks0;
-                        sc[nt][2 + e] *= fac[nt][e] * ks1;
-                    }
-            }
-            uint32_t pb[NT][2][NQ];   // weights as B fragments
             bool grew = false;
             float corr[NT][2];
 #pragma unroll
@@ -674,7 +686,17 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                 {
-                    float x = fmaxf(sc[nt][e] + ev0, sc[nt][2 + e] + ev1);
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                        {
+                            float& y = sc[hv][nt][2 * r + e];
+                            y *= F16 ? fac[nt][e] * kf[hv][r] : fac[nt][e];
+                            if (!whole && !((seen >> (((hv * 2 + r) * NT + nt) * 2 + e)) & 1u)) y = -INFINITY;
+                            x = fmaxf(x, F16 ? y + ev[hv][r] : y);
+                        }
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -686,10 +708,20 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                         grew = true;
                     }
                     const float mm = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-                    // (a NaN score stays one: exp2f(NaN) is NaN)
-                    sc[nt][e] = exp2f(sc[nt][e] - mm);
-                    sc[nt][2 + e] = exp2f(sc[nt][2 + e] - mm);
-                    l[nt][e] = l[nt][e] * corr[nt][e] + (sc[nt][e] + sc[nt][2 + e]);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                        {
+                            float& y = sc[hv][nt][2 * r + e];
+                            y = exp2f(y - mm);   // (a NaN score stays one)
+                            sum += y;
+                            // A scale of NaN must not meet a weight of zero that stands for "not seen".
+                            if constexpr (F16)
+                                y = (!whole && !((seen >> (((hv * 2 + r) * NT + nt) * 2 + e)) & 1u)) ? 0.f : y * vs[hv][r];
+                        }
+                    l[nt][e] = l[nt][e] * corr[nt][e] + sum;
                 }
             }
             if (__any_sync(0xffffffffu, grew))
@@ -705,20 +737,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                         acc[nt][x][3] *= corr[nt][1];
                     }
             }
-            if constexpr (F16)
-            {
-                // A scale of NaN must not meet a weight of zero that stands for "not seen".
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                    {
-                        const bool z0 = !whole && !(((live >> g) & 1u) && paged_sees(a, pos[nt][e], key_of(u0 + g)));
-                        const bool z1 = !whole && !(((live >> (g + 8)) & 1u) && paged_sees(a, pos[nt][e], key_of(u0 + g + 8)));
-                        sc[nt][e] = z0 ? 0.f : sc[nt][e] * vs0;
-                        sc[nt][2 + e] = z1 ? 0.f : sc[nt][2 + e] * vs1;
-                    }
-            }
             // Values that some column must not see may be infinite or NaN, and 0 times those is NaN:
             // if there are any in such a step, its products are taken one by one.
             if constexpr (!F16)
@@ -726,7 +744,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                 if (__any_sync(0xffffffffu, hidden))
                 {
                     bool odd = false;
-                    for (int x = lane; x < 16 * CPR; x += 32)
+                    for (int x = lane; x < KEYS * CPR; x += 32)
                     {
                         const uint4 w = lds128(vb + x * 16);
                         const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
@@ -736,119 +754,130 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                     }
                     if (__any_sync(0xffffffffu, odd))
                     {
-                        for (int j = 0; j < 16; ++j)
+#pragma unroll
+                        for (int hr = 0; hr < 2 * HV; ++hr)
                         {
-                            const int src = (j & 7) * 4 + t, key = key_of(u0 + j);
+                            const unsigned char* const vst = ring + slot * Sh::STAGE + KEYS * RB;
+#pragma unroll 1
+                            for (int k = 0; k < 8; ++k)
+                            {
+                                const int row = 8 * hr + k, key = key_of(u0 + row);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
+                                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                {
-                                    const float p = __shfl_sync(0xffffffffu, j < 8 ? sc[nt][e] : sc[nt][2 + e], src);
-                                    if (!((live >> j) & 1u) || !paged_sees(a, pos[nt][e], key)) continue;
+                                    for (int e = 0; e < 2; ++e)
+                                    {
+                                        const float p = __shfl_sync(0xffffffffu, sc[hr >> 1][nt][2 * (hr & 1) + e], k * 4 + t);
+                                        if (!((live >> row) & 1u) || !paged_sees(a, pos[nt][e], key)) continue;
 #pragma unroll
-                                    for (int x = 0; x < MTS; ++x)
+                                        for (int x = 0; x < MTS; ++x)
 #pragma unroll
-                                        for (int hf = 0; hf < 2; ++hf)
-                                        {
-                                            const int d = split_dim<CT, D>(x, hf, g), by = d * static_cast<int>(sizeof(CT));
-                                            const unsigned char* at = ring + slot * Sh::STAGE + 16 * RB +
-                                                                      split_v_at<CT, D>(j, by >> 4) + (by & 15);
-                                            if constexpr (!F16) acc[nt][x][2 * hf + e] += p * to_f32<CT>(*reinterpret_cast<const CT*>(at));
-                                        }
-                                }
+                                            for (int hf = 0; hf < 2; ++hf)
+                                            {
+                                                const int by = split_dim<CT, D>(x, hf, g) * static_cast<int>(sizeof(CT));
+                                                acc[nt][x][2 * hf + e] +=
+                                                    p * to_f32<CT>(*reinterpret_cast<const CT*>(vst + split_v_at<CT, D>(row, by >> 4) + (by & 15)));
+                                            }
+                                    }
+                            }
                         }
                         continue;
                     }
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int hv = 0; hv < HV; ++hv)
             {
-                uint32_t p0[NQ], p1[NQ];
-                split_pair<F16, NQ>(sc[nt][0], sc[nt][1], p0);
-                split_pair<F16, NQ>(sc[nt][2], sc[nt][3], p1);
-#pragma unroll
-                for (int j = 0; j < NQ; ++j)
-                {
-                    pb[nt][0][j] = movmatrix(p0[j]);
-                    pb[nt][1][j] = movmatrix(p1[j]);
-                }
-            }
-            auto pv = [&](int mt, const uint32_t (&va)[NK][4]) {
+                uint32_t pb[NT][2][NQ];   // weights as B fragments
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = NQ - 1; j >= 0; --j)
-#pragma unroll
-                        for (int n = NK - 1; n >= 0; --n)
-                            if (n + j <= 2) mma16816<F16>(acc[nt][mt], va[n], pb[nt][0][j], pb[nt][1][j]);
-            };
-            if constexpr (sizeof(CT) == 2)
-            {
-#pragma unroll
-                for (int mt = 0; mt < MTS; ++mt)
                 {
-                    uint32_t va[1][4];
-                    ldmatrix4_trans(va[0], vb + split_v_at<CT, D>((lane & 7) + ((lane >> 4) << 3), 2 * mt + ((lane >> 3) & 1)));
-                    pv(mt, va);
-                }
-            }
-            else if constexpr (sizeof(CT) == 4)
-            {
+                    uint32_t p0[NQ], p1[NQ];
+                    split_pair<F16, NQ>(sc[hv][nt][0], sc[hv][nt][1], p0);
+                    split_pair<F16, NQ>(sc[hv][nt][2], sc[hv][nt][3], p1);
 #pragma unroll
-                for (int x = 0; x < D / 32; ++x)
-                {
-                    const uint4 f0 = lds128(vb + split_v_at<CT, D>(2 * t, 8 * x + g)), f1 = lds128(vb + split_v_at<CT, D>(2 * t + 1, 8 * x + g));
-                    const uint4 f2 = lds128(vb + split_v_at<CT, D>(2 * t + 8, 8 * x + g)), f3 = lds128(vb + split_v_at<CT, D>(2 * t + 9, 8 * x + g));
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
+                    for (int j = 0; j < NQ; ++j)
                     {
-                        uint32_t va[NK][4], p[NK];
-                        auto put = [&](int at, uint32_t lo, uint32_t hi) {
-                            split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
-#pragma unroll
-                            for (int n = 0; n < NK; ++n) va[n][at] = p[n];
-                        };
-                        put(0, y ? f0.z : f0.x, y ? f1.z : f1.x);
-                        put(1, y ? f0.w : f0.y, y ? f1.w : f1.y);
-                        put(2, y ? f2.z : f2.x, y ? f3.z : f3.x);
-                        put(3, y ? f2.w : f2.y, y ? f3.w : f3.y);
-                        pv(2 * x + y, va);
+                        pb[nt][0][j] = movmatrix(p0[j]);
+                        pb[nt][1][j] = movmatrix(p1[j]);
                     }
                 }
-            }
-            else
-            {
-                // Rows 2t, 2t + 1, 2t + 8, 2t + 9; D / 8 consecutive dimensions of each.
-                constexpr int W = D / 32;   // words
-                uint32_t f[4][W];
+                auto pv = [&](int mt, const uint32_t (&va)[NK][4]) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = NQ - 1; j >= 0; --j)
+#pragma unroll
+                            for (int n = NK - 1; n >= 0; --n)
+                                if (n + j <= 2) mma16816<F16>(acc[nt][mt], va[n], pb[nt][0][j], pb[nt][1][j]);
+                };
+                if constexpr (sizeof(CT) == 2)
                 {
-                    const int row = 2 * t + (r & 1) + (r >> 1) * 8;
-                    if constexpr (D == 128)
+#pragma unroll
+                    for (int mt = 0; mt < MTS; ++mt)
                     {
-                        const uint4 x = lds128(vb + split_v_at<CT, D>(row, g));
-                        f[r][0] = x.x; f[r][1] = x.y; f[r][2] = x.z; f[r][3] = x.w;
-                    }
-                    else
-                    {
-                        const uint2 x = lds64(vb + split_v_at<CT, D>(row, g >> 1) + (g & 1) * 8);
-                        f[r][0] = x.x; f[r][1] = x.y;
+                        uint32_t va[1][4];
+                        ldmatrix4_trans(va[0], vb + split_v_at<CT, D>(16 * hv + (lane & 7) + ((lane >> 4) << 3), 2 * mt + ((lane >> 3) & 1)));
+                        pv(mt, va);
                     }
                 }
-#pragma unroll
-                for (int mt = 0; mt < MTS; ++mt)
+                else if constexpr (sizeof(CT) == 4)
                 {
-                    const int wd = mt >> 1;
-                    const uint32_t s0 = (mt & 1) ? 0x62u : 0x40u, s1 = (mt & 1) ? 0x73u : 0x51u;
-                    uint32_t va[1][4];
-                    va[0][0] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s0));
-                    va[0][1] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s1));
-                    va[0][2] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s0));
-                    va[0][3] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s1));
-                    pv(mt, va);
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x)
+                    {
+                        const int r0 = 16 * hv + 2 * t, c = 8 * x + g;
+                        const uint4 f0 = lds128(vb + split_v_at<CT, D>(r0, c)), f1 = lds128(vb + split_v_at<CT, D>(r0 + 1, c));
+                        const uint4 f2 = lds128(vb + split_v_at<CT, D>(r0 + 8, c)), f3 = lds128(vb + split_v_at<CT, D>(r0 + 9, c));
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                        {
+                            uint32_t va[NK][4], p[NK];
+                            auto put = [&](int at, uint32_t lo, uint32_t hi) {
+                                split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
+#pragma unroll
+                                for (int n = 0; n < NK; ++n) va[n][at] = p[n];
+                            };
+                            put(0, y ? f0.z : f0.x, y ? f1.z : f1.x);
+                            put(1, y ? f0.w : f0.y, y ? f1.w : f1.y);
+                            put(2, y ? f2.z : f2.x, y ? f3.z : f3.x);
+                            put(3, y ? f2.w : f2.y, y ? f3.w : f3.y);
+                            pv(2 * x + y, va);
+                        }
+                    }
+                }
+                else
+                {
+                    // Rows 2t, 2t + 1, 2t + 8, 2t + 9; D / 8 consecutive dimensions of each.
+                    constexpr int W = D / 32;   // words
+                    uint32_t f[4][W];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                    {
+                        const int row = 16 * hv + 2 * t + (r & 1) + (r >> 1) * 8;
+                        if constexpr (D == 128)
+                        {
+                            const uint4 x = lds128(vb + split_v_at<CT, D>(row, g));
+                            f[r][0] = x.x; f[r][1] = x.y; f[r][2] = x.z; f[r][3] = x.w;
+                        }
+                        else
+                        {
+                            const uint2 x = lds64(vb + split_v_at<CT, D>(row, g >> 1) + (g & 1) * 8);
+                            f[r][0] = x.x; f[r][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MTS; ++mt)
+                    {
+                        const int wd = mt >> 1;
+                        const uint32_t s0 = (mt & 1) ? 0x62u : 0x40u, s1 = (mt & 1) ? 0x73u : 0x51u;
+                        uint32_t va[1][4];
+                        va[0][0] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s0));
+                        va[0][1] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s1));
+                        va[0][2] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s0));
+                        va[0][3] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s1));
+                        pv(mt, va);
+                    }
                 }
             }
         }
@@ -923,11 +952,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
         {
             // This CTA starts the item: its parts are here and in the CTAs up to the one with the item's last tile.
             const long long x_last = st.x1 - left - n_tiles + it.tiles - 1 - tile0;   // (global index of that tile)
-            long long last = x_last * st.ctas / st.total;
-            while (st.total * (last + 1) / st.ctas <= x_last) ++last;
-            while (st.total * last / st.ctas > x_last) --last;
+            const int last = static_cast<int>(x_last / st.share);
             PagedJoin d;
-            d.count = static_cast<int>(last) - static_cast<int>(blockIdx.x) + 1;
+            d.count = last - static_cast<int>(blockIdx.x) + 1;
             d.first_slot = part_slot;
             d.first_cta = blockIdx.x;
             d.row0 = it.q.row0;
@@ -954,7 +981,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                 if (it.seq >= a.b.num_seqs) break;   // (the arrays changed under the call)
             }
             it.w = paged_span(a, it.q, it.tile * COLS, COLS);
-            it.tiles = split_tiles(it.w.n);
+            it.tiles = split_tiles<Sh::TILE>(it.w.n);
         }
         __syncthreads();   // the sums were read; the ring is free
     }

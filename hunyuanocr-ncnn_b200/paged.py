@@ -23,6 +23,7 @@ _STATUS = {1: "a page number lies outside the cache", 2: "a kv_len does not fit 
            4: "q_start is not ascending or leaves the rows", 8: "a bounded wait inside a kernel gave up"}
 
 _I, _L, _P = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
+_raw_stream = torch._C._cuda_getCurrentRawStream   # the handle alone, without building a torch.cuda.Stream
 
 
 class _Cache(ctypes.Structure):
@@ -72,7 +73,7 @@ class PagedBatch:
               "q_start, kv_len and the rows of block_table must be contiguous")
         _need(q_start.device == kv_len.device == block_table.device, "the batch's arrays must be on one device")
         self.q_start, self.kv_len, self.block_table, self.max_rows = q_start, kv_len, block_table, max_rows
-        self.device = kv_len.device
+        self.num_seqs, self.index = n, kv_len.get_device()
         self._c = _Batch(n, max_rows, block_table.shape[1], block_table.stride(0), q_start.data_ptr(),
                          kv_len.data_ptr(), block_table.data_ptr())
         self._ref = ctypes.byref(self._c)
@@ -100,7 +101,7 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         pages, heads, rows, dim = k.shape
-        self._heads, self._dim = heads, dim
+        self._heads, self._dim, self._index, self._workspace = heads, dim, k.device.index, {}
         self._c = _Cache(_CACHE_DTYPES[k.dtype], pages, heads, rows, dim, k.device.index, k.data_ptr(), v.data_ptr(),
                          *k.stride()[:3], None if k_scale is None else k_scale.data_ptr(),
                          None if v_scale is None else v_scale.data_ptr(), *strides, self.status.data_ptr())
@@ -120,8 +121,9 @@ class PagedKVCache:
     def _rows(self, t: torch.Tensor, heads: int, name: str) -> int:
         """Checks a row tensor [rows, heads, head_dim]; its type."""
         dtype = _ROW_DTYPES.get(t.dtype)
-        if (dtype is None or t.dim() != 3 or t.shape[2] != self._dim or (heads and t.shape[1] != heads) or
-                t.device != self.device or t.stride(2) != 1):
+        shape = t.shape
+        if (dtype is None or len(shape) != 3 or shape[2] != self._dim or (heads and shape[1] != heads) or
+                t.get_device() != self._index or t.stride(2) != 1):
             raise HyError(HY_ERR_INVALID_ARGUMENT, f"{name} must be a float32 or bfloat16 tensor [rows, heads, "
                           f"{self._dim}] on {self.device} with contiguous heads")
         if t.requires_grad and torch.is_grad_enabled():
@@ -132,10 +134,14 @@ class PagedKVCache:
         dtype = self._rows(k, self._heads, "k")
         if self._rows(v, self._heads, "v") != dtype or v.shape != k.shape:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "k and v must have one shape and type")
-        _need(batch.device == self.device, "the batch must be on the cache's device")
-        ks, vs = k.stride(), v.stride()
-        _check(fn(self._ref, batch._ref, k.shape[0], dtype, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                  torch.cuda.current_stream(self.device).cuda_stream))
+        if batch.index != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        rc = fn(self._ref, batch._ref, k.shape[0], dtype, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
+                _raw_stream(self._index))
+        if rc:
+            _check(rc)
 
     def write(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Writes rows k, v [rows, kv heads, head_dim] at their positions (hy_paged_kv_write)."""
@@ -146,8 +152,11 @@ class PagedKVCache:
         """The batch's positions as rows k, v [rows, kv heads, head_dim] (hy_paged_kv_read). Rows of `out` that
         belong to no sequence are left as they were; without `out` they hold anything."""
         if out is None:
-            out = tuple(torch.empty((rows, self._heads, self._dim), dtype=dtype, device=self.device) for _ in range(2))
-        _need(out[0].shape[0] == rows and out[0].dtype == dtype, "out must hold `rows` rows of `dtype`")
+            shape = (rows, self._heads, self._dim)
+            k = torch.empty(shape, dtype=dtype, device=self.device)
+            out = (k, torch.empty_like(k))
+        else:
+            _need(out[0].shape[0] == rows and out[0].dtype == dtype, "out must hold `rows` rows of `dtype`")
         self._pair(batch, *out, self._lib.hy_paged_kv_read)
         return out
 
@@ -158,19 +167,29 @@ class PagedKVCache:
         false. The workspace comes from torch's allocator, one for each call."""
         dtype = self._rows(q, 0, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = q.new_empty(q.shape)
         elif self._rows(out, q.shape[1], "out") != dtype or out.shape != q.shape:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "q and out must have one shape and type")
-        _need(batch.device == self.device, "the batch must be on the cache's device")
-        rows, heads = q.shape[0], q.shape[1]
-        need = ctypes.c_size_t()
-        _check(self._lib.hy_paged_attention_workspace(self._ref, batch._ref, rows, heads, dtype, ctypes.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-        qs, os = q.stride(), out.stride()
-        _check(self._lib.hy_paged_attention(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), qs[0], qs[1],
-                                            out.data_ptr(), os[0], os[1], scale, causal, window, sinks,
-                                            None if work is None else work.data_ptr(), need.value,
-                                            torch.cuda.current_stream(self.device).cuda_stream))
+        if batch.index != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
+        rows, heads, _ = q.shape
+        key = (rows, heads, dtype, batch.num_seqs, batch.max_rows)
+        need = self._workspace.get(key)   # bytes; they depend on nothing else
+        if need is None:
+            size = ctypes.c_size_t()
+            _check(self._lib.hy_paged_attention_workspace(self._ref, batch._ref, rows, heads, dtype,
+                                                          ctypes.byref(size)))
+            if len(self._workspace) > 256:
+                self._workspace.clear()
+            need = self._workspace[key] = size.value
+        work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        q0, q1, _ = q.stride()
+        o0, o1, _ = out.stride()
+        rc = self._lib.hy_paged_attention(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), q0, q1,
+                                          out.data_ptr(), o0, o1, scale, causal, window, sinks, work.data_ptr(), need,
+                                          _raw_stream(self._index))
+        if rc:
+            _check(rc)
         return out
 
     def check(self) -> None:
