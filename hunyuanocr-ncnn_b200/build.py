@@ -19,8 +19,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libhy_decode.so")
 RECORD = os.path.join(HERE, "libhy_decode.build.json")   # what the last in-tree build compiled, and how
-SOURCES = [os.path.join(HERE, "csrc", "hy_capi.cu"), os.path.join(HERE, "csrc", "hy_paged.cu"),
-           os.path.join(HERE, "csrc", "hy_package.cpp")]
+SOURCES = [os.path.join(HERE, "csrc", f) for f in (
+    "hy_capi.cu", "hy_paged.cu", "hy_paged_attn_f32.cu", "hy_paged_attn_bf16.cu", "hy_package.cpp")]
 DEPS = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))] + [
     os.path.join(REPO, "include", "hy_decode.h"), os.path.join(REPO, "include", "hy_paged.h")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -3,18 +3,16 @@
 // the first CUDA call.
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <climits>
 #include <string>
-#include <type_traits>
 
 #include "hy_paged.cuh"
-#include "hy_paged_attn.cuh"
+#include "hy_paged_launch.cuh"
 #include "hy_paged.h"
 
 namespace hy_internal {
 void set_last_error(const std::string& msg);
-}
+}  // namespace hy_internal
 
 using namespace hy;
 
@@ -151,31 +149,6 @@ PagedBatch device_batch(const hy_paged_batch* b, int rows)
     return {b->q_start_dev, b->kv_len_dev, b->block_table_dev, b->table_stride, b->table_width, b->num_seqs, rows};
 }
 
-template <typename T>
-struct Tag {
-    using type = T;
-};
-
-// f(row type, cache type, head_dim) with the run-time types as types.
-template <typename F>
-auto with_types(int row_dtype, int cache_dtype, int head_dim, F&& f)
-{
-    auto dim = [&](auto rt, auto ct) {
-        return head_dim == 64 ? f(rt, ct, std::integral_constant<int, 64>{})
-                              : f(rt, ct, std::integral_constant<int, 128>{});
-    };
-    auto cache = [&](auto rt) {
-        switch (cache_dtype)
-        {
-        case HY_DTYPE_F32: return dim(rt, Tag<float>{});
-        case HY_DTYPE_BF16: return dim(rt, Tag<__nv_bfloat16>{});
-        case HY_DTYPE_E4M3: return dim(rt, Tag<E4M3>{});
-        default: return dim(rt, Tag<Int8>{});
-        }
-    };
-    return row_dtype == HY_DTYPE_F32 ? cache(Tag<float>{}) : cache(Tag<__nv_bfloat16>{});
-}
-
 int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int dtype, void* k,
                long long krs, long long khs, void* v, long long vrs, long long vhs, void* stream)
 {
@@ -190,7 +163,7 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     const PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, krs, khs, vrs, vhs};
-    with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
+    with_row_type(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
         using RT = typename decltype(rt)::type;
         using CT = typename decltype(ct)::type;
         const dim3 grid(rows), block(kRowWarps * 32);
@@ -202,46 +175,13 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     return e == cudaSuccess ? HY_OK : cuda_fail(write ? "paged write" : "paged read", e);
 }
 
-// Lets Kernel have `smem` bytes of dynamic shared memory; set once per device.
-template <auto Kernel>
-cudaError_t allow_smem(int smem, int device)
-{
-    static std::atomic<unsigned long long> done{0};
-    const unsigned long long bit = 1ull << (device & 63);
-    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-    const cudaError_t e =
-        cudaFuncSetAttribute(reinterpret_cast<const void*>(Kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
-
-// Columns of a tile in units of 8 (see paged_split_kernel): as many as a sequence's rows need, up to 32.
-int split_tiles_n(int max_rows, int group)
+// Columns of a tile of the split kernels: as many as a sequence's rows need, up
+// to 32; fp32 caches have tiles of 2 and 4 (FmaEngine).
+int split_columns(int max_rows, int group, int cache_dtype)
 {
     const long long cols = static_cast<long long>(max_rows) * group;
-    return cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-}
-
-template <typename QT, typename CT, int D, int NT>
-cudaError_t launch_split(const PagedAttnArgs& a, int device, cudaStream_t s)
-{
-    using Sh = SplitShape<QT, CT, D, NT>;
-    cudaError_t e = allow_smem<paged_split_kernel<QT, CT, D, NT>>(Sh::SMEM, device);
-    if (e != cudaSuccess) return e;
-    paged_split_kernel<QT, CT, D, NT><<<Sh::GRID, kSplitThreads, Sh::SMEM, s>>>(a);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    // The join may start while the split kernel runs; it waits for its end.
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(Sh::GRID);
-    cfg.blockDim = dim3(128);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_join_kernel<QT, Sh::F16, D, NT>, a);
+    if (cache_dtype == HY_DTYPE_F32 && cols <= 4) return cols <= 2 ? 2 : 4;
+    return cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
 }
 
 int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype)
@@ -261,7 +201,7 @@ int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, in
 // Descriptions and two parts for every CTA.
 size_t attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int q_heads)
 {
-    const int cols = 8 * split_tiles_n(batch->max_rows, q_heads / cache->num_kv_heads);
+    const int cols = split_columns(batch->max_rows, q_heads / cache->num_kv_heads, cache->dtype);
     return kSplitDescBytes + static_cast<size_t>(2 * kSplitMaxCtas) * cols * (cache->head_dim + 2) * sizeof(float);
 }
 
@@ -320,16 +260,10 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
                           power_of_two(cache->page_size), scale * 1.4426950408889634f, workspace_dev};
-    const int nt = split_tiles_n(batch->max_rows, group);
+    const int cols = split_columns(batch->max_rows, group, cache->dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = with_types(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
-        using RT = typename decltype(rt)::type;
-        using CT = typename decltype(ct)::type;
-        constexpr int D = decltype(d)::value;
-        return nt == 1   ? launch_split<RT, CT, D, 1>(a, cache->device, s)
-               : nt == 2 ? launch_split<RT, CT, D, 2>(a, cache->device, s)
-                         : launch_split<RT, CT, D, 4>(a, cache->device, s);
-    });
+    const auto launch = dtype == HY_DTYPE_F32 ? hy_internal::paged_attention_f32 : hy_internal::paged_attention_bf16;
+    const cudaError_t e = launch(a, cache->dtype, cache->head_dim, cols, cache->device, s);
     return e == cudaSuccess ? HY_OK : cuda_fail("paged attention", e);
 }
 

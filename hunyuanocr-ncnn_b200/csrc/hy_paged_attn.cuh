@@ -177,7 +177,7 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x)
 // ---------------------------------------------------------------------------
 // Few rows per sequence: the keys are split over the GPU.
 //
-// The work is the list of (sequence, tile of 8 NT columns, KV head) items, each
+// The work is the list of (sequence, tile of COLS columns, KV head) items, each
 // of ceil(keys / TILE) tiles (at least one), T in all; CTA i of G takes the next
 // ceil(T / G) tiles of the whole list, whatever items they belong to, so every CTA
 // streams the same number of keys however ragged the lengths are. Memory bounds it
@@ -185,22 +185,13 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x)
 // never pause: every warp owns a quarter of a tile's keys and a cp.async ring of its
 // own, and the warps meet only at the end of an item.
 //
-// The products are taken transposed, S^T[key x column] = K Q^T and O^T[dim x
-// column] = V^T P^T: with the columns in the 8-wide dimension a decode step of
-// two heads wastes 6 of 8 lanes instead of 14 of 16, the accumulators of
-// 128 dimensions are 32 registers, and a column's softmax state lies in the same lane for
-// the scores and for the output.
-//
-// Operands: bf16 and fp32 caches in bf16 (an fp32 number as three terms, products
-// of terms i + j <= 2: exact to 2^-23), 8-bit caches in f16, where their codes and
-// the query (each row times a power of two) are exact; fp32 queries take two f16
-// terms there. Which dimensions a lane takes from a row is free as long as q
-// agrees, so 8-bit and fp32 keys are read from shared memory in 16-byte pieces.
-//
 // A CTA's first and last items may be shared with its neighbours: those leave
 // (m, l, sum) parts in the workspace, slot 2 i for the first item and 2 i + 1 for a
 // later one, and paged_join_kernel adds up the parts of an item. The CTA that
 // starts such an item leaves its description.
+//
+// What a step of a warp computes is an engine's: MmaEngine (tensor cores) or
+// FmaEngine (fp32 caches and up to 4 columns).
 // ---------------------------------------------------------------------------
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
@@ -210,85 +201,765 @@ struct PagedJoin {   // description of an item whose parts are joined; count 0: 
     int count, first_slot, first_cta, row0, col0, cols, head, pad;
 };
 
-template <typename QT, typename CT, int D, int NT>
-struct SplitShape {
-    static constexpr bool F16 = kCodes<CT>;
-    static constexpr int NQ = std::is_same_v<QT, float> ? (F16 ? 2 : 3) : 1;   // terms of q and of the weights
-    static constexpr int NK = std::is_same_v<CT, float> ? 3 : 1;               // terms of k and v
-    static constexpr int COLS = 8 * NT;
-    static constexpr int RB = D * static_cast<int>(sizeof(CT));                // bytes of a row
-    // Keys of a warp's step: 32 where that is 8 KB or less (the work that a step
-    // costs whatever its keys - addresses, maxima, shuffles - is halved), else 16.
-    static constexpr int KEYS = RB <= 128 ? 32 : 16;
-    static constexpr int TILE = kSplitWarps * KEYS;
-    static constexpr int STAGE = 2 * KEYS * RB;                                // a warp's keys and values
-    static constexpr int SCALES = F16 ? 2 * KEYS * 4 : 0;
-    static constexpr int QB = (D / 16) * NT * NQ * 256;
-    static constexpr int FIX = QB + 2 * COLS * 4 + kSplitWarps * COLS * 8 + 64;
-    static constexpr int fit(int kb, int most)
-    {
-        const int n = (kb * 1024 - FIX) / (kSplitWarps * (STAGE + SCALES + 16));
-        return n < most ? n : most;
-    }
-    static constexpr int OCC = (NT == 1 && fit(74, 4) >= 2) ? 3 : fit(112, 4) >= 2 ? 2 : 1;
-    static constexpr int S = OCC == 3 ? fit(74, 4) : OCC == 2 ? fit(112, 4) : fit(224, 4);
-    static constexpr int RING = kSplitWarps * S * STAGE;
-    static constexpr int MERGE = kSplitWarps * COLS * (D + 4) * 4;   // the warps' sums, over the drained ring
-    static constexpr int BODY = RING > MERGE ? RING : MERGE;
-    static constexpr int SC_OFF = BODY;
-    static constexpr int MASK_OFF = SC_OFF + kSplitWarps * S * SCALES;   // a bit for every key that is there
-    static constexpr int Q_OFF = (MASK_OFF + kSplitWarps * S * 4 + 127) / 128 * 128;
-    static constexpr int QS_OFF = Q_OFF + QB;                        // [COLS] 2^-k of a column's q
-    static constexpr int ML_OFF = QS_OFF + COLS * 4;                 // [warps][COLS] (m, l)
-    static constexpr int SMEM = ML_OFF + kSplitWarps * COLS * 8;
-    static_assert(S >= 2 && SMEM <= 227 * 1024, "shared memory");
-    static constexpr int GRID = 148 * OCC;
-    static constexpr bool QREG = (D / 16) * NT * 2 * NQ <= 32;       // q stays in registers
-    // Part of an item in the workspace: [COLS] (m, l), then [COLS][D].
-    static constexpr int PART = COLS * (D + 2);
-};
-
 // Bytes before the parts: the descriptions.
 constexpr size_t kSplitDescBytes = kSplitMaxCtas * sizeof(PagedJoin);
-
-// Output dimension of accumulator row (m tile, half) of lane group g, by how V's fragments are read.
-template <typename CT, int D>
-__device__ __forceinline__ int split_dim(int mt, int half, int g)
-{
-    if constexpr (sizeof(CT) == 4) return 32 * (mt >> 1) + 4 * g + 2 * (mt & 1) + half;
-    else if constexpr (sizeof(CT) == 2) return 16 * mt + 8 * half + g;
-    else return (D / 8) * g + 2 * mt + half;
-}
-// Where 16-byte piece c of key row r lies in a stage (bytes), for K and for V: the
-// rotations keep the lanes of each shared-memory phase on different banks.
-template <typename CT, int D>
-__device__ __forceinline__ int split_k_at(int r, int c)
-{
-    constexpr int RB = D * static_cast<int>(sizeof(CT));
-    if constexpr (sizeof(CT) == 2) return r * RB + ((c ^ (r & 7)) << 4);
-    else if constexpr (RB >= 128) return r * RB + ((c ^ ((r & 1) << 2)) << 4);
-    else return r * RB + (c << 4);
-}
-template <typename CT, int D>
-__device__ __forceinline__ int split_v_at(int r, int c)
-{
-    constexpr int RB = D * static_cast<int>(sizeof(CT));
-    if constexpr (sizeof(CT) == 2) return r * RB + ((c ^ (r & 7)) << 4);
-    else if constexpr (RB >= 128) return r * RB + ((c ^ (r & 6)) << 4);
-    else
-    {
-        // 64-byte rows: even rows first, so that rows 0, 2, 4, 6 span both halves of the banks.
-        const int pos = (r & ~7) | ((r & 1) << 2) | ((r & 6) >> 1);
-        return pos * RB + ((c ^ (pos & 2)) << 4);
-    }
-}
 
 struct SplitItem {
     PagedSeq q;
     PagedSpan w;
     int seq, tile, head, tiles;
+    int cols;   // columns that are there
+};
+__device__ __forceinline__ int split_key(const SplitItem& it, int u) { return u < it.w.sinks ? u : it.w.lo + u - it.w.sinks; }
+// Row tensor offset of column c of an item.
+__device__ __forceinline__ long long split_q_at(const PagedAttnArgs& a, const SplitItem& it, int tile_cols, int c)
+{
+    const int cc = it.tile * tile_cols + c, row = cc / a.group;
+    return (it.q.row0 + row) * a.q_row_stride + (it.head * a.group + cc - row * a.group) * a.q_head_stride;
+}
+__device__ __forceinline__ int split_pos(const PagedAttnArgs& a, const SplitItem& it, int tile_cols, int c)
+{
+    return c < it.cols ? it.q.kv - it.q.n + (it.tile * tile_cols + c) / a.group : -1;
+}
+// Every column sees every one of the KEYS keys from u0 on (`live` tells which are there).
+template <int KEYS>
+__device__ __forceinline__ bool split_whole(const PagedAttnArgs& a, const SplitItem& it, int u0, uint32_t live)
+{
+    const int j_first = split_key(it, u0), j_last = split_key(it, min(u0 + KEYS - 1, it.w.n - 1));
+    return live == (KEYS == 32 ? 0xffffffffu : (1u << (KEYS & 31)) - 1u) && it.w.p_first >= 0 &&
+           (!a.causal || (j_last <= it.w.p_first &&
+                          (a.window == 0 || j_first > it.w.p_last - a.window || j_last < a.sinks)));
+}
+
+// Sizes that follow from an engine's: ring stages and CTAs per SM. Three CTAs
+// for narrow tiles (168 registers a thread), else two, else (16 KB a step) one.
+template <typename E>
+struct SplitShape {
+    static constexpr int TILE = kSplitWarps * E::KEYS;
+    static constexpr int STAGE = 2 * E::KEYS * E::RB;
+    static constexpr int SCALES = E::F16 ? 2 * E::KEYS * 4 : 0;
+    static constexpr int FIX = E::Q_SMEM + E::COLS * 4 + kSplitWarps * E::COLS * 8 + 256;
+    static constexpr int fit(int kb, int most)
+    {
+        const int n = (kb * 1024 - FIX) / (kSplitWarps * (STAGE + SCALES + 4));
+        return n < most ? n : most;
+    }
+    static constexpr int OCC = (E::MAX_OCC == 3 && fit(74, 4) >= 2) ? 3 : fit(112, 4) >= 2 ? 2 : 1;
+    static constexpr int S = OCC == 3 ? fit(74, 4) : OCC == 2 ? fit(112, 4) : fit(224, 4);
+    static constexpr int RING = kSplitWarps * S * STAGE;
+    static constexpr int MERGE = kSplitWarps * E::COLS * (E::D + 4) * 4;   // the warps' sums, over the drained ring
+    static constexpr int SC_OFF = RING > MERGE ? RING : MERGE;
+    static constexpr int MASK_OFF = SC_OFF + kSplitWarps * S * SCALES;     // a bit for every key that is there
+    static constexpr int Q_OFF = (MASK_OFF + kSplitWarps * S * 4 + 127) / 128 * 128;
+    static constexpr int MAX_OFF = Q_OFF + E::Q_SMEM;                      // [COLS] bits of a column's largest |q|
+    static constexpr int ML_OFF = (MAX_OFF + E::COLS * 4 + 7) / 8 * 8;     // [warps][COLS] (m, l)
+    static constexpr int SMEM = ML_OFF + kSplitWarps * E::COLS * 8;
+    static_assert(S >= 2 && SMEM <= 227 * 1024, "shared memory");
+    static constexpr int GRID = 148 * OCC;
+    static constexpr int PART = E::COLS * (E::D + 2);   // a part: [COLS] (m, l), then [COLS][D]
 };
 
+// ---------------------------------------------------------------------------
+// The products on the tensor cores, taken transposed: S^T[key x column] = K Q^T
+// and O^T[dim x column] = V^T P^T. With the columns in the 8-wide dimension a
+// decode step of two heads wastes 6 of 8 lanes instead of 14 of 16, the
+// accumulators of 128 dimensions are 32 registers, and a column's softmax state
+// lies in the same lane for the scores and for the output.
+//
+// bf16 and fp32 caches multiply in bf16 (an fp32 number as three terms, products
+// of terms i + j <= 2: exact to 2^-23); 8-bit caches in f16, where their codes and
+// the query (each row times a power of two) are exact, fp32 queries as two f16
+// terms. Which dimensions a lane takes from a row is free as long as q
+// agrees, so 8-bit and fp32 keys are read from shared memory in 16-byte pieces.
+// ---------------------------------------------------------------------------
+template <typename QT_, typename CT_, int D_, int NT>
+struct MmaEngine {
+    using QT = QT_;
+    using CT = CT_;
+    static constexpr int D = D_, COLS = 8 * NT;
+    static constexpr bool F16 = kCodes<CT>;
+    static constexpr int NQ = std::is_same_v<QT, float> ? (F16 ? 2 : 3) : 1;   // terms of q and of the weights
+    static constexpr int NK = std::is_same_v<CT, float> ? 3 : 1;               // terms of k and v
+    static constexpr int RB = D * static_cast<int>(sizeof(CT));                // bytes of a row
+    // Keys of a warp's step: 32 where that is 8 KB or less (the work that a step
+    // costs whatever its keys - addresses, maxima, shuffles - is halved) and the registers allow it, else 16.
+    static constexpr int KEYS = RB <= 128 && NT < 4 ? 32 : 16;
+    static constexpr int MAX_OCC = NT == 1 ? 3 : 2;   // CTAs per SM that the registers allow
+    static constexpr int KS = D / 16, MTS = D / 16, HV = KEYS / 16;
+    static constexpr int Q_SMEM = KS * NT * NQ * 256;
+    static constexpr int QI = KS * NT / kSplitWarps;                           // q fragments that a thread makes
+    static constexpr bool QREG = KS * NT * 2 * NQ <= 32;                       // q stays in registers
+    static constexpr int NA = NT >= 4 ? 1 : NQ * NK == 1 ? 2 : NQ > NK ? NQ : NK;   // chains of products per score
+    static constexpr int MG = NT >= 4 ? 1 : 2;                                      // m tiles whose products alternate
+    static constexpr float OUT = F16 ? 1.f / 16384.f : 1.f;                         // the sums' unit
+
+    uint2 qreg[QREG ? NQ * KS * NT : 1];
+    const uint2* qf;
+    int pos[NT][2];       // positions and score factors of this lane's columns (2t, 2t + 1 of every n tile)
+    float fac[NT][2];
+    float m[NT][2], l[NT][2], acc[NT][MTS][4];
+
+    // Where 16-byte piece c of key row r lies in a stage (bytes), for K and for V: the
+    // rotations keep the lanes of each shared-memory phase on different banks.
+    static __device__ __forceinline__ int k_at(int r, int c)
+    {
+        if constexpr (sizeof(CT) == 2) return r * RB + ((c ^ (r & 7)) << 4);
+        else if constexpr (RB >= 128) return r * RB + ((c ^ ((r & 1) << 2)) << 4);
+        else return r * RB + (c << 4);
+    }
+    static __device__ __forceinline__ int v_at(int r, int c)
+    {
+        if constexpr (sizeof(CT) == 2) return r * RB + ((c ^ (r & 7)) << 4);
+        else if constexpr (RB >= 128) return r * RB + ((c ^ (r & 6)) << 4);
+        else
+        {
+            // 64-byte rows: even rows first, so that rows 0, 2, 4, 6 span both halves of the banks.
+            const int at = (r & ~7) | ((r & 1) << 2) | ((r & 6) >> 1);
+            return at * RB + ((c ^ (at & 2)) << 4);
+        }
+    }
+    // Output dimension of accumulator row (m tile, half) of lane group g, by how V's fragments are read.
+    static __device__ __forceinline__ int dim_of(int mt, int half, int g)
+    {
+        if constexpr (sizeof(CT) == 4) return 32 * (mt >> 1) + 4 * g + 2 * (mt & 1) + half;
+        else if constexpr (sizeof(CT) == 2) return 16 * mt + 8 * half + g;
+        else return (D / 8) * g + 2 * mt + half;
+    }
+
+    // q of the fragments that this thread makes, straight from memory; fragment i of
+    // thread tid: lane tid % 32 of n tile x % NT, k step x / NT, x = tid / 32 + 4 i.
+    float raw[QI][4];
+    __device__ __forceinline__ void fetch_q(const PagedAttnArgs& a, const SplitItem& it)
+    {
+        const int ln = threadIdx.x & 31, gg = ln >> 2, tt = ln & 3;
+        long long at[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) at[nt] = split_q_at(a, it, COLS, min(nt * 8 + gg, it.cols - 1));
+#pragma unroll
+        for (int i = 0; i < QI; ++i)
+        {
+            const int x = (threadIdx.x >> 5) + kSplitWarps * i, nt = x % NT, ks = x / NT;
+            const long long o = NT == 1 ? at[0] : at[nt % NT];
+            if constexpr (sizeof(CT) == 2)
+            {
+                const QT* p = static_cast<const QT*>(a.q) + o + 16 * ks + 2 * tt;
+                if constexpr (sizeof(QT) == 4)
+                {
+                    const float2 u = __ldg(reinterpret_cast<const float2*>(p)), w = __ldg(reinterpret_cast<const float2*>(p + 8));
+                    raw[i][0] = u.x; raw[i][1] = u.y; raw[i][2] = w.x; raw[i][3] = w.y;
+                }
+                else
+                {
+                    const uint32_t u = __ldg(reinterpret_cast<const uint32_t*>(p)), w = __ldg(reinterpret_cast<const uint32_t*>(p + 8));
+                    raw[i][0] = __uint_as_float(u << 16); raw[i][1] = __uint_as_float(u & 0xFFFF0000u);
+                    raw[i][2] = __uint_as_float(w << 16); raw[i][3] = __uint_as_float(w & 0xFFFF0000u);
+                }
+            }
+            else
+            {
+                load_row<QT, 4>(a.q, o + (sizeof(CT) == 4 ? 16 * ks + 4 * tt : 64 * (ks >> 2) + 16 * tt + 4 * (ks & 3)), raw[i]);
+            }
+            if (nt * 8 + gg >= it.cols) raw[i][0] = raw[i][1] = raw[i][2] = raw[i][3] = 0.f;
+        }
+    }
+    // The fragments, through shared memory (all warps need all of them). colmax is zero on entry.
+    __device__ __forceinline__ void make_q(const PagedAttnArgs& a, const SplitItem& it, unsigned char* smem_q, uint32_t* colmax)
+    {
+        const int ln = threadIdx.x & 31, gg = ln >> 2, t = ln & 3;
+        uint2* const q = reinterpret_cast<uint2*>(smem_q);   // [term][ks][nt][lane]
+        if constexpr (F16)
+        {
+            // A column's power of two: its largest magnitude comes to lie in [2^14, 2^15).
+#pragma unroll
+            for (int i = 0; i < QI; ++i)
+            {
+                uint32_t x = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x = max(x, __float_as_uint(raw[i][e]) & 0x7fffffffu);
+                x = max(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = max(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                if (t == 0) atomicMax(colmax + ((threadIdx.x >> 5) + kSplitWarps * i) % NT * 8 + gg, x);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < QI; ++i)
+        {
+            const int x = (threadIdx.x >> 5) + kSplitWarps * i, nt = x % NT, ks = x / NT;
+            if constexpr (F16)
+            {
+                const float up = __uint_as_float((254u << 23) - down_bits(colmax[nt * 8 + gg]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) raw[i][e] *= up;
+            }
+            uint32_t b0[NQ], b1[NQ];
+            split_pair<F16, NQ>(raw[i][0], raw[i][1], b0);
+            split_pair<F16, NQ>(raw[i][2], raw[i][3], b1);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) q[((j * KS + ks) * NT + nt) * 32 + ln] = make_uint2(b0[j], b1[j]);
+        }
+        __syncthreads();
+        qf = q;
+        if constexpr (QREG)
+#pragma unroll
+            for (int i = 0; i < NQ * KS * NT; ++i) qreg[i] = q[i * 32 + ln];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+        {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                const int c = nt * 8 + 2 * t + e;
+                pos[nt][e] = split_pos(a, it, COLS, c);
+                fac[nt][e] = F16 ? a.scale_log2 * __uint_as_float(down_bits(colmax[c])) : a.scale_log2;
+                m[nt][e] = -INFINITY;
+                l[nt][e] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < MTS; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+        }
+    }
+    // Bits of 2^-k, k = 14 - exponent of the largest magnitude, kept within the normal numbers.
+    static __device__ __forceinline__ uint32_t down_bits(uint32_t largest)
+    {
+        return (min(max(largest >> 23, 16u), 254u) - 14u) << 23;
+    }
+    __device__ __forceinline__ uint2 q_frag(int term, int ks, int nt) const
+    {
+        const int i = (term * KS + ks) * NT + nt;
+        if constexpr (QREG) return qreg[i];
+        else return qf[i * 32 + (threadIdx.x & 31)];
+    }
+
+    // A step: KEYS keys of virtual positions u0 .., in shared memory at kb (keys, then values), scales at sc_u.
+    __device__ __forceinline__ void step(const PagedAttnArgs& a, const SplitItem& it, int u0, uint32_t live,
+                                         const unsigned char* stage, uint32_t kb, uint32_t sc_u)
+    {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const uint32_t vb = kb + KEYS * RB;
+        // Scores of the step's keys: sc[hv][nt] holds keys 16 hv + g and + 8.
+        float sc[HV][NT][4];
+#pragma unroll
+        for (int hv = 0; hv < HV; ++hv)
+        {
+            float part[NA][NT][4];   // chains of products that do not wait for one another
+#pragma unroll
+            for (int n = 0; n < NA; ++n)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) part[n][nt][0] = part[n][nt][1] = part[n][nt][2] = part[n][nt][3] = 0.f;
+                uint4 w0, w1;   // 8-bit keys: 64 dimensions of rows g and g + 8
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+            {
+                uint32_t ka[NK][4];
+                if constexpr (sizeof(CT) == 2)
+                {
+                    ldmatrix4(ka[0], kb + k_at(16 * hv + (lane & 15), 2 * ks + (lane >> 4)));
+                }
+                else if constexpr (sizeof(CT) == 4)
+                {
+                    const uint4 x = lds128(kb + k_at(16 * hv + g, 4 * ks + t)),
+                                y = lds128(kb + k_at(16 * hv + g + 8, 4 * ks + t));
+                    uint32_t p[NK];
+                    auto put = [&](int at, uint32_t lo, uint32_t hi) {
+                        split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) ka[n][at] = p[n];
+                    };
+                    put(0, x.x, x.y);
+                    put(1, y.x, y.y);
+                    put(2, x.z, x.w);
+                    put(3, y.z, y.w);
+                }
+                else
+                {
+                    if (ks % 4 == 0)
+                    {
+                        w0 = lds128(kb + k_at(16 * hv + g, ks + t));
+                        w1 = lds128(kb + k_at(16 * hv + g + 8, ks + t));
+                    }
+                    const uint32_t x = ks % 4 == 0 ? w0.x : ks % 4 == 1 ? w0.y : ks % 4 == 2 ? w0.z : w0.w;
+                    const uint32_t y = ks % 4 == 0 ? w1.x : ks % 4 == 1 ? w1.y : ks % 4 == 2 ? w1.z : w1.w;
+                    ka[0][0] = codes_f16<CT>(x);
+                    ka[0][1] = codes_f16<CT>(y);
+                    ka[0][2] = codes_f16<CT>(x >> 16);
+                    ka[0][3] = codes_f16<CT>(y >> 16);
+                }
+#pragma unroll
+                for (int j = NQ - 1; j >= 0; --j)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                    {
+                        const uint2 b = q_frag(j, ks, nt);
+#pragma unroll
+                        for (int n = NK - 1; n >= 0; --n)
+                            if (n + j <= 2)
+                                mma16816<F16>(part[NA == 1 ? 0 : NQ * NK == 1 ? ks % NA : (n + j) % NA][nt], ka[n], b.x, b.y);
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    sc[hv][nt][e] = part[NA - 1][nt][e];   // the small terms first
+#pragma unroll
+                    for (int n = NA - 2; n >= 0; --n) sc[hv][nt][e] += part[n][nt][e];
+                }
+        }
+
+        // Scores in units of log 2, masks, the weights' exponents. Index [hv][r]: key 16 hv + 8 r + g.
+        float vs[HV][2], ev[HV][2], kf[HV][2];
+#pragma unroll
+        for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+            {
+                kf[hv][r] = vs[hv][r] = 1.f;
+                ev[hv][r] = 0.f;
+                if constexpr (F16)
+                {
+                    const uint32_t at = sc_u + (16 * hv + 8 * r + g) * 4;
+                    kf[hv][r] = lds_f32(at);
+                    const float v = lds_f32(at + KEYS * 4);
+                    // The maximum is taken over the score plus the exponent of the value's scale, so that
+                    // a weight times its scale is below 2 and fits f16 (times 2^14).
+                    ev[hv][r] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(v) >> 23) - 127, -100), 100));
+                    vs[hv][r] = v * 16384.f;
+                }
+            }
+        const bool whole = split_whole<KEYS>(a, it, u0, live);
+        uint32_t seen = 0xffffffffu;   // bit ((hv * 2 + r) * NT + nt) * 2 + e: the column sees the key
+        bool hidden = false;           // some column does not see a key that was loaded
+        if (!whole)
+        {
+#pragma unroll
+            for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                {
+                    const int in16 = 16 * hv + 8 * r + g, j = split_key(it, u0 + in16);
+                    const bool there = (live >> in16) & 1u;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                        {
+                            const bool v = there && paged_sees(a, pos[nt][e], j);
+                            hidden |= there && !v;
+                            if (!v) seen &= ~(1u << (((hv * 2 + r) * NT + nt) * 2 + e));
+                        }
+                }
+        }
+        bool grew = false;
+        float corr[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+        {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                float x = -INFINITY;
+#pragma unroll
+                for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                    {
+                        float& y = sc[hv][nt][2 * r + e];
+                        y *= F16 ? fac[nt][e] * kf[hv][r] : fac[nt][e];
+                        if (!whole && !((seen >> (((hv * 2 + r) * NT + nt) * 2 + e)) & 1u)) y = -INFINITY;
+                        x = fmaxf(x, F16 ? y + ev[hv][r] : y);
+                    }
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                corr[nt][e] = 1.f;
+                if (x > m[nt][e])
+                {
+                    corr[nt][e] = exp2f(m[nt][e] - x);
+                    m[nt][e] = x;
+                    grew = true;
+                }
+                const float mm = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+                float sum = 0.f;
+#pragma unroll
+                for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                    {
+                        float& y = sc[hv][nt][2 * r + e];
+                        y = exp2f(y - mm);   // (a NaN score stays one)
+                        sum += y;
+                        // A scale of NaN must not meet a weight of zero that stands for "not seen".
+                        if constexpr (F16)
+                            y = (!whole && !((seen >> (((hv * 2 + r) * NT + nt) * 2 + e)) & 1u)) ? 0.f : y * vs[hv][r];
+                    }
+                l[nt][e] = l[nt][e] * corr[nt][e] + sum;
+            }
+        }
+        if (__any_sync(0xffffffffu, grew))
+        {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int x = 0; x < MTS; ++x)
+                {
+                    acc[nt][x][0] *= corr[nt][0];
+                    acc[nt][x][1] *= corr[nt][1];
+                    acc[nt][x][2] *= corr[nt][0];
+                    acc[nt][x][3] *= corr[nt][1];
+                }
+        }
+        // Values that some column must not see may be infinite or NaN, and 0 times those is NaN:
+        // if there are any in such a step, its products are taken one by one.
+        if constexpr (!F16)
+        {
+            if (__any_sync(0xffffffffu, hidden))
+            {
+                bool odd = false;
+                for (int x = lane; x < KEYS * RB / 16; x += 32)
+                {
+                    const uint4 w = lds128(vb + x * 16);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        odd |= (ws[e] & 0x7f800000u) == 0x7f800000u || (sizeof(CT) == 2 && (ws[e] & 0x7f80u) == 0x7f80u);
+                }
+                if (__any_sync(0xffffffffu, odd))
+                {
+#pragma unroll
+                    for (int hr = 0; hr < 2 * HV; ++hr)
+                    {
+                        const unsigned char* const vst = stage + KEYS * RB;
+#pragma unroll 1
+                        for (int k = 0; k < 8; ++k)
+                        {
+                            const int row = 8 * hr + k, key = split_key(it, u0 + row);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                {
+                                    const float p = __shfl_sync(0xffffffffu, sc[hr >> 1][nt][2 * (hr & 1) + e], k * 4 + t);
+                                    if (!((live >> row) & 1u) || !paged_sees(a, pos[nt][e], key)) continue;
+#pragma unroll
+                                    for (int x = 0; x < MTS; ++x)
+#pragma unroll
+                                        for (int hf = 0; hf < 2; ++hf)
+                                        {
+                                            const int by = dim_of(x, hf, g) * static_cast<int>(sizeof(CT));
+                                            acc[nt][x][2 * hf + e] +=
+                                                p * to_f32<CT>(*reinterpret_cast<const CT*>(vst + v_at(row, by >> 4) + (by & 15)));
+                                        }
+                                }
+                        }
+                    }
+                    return;
+                }
+            }
+        }
+#pragma unroll
+        for (int hv = 0; hv < HV; ++hv)
+        {
+            uint32_t pb[NT][2][NQ];   // weights as B fragments
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+            {
+                uint32_t p0[NQ], p1[NQ];
+                split_pair<F16, NQ>(sc[hv][nt][0], sc[hv][nt][1], p0);
+                split_pair<F16, NQ>(sc[hv][nt][2], sc[hv][nt][3], p1);
+#pragma unroll
+                for (int j = 0; j < NQ; ++j)
+                {
+                    pb[nt][0][j] = movmatrix(p0[j]);
+                    pb[nt][1][j] = movmatrix(p1[j]);
+                }
+            }
+            auto pv = [&](int mt, const uint32_t (&va)[MG][NK][4]) {   // m tiles mt .. mt + MG - 1
+#pragma unroll
+                for (int j = NQ - 1; j >= 0; --j)
+#pragma unroll
+                    for (int n = NK - 1; n >= 0; --n)
+#pragma unroll
+                        for (int x = 0; x < MG; ++x)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                if (n + j <= 2) mma16816<F16>(acc[nt][mt + x], va[x][n], pb[nt][0][j], pb[nt][1][j]);
+            };
+            if constexpr (sizeof(CT) == 2)
+            {
+#pragma unroll
+                for (int mt = 0; mt < MTS; mt += MG)
+                {
+                    uint32_t va[MG][1][4];
+#pragma unroll
+                    for (int x = 0; x < MG; ++x)
+                        ldmatrix4_trans(va[x][0], vb + v_at(16 * hv + (lane & 7) + ((lane >> 4) << 3),
+                                                                         2 * (mt + x) + ((lane >> 3) & 1)));
+                    pv(mt, va);
+                }
+            }
+            else if constexpr (sizeof(CT) == 4)
+            {
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x)
+                {
+                    const int r0 = 16 * hv + 2 * t, c = 8 * x + g;
+                    const uint4 f0 = lds128(vb + v_at(r0, c)), f1 = lds128(vb + v_at(r0 + 1, c));
+                    const uint4 f2 = lds128(vb + v_at(r0 + 8, c)), f3 = lds128(vb + v_at(r0 + 9, c));
+#pragma unroll
+                    for (int y0 = 0; y0 < 2; y0 += MG)
+                    {
+                        uint32_t va[MG][NK][4], p[NK];
+#pragma unroll
+                        for (int y = y0; y < y0 + MG; ++y)
+                        {
+                            auto put = [&](int at, uint32_t lo, uint32_t hi) {
+                                split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
+#pragma unroll
+                                for (int n = 0; n < NK; ++n) va[y - y0][n][at] = p[n];
+                            };
+                            put(0, y ? f0.z : f0.x, y ? f1.z : f1.x);
+                            put(1, y ? f0.w : f0.y, y ? f1.w : f1.y);
+                            put(2, y ? f2.z : f2.x, y ? f3.z : f3.x);
+                            put(3, y ? f2.w : f2.y, y ? f3.w : f3.y);
+                        }
+                        pv(2 * x + y0, va);
+                    }
+                }
+            }
+            else
+            {
+                // Rows 2t, 2t + 1, 2t + 8, 2t + 9; D / 8 consecutive dimensions of each.
+                constexpr int W = D / 32;   // words
+                uint32_t f[4][W];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                {
+                    const int row = 16 * hv + 2 * t + (r & 1) + (r >> 1) * 8;
+                    if constexpr (D == 128)
+                    {
+                        const uint4 x = lds128(vb + v_at(row, g));
+                        f[r][0] = x.x; f[r][1] = x.y; f[r][2] = x.z; f[r][3] = x.w;
+                    }
+                    else
+                    {
+                        const uint2 x = lds64(vb + v_at(row, g >> 1) + (g & 1) * 8);
+                        f[r][0] = x.x; f[r][1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MTS; mt += MG)
+                {
+                    uint32_t va[MG][1][4];
+#pragma unroll
+                    for (int x = 0; x < MG; ++x)
+                    {
+                        const int wd = (mt + x) >> 1;
+                        const uint32_t s0 = ((mt + x) & 1) ? 0x62u : 0x40u, s1 = ((mt + x) & 1) ? 0x73u : 0x51u;
+                        va[x][0][0] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s0));
+                        va[x][0][1] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s1));
+                        va[x][0][2] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s0));
+                        va[x][0][3] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s1));
+                    }
+                    pv(mt, va);
+                }
+            }
+        }
+    }
+
+    // This warp's part: (m, l) of the columns, and their sums [COLS][D + 4].
+    __device__ __forceinline__ void put(int cols, float* sums, float2* ml)
+    {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
+                const int c = nt * 8 + 2 * t + e;
+                if (g == 0) ml[c] = make_float2(m[nt][e], l[nt][e]);
+                if (c >= cols) continue;
+#pragma unroll
+                for (int x = 0; x < MTS; ++x)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) sums[c * (D + 4) + dim_of(x, hf, g)] = acc[nt][x][2 * hf + e];
+            }
+    }
+};
+
+// ---------------------------------------------------------------------------
+// fp32 caches, up to 4 columns: plain fp32 multiply-adds. Splitting an fp32 key
+// into terms for the tensor cores costs a lane some 700 operations a step of 16 keys, the
+// multiply-adds of two columns 256. Eight lanes share a key (each D / 8 of its dimensions in 16-byte
+// pieces), the warp takes four keys at a time; each group of eight lanes keeps
+// a softmax state of its own.
+// ---------------------------------------------------------------------------
+template <typename QT_, int D_, int NC>
+struct FmaEngine {
+    using QT = QT_;
+    using CT = float;
+    static constexpr int D = D_, COLS = NC;
+    static constexpr bool F16 = false;
+    static constexpr int RB = D * 4, KEYS = 4096 / RB, Q_SMEM = 0;   // a step is 8 KB
+    static constexpr int MAX_OCC = D * NC > 256 ? 2 : 3;
+    static constexpr int P = D / 32, KK = KEYS / 4;                   // 16-byte pieces of a lane; keys of a group
+    static constexpr float OUT = 1.f;
+
+    float4 q[NC][P], acc[NC][P];
+    int pos[NC];
+    float m[NC], l[NC];
+
+    static __device__ __forceinline__ int k_at(int r, int c) { return r * RB + (c << 4); }
+    static __device__ __forceinline__ int v_at(int r, int c) { return r * RB + (c << 4); }
+
+    __device__ __forceinline__ void fetch_q(const PagedAttnArgs& a, const SplitItem& it)
+    {
+        const int dl = threadIdx.x & 7;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+        {
+            const long long at = split_q_at(a, it, NC, min(c, it.cols - 1));
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+            {
+                float x[4];
+                load_row<QT, 4>(a.q, at + (dl + 8 * p) * 4, x);
+                q[c][p] = make_float4(x[0], x[1], x[2], x[3]);
+            }
+        }
+    }
+    __device__ __forceinline__ void make_q(const PagedAttnArgs& a, const SplitItem& it, unsigned char*, uint32_t*)
+    {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+        {
+            pos[c] = split_pos(a, it, NC, c);
+            m[c] = -INFINITY;
+            l[c] = 0.f;
+#pragma unroll
+            for (int p = 0; p < P; ++p) acc[c][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+
+    __device__ __forceinline__ void step(const PagedAttnArgs& a, const SplitItem& it, int u0, uint32_t live,
+                                         const unsigned char*, uint32_t kb, uint32_t)
+    {
+        const int lane = threadIdx.x & 31, dl = lane & 7, kg = lane >> 3;
+        float s[KK][NC];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+        {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[kk][c] = 0.f;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+            {
+                const uint4 x = lds128(kb + k_at(4 * kk + kg, dl + 8 * p));
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    s[kk][c] += dot4(q[c][p], make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)));
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s[kk][c] += __shfl_xor_sync(0xffffffffu, s[kk][c], o);
+        const bool whole = split_whole<KEYS>(a, it, u0, live);
+        uint32_t seen = 0xffffffffu;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+            {
+                s[kk][c] *= a.scale_log2;
+                if (!whole && !(((live >> (4 * kk + kg)) & 1u) && paged_sees(a, pos[c], split_key(it, u0 + 4 * kk + kg))))
+                {
+                    s[kk][c] = -INFINITY;
+                    seen &= ~(1u << (kk * NC + c));
+                }
+            }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+        {
+            float top = s[0][c];
+#pragma unroll
+            for (int kk = 1; kk < KK; ++kk) top = fmaxf(top, s[kk][c]);
+            float corr = 1.f;
+            if (top > m[c])
+            {
+                corr = exp2f(m[c] - top);
+                m[c] = top;
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                {
+                    acc[c][p].x *= corr; acc[c][p].y *= corr; acc[c][p].z *= corr; acc[c][p].w *= corr;
+                }
+            }
+            const float mm = m[c] == -INFINITY ? 0.f : m[c];
+            l[c] *= corr;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+            {
+                s[kk][c] = exp2f(s[kk][c] - mm);   // (a NaN score stays one)
+                l[c] += s[kk][c];
+            }
+        }
+        const uint32_t vb = kb + KEYS * RB;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+            {
+                const uint4 x = lds128(vb + v_at(4 * kk + kg, dl + 8 * p));
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                {
+                    // (what a column does not see may hold anything: it is not even multiplied by 0)
+                    if (!whole && !((seen >> (kk * NC + c)) & 1u)) continue;
+                    acc[c][p].x = fmaf(s[kk][c], __uint_as_float(x.x), acc[c][p].x);
+                    acc[c][p].y = fmaf(s[kk][c], __uint_as_float(x.y), acc[c][p].y);
+                    acc[c][p].z = fmaf(s[kk][c], __uint_as_float(x.z), acc[c][p].z);
+                    acc[c][p].w = fmaf(s[kk][c], __uint_as_float(x.w), acc[c][p].w);
+                }
+            }
+    }
+
+    __device__ __forceinline__ void put(int cols, float* sums, float2* ml)
+    {
+        const int lane = threadIdx.x & 31, dl = lane & 7;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+        {
+            float top = m[c];
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float f = m[c] == top ? 1.f : exp2f(m[c] - top);
+            auto all = [&](float x) {
+                x *= f;
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                return x + __shfl_xor_sync(0xffffffffu, x, 16);
+            };
+            l[c] = all(l[c]);
+            if (lane == 0) ml[c] = make_float2(top, l[c]);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+            {
+                const float4 v = make_float4(all(acc[c][p].x), all(acc[c][p].y), all(acc[c][p].z), all(acc[c][p].w));
+                if (lane < 8 && c < cols) *reinterpret_cast<float4*>(sums + c * (D + 4) + (dl + 8 * p) * 4) = v;
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
+// The schedule.
+// ---------------------------------------------------------------------------
 template <int COLS>
 __device__ __forceinline__ int split_row_tiles(const PagedAttnArgs& a, int n)
 {
@@ -309,8 +980,7 @@ __device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
     return c * a.c.kv_heads;
 }
 
-// Finds the CTA's range of tiles and the item its first tile belongs to; every
-// thread returns the same. scan: shared memory for 4 + 2 long longs and 2 ints.
+// The CTA's range of tiles and the sequence of its first tile; every thread returns the same.
 struct SplitStart {
     long long x0, x1, total;   // the CTA's tiles; of all
     long long in_seq;          // x0 counted from its sequence's first tile
@@ -326,7 +996,11 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     o.total = 0;
     const int rounds = (a.b.num_seqs + kSplitThreads - 1) / kSplitThreads;
     long long mine = 0;
-    for (int r = 0; r < rounds; ++r) mine = split_cost<COLS, TILE>(a, r * kSplitThreads + tid), o.total += mine;
+    for (int r = 0; r < rounds; ++r)
+    {
+        mine = split_cost<COLS, TILE>(a, r * kSplitThreads + tid);
+        o.total += mine;
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) o.total += __shfl_xor_sync(0xffffffffu, o.total, d);
     if (lane == 0) scan[warp] = o.total;
@@ -370,27 +1044,26 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     return o;
 }
 
-template <typename QT, typename CT, int D, int NT>
-__global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC) paged_split_kernel(const PagedAttnArgs a)
+template <typename E>
+__global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split_kernel(const PagedAttnArgs a)
 {
-    using Sh = SplitShape<QT, CT, D, NT>;
-    constexpr bool F16 = Sh::F16;
-    constexpr int NQ = Sh::NQ, NK = Sh::NK, COLS = Sh::COLS, S = Sh::S, RB = Sh::RB, CPR = RB / 16;
-    constexpr int KS = D / 16, MTS = D / 16, KEYS = Sh::KEYS, TILE = Sh::TILE, HV = KEYS / 16;
+    using Sh = SplitShape<E>;
+    using CT = typename E::CT;
+    using QT = typename E::QT;
+    constexpr int COLS = E::COLS, S = Sh::S, RB = E::RB, CPR = RB / 16, KEYS = E::KEYS, TILE = Sh::TILE, D = E::D;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan[6];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    pdl_launch();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     PagedJoin* const desc = static_cast<PagedJoin*>(a.work) + blockIdx.x;
     float* const parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.work) + kSplitDescBytes);
+    uint32_t* const colmax = reinterpret_cast<uint32_t*>(smem + Sh::MAX_OFF);
+    if (tid < COLS) colmax[tid] = 0;
+    pdl_wait();
+    pdl_launch();
 
-    const SplitStart st = split_start<COLS, Sh::TILE>(a, scan);
-    if (st.x0 >= st.x1)
-    {
-        if (tid == 0) desc->count = 0;
-        return;
-    }
-    if (tid == 0) desc->count = 0;   // (rewritten below by the same thread)
+    const SplitStart st = split_start<COLS, TILE>(a, scan);
+    if (tid == 0) desc->count = 0;   // (rewritten below, by the same thread, if an item's parts are to be joined)
+    if (st.x0 >= st.x1) return;
 
     // The first item.
     SplitItem it;
@@ -400,52 +1073,49 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
     for (it.tile = 0;; ++it.tile)
     {
         it.w = paged_span(a, it.q, it.tile * COLS, COLS);
-        it.tiles = split_tiles<Sh::TILE>(it.w.n);
+        it.tiles = split_tiles<TILE>(it.w.n);
         if (in < static_cast<long long>(it.tiles) * a.c.kv_heads) break;
         if ((it.tile + 1) * COLS >= it.q.n * a.group) return;   // (the arrays changed under the call)
         in -= static_cast<long long>(it.tiles) * a.c.kv_heads;
     }
     it.head = static_cast<int>(in / it.tiles);
-    int tile0 = static_cast<int>(in % it.tiles);
+    int tile0 = static_cast<int>(in - static_cast<long long>(it.head) * it.tiles);
 
     unsigned char* const ring = smem + warp * S * Sh::STAGE;
     const uint32_t ring_u = smem_u32(ring);
     const uint32_t sc_u = smem_u32(smem + Sh::SC_OFF + warp * S * Sh::SCALES);
     volatile uint32_t* const masks = reinterpret_cast<volatile uint32_t*>(smem + Sh::MASK_OFF) + warp * S;
-    uint2* const qf = reinterpret_cast<uint2*>(smem + Sh::Q_OFF);   // [term][ks][nt][lane]
-    float* const qscale = reinterpret_cast<float*>(smem + Sh::QS_OFF);
 
     long long left = st.x1 - st.x0;
     bool first = true;
+    E eng;
     while (true)
     {
         const int tile1 = static_cast<int>(min(static_cast<long long>(it.tiles), tile0 + left));
         const int n_tiles = tile1 - tile0;
-        const int cols = min(COLS, it.q.n * a.group - it.tile * COLS);
+        it.cols = min(COLS, it.q.n * a.group - it.tile * COLS);
         const int* const table = a.b.table + it.seq * a.b.table_stride;
 
         // ---- loads: this warp's keys of tile tile0 + i into slot i % S ----
         const int kr = lane % KEYS;
-        auto key_of = [&](int u) { return u < it.w.sinks ? u : it.w.lo + u - it.w.sinks; };
-        // Page and row in it of this lane's key of a tile, looked up a step ahead of the load.
-        int pg_next = 0, in_next = 0;
-        auto look_up = [&](int i) {
+        // Page and row in it of this lane's key of a tile: looked up ahead of the load.
+        auto look_up = [&](int i, int& pg, int& row) {
             const int u = (tile0 + i) * TILE + warp * KEYS + kr;
             if (i >= n_tiles || u >= it.w.n) return;
-            const int j = key_of(u), pg = a.page_shift >= 0 ? j >> a.page_shift : j / a.c.page_size;
-            in_next = j - pg * a.c.page_size;
-            pg_next = __ldg(table + pg);
+            const int j = split_key(it, u), x = a.page_shift >= 0 ? j >> a.page_shift : j / a.c.page_size;
+            row = j - x * a.c.page_size;
+            pg = __ldg(table + x);
         };
-        look_up(0);
-        auto load = [&](int i) {
+        auto load = [&](int i, int pg, int row) {
             if (i < n_tiles)
             {
                 const int slot = i % S;
                 const bool live = (tile0 + i) * TILE + warp * KEYS + kr < it.w.n;
-                const bool ok = live && pg_next >= 0 && pg_next < a.c.num_pages;
+                const bool ok = live && pg >= 0 && pg < a.c.num_pages;
                 if (live && !ok) paged_status(a.c.status, kPagedBadPage);
-                const long long off = ok ? pg_next * a.c.page_stride + in_next * a.c.row_stride + it.head * a.c.head_stride : 0;
-                const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+                const long long off = ok ? pg * a.c.page_stride + row * a.c.row_stride + it.head * a.c.head_stride : 0;
+                uint32_t mask = __ballot_sync(0xffffffffu, ok);
+                if constexpr (KEYS < 32) mask &= (1u << KEYS) - 1u;
                 if (lane == 0) masks[slot] = mask;
                 const uint32_t base = ring_u + slot * Sh::STAGE;
 #pragma unroll
@@ -454,467 +1124,53 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                     const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
                     const long long o = __shfl_sync(0xffffffffu, off, r) + c * (16 / static_cast<int>(sizeof(CT)));
                     const bool pr = (mask >> r) & 1u;
-                    cp_async16_zfill(base + split_k_at<CT, D>(r, c), static_cast<const CT*>(a.c.k) + o, pr);
-                    cp_async16_zfill(base + KEYS * RB + split_v_at<CT, D>(r, c), static_cast<const CT*>(a.c.v) + o, pr);
+                    cp_async16_zfill(base + E::k_at(r, c), static_cast<const CT*>(a.c.k) + o, pr);
+                    cp_async16_zfill(base + KEYS * RB + E::v_at(r, c), static_cast<const CT*>(a.c.v) + o, pr);
                 }
-                if constexpr (F16)
+                if constexpr (E::F16)
                 {
-                    const long long so = ok ? pg_next * a.c.s_page_stride + in_next * a.c.s_row_stride + it.head * a.c.s_head_stride : 0;
+                    const long long so = ok ? pg * a.c.s_page_stride + row * a.c.s_row_stride + it.head * a.c.s_head_stride : 0;
                     const uint32_t dst = sc_u + slot * Sh::SCALES + kr * 4;
                     cp_async4_zfill(dst, a.c.k_scale + so, ok);
                     cp_async4_zfill(dst + KEYS * 4, a.c.v_scale + so, ok);
                 }
-                look_up(i + 1);
             }
             cp_commit();
         };
+        int pg[S] = {}, row[S] = {};
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i) load(i);
-
-        // ---- q as B fragments ----
-        if constexpr (F16)
-        {
-            // A column's power of two: its largest magnitude comes to lie in [2^14, 2^15).
-            for (int c = warp; c < COLS; c += kSplitWarps)
-            {
-                uint32_t m = 0;
-                if (c < cols)
-                {
-                    const int cc = it.tile * COLS + c, row = it.q.row0 + cc / a.group, h = it.head * a.group + cc % a.group;
-                    float x[4];
-                    if (lane < D / 4) load_row<QT, 4>(a.q, row * a.q_row_stride + h * a.q_head_stride + lane * 4, x);
+        for (int i = 0; i < S; ++i) look_up(i, pg[i], row[i]);
+        eng.fetch_q(a, it);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (lane < D / 4) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
-                }
-                m = __reduce_max_sync(0xffffffffu, m);
-                // 2^k with k = 14 - exponent, kept within the normal numbers; not finite: 1.
-                const int e = min(max(static_cast<int>(m >> 23), 16), 254);
-                if (lane == 0) qscale[c] = __uint_as_float(static_cast<uint32_t>(e - 14) << 23);   // its inverse
-            }
-            __syncthreads();
-        }
-        for (int x = tid; x < KS * NT * 32; x += kSplitThreads)
-        {
-            const int ln = x & 31, nt = (x >> 5) % NT, ks = (x >> 5) / NT, gg = ln >> 2, tt = ln & 3;
-            const int c = nt * 8 + gg;
-            float v[4] = {};
-            if (c < cols)
-            {
-                const int cc = it.tile * COLS + c, row = it.q.row0 + cc / a.group, h = it.head * a.group + cc % a.group;
-                const long long o = row * a.q_row_stride + h * a.q_head_stride;
-                if constexpr (sizeof(CT) == 2)
-                {
-                    const QT* p = static_cast<const QT*>(a.q) + o + 16 * ks + 2 * tt;
-                    v[0] = to_f32<QT>(p[0]); v[1] = to_f32<QT>(p[1]); v[2] = to_f32<QT>(p[8]); v[3] = to_f32<QT>(p[9]);
-                }
-                else
-                {
-                    const int d = sizeof(CT) == 4 ? 16 * ks + 4 * tt : 64 * (ks >> 2) + 16 * tt + 4 * (ks & 3);
-                    load_row<QT, 4>(a.q, o + d, v);
-                }
-                if constexpr (F16)
-                {
-                    const float up = __uint_as_float((254u << 23) - __float_as_uint(qscale[c]));   // 2^k
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= up;
-                }
-            }
-            uint32_t b0[NQ], b1[NQ];
-            split_pair<F16, NQ>(v[0], v[1], b0);
-            split_pair<F16, NQ>(v[2], v[3], b1);
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) qf[((i * KS + ks) * NT + nt) * 32 + ln] = make_uint2(b0[i], b1[i]);
-        }
-        __syncthreads();
-        uint2 qreg[Sh::QREG ? NQ * KS * NT : 1];
-        if constexpr (Sh::QREG)
-#pragma unroll
-            for (int i = 0; i < NQ * KS * NT; ++i) qreg[i] = qf[i * 32 + lane];
-        auto q_frag = [&](int term, int ks, int nt) {
-            const int i = (term * KS + ks) * NT + nt;
-            if constexpr (Sh::QREG) return qreg[i];
-            else return qf[i * 32 + lane];
-        };
-        // Positions and score factors of this lane's columns (2t, 2t + 1 of every n tile).
-        int pos[NT][2];
-        float fac[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-                const int c = nt * 8 + 2 * t + e;
-                pos[nt][e] = c < cols ? it.q.kv - it.q.n + (it.tile * COLS + c) / a.group : -1;
-                fac[nt][e] = F16 ? a.scale_log2 * qscale[c] : a.scale_log2;
-            }
-
-        float m[NT][2], l[NT][2], acc[NT][MTS][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-        {
-            m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-            for (int i = 0; i < MTS; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
-        }
+        for (int i = 0; i < S - 1; ++i) load(i, pg[i], row[i]);
+        int pg_next = pg[S - 1], row_next = row[S - 1];
+        eng.make_q(a, it, smem + Sh::Q_OFF, colmax);
 
         // ---- the keys ----
         for (int i = 0; i < n_tiles; ++i)
         {
             cp_wait<S - 2>();
             __syncwarp();
-            load(i + S - 1);
+            load(i + S - 1, pg_next, row_next);
+            look_up(i + S, pg_next, row_next);
             const int u0 = (tile0 + i) * TILE + warp * KEYS;
             if (u0 >= it.w.n) continue;   // nothing for this warp in the item's last tile
             const int slot = i % S;
-            const uint32_t kb = ring_u + slot * Sh::STAGE, vb = kb + KEYS * RB;
-            const uint32_t live = masks[slot];
-
-            // Scores of the step's keys: sc[hv][nt] holds keys 16 hv + g and + 8.
-            float sc[HV][NT][4];
-#pragma unroll
-            for (int hv = 0; hv < HV; ++hv)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) sc[hv][nt][0] = sc[hv][nt][1] = sc[hv][nt][2] = sc[hv][nt][3] = 0.f;
-#pragma unroll
-            for (int hv = 0; hv < HV; ++hv)
-            {
-                uint4 w0, w1;   // 8-bit keys: 64 dimensions of rows g and g + 8
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                {
-                    uint32_t ka[NK][4];
-                    if constexpr (sizeof(CT) == 2)
-                    {
-                        ldmatrix4(ka[0], kb + split_k_at<CT, D>(16 * hv + (lane & 15), 2 * ks + (lane >> 4)));
-                    }
-                    else if constexpr (sizeof(CT) == 4)
-                    {
-                        const uint4 x = lds128(kb + split_k_at<CT, D>(16 * hv + g, 4 * ks + t)),
-                                    y = lds128(kb + split_k_at<CT, D>(16 * hv + g + 8, 4 * ks + t));
-                        uint32_t p[NK];
-                        auto put = [&](int at, uint32_t lo, uint32_t hi) {
-                            split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
-#pragma unroll
-                            for (int n = 0; n < NK; ++n) ka[n][at] = p[n];
-                        };
-                        put(0, x.x, x.y);
-                        put(1, y.x, y.y);
-                        put(2, x.z, x.w);
-                        put(3, y.z, y.w);
-                    }
-                    else
-                    {
-                        if (ks % 4 == 0)
-                        {
-                            w0 = lds128(kb + split_k_at<CT, D>(16 * hv + g, ks + t));
-                            w1 = lds128(kb + split_k_at<CT, D>(16 * hv + g + 8, ks + t));
-                        }
-                        const uint32_t x = ks % 4 == 0 ? w0.x : ks % 4 == 1 ? w0.y : ks % 4 == 2 ? w0.z : w0.w;
-                        const uint32_t y = ks % 4 == 0 ? w1.x : ks % 4 == 1 ? w1.y : ks % 4 == 2 ? w1.z : w1.w;
-                        ka[0][0] = codes_f16<CT>(x);
-                        ka[0][1] = codes_f16<CT>(y);
-                        ka[0][2] = codes_f16<CT>(x >> 16);
-                        ka[0][3] = codes_f16<CT>(y >> 16);
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int j = NQ - 1; j >= 0; --j)
-                        {
-                            const uint2 b = q_frag(j, ks, nt);
-#pragma unroll
-                            for (int n = NK - 1; n >= 0; --n)
-                                if (n + j <= 2) mma16816<F16>(sc[hv][nt], ka[n], b.x, b.y);
-                        }
-                }
-            }
-
-            // Scores in units of log 2, masks, the weights' exponents. Index [hv][r]: key 16 hv + 8 r + g.
-            float vs[HV][2], ev[HV][2], kf[HV][2];
-#pragma unroll
-            for (int hv = 0; hv < HV; ++hv)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-                {
-                    kf[hv][r] = vs[hv][r] = 1.f;
-                    ev[hv][r] = 0.f;
-                    if constexpr (F16)
-                    {
-                        const uint32_t at = sc_u + slot * Sh::SCALES + (16 * hv + 8 * r + g) * 4;
-                        kf[hv][r] = lds_f32(at);
-                        const float v = lds_f32(at + KEYS * 4);
-                        // The maximum is taken over the score plus the exponent of the value's scale, so that
-                        // a weight times its scale is below 2 and fits f16 (times 2^14).
-                        ev[hv][r] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(v) >> 23) - 127, -100), 100));
-                        vs[hv][r] = v * 16384.f;
-                    }
-                }
-            const int j_first = key_of(u0), j_last = key_of(min(u0 + KEYS - 1, it.w.n - 1));
-            const bool whole = live == (KEYS == 32 ? 0xffffffffu : 0xffffu) &&
-                               (!a.causal || (j_last <= it.w.p_first &&
-                                              (a.window == 0 || j_first > it.w.p_last - a.window || j_last < a.sinks))) &&
-                               it.w.p_first >= 0;
-            uint32_t seen = 0xffffffffu;   // bit ((hv * 2 + r) * NT + nt) * 2 + e: the column sees the key
-            bool hidden = false;           // some column does not see a key that was loaded
-            if (!whole)
-            {
-#pragma unroll
-                for (int hv = 0; hv < HV; ++hv)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                    {
-                        const int in16 = 16 * hv + 8 * r + g, j = key_of(u0 + in16);
-                        const bool there = (live >> in16) & 1u;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                            {
-                                const bool v = there && paged_sees(a, pos[nt][e], j);
-                                hidden |= there && !v;
-                                if (!v) seen &= ~(1u << (((hv * 2 + r) * NT + nt) * 2 + e));
-                            }
-                    }
-            }
-            bool grew = false;
-            float corr[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-            {
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                {
-                    float x = -INFINITY;
-#pragma unroll
-                    for (int hv = 0; hv < HV; ++hv)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                        {
-                            float& y = sc[hv][nt][2 * r + e];
-                            y *= F16 ? fac[nt][e] * kf[hv][r] : fac[nt][e];
-                            if (!whole && !((seen >> (((hv * 2 + r) * NT + nt) * 2 + e)) & 1u)) y = -INFINITY;
-                            x = fmaxf(x, F16 ? y + ev[hv][r] : y);
-                        }
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    corr[nt][e] = 1.f;
-                    if (x > m[nt][e])
-                    {
-                        corr[nt][e] = exp2f(m[nt][e] - x);
-                        m[nt][e] = x;
-                        grew = true;
-                    }
-                    const float mm = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-                    float sum = 0.f;
-#pragma unroll
-                    for (int hv = 0; hv < HV; ++hv)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                        {
-                            float& y = sc[hv][nt][2 * r + e];
-                            y = exp2f(y - mm);   // (a NaN score stays one)
-                            sum += y;
-                            // A scale of NaN must not meet a weight of zero that stands for "not seen".
-                            if constexpr (F16)
-                                y = (!whole && !((seen >> (((hv * 2 + r) * NT + nt) * 2 + e)) & 1u)) ? 0.f : y * vs[hv][r];
-                        }
-                    l[nt][e] = l[nt][e] * corr[nt][e] + sum;
-                }
-            }
-            if (__any_sync(0xffffffffu, grew))
-            {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int x = 0; x < MTS; ++x)
-                    {
-                        acc[nt][x][0] *= corr[nt][0];
-                        acc[nt][x][1] *= corr[nt][1];
-                        acc[nt][x][2] *= corr[nt][0];
-                        acc[nt][x][3] *= corr[nt][1];
-                    }
-            }
-            // Values that some column must not see may be infinite or NaN, and 0 times those is NaN:
-            // if there are any in such a step, its products are taken one by one.
-            if constexpr (!F16)
-            {
-                if (__any_sync(0xffffffffu, hidden))
-                {
-                    bool odd = false;
-                    for (int x = lane; x < KEYS * CPR; x += 32)
-                    {
-                        const uint4 w = lds128(vb + x * 16);
-                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            odd |= (ws[e] & 0x7f800000u) == 0x7f800000u || (sizeof(CT) == 2 && (ws[e] & 0x7f80u) == 0x7f80u);
-                    }
-                    if (__any_sync(0xffffffffu, odd))
-                    {
-#pragma unroll
-                        for (int hr = 0; hr < 2 * HV; ++hr)
-                        {
-                            const unsigned char* const vst = ring + slot * Sh::STAGE + KEYS * RB;
-#pragma unroll 1
-                            for (int k = 0; k < 8; ++k)
-                            {
-                                const int row = 8 * hr + k, key = key_of(u0 + row);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e)
-                                    {
-                                        const float p = __shfl_sync(0xffffffffu, sc[hr >> 1][nt][2 * (hr & 1) + e], k * 4 + t);
-                                        if (!((live >> row) & 1u) || !paged_sees(a, pos[nt][e], key)) continue;
-#pragma unroll
-                                        for (int x = 0; x < MTS; ++x)
-#pragma unroll
-                                            for (int hf = 0; hf < 2; ++hf)
-                                            {
-                                                const int by = split_dim<CT, D>(x, hf, g) * static_cast<int>(sizeof(CT));
-                                                acc[nt][x][2 * hf + e] +=
-                                                    p * to_f32<CT>(*reinterpret_cast<const CT*>(vst + split_v_at<CT, D>(row, by >> 4) + (by & 15)));
-                                            }
-                                    }
-                            }
-                        }
-                        continue;
-                    }
-                }
-            }
-#pragma unroll
-            for (int hv = 0; hv < HV; ++hv)
-            {
-                uint32_t pb[NT][2][NQ];   // weights as B fragments
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                {
-                    uint32_t p0[NQ], p1[NQ];
-                    split_pair<F16, NQ>(sc[hv][nt][0], sc[hv][nt][1], p0);
-                    split_pair<F16, NQ>(sc[hv][nt][2], sc[hv][nt][3], p1);
-#pragma unroll
-                    for (int j = 0; j < NQ; ++j)
-                    {
-                        pb[nt][0][j] = movmatrix(p0[j]);
-                        pb[nt][1][j] = movmatrix(p1[j]);
-                    }
-                }
-                auto pv = [&](int mt, const uint32_t (&va)[NK][4]) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int j = NQ - 1; j >= 0; --j)
-#pragma unroll
-                            for (int n = NK - 1; n >= 0; --n)
-                                if (n + j <= 2) mma16816<F16>(acc[nt][mt], va[n], pb[nt][0][j], pb[nt][1][j]);
-                };
-                if constexpr (sizeof(CT) == 2)
-                {
-#pragma unroll
-                    for (int mt = 0; mt < MTS; ++mt)
-                    {
-                        uint32_t va[1][4];
-                        ldmatrix4_trans(va[0], vb + split_v_at<CT, D>(16 * hv + (lane & 7) + ((lane >> 4) << 3), 2 * mt + ((lane >> 3) & 1)));
-                        pv(mt, va);
-                    }
-                }
-                else if constexpr (sizeof(CT) == 4)
-                {
-#pragma unroll
-                    for (int x = 0; x < D / 32; ++x)
-                    {
-                        const int r0 = 16 * hv + 2 * t, c = 8 * x + g;
-                        const uint4 f0 = lds128(vb + split_v_at<CT, D>(r0, c)), f1 = lds128(vb + split_v_at<CT, D>(r0 + 1, c));
-                        const uint4 f2 = lds128(vb + split_v_at<CT, D>(r0 + 8, c)), f3 = lds128(vb + split_v_at<CT, D>(r0 + 9, c));
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                        {
-                            uint32_t va[NK][4], p[NK];
-                            auto put = [&](int at, uint32_t lo, uint32_t hi) {
-                                split_pair<false, NK>(__uint_as_float(lo), __uint_as_float(hi), p);
-#pragma unroll
-                                for (int n = 0; n < NK; ++n) va[n][at] = p[n];
-                            };
-                            put(0, y ? f0.z : f0.x, y ? f1.z : f1.x);
-                            put(1, y ? f0.w : f0.y, y ? f1.w : f1.y);
-                            put(2, y ? f2.z : f2.x, y ? f3.z : f3.x);
-                            put(3, y ? f2.w : f2.y, y ? f3.w : f3.y);
-                            pv(2 * x + y, va);
-                        }
-                    }
-                }
-                else
-                {
-                    // Rows 2t, 2t + 1, 2t + 8, 2t + 9; D / 8 consecutive dimensions of each.
-                    constexpr int W = D / 32;   // words
-                    uint32_t f[4][W];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                    {
-                        const int row = 16 * hv + 2 * t + (r & 1) + (r >> 1) * 8;
-                        if constexpr (D == 128)
-                        {
-                            const uint4 x = lds128(vb + split_v_at<CT, D>(row, g));
-                            f[r][0] = x.x; f[r][1] = x.y; f[r][2] = x.z; f[r][3] = x.w;
-                        }
-                        else
-                        {
-                            const uint2 x = lds64(vb + split_v_at<CT, D>(row, g >> 1) + (g & 1) * 8);
-                            f[r][0] = x.x; f[r][1] = x.y;
-                        }
-                    }
-#pragma unroll
-                    for (int mt = 0; mt < MTS; ++mt)
-                    {
-                        const int wd = mt >> 1;
-                        const uint32_t s0 = (mt & 1) ? 0x62u : 0x40u, s1 = (mt & 1) ? 0x73u : 0x51u;
-                        uint32_t va[1][4];
-                        va[0][0] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s0));
-                        va[0][1] = codes_f16<CT>(__byte_perm(f[0][wd], f[1][wd], s1));
-                        va[0][2] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s0));
-                        va[0][3] = codes_f16<CT>(__byte_perm(f[2][wd], f[3][wd], s1));
-                        pv(mt, va);
-                    }
-                }
-            }
+            eng.step(a, it, u0, masks[slot], ring + slot * Sh::STAGE, ring_u + slot * Sh::STAGE, sc_u + slot * Sh::SCALES);
         }
         cp_wait<0>();
 
         // ---- the warps' parts into one ----
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
-                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
-                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
-            }
         __syncthreads();   // every ring is drained
-        float* const sums = reinterpret_cast<float*>(smem);                       // [warp][COLS][D + 4]
-        float2* const ml = reinterpret_cast<float2*>(smem + Sh::ML_OFF);           // [warp][COLS]
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-                const int c = nt * 8 + 2 * t + e;
-                if (g == 0) ml[warp * COLS + c] = make_float2(m[nt][e], l[nt][e]);
-                if (c < cols)
-#pragma unroll
-                    for (int x = 0; x < MTS; ++x)
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf)
-                            sums[(warp * COLS + c) * (D + 4) + split_dim<CT, D>(x, hf, g)] = acc[nt][x][2 * hf + e];
-            }
+        float* const sums = reinterpret_cast<float*>(smem);                // [warp][COLS][D + 4]
+        float2* const ml = reinterpret_cast<float2*>(smem + Sh::ML_OFF);   // [warp][COLS]
+        eng.put(it.cols, sums + warp * COLS * (D + 4), ml + warp * COLS);
         __syncthreads();
+        if (tid < COLS) colmax[tid] = 0;
         const bool complete = tile0 == 0 && tile1 == it.tiles;
         const int part_slot = 2 * blockIdx.x + (first ? 0 : 1);
         float* const part = parts + static_cast<long long>(part_slot) * Sh::PART;
-        for (int x = tid; x < cols * (D / 4); x += kSplitThreads)
+        for (int x = tid; x < it.cols * (D / 4); x += kSplitThreads)
         {
             const int c = x / (D / 4), d = (x % (D / 4)) * 4;
             float2 w[kSplitWarps];
@@ -935,11 +1191,11 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
             }
             if (complete)
             {
-                const float inv = L == 0.f ? 0.f : (F16 ? 1.f / 16384.f : 1.f) / L;
+                const float inv = L == 0.f ? 0.f : E::OUT / L;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] *= inv;
-                const int cc = it.tile * COLS + c, row = it.q.row0 + cc / a.group, h = it.head * a.group + cc % a.group;
-                store_row<QT, 4>(a.out, row * a.o_row_stride + h * a.o_head_stride + d, o);
+                const int cc = it.tile * COLS + c, rw = cc / a.group;
+                store_row<QT, 4>(a.out, (it.q.row0 + rw) * a.o_row_stride + (it.head * a.group + cc - rw * a.group) * a.o_head_stride + d, o);
             }
             else
             {
@@ -951,15 +1207,14 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
         if (!complete && tile0 == 0 && tid == 0)
         {
             // This CTA starts the item: its parts are here and in the CTAs up to the one with the item's last tile.
-            const long long x_last = st.x1 - left - n_tiles + it.tiles - 1 - tile0;   // (global index of that tile)
-            const int last = static_cast<int>(x_last / st.share);
+            const long long x_last = st.x1 - left - n_tiles + it.tiles - 1;   // (global index of that tile)
             PagedJoin d;
-            d.count = last - static_cast<int>(blockIdx.x) + 1;
+            d.count = static_cast<int>(x_last / st.share) - static_cast<int>(blockIdx.x) + 1;
             d.first_slot = part_slot;
             d.first_cta = blockIdx.x;
             d.row0 = it.q.row0;
             d.col0 = it.tile * COLS;
-            d.cols = cols;
+            d.cols = it.cols;
             d.head = it.head;
             d.pad = 0;
             *desc = d;
@@ -981,62 +1236,86 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<QT, CT, D, NT>::OCC)
                 if (it.seq >= a.b.num_seqs) break;   // (the arrays changed under the call)
             }
             it.w = paged_span(a, it.q, it.tile * COLS, COLS);
-            it.tiles = split_tiles<Sh::TILE>(it.w.n);
+            it.tiles = split_tiles<TILE>(it.w.n);
         }
         __syncthreads();   // the sums were read; the ring is free
     }
 }
 
-// Joins the parts of the item that CTA blockIdx.x of the split kernel started, if it did.
-template <typename QT, bool F16, int D, int NT>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a)
+// Joins the parts of the item that CTA blockIdx.x of the split kernel started, if it
+// did; blockIdx.y takes 8 of its columns. A float4 of a column is a group of D / 4 threads'; the
+// groups are dealt to the columns that there are, several to a column where
+// columns are few, each adding up every so manyth part.
+constexpr int kJoinThreads = 512;
+template <typename E>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a)
 {
-    constexpr int COLS = 8 * NT, PART = COLS * (D + 2);
+    constexpr int COLS = E::COLS, D = E::D, PART = SplitShape<E>::PART, LANES = D / 4, GROUPS = kJoinThreads / LANES;
+    __shared__ float2 ml[GROUPS];
+    __shared__ float4 vec[GROUPS][LANES];
     pdl_wait();
     const PagedJoin j = static_cast<const PagedJoin*>(a.work)[blockIdx.x];
-    if (j.count == 0) return;
+    const int c0 = blockIdx.y * 8, cols = min(8, j.cols - c0);
+    if (j.count == 0 || cols <= 0) return;
     const float* const parts = reinterpret_cast<const float*>(static_cast<const unsigned char*>(a.work) + kSplitDescBytes);
-    for (int x = threadIdx.x; x < j.cols * (D / 4); x += 128)
+    const int grp = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
+    const int width = cols <= 1 ? 1 : cols <= 2 ? 2 : cols <= 4 ? 4 : 8;   // columns, rounded up to a power of two
+    const int per = GROUPS / width, c = c0 + grp % width, sub = grp / width;
+    float M = -INFINITY, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto at = [&](int k) { return parts + static_cast<long long>(k == 0 ? j.first_slot : 2 * (j.first_cta + k)) * PART; };
+    constexpr int U = 8;   // parts in flight
+    if (c < c0 + cols)
     {
-        const int c = x / (D / 4), d = (x % (D / 4)) * 4;
-        float M = -INFINITY, L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto at = [&](int k) {
-            return parts + static_cast<long long>(k == 0 ? j.first_slot : 2 * (j.first_cta + k)) * PART;
-        };
-        constexpr int U = 8;   // parts in flight
-        for (int k0 = 0; k0 < j.count; k0 += U)
+        for (int k0 = sub; k0 < j.count; k0 += U * per)
         {
             float2 w[U];
             float4 v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int x = 0; x < U; ++x)
             {
-                const int k = min(k0 + u, j.count - 1);
-                w[u] = reinterpret_cast<const float2*>(at(k))[c];
-                v[u] = *reinterpret_cast<const float4*>(at(k) + 2 * COLS + c * D + d);
+                if (k0 + x * per >= j.count) break;
+                w[x] = reinterpret_cast<const float2*>(at(k0 + x * per))[c];
+                v[x] = *reinterpret_cast<const float4*>(at(k0 + x * per) + 2 * COLS + c * D + d);
             }
             float top = M;
 #pragma unroll
-            for (int u = 0; u < U; ++u) top = fmaxf(top, w[u].x);
+            for (int x = 0; x < U; ++x)
+                if (k0 + x * per < j.count) top = fmaxf(top, w[x].x);
             const float f0 = M == top ? 1.f : exp2f(M - top);
             L *= f0;
             o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int x = 0; x < U; ++x)
             {
-                if (k0 + u >= j.count) break;
-                const float f = w[u].x == top ? 1.f : exp2f(w[u].x - top);
-                L += f * w[u].y;
-                o.x += f * v[u].x; o.y += f * v[u].y; o.z += f * v[u].z; o.w += f * v[u].w;
+                if (k0 + x * per >= j.count) break;
+                const float f = w[x].x == top ? 1.f : exp2f(w[x].x - top);
+                L += f * w[x].y;
+                o.x += f * v[x].x; o.y += f * v[x].y; o.z += f * v[x].z; o.w += f * v[x].w;
             }
             M = top;
         }
-        const float inv = L == 0.f ? 0.f : (F16 ? 1.f / 16384.f : 1.f) / L;
-        const float r[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-        const int cc = j.col0 + c, row = j.row0 + cc / a.group, h = j.head * a.group + cc % a.group;
-        store_row<QT, 4>(a.out, row * a.o_row_stride + h * a.o_head_stride + d, r);
     }
+    if (d == 0) ml[grp] = make_float2(M, L);
+    vec[grp][d / 4] = o;
+    __syncthreads();
+    if (sub != 0 || c >= c0 + cols) return;
+    float top = -INFINITY;
+    for (int x = 0; x < per; ++x) top = fmaxf(top, ml[grp + x * width].x);
+    L = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = 0; x < per; ++x)
+    {
+        const float2 w = ml[grp + x * width];
+        const float f = w.x == top ? 1.f : exp2f(w.x - top);
+        const float4 v = vec[grp + x * width][d / 4];
+        L += f * w.y;
+        o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+    }
+    const float inv = L == 0.f ? 0.f : E::OUT / L;
+    const float r[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    const int cc = j.col0 + c, rw = cc / a.group;
+    store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + d, r);
 }
 
 }  // namespace hy

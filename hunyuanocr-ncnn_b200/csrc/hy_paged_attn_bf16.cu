@@ -1,0 +1,8 @@
+// Paged attention of bf16 rows.
+#include "hy_paged_launch.cuh"
+
+cudaError_t hy_internal::paged_attention_bf16(const hy::PagedAttnArgs& a, int cache_dtype, int head_dim, int cols, int device,
+                                             cudaStream_t s)
+{
+    return hy::launch_split_typed<__nv_bfloat16>(a, cache_dtype, head_dim, cols, device, s);
+}

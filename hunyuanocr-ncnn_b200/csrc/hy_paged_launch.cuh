@@ -1,0 +1,105 @@
+// Launches of the paged attention, one translation unit per row type
+// (hy_paged_attn_f32.cu, hy_paged_attn_bf16.cu).
+#pragma once
+
+#include <atomic>
+#include <type_traits>
+
+#include "hy_decode.h"
+#include "hy_paged_attn.cuh"
+#include "hy_paged.h"
+
+namespace hy_internal {
+cudaError_t paged_attention_f32(const hy::PagedAttnArgs& a, int cache_dtype, int head_dim, int cols, int device, cudaStream_t s);
+cudaError_t paged_attention_bf16(const hy::PagedAttnArgs& a, int cache_dtype, int head_dim, int cols, int device, cudaStream_t s);
+}  // namespace hy_internal
+
+namespace hy {
+
+template <typename T>
+struct Tag {
+    using type = T;
+};
+
+// f(row type, cache type, head_dim) with the run-time types as types.
+template <typename RT, typename F>
+auto with_types(RT rt, int cache_dtype, int head_dim, F&& f)
+{
+    auto dim = [&](auto ct) {
+        return head_dim == 64 ? f(rt, ct, std::integral_constant<int, 64>{})
+                              : f(rt, ct, std::integral_constant<int, 128>{});
+    };
+    switch (cache_dtype)
+    {
+    case HY_DTYPE_F32: return dim(Tag<float>{});
+    case HY_DTYPE_BF16: return dim(Tag<__nv_bfloat16>{});
+    case HY_DTYPE_E4M3: return dim(Tag<E4M3>{});
+    default: return dim(Tag<Int8>{});
+    }
+}
+template <typename F>
+auto with_row_type(int row_dtype, int cache_dtype, int head_dim, F&& f)
+{
+    return row_dtype == HY_DTYPE_F32 ? with_types(Tag<float>{}, cache_dtype, head_dim, f)
+                                     : with_types(Tag<__nv_bfloat16>{}, cache_dtype, head_dim, f);
+}
+
+// Lets Kernel have `smem` bytes of dynamic shared memory; set once per device.
+template <auto Kernel>
+cudaError_t allow_smem(int smem, int device)
+{
+    static std::atomic<unsigned long long> done{0};
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    const cudaError_t e =
+        cudaFuncSetAttribute(reinterpret_cast<const void*>(Kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+// A launch that may be prepared while the kernel before it in the stream runs (the kernels wait for its end).
+template <typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Args...), dim3 grid, int threads, int smem, cudaStream_t s, const Args&... args)
+{
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename E>
+cudaError_t launch_split(const PagedAttnArgs& a, int device, cudaStream_t s)
+{
+    using Sh = SplitShape<E>;
+    cudaError_t e = allow_smem<paged_split_kernel<E>>(Sh::SMEM, device);
+    if (e == cudaSuccess) e = launch_pdl(paged_split_kernel<E>, dim3(Sh::GRID), kSplitThreads, Sh::SMEM, s, a);
+    if (e == cudaSuccess)
+        e = launch_pdl(paged_join_kernel<E>, dim3(Sh::GRID, (E::COLS + 7) / 8), kJoinThreads, 0, s, a);
+    return e;
+}
+
+template <typename QT>
+cudaError_t launch_split_typed(const PagedAttnArgs& a, int cache_dtype, int head_dim, int cols, int device, cudaStream_t s)
+{
+    return with_types(Tag<QT>{}, cache_dtype, head_dim, [&](auto, auto ct, auto d) {
+        using CT = typename decltype(ct)::type;
+        constexpr int D = decltype(d)::value;
+        if constexpr (std::is_same_v<CT, float>)
+        {
+            if (cols == 2) return launch_split<FmaEngine<QT, D, 2>>(a, device, s);
+            if (cols == 4) return launch_split<FmaEngine<QT, D, 4>>(a, device, s);
+        }
+        return cols <= 8    ? launch_split<MmaEngine<QT, CT, D, 1>>(a, device, s)
+               : cols == 16 ? launch_split<MmaEngine<QT, CT, D, 2>>(a, device, s)
+                            : launch_split<MmaEngine<QT, CT, D, 4>>(a, device, s);
+    });
+}
+
+}  // namespace hy
