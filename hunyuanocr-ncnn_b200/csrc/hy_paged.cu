@@ -175,12 +175,14 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     return e == cudaSuccess ? HY_OK : cuda_fail(write ? "paged write" : "paged read", e);
 }
 
-// Columns of a tile of the split kernels: as many as a sequence's rows need, up
-// to 32; fp32 caches have tiles of 2 and 4 (FmaEngine).
-int split_columns(int max_rows, int group, int cache_dtype)
+// Columns of a tile: as many as a sequence's rows need, up to 32, in the split
+// kernels (fp32 caches have tiles of 2 and 4 too, FmaEngine), else 256, for which
+// bf16 rows take the tcgen05 kernel; fp32 rows and fp32 caches stay at 32.
+int tile_columns(int max_rows, int group, int dtype, int cache_dtype)
 {
     const long long cols = static_cast<long long>(max_rows) * group;
     if (cache_dtype == HY_DTYPE_F32 && cols <= 4) return cols <= 2 ? 2 : 4;
+    if (cols > 32 && dtype == HY_DTYPE_BF16 && cache_dtype != HY_DTYPE_F32) return 256;
     return cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
 }
 
@@ -199,10 +201,10 @@ int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, in
 }
 
 // Descriptions and two parts for every CTA.
-size_t attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int q_heads)
+size_t attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int q_heads, int dtype)
 {
-    const int cols = split_columns(batch->max_rows, q_heads / cache->num_kv_heads, cache->dtype);
-    return kSplitDescBytes + static_cast<size_t>(2 * kSplitMaxCtas) * cols * (cache->head_dim + 2) * sizeof(float);
+    const int cols = tile_columns(batch->max_rows, q_heads / cache->num_kv_heads, dtype, cache->dtype);
+    return kSplitDescBytes + static_cast<size_t>(2 * (cols == 256 ? 148 : kSplitMaxCtas)) * cols * (cache->head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -231,7 +233,7 @@ int hy_paged_attention_workspace(const hy_paged_cache* cache, const hy_paged_bat
     const int rc = check_attention(cache, batch, rows, q_heads, dtype);
     if (rc) return rc;
     if (!bytes) return fail(HY_ERR_INVALID_ARGUMENT, "bytes is null");
-    *bytes = attention_workspace(cache, batch, q_heads);
+    *bytes = attention_workspace(cache, batch, q_heads, dtype);
     return HY_OK;
 }
 
@@ -244,7 +246,8 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     if (rc) return rc;
     if (window < 0 || sinks < 0) return fail(HY_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
     if (!causal && window > 0) return fail(HY_ERR_UNSUPPORTED, "a window needs causal attention");
-    if (!(scale == scale) || scale - scale != 0.f) return fail(HY_ERR_INVALID_ARGUMENT, "scale must be finite");
+    if (!(scale > 0.f) || scale - scale != 0.f)
+        return fail(HY_ERR_INVALID_ARGUMENT, "scale must be finite and positive");
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
     rc = check_rows("q", q_dev, q_row_stride, q_head_stride, dtype);
     if (!rc) rc = check_rows("out", out_dev, out_row_stride, out_head_stride, dtype);
@@ -252,7 +255,7 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     if (q_dev == out_dev) return fail(HY_ERR_INVALID_ARGUMENT, "q and out must not overlap");
     if (!workspace_dev || !aligned16(workspace_dev))
         return fail(HY_ERR_INVALID_ARGUMENT, "the workspace is null or not on 16 bytes");
-    if (workspace_bytes < attention_workspace(cache, batch, q_heads))
+    if (workspace_bytes < attention_workspace(cache, batch, q_heads, dtype))
         return fail(HY_ERR_CAPACITY, "the workspace is too small");
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
@@ -260,7 +263,7 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
                           power_of_two(cache->page_size), scale * 1.4426950408889634f, workspace_dev};
-    const int cols = split_columns(batch->max_rows, group, cache->dtype);
+    const int cols = tile_columns(batch->max_rows, group, dtype, cache->dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto launch = dtype == HY_DTYPE_F32 ? hy_internal::paged_attention_f32 : hy_internal::paged_attention_bf16;
     const cudaError_t e = launch(a, cache->dtype, cache->head_dim, cols, cache->device, s);

@@ -116,6 +116,13 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// 2^x, off by less than 2^-22; 0 below 2^-126.
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
 {
     const __half2 v = __floats2half2_rn(lo, hi);
@@ -576,7 +583,7 @@ struct MmaEngine {
                 corr[nt][e] = 1.f;
                 if (x > m[nt][e])
                 {
-                    corr[nt][e] = exp2f(m[nt][e] - x);
+                    corr[nt][e] = ex2(m[nt][e] - x);
                     m[nt][e] = x;
                     grew = true;
                 }
@@ -588,7 +595,7 @@ struct MmaEngine {
                     for (int r = 0; r < 2; ++r)
                     {
                         float& y = sc[hv][nt][2 * r + e];
-                        y = exp2f(y - mm);   // (a NaN score stays one)
+                        y = ex2(y - mm);   // (a NaN score stays one)
                         sum += y;
                         // A scale of NaN must not meet a weight of zero that stands for "not seen".
                         if constexpr (F16)
@@ -893,7 +900,7 @@ struct FmaEngine {
             float corr = 1.f;
             if (top > m[c])
             {
-                corr = exp2f(m[c] - top);
+                corr = ex2(m[c] - top);
                 m[c] = top;
 #pragma unroll
                 for (int p = 0; p < P; ++p)
@@ -906,7 +913,7 @@ struct FmaEngine {
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
             {
-                s[kk][c] = exp2f(s[kk][c] - mm);   // (a NaN score stays one)
+                s[kk][c] = ex2(s[kk][c] - mm);   // (a NaN score stays one)
                 l[c] += s[kk][c];
             }
         }
@@ -939,7 +946,7 @@ struct FmaEngine {
             float top = m[c];
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float f = m[c] == top ? 1.f : exp2f(m[c] - top);
+            const float f = m[c] == top ? 1.f : ex2(m[c] - top);
             auto all = [&](float x) {
                 x *= f;
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
@@ -987,18 +994,20 @@ struct SplitStart {
     long long share;           // tiles per CTA
     int seq;
 };
-template <int COLS, int TILE>
+// scan: shared memory for a long long per warp and one more.
+template <int COLS, int TILE, int THREADS>
 __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long long* scan)
 {
+    constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __shared__ int s_seq;
     SplitStart o;
     o.total = 0;
-    const int rounds = (a.b.num_seqs + kSplitThreads - 1) / kSplitThreads;
+    const int rounds = (a.b.num_seqs + THREADS - 1) / THREADS;
     long long mine = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        mine = split_cost<COLS, TILE>(a, r * kSplitThreads + tid);
+        mine = split_cost<COLS, TILE>(a, r * THREADS + tid);
         o.total += mine;
     }
 #pragma unroll
@@ -1006,7 +1015,7 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     if (lane == 0) scan[warp] = o.total;
     __syncthreads();
     o.total = 0;
-    for (int w = 0; w < kSplitWarps; ++w) o.total += scan[w];
+    for (int w = 0; w < WARPS; ++w) o.total += scan[w];
     o.share = max(1ll, (o.total + gridDim.x - 1) / gridDim.x);
     o.x0 = min(o.total, o.share * blockIdx.x);
     o.x1 = min(o.total, o.x0 + o.share);
@@ -1016,7 +1025,7 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     long long base = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        if (rounds > 1) mine = split_cost<COLS, TILE>(a, r * kSplitThreads + tid);
+        if (rounds > 1) mine = split_cost<COLS, TILE>(a, r * THREADS + tid);
         long long inc = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1)
@@ -1029,18 +1038,18 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
         __syncthreads();
         long long before = base;
         for (int w = 0; w < warp; ++w) before += scan[w];
-        for (int w = 0; w < kSplitWarps; ++w) base += scan[w];
+        for (int w = 0; w < WARPS; ++w) base += scan[w];
         const long long lo = before + inc - mine;
         if (o.x0 >= lo && o.x0 < lo + mine)
         {
-            s_seq = r * kSplitThreads + tid;
-            scan[4] = o.x0 - lo;
+            s_seq = r * THREADS + tid;
+            scan[WARPS] = o.x0 - lo;
         }
         if (o.x0 < base) break;   // uniform: found in this round
     }
     __syncthreads();
     o.seq = s_seq;
-    o.in_seq = scan[4];
+    o.in_seq = scan[WARPS];
     return o;
 }
 
@@ -1052,7 +1061,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
     using QT = typename E::QT;
     constexpr int COLS = E::COLS, S = Sh::S, RB = E::RB, CPR = RB / 16, KEYS = E::KEYS, TILE = Sh::TILE, D = E::D;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long scan[6];
+    __shared__ long long scan[kSplitWarps + 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     PagedJoin* const desc = static_cast<PagedJoin*>(a.work) + blockIdx.x;
     float* const parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.work) + kSplitDescBytes);
@@ -1061,7 +1070,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
     pdl_wait();
     pdl_launch();
 
-    const SplitStart st = split_start<COLS, TILE>(a, scan);
+    const SplitStart st = split_start<COLS, TILE, kSplitThreads>(a, scan);
     if (tid == 0) desc->count = 0;   // (rewritten below, by the same thread, if an item's parts are to be joined)
     if (st.x0 >= st.x1) return;
 
@@ -1184,7 +1193,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
 #pragma unroll
             for (int k = 0; k < kSplitWarps; ++k)
             {
-                const float f = w[k].x == M ? 1.f : exp2f(w[k].x - M);
+                const float f = w[k].x == M ? 1.f : ex2(w[k].x - M);
                 const float4 v = *reinterpret_cast<const float4*>(sums + (k * COLS + c) * (D + 4) + d);
                 L += f * w[k].y;
                 o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
@@ -1250,7 +1259,7 @@ constexpr int kJoinThreads = 512;
 template <typename E>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a)
 {
-    constexpr int COLS = E::COLS, D = E::D, PART = SplitShape<E>::PART, LANES = D / 4, GROUPS = kJoinThreads / LANES;
+    constexpr int COLS = E::COLS, D = E::D, PART = COLS * (D + 2), LANES = D / 4, GROUPS = kJoinThreads / LANES;
     __shared__ float2 ml[GROUPS];
     __shared__ float4 vec[GROUPS][LANES];
     pdl_wait();
@@ -1282,14 +1291,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
 #pragma unroll
             for (int x = 0; x < U; ++x)
                 if (k0 + x * per < j.count) top = fmaxf(top, w[x].x);
-            const float f0 = M == top ? 1.f : exp2f(M - top);
+            const float f0 = M == top ? 1.f : ex2(M - top);
             L *= f0;
             o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
 #pragma unroll
             for (int x = 0; x < U; ++x)
             {
                 if (k0 + x * per >= j.count) break;
-                const float f = w[x].x == top ? 1.f : exp2f(w[x].x - top);
+                const float f = w[x].x == top ? 1.f : ex2(w[x].x - top);
                 L += f * w[x].y;
                 o.x += f * v[x].x; o.y += f * v[x].y; o.z += f * v[x].z; o.w += f * v[x].w;
             }
@@ -1307,7 +1316,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     for (int x = 0; x < per; ++x)
     {
         const float2 w = ml[grp + x * width];
-        const float f = w.x == top ? 1.f : exp2f(w.x - top);
+        const float f = w.x == top ? 1.f : ex2(w.x - top);
         const float4 v = vec[grp + x * width][d / 4];
         L += f * w.y;
         o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;

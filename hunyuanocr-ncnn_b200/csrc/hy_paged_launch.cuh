@@ -7,6 +7,7 @@
 
 #include "hy_decode.h"
 #include "hy_paged_attn.cuh"
+#include "hy_paged_chunk.cuh"
 #include "hy_paged.h"
 
 namespace hy_internal {
@@ -85,6 +86,16 @@ cudaError_t launch_split(const PagedAttnArgs& a, int device, cudaStream_t s)
     return e;
 }
 
+template <typename CT, int D>
+cudaError_t launch_chunk(const PagedAttnArgs& a, int device, cudaStream_t s)
+{
+    using E = ChunkEngine<CT, D>;
+    cudaError_t e = allow_smem<paged_chunk_kernel<CT, D>>(E::SMEM, device);
+    if (e == cudaSuccess) e = launch_pdl(paged_chunk_kernel<CT, D>, dim3(148), kChunkThreads, E::SMEM, s, a);
+    if (e == cudaSuccess) e = launch_pdl(paged_join_kernel<E>, dim3(148, E::COLS / 8), kJoinThreads, 0, s, a);
+    return e;
+}
+
 template <typename QT>
 cudaError_t launch_split_typed(const PagedAttnArgs& a, int cache_dtype, int head_dim, int cols, int device, cudaStream_t s)
 {
@@ -96,6 +107,8 @@ cudaError_t launch_split_typed(const PagedAttnArgs& a, int cache_dtype, int head
             if (cols == 2) return launch_split<FmaEngine<QT, D, 2>>(a, device, s);
             if (cols == 4) return launch_split<FmaEngine<QT, D, 4>>(a, device, s);
         }
+        if constexpr (std::is_same_v<QT, __nv_bfloat16> && !std::is_same_v<CT, float>)
+            if (cols == 256) return launch_chunk<CT, D>(a, device, s);
         return cols <= 8    ? launch_split<MmaEngine<QT, CT, D, 1>>(a, device, s)
                : cols == 16 ? launch_split<MmaEngine<QT, CT, D, 2>>(a, device, s)
                             : launch_split<MmaEngine<QT, CT, D, 4>>(a, device, s);

@@ -110,7 +110,7 @@ int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, i
  *   causal == 0: every j < kv_len (window must be 0).
  * A row that sees nothing gives zeros. Positions that a row does not see do
  * not reach its output, whatever they hold (infinities and NaN included).
- * q and out have the same dtype and must not overlap. Products and softmax
+ * scale must be positive. q and out have the same dtype and must not overlap. Products and softmax
  * sums are in fp32. F32 rows: every product is exact to 2^-22 or better. BF16
  * rows: probabilities are rounded to bf16 before they multiply v. */
 int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
