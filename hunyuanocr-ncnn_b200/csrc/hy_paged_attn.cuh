@@ -33,6 +33,8 @@ struct PagedSpan {
     int p_first, p_last;   // positions of the first and last row
     int sinks, lo, n;      // virtual position u < sinks: u, else lo + u - sinks; n of them
 };
+// ALIGN: the run's parts start and the sinks end at multiples of it (what that adds is masked).
+template <int ALIGN = 1>
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const PagedSeq& s, int c0, int cols)
 {
     PagedSpan o;
@@ -40,8 +42,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
     o.p_first = s.kv - s.n + c0 / a.group;
     o.p_last = s.kv - s.n + last / a.group;
     const int hi = o.p_last < 0 ? 0 : a.causal ? o.p_last + 1 : s.kv;
-    o.lo = (a.window > 0) ? min(hi, max(0, o.p_first - a.window + 1)) : 0;
-    o.sinks = min(o.lo, a.sinks);
+    o.lo = (a.window > 0) ? min(hi, max(0, o.p_first - a.window + 1)) / ALIGN * ALIGN : 0;
+    o.sinks = a.sinks >= o.lo ? o.lo : (a.sinks + ALIGN - 1) / ALIGN * ALIGN;
     o.n = o.sinks + hi - o.lo;
     return o;
 }
@@ -976,14 +978,14 @@ template <int TILE>
 __device__ __forceinline__ int split_tiles(int keys) { return max(1, (keys + TILE - 1) / TILE); }
 
 // Tiles of sequence s, all its items.
-template <int COLS, int TILE>
+template <int COLS, int TILE, int ALIGN>
 __device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
 {
     PagedSeq q;
     if (s >= a.b.num_seqs || !paged_seq(a.b, s, a.c.page_size, a.c.status, q)) return 0;
     long long c = 0;
     const int rt = split_row_tiles<COLS>(a, q.n);
-    for (int t = 0; t < rt; ++t) c += split_tiles<TILE>(paged_span(a, q, t * COLS, COLS).n);
+    for (int t = 0; t < rt; ++t) c += split_tiles<TILE>(paged_span<ALIGN>(a, q, t * COLS, COLS).n);
     return c * a.c.kv_heads;
 }
 
@@ -995,7 +997,7 @@ struct SplitStart {
     int seq;
 };
 // scan: shared memory for a long long per warp and one more.
-template <int COLS, int TILE, int THREADS>
+template <int COLS, int TILE, int THREADS, int ALIGN = 1>
 __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long long* scan)
 {
     constexpr int WARPS = THREADS / 32;
@@ -1007,7 +1009,7 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     long long mine = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        mine = split_cost<COLS, TILE>(a, r * THREADS + tid);
+        mine = split_cost<COLS, TILE, ALIGN>(a, r * THREADS + tid);
         o.total += mine;
     }
 #pragma unroll
@@ -1025,7 +1027,7 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     long long base = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        if (rounds > 1) mine = split_cost<COLS, TILE>(a, r * THREADS + tid);
+        if (rounds > 1) mine = split_cost<COLS, TILE, ALIGN>(a, r * THREADS + tid);
         long long inc = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1)

@@ -11,19 +11,27 @@
 //     from tensor memory, the weights go back to it as the next product's operand;
 //     the output is rescaled in tensor memory, and only when a column's maximum has
 //     grown by more than 2^8 since it was last (the weights stay below 2^8);
-//   warps 8-11: loads. Every thread looks up the page of one key of a block;
-//     rows go to shared memory by cp.async (bf16) or through registers as f16 (8-bit codes, exact),
-//     in the 128-byte-swizzled layout that serves K as the K-major operand of
-//     q k^T and V as the MN-major operand of p v;
-//   warp 12: one thread issues the products (13-15 make the warpgroup whole). Tile 0's and 1's alternate, so
-//     that the tensor cores work on one tile while the other's softmax runs:
-//     p v of block j, then q k^T of block j + 1, whose scores take the place of the weights just used.
+//   warps 8-11: loads, and the walk over the items (the other roles read an item's
+//     description from shared memory when its q is there). bf16 blocks arrive in the
+//     128-byte-swizzled layout that serves K as the K-major operand of q k^T
+//     and V as the MN-major operand of p v; 8-bit blocks arrive as codes in a
+//     staging ring and are written to that layout as f16 (exact);
+//   warp 12: one thread issues the products (13-15 make the warpgroup whole).
+//     Tile 0's and 1's alternate, so that the tensor cores work on one tile while the
+//     other's softmax runs: p v of block j, then q k^T of block j + 1, whose
+//     scores take the place of the weights just used.
+//
+// Where pages hold a multiple of 16 rows, blocks are fetched by TMA, 16 rows of a
+// page at a time (the window's start is rounded down to 16, masks do the rest);
+// for other page sizes the loading warps copy row by row.
 //
 // Tensor memory (512 columns): scores of the two tiles (128 each; the
 // weights, 16 bits, in the upper 64 of them), outputs of the two tiles (128 each).
 // Every wait is bounded; a wait that gives up sets a status bit, and the CTA
 // runs on to free its tensor memory.
 #pragma once
+
+#include <cuda.h>
 
 #include "hy_paged_attn.cuh"
 #include "hy_tcgen05.cuh"
@@ -38,21 +46,36 @@ struct ChunkEngine {
     static constexpr bool F16 = kCodes<CT>;
     // f16 weights carry 2^6: below 2^(6 + 8 + 1), and exact to 11 bits down to 2^-20 of the largest.
     static constexpr float OUT = F16 ? 1.f / 64.f : 1.f;
-    static constexpr int RB = D * 2;                       // bytes of a row in shared memory
+    static constexpr int RB = D * 2;                       // bytes of a row in operand layout
     static constexpr int TILE_B = 128 * RB;                // a block of K or V, a tile of q
-    static constexpr int SLOTS = 4;                        // ring of K and V blocks
-    static constexpr int Q_OFF = 0, RING_OFF = 2 * TILE_B;
+    static constexpr int SLOTS = F16 ? 3 : 4;              // ring of K and V blocks
+    static constexpr int CODES_B = 128 * D, STAGES = F16 ? 3 : 0;   // staging ring of 8-bit blocks
+    static constexpr int Q_OFF = 0, RING_OFF = 2 * TILE_B, STAGE_OFF = RING_OFF + SLOTS * TILE_B;
     // Scales of the last 4 blocks: k, v times the weights' unit, exponent of v's (fp32, 128 each).
-    static constexpr int SCALE_B = 3 * 128 * 4, SCALE_OFF = RING_OFF + SLOTS * TILE_B;
+    static constexpr int SCALE_B = 3 * 128 * 4, SCALE_OFF = STAGE_OFF + STAGES * CODES_B;
     static constexpr int LIVE_OFF = SCALE_OFF + (F16 ? 4 * SCALE_B : 0);   // [4 blocks][4] words, a bit for every key
-    static constexpr int QS_OFF = LIVE_OFF + 64;                      // [256] 2^-k of a column's q
-    static constexpr int BAR_OFF = QS_OFF + 1024;
-    static constexpr int SMEM = BAR_OFF + 256 + 1024;                 // + alignment of the base to 1024
+    static constexpr int QS_OFF = LIVE_OFF + 64;                           // [256] 2^-k of a column's q
+    static constexpr int ITEM_OFF = QS_OFF + 1024;                         // [2] ChunkItem
+    static constexpr int BAR_OFF = ITEM_OFF + 2 * 64;
+    static constexpr int SMEM = BAR_OFF + 256 + 1024;                      // + alignment of the base to 1024
+    static_assert(SMEM <= 227 * 1024, "shared memory");
     static constexpr int S_COL = 0, O_COL = 256;           // tensor memory columns of tile 0; tile 1: + 128
+};
+
+// What the softmax and product roles need of an item.
+struct ChunkItem {
+    int row0, kv, n;            // the sequence
+    int tile, head, cols;
+    int sinks, lo, keys;        // virtual positions (PagedSpan)
+    int b0, b1, tiles;          // this CTA's blocks [b0, b1) of tiles; b1 == b0: no more items
+    int first;                  // the CTA's first item
+    int lim[2];                 // where the blocks end that tile 0 / 1 sees something of, at most b1
+    int last_cta;               // the CTA that has the item's last block
 };
 
 constexpr int kChunkThreads = 16 * 32;
 constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 12;
+constexpr int kChunkCubic = 1, kChunkCubicOf = 4;   // pairs of weights by the cubic, of so many
 // Registers a thread: 128 at launch; 256 softmax threads take 184, the other 256 keep 72
 // (184 + 72 = 2 x 128: what one half gives up is what the other asks for).
 constexpr int kChunkRegsSoftmax = 184, kChunkRegsOther = 72;
@@ -124,6 +147,21 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int c1, int c2, int c3, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Byte offset of 16-byte piece c of row r in a 128-row tile: 64 dimensions (128 bytes) to a
@@ -133,7 +171,7 @@ __device__ __forceinline__ uint32_t sw128_at(int r, int c)
     return static_cast<uint32_t>((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// A CTA's walk over its share of the list of blocks; every role keeps its own.
+// A CTA's walk over its share of the list of blocks.
 template <int COLS, int TILE>
 struct ItemWalk {
     SplitItem it;
@@ -152,7 +190,7 @@ struct ItemWalk {
         long long in = st.in_seq;
         for (it.tile = 0;; ++it.tile)
         {
-            it.w = paged_span(a, it.q, it.tile * COLS, COLS);
+            it.w = paged_span<16>(a, it.q, it.tile * COLS, COLS);
             it.tiles = split_tiles<TILE>(it.w.n);
             if (in < static_cast<long long>(it.tiles) * a.c.kv_heads) break;
             if ((it.tile + 1) * COLS >= it.q.n * a.group) return false;   // (the arrays changed under the call)
@@ -188,7 +226,7 @@ struct ItemWalk {
                 } while (it.seq < a.b.num_seqs && (!paged_seq(a.b, it.seq, a.c.page_size, nullptr, it.q) || it.q.n == 0));
                 if (it.seq >= a.b.num_seqs) return false;   // (the arrays changed under the call)
             }
-            it.w = paged_span(a, it.q, it.tile * COLS, COLS);
+            it.w = paged_span<16>(a, it.q, it.tile * COLS, COLS);
             it.tiles = split_tiles<TILE>(it.w.n);
         }
         set(a);
@@ -208,8 +246,70 @@ struct ItemWalk {
     }
 };
 
+// Two fp32 at once.
+__device__ __forceinline__ uint64_t f2(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Largest of three; a NaN among them comes out.
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair on the multiply-add units: x = n + f, |f| <= 1/2, and a cubic that
+// is within 7.5e-5 of 2^f (equal ripple of the relative error; the weights it makes
+// are rounded to 2^-8 or 2^-11). For x in [-inf, 126); below -126 it stays at 2^-126.
+__device__ __forceinline__ uint64_t f2_exp2_cubic(uint64_t x)
+{
+    float a, b;
+    f2_get(x, a, b);
+    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t magic = f2(12582912.f, 12582912.f);   // 1.5 * 2^23: the sum's low bits are n
+    const uint64_t r = f2_add(x, magic);
+    const uint64_t f = f2_add(x, f2_mul(f2_add(r, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f)));
+    uint64_t y = f2_fma(f, f2(0.05517149f, 0.05517149f), f2(0.24261094f, 0.24261094f));
+    y = f2_fma(y, f, f2(0.69326099f, 0.69326099f));
+    y = f2_fma(y, f, f2(0.99992808f, 0.99992808f));
+    float n0, n1;
+    f2_get(r, n0, n1);
+    f2_get(y, a, b);
+    return f2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23)),
+              __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23)));
+}
+
+// Fetching by TMA: tensor maps of K and V over (dim, page, head, row), the last three in
+// the order of their strides; where[i]: the coordinate (1..3) of row, head and page.
+struct ChunkTma {
+    CUtensorMap k, v;
+    int on;
+    int row_c, head_c, page_c;
+};
+
 template <typename CT, int D>
-__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const PagedAttnArgs a)
+__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const PagedAttnArgs a, const __grid_constant__ ChunkTma tma)
 {
     using E = ChunkEngine<CT, D>;
     using Walk = ItemWalk<256, 128>;
@@ -219,10 +319,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     unsigned char* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     const uint32_t sm = smem_u32(smem);
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + E::BAR_OFF);
-    uint64_t* const kv_full = bars;               // [SLOTS] 128 loading threads
-    uint64_t* const kv_empty = kv_full + SLOTS;   // [SLOTS] products that read it are done
-    uint64_t* const q_full = kv_empty + SLOTS;    // 128
-    uint64_t* const q_empty = q_full + 1;         // products with q are done, qscale was read (256)
+    uint64_t* const kv_full = bars;               // [4] the block is in operand layout
+    uint64_t* const kv_empty = kv_full + 4;       // [4] products that read it are done
+    uint64_t* const st_full = kv_empty + 4;       // [3] codes are in the staging ring; bf16: [0] a block to be mended
+    uint64_t* const st_empty = st_full + 3;       // [3] codes were read (4 warps)
+    uint64_t* const q_full = st_empty + 3;        // q and the item's description are there (128)
+    uint64_t* const q_empty = q_full + 1;         // products with q are done, the description was read (256)
     uint64_t* const s_full = q_empty + 1;         // [2] scores are there
     uint64_t* const p_full = s_full + 2;          // [2] weights are there (128), output rescaled
     uint64_t* const o_full = p_full + 2;          // [2] weights times values added
@@ -230,8 +332,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     int* const pv_skip = reinterpret_cast<int*>(done + 1);   // [2] this block's product was taken by the softmax warps
     uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(pv_skip + 2);
     float* const qscale = reinterpret_cast<float*>(smem + E::QS_OFF);
+    ChunkItem* const items_s = reinterpret_cast<ChunkItem*>(smem + E::ITEM_OFF);
     volatile uint32_t* const live_w = reinterpret_cast<volatile uint32_t*>(smem + E::LIVE_OFF);
     __shared__ long long scan[kChunkThreads / 32 + 1];
+    static_assert(sizeof(ChunkItem) == 64, "item ring");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (warp == kChunkMmaWarp)
@@ -241,20 +345,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     }
     if (tid == 0)
     {
-        for (int i = 0; i < SLOTS; ++i)
+        // (bf16 blocks by TMA: one arrival, of the thread that announces the bytes)
+        for (int i = 0; i < 4; ++i)
         {
-            mbar_init(&kv_full[i], 128);
+            mbar_init(&kv_full[i], (!F16 && tma.on) ? 1 : 128);
             mbar_init(&kv_empty[i], 1);
+        }
+        for (int i = 0; i < 3; ++i)
+        {
+            mbar_init(&st_full[i], 1);
+            mbar_init(&st_empty[i], 4);
         }
         mbar_init(q_full, 128);
         mbar_init(q_empty, 1 + 256);
-        mbar_init(done, 1);
         for (int i = 0; i < 2; ++i)
         {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
             mbar_init(&o_full[i], 1);
         }
+        mbar_init(done, 1);
         fence_mbar_init();
     }
     tc_fence_before();
@@ -263,25 +373,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     const uint32_t tmem = *s_tmem;
     pdl_wait();
     pdl_launch();
-    const SplitStart st = split_start<256, 128, kChunkThreads>(a, scan);
-    PagedJoin* const desc = static_cast<PagedJoin*>(a.work) + blockIdx.x;
-    if (tid == 0) desc->count = 0;   // (rewritten below by the same thread)
+    if (tid == 0) static_cast<PagedJoin*>(a.work)[blockIdx.x].count = 0;   // (rewritten below by the same thread)
 
-    Walk w;
-    bool more = w.open(a, st);
+    const SplitStart st = split_start<256, 128, kChunkThreads, 16>(a, scan);
     if (warp >= kChunkLoadWarp && warp < kChunkMmaWarp)
     {
         // ---------------- loads ----------------
         regs_dec<kChunkRegsOther>();
         const int lt = tid - kChunkLoadWarp * 32, lw = lt >> 5;
+        Walk w;
+        bool more = w.open(a, st);
         int n = 0;             // slots filled
-        int blk = 0;           // blocks loaded (index of the scale ring)
-        int items = 0;
+        int blk = 0;           // blocks (index of the scale ring)
+        int items = 0, mended = 0;
         bool ok_all = true;
-        for (; more && ok_all; more = w.next(a), ++items)
+        for (;; ++items)
         {
+            if (items) ok_all = ok_all && mbar_wait(q_empty, (items - 1) & 1, a.c.status, kPagedTimeout);
+            if (lt == 0)
+            {
+                ChunkItem d;
+                d.row0 = w.it.q.row0; d.kv = w.it.q.kv; d.n = w.it.q.n;
+                d.tile = w.it.tile; d.head = w.it.head; d.cols = w.it.cols;
+                d.sinks = w.it.w.sinks; d.lo = w.it.w.lo; d.keys = w.it.w.n;
+                d.b0 = w.b0; d.b1 = w.b1; d.tiles = w.it.tiles;
+                d.first = w.first;
+                d.lim[0] = min(w.b1, w.blocks(a, 0));
+                d.lim[1] = min(w.b1, w.blocks(a, 1));
+                d.last_cta = static_cast<int>((w.start + w.it.tiles - 1) / max(1ll, st.share));
+                if (!more || !ok_all) d.b1 = d.b0;
+                items_s[items & 1] = d;
+            }
+            if (!more || !ok_all)
+            {
+                mbar_arrive(q_full);
+                break;
+            }
             // q: rows of the two tiles, 256 columns, zero where there is no column.
-            if (items) ok_all = mbar_wait(q_empty, (items - 1) & 1, a.c.status, kPagedTimeout);
             constexpr int QP = E::RB / 16;   // 16-byte pieces of a row
             if constexpr (!F16)
             {
@@ -299,120 +427,268 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             else
             {
                 // As f16, times the power of two that brings the column's largest magnitude to [2^14, 2^15).
-                constexpr int LPC = QP;   // lanes of a column
-                for (int x = lt; x < 256 * QP; x += 128)
+                constexpr int U = 4;
+#pragma unroll 1
+                for (int x0 = lt; x0 < 256 * QP; x0 += 128 * U)
                 {
-                    const int c = x / QP, p = x % QP;
-                    float v[8];
-                    load_row<__nv_bfloat16, 8>(a.q, split_q_at(a, w.it, 256, min(c, w.it.cols - 1)) + p * 8, v);
-                    uint32_t m = 0;
+                    uint4 raw[U];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+                    for (int y = 0; y < U; ++y)
                     {
-                        if (c >= w.it.cols) v[e] = 0.f;
-                        m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+                        const int c = (x0 + 128 * y) / QP, p = (x0 + 128 * y) % QP;
+                        raw[y] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
+                                                                     split_q_at(a, w.it, 256, min(c, w.it.cols - 1)) + p * 8));
+                        if (c >= w.it.cols) raw[y] = make_uint4(0, 0, 0, 0);
                     }
 #pragma unroll
-                    for (int o = 1; o < LPC; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    const uint32_t down = (min(max(m >> 23, 16u), 254u) - 14u) << 23;
-                    const float up = __uint_as_float((254u << 23) - down);
-                    if (p == 0) qscale[c] = __uint_as_float(down);
-                    *reinterpret_cast<uint4*>(smem + E::Q_OFF + (c >> 7) * E::TILE_B + sw128_at(c & 127, p)) =
-                        make_uint4(pack_f16(v[0] * up, v[1] * up), pack_f16(v[2] * up, v[3] * up),
-                                   pack_f16(v[4] * up, v[5] * up), pack_f16(v[6] * up, v[7] * up));
+                    for (int y = 0; y < U; ++y)
+                    {
+                        const int c = (x0 + 128 * y) / QP, p = (x0 + 128 * y) % QP;
+                        const uint32_t ws[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
+                        uint32_t m = 0, h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) m = max(m, max((ws[e] << 16) & 0x7fffffffu, ws[e] & 0x7fff0000u));
+#pragma unroll
+                        for (int o = 1; o < QP; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const uint32_t down = (min(max(m >> 23, 16u), 254u) - 14u) << 23;
+                        const float up = __uint_as_float((254u << 23) - down);
+                        if (p == 0) qscale[c] = __uint_as_float(down);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            h[e] = pack_f16(__uint_as_float(ws[e] << 16) * up, __uint_as_float(ws[e] & 0xFFFF0000u) * up);
+                        *reinterpret_cast<uint4*>(smem + E::Q_OFF + (c >> 7) * E::TILE_B + sw128_at(c & 127, p)) =
+                            make_uint4(h[0], h[1], h[2], h[3]);
+                    }
                 }
             }
             fence_async_smem();
             mbar_arrive(q_full);
 
             const int* const table = a.b.table + w.it.seq * a.b.table_stride;
-            int pg_next = 0, row_next = 0;
-            auto look_up = [&](int b) {
-                const int u = b * 128 + lt;
+            auto find = [&](int b, int in_block, int& pg, int& row) {
+                const int u = b * 128 + in_block;
                 if (b >= w.b1 || u >= w.it.w.n) return;
                 const int j = split_key(w.it, u), x = a.page_shift >= 0 ? j >> a.page_shift : j / a.c.page_size;
-                row_next = j - x * a.c.page_size;
-                pg_next = __ldg(table + x);
+                row = j - x * a.c.page_size;
+                pg = __ldg(table + x);
             };
-            look_up(w.b0);
-            const int n_item = n;
-            for (int b = w.b0; b < w.b1 && ok_all; ++b, ++blk)
-            {
-                const bool there = b * 128 + lt < w.it.w.n;
-                const bool ok = there && pg_next >= 0 && pg_next < a.c.num_pages;
-                if (there && !ok) paged_status(a.c.status, kPagedBadPage);
-                const long long off = ok ? pg_next * a.c.page_stride + row_next * a.c.row_stride + w.it.head * a.c.head_stride : 0;
-                const uint32_t mask = __ballot_sync(0xffffffffu, ok);
-                if constexpr (F16)
+            constexpr int CPR = D * static_cast<int>(sizeof(CT)) / 16;   // 16-byte pieces of a row in memory
+            // Page and row: of this thread's key of a block, and (TMA) of the group of 16 that lane / 2 is of.
+            int pg = 0, row = 0, gpg = 0, grow = 0;
+            // Announces and fetches a block by TMA: lane 2 g (+ 1: the upper 64 dimensions of bf16 rows) takes group g.
+            auto fetch = [&](int b, int kv, uint32_t dst, uint64_t* bar) {
+                if (lane == 0) mbar_arrive_expect_tx(bar, 128 * D * static_cast<int>(sizeof(CT)));
+                __syncwarp();
+                constexpr int HALVES = (!F16 && D == 128) ? 2 : 1;
+                const int g = lane >> 1, half = lane & 1;
+                if (g < 8 && half < HALVES)
                 {
-                    const long long so = ok ? pg_next * a.c.s_page_stride + row_next * a.c.s_row_stride + w.it.head * a.c.s_head_stride : 0;
-                    float* const sc = reinterpret_cast<float*>(smem + E::SCALE_OFF + (blk & 3) * E::SCALE_B);
-                    const float vs = ok ? __ldg(a.c.v_scale + so) : 0.f;
-                    sc[lt] = ok ? __ldg(a.c.k_scale + so) : 0.f;
-                    sc[128 + lt] = vs * 64.f;
-                    sc[256 + lt] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(vs) >> 23) - 127, -100), 100));
+                    const bool ok = b * 128 + g * 16 < w.it.w.n && gpg >= 0 && gpg < a.c.num_pages;
+                    const int page = ok ? gpg : a.c.num_pages;   // (past the last page: zeros)
+                    const int c1 = tma.row_c == 1 ? grow : tma.head_c == 1 ? w.it.head : page;
+                    const int c2 = tma.row_c == 2 ? grow : tma.head_c == 2 ? w.it.head : page;
+                    const int c3 = tma.row_c == 3 ? grow : tma.head_c == 3 ? w.it.head : page;
+                    tma_load_4d(dst + (F16 ? g * 16 * D : half * 16384 + g * 2048), kv ? &tma.v : &tma.k, half * 64, c1, c2, c3, bar);
                 }
-                if (lane == 0) live_w[(blk & 3) * 4 + lw] = mask;
-                look_up(b + 1);
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv, ++n)
+                __syncwarp();
+            };
+            if constexpr (!F16)
+            {
+                if (tma.on)
                 {
-                    const int slot = n % SLOTS;
-                    const CT* const base = static_cast<const CT*>(kv ? a.c.v : a.c.k);
-                    constexpr int CPR = D * static_cast<int>(sizeof(CT)) / 16;   // pieces of a row in memory
-                    if constexpr (!F16)
+                    if (lw == 0)
                     {
-                        if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
-                        const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
+                        find(w.b0, (lane >> 1) * 16, gpg, grow);
+                        for (int b = w.b0; b < w.b1 && ok_all; ++b, ++blk)
+                        {
+                            const int left = w.it.w.n - b * 128;
+                            // live bits: 16 per group, two groups a word
+                            const bool page_ok = gpg >= 0 && gpg < a.c.num_pages;
+                            const int cnt = lane < 16 ? min(max(left - (lane >> 1) * 16, 0), 16) : 0;
+                            if (cnt && !page_ok) paged_status(a.c.status, kPagedBadPage);
+                            const uint32_t bits = page_ok ? (1u << cnt) - 1u : 0u;
+                            const uint32_t b_lo = __shfl_sync(0xffffffffu, bits, (lane & 3) * 4), b_hi = __shfl_sync(0xffffffffu, bits, (lane & 3) * 4 + 2);
+                            if (lane < 4) live_w[(blk & 3) * 4 + lane] = b_lo | (b_hi << 16);
+                            __syncwarp();
+                            const int mend = left < 128 && (left & 15);   // rows behind the last key came along
 #pragma unroll
-                        for (int x = 0; x < CPR; ++x)
-                        {
-                            const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
-                            const long long o = __shfl_sync(0xffffffffu, off, r) + c * 8;
-                            cp_async16_zfill(dst + sw128_at(lw * 32 + r, c), base + o, (mask >> r) & 1u);
-                        }
-                        cp_commit();
-                        if (n - n_item >= 2)
-                        {
-                            cp_wait<2>();
-                            fence_async_smem();
-                            mbar_arrive(&kv_full[(n - 2) % SLOTS]);
+                            for (int kv = 0; kv < 2; ++kv, ++n)
+                            {
+                                const int slot = n % SLOTS;
+                                if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                                const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
+                                if (kv && mend)
+                                {
+                                    // They may hold anything: zeros before the products see them.
+                                    fetch(b, kv, dst, &st_full[0]);
+                                    ok_all = ok_all && mbar_wait(&st_full[0], mended & 1, a.c.status, kPagedTimeout);
+                                    ++mended;
+                                    constexpr int QP = E::RB / 16;
+                                    for (int x = lane; x < (16 - (left & 15)) * QP; x += 32)
+                                        *reinterpret_cast<uint4*>(smem + E::RING_OFF + slot * E::TILE_B + sw128_at(left + x / QP, x % QP)) = make_uint4(0, 0, 0, 0);
+                                    fence_async_smem();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive(&kv_full[slot]);
+                                }
+                                else
+                                {
+                                    fetch(b, kv, dst, &kv_full[slot]);
+                                }
+                            }
+                            find(b + 1, (lane >> 1) * 16, gpg, grow);
                         }
                     }
                     else
                     {
-                        uint4 v[CPR];
+                        n += 2 * (w.b1 - w.b0);
+                        blk += w.b1 - w.b0;
+                    }
+                }
+                else
+                {
+                    find(w.b0, lt, pg, row);
+                    int sent = n;   // slots announced
+                    auto drain = [&]() {
+                        cp_wait<0>();
+                        fence_async_smem();
+                        for (; sent < n; ++sent) mbar_arrive(&kv_full[sent % SLOTS]);
+                    };
+                    for (int b = w.b0; b < w.b1 && ok_all; ++b, ++blk)
+                    {
+                        const bool there = b * 128 + lt < w.it.w.n;
+                        const bool ok = there && pg >= 0 && pg < a.c.num_pages;
+                        if (there && !ok) paged_status(a.c.status, kPagedBadPage);
+                        const long long off = ok ? pg * a.c.page_stride + row * a.c.row_stride + w.it.head * a.c.head_stride : 0;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+                        if (lane == 0) live_w[(blk & 3) * 4 + lw] = mask;
+                        find(b + 1, lt, pg, row);
 #pragma unroll
-                        for (int x = 0; x < CPR; ++x)
+                        for (int kv = 0; kv < 2; ++kv, ++n)
                         {
-                            const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
-                            const long long o = __shfl_sync(0xffffffffu, off, r) + c * 16;
-                            v[x] = ((mask >> r) & 1u) ? __ldg(reinterpret_cast<const uint4*>(base + o)) : make_uint4(0, 0, 0, 0);
+                            const int slot = n % SLOTS;
+                            const CT* const base = static_cast<const CT*>(kv ? a.c.v : a.c.k);
+                            if (n >= SLOTS && !mbar_try_wait(&kv_empty[slot], (n / SLOTS - 1) & 1))
+                            {
+                                drain();   // what was fetched is on its way before this waits
+                                ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                            }
+                            const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
+#pragma unroll 8
+                            for (int x = 0; x < CPR; ++x)
+                            {
+                                const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
+                                const long long o = __shfl_sync(0xffffffffu, off, r) + c * 8;
+                                cp_async16_zfill(dst + sw128_at(lw * 32 + r, c), base + o, (mask >> r) & 1u);
+                            }
+                            cp_commit();
+                            if (n - sent >= 2)
+                            {
+                                cp_wait<2>();
+                                fence_async_smem();
+                                mbar_arrive(&kv_full[sent % SLOTS]);
+                                ++sent;
+                            }
+                        }
+                    }
+                    drain();
+                }
+            }
+            else
+            {
+                // Codes to the staging ring two slots ahead, then to the operand ring as f16.
+                const int n0 = n, n1 = n + 2 * (w.b1 - w.b0);
+                int fb = w.b0;   // block of the next fetch
+                if (tma.on) find(fb, (lane >> 1) * 16, gpg, grow);
+                else find(fb, lt, pg, row);
+                auto ahead = [&](int x) {   // fetch slot x
+                    if (x < n1)
+                    {
+                        const int kv = (x - n0) & 1, sg = x % 3;
+                        if (tma.on)
+                        {
+                            if (lw == 0)
+                            {
+                                if (x >= 3) ok_all = ok_all && mbar_wait(&st_empty[sg], (x / 3 - 1) & 1, a.c.status, kPagedTimeout);
+                                fetch(fb, kv, sm + E::STAGE_OFF + sg * E::CODES_B, &st_full[sg]);
+                            }
+                            if (kv) find(++fb, (lane >> 1) * 16, gpg, grow);
+                        }
+                        else
+                        {
+                            const bool ok = fb * 128 + lt < w.it.w.n && pg >= 0 && pg < a.c.num_pages;
+                            const long long off = ok ? pg * a.c.page_stride + row * a.c.row_stride + w.it.head * a.c.head_stride : 0;
+                            const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+                            const CT* const base = static_cast<const CT*>(kv ? a.c.v : a.c.k);
+#pragma unroll
+                            for (int y = 0; y < CPR; ++y)
+                            {
+                                const int idx = y * 32 + lane, r = idx / CPR, c = idx % CPR;
+                                const long long o = __shfl_sync(0xffffffffu, off, r) + c * 16;
+                                cp_async16_zfill(sm + E::STAGE_OFF + sg * E::CODES_B + (lw * 32 + r) * D + c * 16, base + o, (mask >> r) & 1u);
+                            }
+                            if (kv) find(++fb, lt, pg, row);
+                        }
+                    }
+                    cp_commit();
+                };
+                // Page of this thread's key, for its scales: of block b, a block ahead of the scales themselves.
+                int spg = 0, srow = 0;
+                find(w.b0, lt, spg, srow);
+                ahead(n0);
+                ahead(n0 + 1);
+                for (int b = w.b0; b < w.b1 && ok_all; ++b, ++blk)
+                {
+                    const bool there = b * 128 + lt < w.it.w.n;
+                    const bool ok = there && spg >= 0 && spg < a.c.num_pages;
+                    if (there && !ok) paged_status(a.c.status, kPagedBadPage);
+                    const long long so = ok ? spg * a.c.s_page_stride + srow * a.c.s_row_stride + w.it.head * a.c.s_head_stride : 0;
+                    const float ks = ok ? __ldg(a.c.k_scale + so) : 0.f, vs = ok ? __ldg(a.c.v_scale + so) : 0.f;
+                    const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+                    find(b + 1, lt, spg, srow);
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; ++kv, ++n)
+                    {
+                        const int slot = n % SLOTS, sg = n % 3;
+                        ahead(n + 2);
+                        if (tma.on) ok_all = ok_all && mbar_wait(&st_full[sg], (n / 3) & 1, a.c.status, kPagedTimeout);
+                        else
+                        {
+                            cp_wait<2>();
+                            __syncwarp();
                         }
                         if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                        const uint32_t src = sm + E::STAGE_OFF + sg * E::CODES_B;
                         unsigned char* const dst = smem + E::RING_OFF + slot * E::TILE_B;
 #pragma unroll
                         for (int x = 0; x < CPR; ++x)
                         {
-                            const int idx = x * 32 + lane, r = lw * 32 + idx / CPR, c = idx % CPR;
-                            *reinterpret_cast<uint4*>(dst + sw128_at(r, 2 * c)) =
-                                make_uint4(codes_f16<CT>(v[x].x), codes_f16<CT>(v[x].x >> 16), codes_f16<CT>(v[x].y), codes_f16<CT>(v[x].y >> 16));
-                            *reinterpret_cast<uint4*>(dst + sw128_at(r, 2 * c + 1)) =
-                                make_uint4(codes_f16<CT>(v[x].z), codes_f16<CT>(v[x].z >> 16), codes_f16<CT>(v[x].w), codes_f16<CT>(v[x].w >> 16));
+                            const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR, rr = lw * 32 + r;
+                            uint4 v = lds128(src + rr * D + c * 16);
+                            if (!((mask >> r) & 1u)) v = make_uint4(0, 0, 0, 0);   // (rows behind the last key)
+                            *reinterpret_cast<uint4*>(dst + sw128_at(rr, 2 * c)) =
+                                make_uint4(codes_f16<CT>(v.x), codes_f16<CT>(v.x >> 16), codes_f16<CT>(v.y), codes_f16<CT>(v.y >> 16));
+                            *reinterpret_cast<uint4*>(dst + sw128_at(rr, 2 * c + 1)) =
+                                make_uint4(codes_f16<CT>(v.z), codes_f16<CT>(v.z >> 16), codes_f16<CT>(v.w), codes_f16<CT>(v.w >> 16));
+                        }
+                        if (kv == 0)
+                        {
+                            // (entries of a block are written when the one four before it is long used)
+                            float* const sc = reinterpret_cast<float*>(smem + E::SCALE_OFF + (blk & 3) * E::SCALE_B);
+                            sc[lt] = ks;
+                            sc[128 + lt] = vs * 64.f;
+                            sc[256 + lt] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(vs) >> 23) - 127, -100), 100));
+                            if (lane == 0) live_w[(blk & 3) * 4 + lw] = mask;
                         }
                         fence_async_smem();
                         mbar_arrive(&kv_full[slot]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&st_empty[sg]);
                     }
                 }
-            }
-            if constexpr (!F16)
-            {
                 cp_wait<0>();
-                fence_async_smem();
-                for (int x = max(n_item, n - 2); x < n; ++x) mbar_arrive(&kv_full[x % SLOTS]);
             }
+            more = w.next(a);
         }
-        cp_wait<0>();
     }
     else if (warp >= kChunkMmaWarp)
     {
@@ -421,62 +697,71 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
         if (warp == kChunkMmaWarp && lane == 0)
         {
             constexpr uint32_t ID_QK = idesc_f16(!F16, false, 128, 128), ID_PV = idesc_f16(!F16, true, 128, D);
-            int nb = 0, items = 0;   // blocks before this item
+            int nb = 0;   // blocks before this item
             int p_seen[2] = {0, 0};
             bool ok = true;
             auto qk = [&](int i, int blk) {
                 const uint32_t q = sm + E::Q_OFF + i * E::TILE_B, k = sm + E::RING_OFF + ((2 * blk) % SLOTS) * E::TILE_B;
+                const uint64_t qd = sw128_desc(q, 16, 1024), kd = sw128_desc(k, 16, 1024);
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                 {
-                    const uint32_t o = (ks >> 2) * 16384 + (ks & 3) * 32;
-                    umma_f16_ss(tmem + E::S_COL + i * 128, sw128_desc(q + o, 16, 1024), sw128_desc(k + o, 16, 1024), ID_QK, ks ? 1u : 0u);
+                    const uint64_t o = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+                    umma_f16_ss(tmem + E::S_COL + i * 128, qd + o, kd + o, ID_QK, ks ? 1u : 0u);
                 }
                 umma_commit(&s_full[i]);
             };
             auto pv = [&](int i, int blk, bool add) {
-                const uint32_t v = sm + E::RING_OFF + ((2 * blk + 1) % SLOTS) * E::TILE_B;
+                const uint64_t vd = sw128_desc(sm + E::RING_OFF + ((2 * blk + 1) % SLOTS) * E::TILE_B, 16384, 1024);
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks)
-                    umma_f16_ts(tmem + E::O_COL + i * 128, tmem + E::S_COL + i * 128 + 64 + ks * 8,
-                                sw128_desc(v + ks * 2048, 16384, 1024), ID_PV, (add || ks) ? 1u : 0u);
+                    umma_f16_ts(tmem + E::O_COL + i * 128, tmem + E::S_COL + i * 128 + 64 + ks * 8, vd + ks * 128, ID_PV, (add || ks) ? 1u : 0u);
             };
             auto full = [&](int slot_n) {
                 ok = ok && mbar_wait_spin(&kv_full[slot_n % SLOTS], (slot_n / SLOTS) & 1, a.c.status, kPagedTimeout);
                 tc_fence_after();
             };
-            for (; more && ok; more = w.next(a), ++items)
+            for (int items = 0; ok; ++items)
             {
-                const int lim[2] = {min(w.b1, w.blocks(a, 0)), min(w.b1, w.blocks(a, 1))};
-                const int n_blk = w.b1 - w.b0;
-                ok = ok && mbar_wait_spin(q_full, items & 1, a.c.status, kPagedTimeout);
+                ok = mbar_wait_spin(q_full, items & 1, a.c.status, kPagedTimeout);
+                if (!ok) break;
+                const volatile ChunkItem& it = items_s[items & 1];
+                const int b0 = it.b0, n_blk = it.b1 - b0, lim[2] = {it.lim[0], it.lim[1]};
+                if (n_blk <= 0) break;
                 full(2 * nb);
                 if (!ok) break;
                 for (int i = 0; i < 2; ++i)
-                    if (w.b0 < lim[i]) qk(i, nb);
+                    if (b0 < lim[i]) qk(i, nb);
                 umma_commit(&kv_empty[(2 * nb) % SLOTS]);
                 if (n_blk == 1) umma_commit(q_empty);
                 for (int j = 0; j < n_blk && ok; ++j)
                 {
                     const int blk = nb + j;
-                    full(2 * blk + 1);
-                    if (j + 1 < n_blk) full(2 * blk + 2);
+                    const bool more = j + 1 < n_blk;
+                    bool v_there = false, k_there = false;
                     for (int i = 0; i < 2 && ok; ++i)
                     {
-                        if (w.b0 + j < lim[i])
+                        if (b0 + j < lim[i])
                         {
                             ok = mbar_wait_spin(&p_full[i], p_seen[i] & 1, a.c.status, kPagedTimeout);
                             ++p_seen[i];
+                            if (!v_there) full(2 * blk + 1);
+                            v_there = true;
                             if (!ok) break;
                             tc_fence_after();
                             if (F16 || !*reinterpret_cast<volatile int*>(&pv_skip[i])) pv(i, blk, j > 0);
                             umma_commit(&o_full[i]);
                         }
-                        if (j + 1 < n_blk && w.b0 + j + 1 < lim[i]) qk(i, blk + 1);
+                        if (more && b0 + j + 1 < lim[i])
+                        {
+                            if (!k_there) full(2 * blk + 2);
+                            k_there = true;
+                            if (ok) qk(i, blk + 1);
+                        }
                     }
                     if (!ok) break;
                     umma_commit(&kv_empty[(2 * blk + 1) % SLOTS]);
-                    if (j + 1 < n_blk) umma_commit(&kv_empty[(2 * blk + 2) % SLOTS]);
+                    if (more) umma_commit(&kv_empty[(2 * blk + 2) % SLOTS]);
                     if (j + 2 == n_blk) umma_commit(q_empty);
                 }
                 nb += n_blk;
@@ -493,43 +778,73 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
         const int i = warp >> 2, c_in = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + E::S_COL + i * 128 + lanes, to = tmem + E::O_COL + i * 128 + lanes;
-        float* const parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.work) + kSplitDescBytes);
-        int nb = 0, seen = 0, items = 0;   // blocks of earlier items; blocks of this tile; items
+        int nb = 0, seen = 0;   // blocks of earlier items; blocks of this tile
         bool ok = true;
-        for (; more && ok; more = w.next(a), ++items)
+        for (int items = 0;; ++items)
         {
-            const int lim = min(w.b1, w.blocks(a, i));
-            const int c = i * 128 + c_in, cc = w.it.tile * 256 + c, rw = cc / a.group;
-            const bool col = c < w.it.cols;
-            const int p = col ? w.it.q.kv - w.it.q.n + rw : -1;
-            // The tile's first and last positions.
-            const int p_lo = w.it.q.kv - w.it.q.n + (w.it.tile * 256 + i * 128) / a.group;
-            const int p_hi = w.it.q.kv - w.it.q.n + (w.it.tile * 256 + min(w.it.cols, i * 128 + 128) - 1) / a.group;
             ok = mbar_wait(q_full, items & 1, a.c.status, kPagedTimeout);
             if (!ok) break;
+            const ChunkItem it = items_s[items & 1];
+            const int c = i * 128 + c_in;
             const float fac = F16 ? a.scale_log2 * qscale[c] : a.scale_log2;
             mbar_arrive(q_empty);
+            if (it.b1 == it.b0) break;
+            const int lim = it.lim[i];
+            const bool col = c < it.cols;
+            const int p_0 = it.kv - it.n;
+            const int p = col ? p_0 + (it.tile * 256 + c) / a.group : -1;
+            // The tile's first and last positions.
+            const int p_lo = p_0 + (it.tile * 256 + i * 128) / a.group;
+            const int p_hi = p_0 + (it.tile * 256 + min(it.cols, i * 128 + 128) - 1) / a.group;
+            auto key = [&](int u) { return u < it.sinks ? u : it.lo + u - it.sinks; };
             float m = -INFINITY, l = 0.f;
-            for (int b = w.b0; b < lim && ok; ++b, ++seen)
+            for (int b = it.b0; b < lim && ok; ++b, ++seen)
             {
-                const int blk = nb + b - w.b0, ring = blk & 3, vslot = (2 * blk + 1) % SLOTS;
+                const int blk = nb + b - it.b0, ring = blk & 3, vslot = (2 * blk + 1) % SLOTS;
                 // (the values' barrier tells that the block's scales and bits are there too, and its slot
                 // cannot be filled anew before this tile's weights are out)
                 ok = mbar_wait(&kv_full[vslot], ((2 * blk + 1) / SLOTS) & 1, a.c.status, kPagedTimeout) &&
                      mbar_wait(&s_full[i], seen & 1, a.c.status, kPagedTimeout);
                 if (!ok) break;
                 tc_fence_after();
+                uint32_t r[128];   // scores, then (packed) weights
+                {
+                    uint32_t(&r0)[32] = *reinterpret_cast<uint32_t(*)[32]>(r);
+                    uint32_t(&r1)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 32);
+                    uint32_t(&r2)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 64);
+                    uint32_t(&r3)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 96);
+                    tmem_ld32(ts, r0);
+                    tmem_ld32(ts + 32, r1);
+                    tmem_ld32(ts + 64, r2);
+                    tmem_ld32(ts + 96, r3);
+                    tmem_ld32_wait(r0);
+                    tmem_ld32_wait(r1);
+                    tmem_ld32_wait(r2);
+                    tmem_ld32_wait(r3);
+                }
                 const float4* const sc = reinterpret_cast<const float4*>(smem + E::SCALE_OFF + ring * E::SCALE_B);
-                const int u0 = b * 128, j_first = split_key(w.it, u0), j_last = split_key(w.it, min(u0 + 127, w.it.w.n - 1));
+                const int u0 = b * 128, j_first = key(u0), j_last = key(min(u0 + 127, it.keys - 1));
                 uint32_t vis[4];   // what the column sees, a bit per key
 #pragma unroll
                 for (int x = 0; x < 4; ++x) vis[x] = live_w[ring * 4 + x];
                 const bool whole = (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu && p_lo >= 0 &&
                                    (!a.causal || (j_last <= p_lo && (a.window == 0 || j_first > p_hi - a.window || j_last < a.sinks)));
                 bool odd = false;
+                if constexpr (F16)
+                {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                    {
+                        const float4 k = sc[e];
+                        r[4 * e] = __float_as_uint(__uint_as_float(r[4 * e]) * k.x);
+                        r[4 * e + 1] = __float_as_uint(__uint_as_float(r[4 * e + 1]) * k.y);
+                        r[4 * e + 2] = __float_as_uint(__uint_as_float(r[4 * e + 2]) * k.z);
+                        r[4 * e + 3] = __float_as_uint(__uint_as_float(r[4 * e + 3]) * k.w);
+                    }
+                }
                 if (!whole)
                 {
-                    if (u0 >= w.it.w.sinks)   // one run of keys
+                    if (u0 >= it.sinks)   // one run of keys
                     {
                         const int hi = p < 0 ? -1 : a.causal ? min(p - j_first, 127) : 127;
                         const int lo = a.window > 0 && p - a.window + 1 > j_first ? p - a.window + 1 - j_first : 0;
@@ -537,12 +852,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         for (int x = 0; x < 4; ++x)
                         {
                             const int h = hi - 32 * x, f = lo - 32 * x;
-                            uint32_t in = h >= 31 ? 0xffffffffu : h < 0 ? 0u : (2u << h) - 1u;
-                            in &= f <= 0 ? 0xffffffffu : f > 31 ? 0u : 0xffffffffu << f;
-                            // (keys below the window may still be sinks)
-                            const int s = min(a.sinks - j_first - 32 * x, 32);
-                            if (a.window > 0 && s > 0) in |= (s >= 32 ? 0xffffffffu : (1u << s) - 1u) & (h >= 31 ? 0xffffffffu : h < 0 ? 0u : (2u << h) - 1u);
-                            vis[x] &= in;
+                            const uint32_t upto = h >= 31 ? 0xffffffffu : h < 0 ? 0u : (2u << h) - 1u;
+                            uint32_t in = f <= 0 ? 0xffffffffu : f > 31 ? 0u : 0xffffffffu << f;
+                            const int s = min(a.sinks - j_first - 32 * x, 32);   // (keys below the window may be sinks)
+                            if (a.window > 0 && s > 0) in |= s >= 32 ? 0xffffffffu : (1u << s) - 1u;
+                            vis[x] &= in & upto;
                         }
                     }
                     else
@@ -552,11 +866,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         {
                             uint32_t in = 0;
 #pragma unroll 1
-                            for (int y = 0; y < 32; ++y)
-                                in |= (paged_sees(a, p, split_key(w.it, u0 + 32 * x + y)) ? 1u : 0u) << y;
+                            for (int y = 0; y < 32; ++y) in |= (paged_sees(a, p, key(u0 + 32 * x + y)) ? 1u : 0u) << y;
                             vis[x] &= in;
                         }
                     }
+#pragma unroll
+                    for (int e = 0; e < 128; ++e)
+                        if (!((vis[e >> 5] >> (e & 31)) & 1u)) r[e] = 0xff800000u;   // -inf
                     if constexpr (!F16)
                     {
                         // 0 times an infinity or NaN is NaN, so a block that some column must not see all of and
@@ -578,71 +894,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         odd = any != 0;
                     }
                 }
-                // Scores of chunk x (32 keys), in units that `fac` makes powers of two; -inf where not seen.
-                auto scores = [&](int x, uint32_t (&r)[32]) {
-                    if constexpr (F16)
-                    {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                        {
-                            const float4 k = sc[x * 8 + e];
-                            r[4 * e] = __float_as_uint(__uint_as_float(r[4 * e]) * k.x);
-                            r[4 * e + 1] = __float_as_uint(__uint_as_float(r[4 * e + 1]) * k.y);
-                            r[4 * e + 2] = __float_as_uint(__uint_as_float(r[4 * e + 2]) * k.z);
-                            r[4 * e + 3] = __float_as_uint(__uint_as_float(r[4 * e + 3]) * k.w);
-                        }
-                    }
-                    if (!whole)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!((vis[x] >> e) & 1u)) r[e] = 0xff800000u;
-                };
-                auto top_of = [&](int x, const uint32_t (&r)[32]) {
+                float top;
+                {
                     float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
-                    if constexpr (F16)
-                    {
+                    auto z = [&](int e, float ev) { return F16 ? fmaf(__uint_as_float(r[e]), fac, ev) : __uint_as_float(r[e]); };
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                        {
-                            const float4 v = sc[64 + x * 8 + e];
-                            t0 = fmaxf(t0, fmaf(__uint_as_float(r[4 * e]), fac, v.x));
-                            t1 = fmaxf(t1, fmaf(__uint_as_float(r[4 * e + 1]), fac, v.y));
-                            t2 = fmaxf(t2, fmaf(__uint_as_float(r[4 * e + 2]), fac, v.z));
-                            t3 = fmaxf(t3, fmaf(__uint_as_float(r[4 * e + 3]), fac, v.w));
-                        }
-                        return fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
-                    }
-                    else
+                    for (int e = 0; e < 128; e += 8)
                     {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
+                        float4 v0 = make_float4(0, 0, 0, 0), v1 = v0;
+                        if constexpr (F16)
                         {
-                            t0 = fmaxf(t0, __uint_as_float(r[4 * e]));
-                            t1 = fmaxf(t1, __uint_as_float(r[4 * e + 1]));
-                            t2 = fmaxf(t2, __uint_as_float(r[4 * e + 2]));
-                            t3 = fmaxf(t3, __uint_as_float(r[4 * e + 3]));
+                            v0 = sc[64 + e / 4];
+                            v1 = sc[65 + e / 4];
                         }
-                        return fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                        t0 = max3_nan(t0, z(e, v0.x), z(e + 1, v0.y));
+                        t1 = max3_nan(t1, z(e + 2, v0.z), z(e + 3, v0.w));
+                        t2 = max3_nan(t2, z(e + 4, v1.x), z(e + 5, v1.y));
+                        t3 = max3_nan(t3, z(e + 6, v1.z), z(e + 7, v1.w));
                     }
-                };
-                uint32_t ra[32], rb[32];
-                tmem_ld32(ts, ra);
-                tmem_ld32(ts + 32, rb);
-                tmem_ld32_wait(ra);
-                tmem_ld32_wait(rb);
-                scores(0, ra);
-                scores(1, rb);
-                float top = fmaxf(top_of(0, ra), top_of(1, rb));
-                tmem_ld32(ts + 64, ra);
-                tmem_ld32(ts + 96, rb);
-                tmem_ld32_wait(ra);
-                tmem_ld32_wait(rb);
-                scores(2, ra);
-                scores(3, rb);
-                top = fmaxf(top, fmaxf(top_of(2, ra), top_of(3, rb)));
-                if constexpr (!F16) top = top == -INFINITY ? top : top * fac;
-                // A new reference only where the maximum has grown by more than 2^8 (or there was none).
-                const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+                    top = max3_nan(max3_nan(t0, t1, t2), t3, t3);
+                    if constexpr (!F16) top *= fac;
+                }
+                if (top == INFINITY) top = __int_as_float(0x7fffffff);   // inf - inf
+                // A new reference only where the maximum has grown by more than 2^8 (or there was none); a NaN becomes one.
+                const bool grow = !(top <= m + 8.f) && !(top == -INFINITY);
                 float corr = 1.f;
                 if (grow)
                 {
@@ -650,80 +925,90 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     l *= corr;
                     m = top;
                 }
-                if (b > w.b0 && __any_sync(0xffffffffu, grow))
+                if (b > it.b0 && __any_sync(0xffffffffu, grow))
                 {
                     ok = mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
                     tc_fence_after();
 #pragma unroll 1
-                    for (int x = 0; x < D / 32; ++x)
+                    for (int x = 0; x < D / 16; ++x)
                     {
-                        uint32_t o[32];
-                        tmem_ld32(to + 32 * x, o);
-                        tmem_ld32_wait(o);
+                        uint32_t o[16];
+                        tmem_ld16(to + 16 * x, o);
+                        tmem_ld_wait(o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                        tmem_st32(to + 32 * x, o);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tmem_st16(to + 16 * x, o);
                     }
                 }
                 const float mm = m == -INFINITY ? 0.f : m;
-                float l0 = 0.f, l1 = 0.f;
-                // The weights of chunks x and x + 1 as the next product's operand, 32 words.
-                auto weights = [&](int x, const uint32_t (&r0)[32], const uint32_t (&r1)[32]) {
-                    uint32_t out[32];
+                const bool cubic = whole && __all_sync(0xffffffffu, m > -INFINITY);
+                const uint64_t fac2 = f2(fac, fac), mm2 = f2(-mm, -mm);
+                uint64_t sum0 = 0, sum1 = 0;   // (pairs of zeros)
+                // Weights; every fourth pair by the cubic: the special-function units make 4 of 2^x a
+                // cycle and quarter of the SM, two tiles' blocks take them 2048 cycles, as long as the products.
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
+                for (int e = 0; e < 64; ++e)
+                {
+                    const uint64_t x = f2_fma(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), fac2, mm2);
+                    uint64_t y;
+                    float w0, w1;
+                    if (e % kChunkCubicOf < kChunkCubic && cubic)
+                    {
+                        y = f2_exp2_cubic(x);
+                    }
+                    else
+                    {
+                        f2_get(x, w0, w1);
+                        y = f2(ex2(w0), ex2(w1));
+                    }
+                    if (e & 1) sum1 = f2_add(sum1, y);
+                    else sum0 = f2_add(sum0, y);
+                    if constexpr (F16)
+                    {
+                        const float2 v = reinterpret_cast<const float2*>(sc)[64 + e];
+                        y = f2_mul(y, f2(v.x, v.y));
+                    }
+                    f2_get(y, w0, w1);
+                    if constexpr (F16)
+                    {
+                        // (a scale of NaN must not meet a weight of zero that stands for "not seen")
+                        if (!whole)
                         {
-                            const uint32_t s0 = h ? r1[2 * e] : r0[2 * e], s1 = h ? r1[2 * e + 1] : r0[2 * e + 1];
-                            float w0 = ex2(fmaf(__uint_as_float(s0), fac, -mm)), w1 = ex2(fmaf(__uint_as_float(s1), fac, -mm));
-                            l0 += w0;
-                            l1 += w1;
-                            if constexpr (F16)
-                            {
-                                const float2 v = reinterpret_cast<const float2*>(sc)[64 + (x + h) * 16 + e];
-                                w0 *= v.x;
-                                w1 *= v.y;
-                                // (a scale of NaN must not meet a weight of zero that stands for "not seen")
-                                if (!whole && !((vis[x + h] >> (2 * e)) & 1u)) w0 = 0.f;
-                                if (!whole && !((vis[x + h] >> (2 * e + 1)) & 1u)) w1 = 0.f;
-                                out[16 * h + e] = pack_f16(w0, w1);
-                            }
-                            else
-                            {
-                                out[16 * h + e] = pack_bf16(w0, w1);
-                            }
+                            if (!((vis[e >> 4] >> (2 * e & 31)) & 1u)) w0 = 0.f;
+                            if (!((vis[e >> 4] >> ((2 * e + 1) & 31)) & 1u)) w1 = 0.f;
                         }
-                    tmem_st32(ts + 64 + 16 * x, out);
-                };
-                weights(2, ra, rb);   // over scores that are in registers
-                tmem_ld32(ts, ra);
-                tmem_ld32(ts + 32, rb);
-                tmem_ld32_wait(ra);
-                tmem_ld32_wait(rb);
-                scores(0, ra);
-                scores(1, rb);
-                weights(0, ra, rb);
-                l += l0 + l1;
+                        r[e] = pack_f16(w0, w1);
+                    }
+                    else
+                    {
+                        r[e] = pack_bf16(w0, w1);
+                    }
+                    if (e == 31) tmem_st32(ts + 64, *reinterpret_cast<uint32_t(*)[32]>(r));
+                }
+                tmem_st32(ts + 96, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+                float s0, s1, s2, s3;
+                f2_get(sum0, s0, s1);
+                f2_get(sum1, s2, s3);
+                l += (s0 + s1) + (s2 + s3);
                 tmem_st_wait();
                 if constexpr (!F16)
                 {
                     if (odd)
                     {
                         // o += p v, key by key, for what the column sees.
-                        if (b > w.b0) ok = ok && mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
+                        if (b > it.b0) ok = ok && mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
                         tc_fence_after();
                         const uint32_t vbase = sm + E::RING_OFF + vslot * E::TILE_B;
                         auto vis_at = [&](int x) { return x == 0 ? vis[0] : x == 1 ? vis[1] : x == 2 ? vis[2] : vis[3]; };
 #pragma unroll 1
-                        for (int x = 0; x < D / 32; ++x)
+                        for (int x = 0; x < D / 16; ++x)
                         {
-                            uint32_t o[32];
-                            tmem_ld32(to + 32 * x, o);
-                            tmem_ld32_wait(o);
-                            if (b == w.b0)
+                            uint32_t o[16];
+                            tmem_ld16(to + 16 * x, o);
+                            tmem_ld_wait(o);
+                            if (b == it.b0)
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = 0;
+                                for (int e = 0; e < 16; ++e) o[e] = 0;
 #pragma unroll 1
                             for (int k = 0; k < 128; ++k)
                             {
@@ -734,9 +1019,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                                 if ((vis_at(k >> 5) >> (k & 31)) & 1u)
                                 {
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e)
+                                    for (int e = 0; e < 2; ++e)
                                     {
-                                        const uint4 v = lds128(vbase + sw128_at(k, 4 * x + e));
+                                        const uint4 v = lds128(vbase + sw128_at(k, 2 * x + e));
                                         const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                                         for (int y = 0; y < 4; ++y)
@@ -750,7 +1035,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                                 }
                                 __syncwarp();
                             }
-                            tmem_st32(to + 32 * x, o);
+                            tmem_st16(to + 16 * x, o);
                         }
                         tmem_st_wait();
                     }
@@ -761,21 +1046,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             }
             if (!ok) break;
             // ---- the item's output, or this CTA's part of it ----
-            const bool any = lim > w.b0;
+            const bool any = lim > it.b0;
             if (any)
             {
                 ok = mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
                 if (!ok) break;
                 tc_fence_after();
             }
-            const bool complete = w.complete();
-            const int part_slot = 2 * blockIdx.x + (w.first ? 0 : 1);
-            float* const part = parts + static_cast<long long>(part_slot) * (256 * (D + 2));
+            const bool complete = it.b0 == 0 && it.b1 == it.tiles;
+            const int part_slot = 2 * blockIdx.x + (it.first ? 0 : 1);
+            float* const part = reinterpret_cast<float*>(static_cast<unsigned char*>(a.work) + kSplitDescBytes) +
+                                static_cast<long long>(part_slot) * (256 * (D + 2));
             const float inv = l == 0.f ? 0.f : E::OUT / l;
-            if (i * 128 < w.it.cols)
+            if (i * 128 < it.cols)
             {
                 if (col && !complete) reinterpret_cast<float2*>(part)[c] = make_float2(m, l);
-                const long long at = (w.it.q.row0 + rw) * a.o_row_stride + (w.it.head * a.group + cc - rw * a.group) * a.o_head_stride;
+                const int cc = it.tile * 256 + c, rw = cc / a.group;
+                const long long at = (it.row0 + rw) * a.o_row_stride + (it.head * a.group + cc - rw * a.group) * a.o_head_stride;
 #pragma unroll 1
                 for (int x = 0; x < D / 32; ++x)
                 {
@@ -808,21 +1095,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 }
                 tc_fence_before();
             }
-            if (tid == 0 && !complete && w.b0 == 0)
+            if (tid == 0 && !complete && it.b0 == 0)
             {
-                const long long x_last = w.start + w.it.tiles - 1;   // global index of the item's last block
                 PagedJoin d;
-                d.count = static_cast<int>(x_last / st.share) - static_cast<int>(blockIdx.x) + 1;
+                d.count = it.last_cta - static_cast<int>(blockIdx.x) + 1;
                 d.first_slot = part_slot;
                 d.first_cta = blockIdx.x;
-                d.row0 = w.it.q.row0;
-                d.col0 = w.it.tile * 256;
-                d.cols = w.it.cols;
-                d.head = w.it.head;
+                d.row0 = it.row0;
+                d.col0 = it.tile * 256;
+                d.cols = it.cols;
+                d.head = it.head;
                 d.pad = 0;
-                *desc = d;
+                static_cast<PagedJoin*>(a.work)[blockIdx.x] = d;
             }
-            nb += w.b1 - w.b0;
+            nb += it.b1 - it.b0;
         }
     }
     __syncwarp();

@@ -2,7 +2,9 @@
 // (hy_paged_attn_f32.cu, hy_paged_attn_bf16.cu).
 #pragma once
 
+#include <algorithm>
 #include <atomic>
+#include <cstring>
 #include <type_traits>
 
 #include "hy_decode.h"
@@ -86,12 +88,63 @@ cudaError_t launch_split(const PagedAttnArgs& a, int device, cudaStream_t s)
     return e;
 }
 
+// Tensor maps of K and V for blocks fetched 16 rows of a page at a time. Pages that do not
+// hold a multiple of 16 rows, and layouts that the maps cannot express, are copied row by row.
+template <typename CT, int D>
+ChunkTma chunk_tma(const PagedAttnArgs& a)
+{
+    using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const EncodeFn encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<EncodeFn>(fn);
+    }();
+    ChunkTma t;
+    std::memset(&t, 0, sizeof t);
+    if (!encode || a.c.page_size % 16 != 0) return t;
+    constexpr int E = sizeof(CT);
+    struct Dim {
+        long long stride;
+        cuuint64_t size;
+        cuuint32_t box;
+        int* where;
+    } dims[3] = {{a.c.row_stride, static_cast<cuuint64_t>(a.c.page_size), 16, &t.row_c},
+                 {a.c.head_stride, static_cast<cuuint64_t>(a.c.kv_heads), 1, &t.head_c},
+                 {a.c.page_stride, static_cast<cuuint64_t>(a.c.num_pages), 1, &t.page_c}};
+    std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+    const cuuint32_t inner = E == 1 ? D : 64;   // 128 bytes of a bf16 row, a row of codes
+    cuuint64_t size[4] = {D}, stride[3];
+    cuuint32_t box[4] = {inner}, step[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 3; ++i)
+    {
+        if (dims[i].stride <= 0 || dims[i].stride * E >= (1ll << 40)) return t;
+        size[i + 1] = dims[i].size;
+        stride[i] = static_cast<cuuint64_t>(dims[i].stride) * E;
+        box[i + 1] = dims[i].box;
+        *dims[i].where = i + 1;
+    }
+    for (int v = 0; v < 2; ++v)
+        if (encode(v ? &t.v : &t.k, E == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v ? a.c.v : a.c.k,
+                   size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   E == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return t;
+    t.on = 1;
+    return t;
+}
+
 template <typename CT, int D>
 cudaError_t launch_chunk(const PagedAttnArgs& a, int device, cudaStream_t s)
 {
     using E = ChunkEngine<CT, D>;
+    const ChunkTma tma = chunk_tma<CT, D>(a);
     cudaError_t e = allow_smem<paged_chunk_kernel<CT, D>>(E::SMEM, device);
-    if (e == cudaSuccess) e = launch_pdl(paged_chunk_kernel<CT, D>, dim3(148), kChunkThreads, E::SMEM, s, a);
+    if (e == cudaSuccess) e = launch_pdl(paged_chunk_kernel<CT, D>, dim3(148), kChunkThreads, E::SMEM, s, a, tma);
     if (e == cudaSuccess) e = launch_pdl(paged_join_kernel<E>, dim3(148, E::COLS / 8), kJoinThreads, 0, s, a);
     return e;
 }
