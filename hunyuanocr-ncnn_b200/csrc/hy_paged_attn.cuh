@@ -1329,4 +1329,75 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + d, r);
 }
 
+// The same for tiles of 256 columns, where many items are shared by two or three
+// CTAs: blockIdx.y takes an eighth of the item's D / 4 x columns float4s, a thread two of them.
+template <typename E>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_wide_kernel(const PagedAttnArgs a)
+{
+    constexpr int COLS = E::COLS, D = E::D, PART = COLS * (D + 2), LANES = D / 4, N = COLS * LANES / 8 / kJoinThreads;
+    static_assert(N >= 1 && N * 8 * kJoinThreads == COLS * LANES, "shares");
+    pdl_wait();
+    const PagedJoin j = static_cast<const PagedJoin*>(a.work)[blockIdx.x];
+    if (j.count == 0) return;
+    const float* const parts = reinterpret_cast<const float*>(static_cast<const unsigned char*>(a.work) + kSplitDescBytes);
+    float M[N], L[N];
+    float4 o[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+    {
+        M[x] = -INFINITY;
+        L[x] = 0.f;
+        o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int e0 = blockIdx.y * (N * kJoinThreads) + threadIdx.x;   // element x: e0 + x * kJoinThreads
+    if (e0 / LANES >= j.cols) return;
+    constexpr int U = 4;   // parts in flight
+    for (int k0 = 0; k0 < j.count; k0 += U)
+    {
+        float2 w[U][N];
+        float4 v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int k = min(k0 + u, j.count - 1);
+            const float* const p = parts + static_cast<long long>(k == 0 ? j.first_slot : 2 * (j.first_cta + k)) * PART;
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+            {
+                const int e = e0 + x * kJoinThreads, c = min(e / LANES, j.cols - 1);
+                if (k0 + u >= j.count) continue;
+                w[u][x] = reinterpret_cast<const float2*>(p)[c];
+                v[u][x] = *reinterpret_cast<const float4*>(p + 2 * COLS + c * D + e % LANES * 4);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            if (k0 + u >= j.count) break;
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+            {
+                const float top = fmaxf(M[x], w[u][x].x);
+                const float f0 = M[x] == top ? 1.f : ex2(M[x] - top), f = w[u][x].x == top ? 1.f : ex2(w[u][x].x - top);
+                L[x] = L[x] * f0 + f * w[u][x].y;
+                o[x].x = o[x].x * f0 + f * v[u][x].x;
+                o[x].y = o[x].y * f0 + f * v[u][x].y;
+                o[x].z = o[x].z * f0 + f * v[u][x].z;
+                o[x].w = o[x].w * f0 + f * v[u][x].w;
+                M[x] = top;
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+    {
+        const int e = e0 + x * kJoinThreads, c = e / LANES;
+        if (c >= j.cols) continue;
+        const float inv = L[x] == 0.f ? 0.f : E::OUT / L[x];
+        const float r[4] = {o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv};
+        const int cc = j.col0 + c, rw = cc / a.group;
+        store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + e % LANES * 4, r);
+    }
+}
+
 }  // namespace hy

@@ -844,31 +844,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 }
                 if (!whole)
                 {
-                    if (u0 >= it.sinks)   // one run of keys
-                    {
-                        const int hi = p < 0 ? -1 : a.causal ? min(p - j_first, 127) : 127;
-                        const int lo = a.window > 0 && p - a.window + 1 > j_first ? p - a.window + 1 - j_first : 0;
+                    // The block is (part of) the run of sinks, then (part of) the window's: of either, the keys
+                    // from the column's window on, and the sinks, up to the column's own position.
+                    auto below = [](int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; };   // bits 0 .. x - 1
+                    const int split = it.sinks - u0;   // keys of the block that belong to the first run
+                    const int last = p < 0 ? -1 : a.causal ? p : it.kv - 1, from = a.window > 0 ? p - a.window + 1 : 0;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                        {
-                            const int h = hi - 32 * x, f = lo - 32 * x;
-                            const uint32_t upto = h >= 31 ? 0xffffffffu : h < 0 ? 0u : (2u << h) - 1u;
-                            uint32_t in = f <= 0 ? 0xffffffffu : f > 31 ? 0u : 0xffffffffu << f;
-                            const int s = min(a.sinks - j_first - 32 * x, 32);   // (keys below the window may be sinks)
-                            if (a.window > 0 && s > 0) in |= s >= 32 ? 0xffffffffu : (1u << s) - 1u;
-                            vis[x] &= in & upto;
-                        }
-                    }
-                    else
+                    for (int x = 0; x < 4; ++x)
                     {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
+                        const int o = 32 * x, k1 = u0 + o, k2 = it.lo - split + o;   // key of bit 0 in the first and in the second run
+                        uint32_t in1 = below(last + 1 - k1), in2 = below(last + 1 - k2);
+                        if (a.window > 0)
                         {
-                            uint32_t in = 0;
-#pragma unroll 1
-                            for (int y = 0; y < 32; ++y) in |= (paged_sees(a, p, key(u0 + 32 * x + y)) ? 1u : 0u) << y;
-                            vis[x] &= in;
+                            in1 &= ~below(from - k1) | below(a.sinks - k1);
+                            in2 &= ~below(from - k2) | below(a.sinks - k2);
                         }
+                        const uint32_t one = below(split - o);
+                        vis[x] &= (in1 & one) | (in2 & ~one);
                     }
 #pragma unroll
                     for (int e = 0; e < 128; ++e)
@@ -944,47 +936,61 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 const bool cubic = whole && __all_sync(0xffffffffu, m > -INFINITY);
                 const uint64_t fac2 = f2(fac, fac), mm2 = f2(-mm, -mm);
                 uint64_t sum0 = 0, sum1 = 0;   // (pairs of zeros)
-                // Weights; every fourth pair by the cubic: the special-function units make 4 of 2^x a
-                // cycle and quarter of the SM, two tiles' blocks take them 2048 cycles, as long as the products.
+                // Weights; some pairs by the cubic: the special-function units make 4 of 2^x a cycle and
+                // quarter of the SM, two tiles' blocks take them 2048 cycles, as long as the products. (The two
+                // cases are whole loops: a branch inside would keep the pairs from overlapping.)
+                auto weights = [&](auto plain) {
+                    constexpr bool PLAIN = decltype(plain)::value;   // the column sees the whole block
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
-                {
-                    const uint64_t x = f2_fma(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), fac2, mm2);
-                    uint64_t y;
-                    float w0, w1;
-                    if (e % kChunkCubicOf < kChunkCubic && cubic)
+                    for (int e = 0; e < 64; ++e)
                     {
-                        y = f2_exp2_cubic(x);
-                    }
-                    else
-                    {
-                        f2_get(x, w0, w1);
-                        y = f2(ex2(w0), ex2(w1));
-                    }
-                    if (e & 1) sum1 = f2_add(sum1, y);
-                    else sum0 = f2_add(sum0, y);
-                    if constexpr (F16)
-                    {
-                        const float2 v = reinterpret_cast<const float2*>(sc)[64 + e];
-                        y = f2_mul(y, f2(v.x, v.y));
-                    }
-                    f2_get(y, w0, w1);
-                    if constexpr (F16)
-                    {
-                        // (a scale of NaN must not meet a weight of zero that stands for "not seen")
-                        if (!whole)
+                        const uint64_t x = f2_fma(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), fac2, mm2);
+                        uint64_t y;
+                        float w0, w1;
+                        if constexpr (PLAIN)
                         {
-                            if (!((vis[e >> 4] >> (2 * e & 31)) & 1u)) w0 = 0.f;
-                            if (!((vis[e >> 4] >> ((2 * e + 1) & 31)) & 1u)) w1 = 0.f;
+                            if (e % kChunkCubicOf < kChunkCubic)
+                            {
+                                y = f2_exp2_cubic(x);
+                            }
+                            else
+                            {
+                                f2_get(x, w0, w1);
+                                y = f2(ex2(w0), ex2(w1));
+                            }
                         }
-                        r[e] = pack_f16(w0, w1);
+                        else
+                        {
+                            f2_get(x, w0, w1);
+                            y = f2(ex2(w0), ex2(w1));
+                        }
+                        if (e & 1) sum1 = f2_add(sum1, y);
+                        else sum0 = f2_add(sum0, y);
+                        if constexpr (F16)
+                        {
+                            const float2 v = reinterpret_cast<const float2*>(sc)[64 + e];
+                            y = f2_mul(y, f2(v.x, v.y));
+                        }
+                        f2_get(y, w0, w1);
+                        if constexpr (F16)
+                        {
+                            // (a scale of NaN must not meet a weight of zero that stands for "not seen")
+                            if constexpr (!PLAIN)
+                            {
+                                if (!((vis[e >> 4] >> (2 * e & 31)) & 1u)) w0 = 0.f;
+                                if (!((vis[e >> 4] >> ((2 * e + 1) & 31)) & 1u)) w1 = 0.f;
+                            }
+                            r[e] = pack_f16(w0, w1);
+                        }
+                        else
+                        {
+                            r[e] = pack_bf16(w0, w1);
+                        }
+                        if (e == 31) tmem_st32(ts + 64, *reinterpret_cast<uint32_t(*)[32]>(r));
                     }
-                    else
-                    {
-                        r[e] = pack_bf16(w0, w1);
-                    }
-                    if (e == 31) tmem_st32(ts + 64, *reinterpret_cast<uint32_t(*)[32]>(r));
-                }
+                };
+                if (cubic) weights(std::true_type{});
+                else weights(std::false_type{});
                 tmem_st32(ts + 96, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
                 float s0, s1, s2, s3;
                 f2_get(sum0, s0, s1);

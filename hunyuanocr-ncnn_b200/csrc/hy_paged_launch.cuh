@@ -145,7 +145,7 @@ cudaError_t launch_chunk(const PagedAttnArgs& a, int device, cudaStream_t s)
     const ChunkTma tma = chunk_tma<CT, D>(a);
     cudaError_t e = allow_smem<paged_chunk_kernel<CT, D>>(E::SMEM, device);
     if (e == cudaSuccess) e = launch_pdl(paged_chunk_kernel<CT, D>, dim3(148), kChunkThreads, E::SMEM, s, a, tma);
-    if (e == cudaSuccess) e = launch_pdl(paged_join_kernel<E>, dim3(148, E::COLS / 8), kJoinThreads, 0, s, a);
+    if (e == cudaSuccess) e = launch_pdl(paged_join_wide_kernel<E>, dim3(148, 8), kJoinThreads, 0, s, a);
     return e;
 }
 
