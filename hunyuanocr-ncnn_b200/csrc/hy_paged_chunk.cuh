@@ -85,6 +85,13 @@ __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.a
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// True in one thread of the (converged) warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // Descriptor of an operand in the 128-byte-swizzled layout (layout type 2 at bits 61-63):
 // rows of 128 bytes, eight rows to a 1024-byte atom.
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo)
@@ -694,65 +701,87 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     {
         // ---------------- products ----------------
         regs_dec<kChunkRegsOther>();
-        if (warp == kChunkMmaWarp && lane == 0)
+        if (warp == kChunkMmaWarp)
         {
+            // The whole warp walks, waits and computes addresses, so that they stay in uniform registers; one
+            // thread issues. (With the whole loop under `lane == 0` an instruction took some 100 cycles to issue.)
             constexpr uint32_t ID_QK = idesc_f16(!F16, false, 128, 128), ID_PV = idesc_f16(!F16, true, 128, D);
+            const bool leader = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             int nb = 0;   // blocks before this item
             int p_seen[2] = {0, 0};
             bool ok = true;
             auto qk = [&](int i, int blk) {
-                const uint32_t q = sm + E::Q_OFF + i * E::TILE_B, k = sm + E::RING_OFF + ((2 * blk) % SLOTS) * E::TILE_B;
-                const uint64_t qd = sw128_desc(q, 16, 1024), kd = sw128_desc(k, 16, 1024);
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
+                const uint64_t qd = sw128_desc(sm + E::Q_OFF + i * E::TILE_B, 16, 1024);
+                const uint64_t kd = sw128_desc(sm + E::RING_OFF + ((2 * blk) % SLOTS) * E::TILE_B, 16, 1024);
+                if (leader)
                 {
-                    const uint64_t o = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
-                    umma_f16_ss(tmem + E::S_COL + i * 128, qd + o, kd + o, ID_QK, ks ? 1u : 0u);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks)
+                    {
+                        const uint64_t o = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+                        umma_f16_ss(tm + E::S_COL + i * 128, qd + o, kd + o, ID_QK, ks ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[i]);
                 }
-                umma_commit(&s_full[i]);
+                __syncwarp();
             };
             auto pv = [&](int i, int blk, bool add) {
                 const uint64_t vd = sw128_desc(sm + E::RING_OFF + ((2 * blk + 1) % SLOTS) * E::TILE_B, 16384, 1024);
+                if (leader)
+                {
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-                    umma_f16_ts(tmem + E::O_COL + i * 128, tmem + E::S_COL + i * 128 + 64 + ks * 8, vd + ks * 128, ID_PV, (add || ks) ? 1u : 0u);
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_f16_ts(tm + E::O_COL + i * 128, tm + E::S_COL + i * 128 + 64 + ks * 8, vd + ks * 128, ID_PV, (add || ks) ? 1u : 0u);
+                }
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (leader) umma_commit(bar);
+                __syncwarp();
             };
             auto full = [&](int slot_n) {
                 ok = ok && mbar_wait_spin(&kv_full[slot_n % SLOTS], (slot_n / SLOTS) & 1, a.c.status, kPagedTimeout);
+                ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
             };
             for (int items = 0; ok; ++items)
             {
-                ok = mbar_wait_spin(q_full, items & 1, a.c.status, kPagedTimeout);
+                ok = __all_sync(0xffffffffu, mbar_wait_spin(q_full, items & 1, a.c.status, kPagedTimeout));
                 if (!ok) break;
-                const volatile ChunkItem& it = items_s[items & 1];
-                const int b0 = it.b0, n_blk = it.b1 - b0, lim[2] = {it.lim[0], it.lim[1]};
+                const ChunkItem it = items_s[items & 1];
+                const int b0 = __shfl_sync(0xffffffffu, it.b0, 0), n_blk = __shfl_sync(0xffffffffu, it.b1, 0) - b0;
+                const int lim[2] = {__shfl_sync(0xffffffffu, it.lim[0], 0), __shfl_sync(0xffffffffu, it.lim[1], 0)};
                 if (n_blk <= 0) break;
                 full(2 * nb);
                 if (!ok) break;
+#pragma unroll
                 for (int i = 0; i < 2; ++i)
                     if (b0 < lim[i]) qk(i, nb);
-                umma_commit(&kv_empty[(2 * nb) % SLOTS]);
-                if (n_blk == 1) umma_commit(q_empty);
+                commit(&kv_empty[(2 * nb) % SLOTS]);
+                if (n_blk == 1) commit(q_empty);
                 for (int j = 0; j < n_blk && ok; ++j)
                 {
                     const int blk = nb + j;
                     const bool more = j + 1 < n_blk;
                     bool v_there = false, k_there = false;
-                    for (int i = 0; i < 2 && ok; ++i)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
                     {
-                        if (b0 + j < lim[i])
+                        if (ok && b0 + j < lim[i])
                         {
-                            ok = mbar_wait_spin(&p_full[i], p_seen[i] & 1, a.c.status, kPagedTimeout);
+                            ok = __all_sync(0xffffffffu, mbar_wait_spin(&p_full[i], p_seen[i] & 1, a.c.status, kPagedTimeout));
                             ++p_seen[i];
                             if (!v_there) full(2 * blk + 1);
                             v_there = true;
-                            if (!ok) break;
                             tc_fence_after();
-                            if (F16 || !*reinterpret_cast<volatile int*>(&pv_skip[i])) pv(i, blk, j > 0);
-                            umma_commit(&o_full[i]);
+                            if (ok)
+                            {
+                                if (F16 || !*reinterpret_cast<volatile int*>(&pv_skip[i])) pv(i, blk, j > 0);
+                                commit(&o_full[i]);
+                            }
                         }
-                        if (more && b0 + j + 1 < lim[i])
+                        if (ok && more && b0 + j + 1 < lim[i])
                         {
                             if (!k_there) full(2 * blk + 2);
                             k_there = true;
@@ -760,13 +789,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         }
                     }
                     if (!ok) break;
-                    umma_commit(&kv_empty[(2 * blk + 1) % SLOTS]);
-                    if (more) umma_commit(&kv_empty[(2 * blk + 2) % SLOTS]);
-                    if (j + 2 == n_blk) umma_commit(q_empty);
+                    commit(&kv_empty[(2 * blk + 1) % SLOTS]);
+                    if (more) commit(&kv_empty[(2 * blk + 2) % SLOTS]);
+                    if (j + 2 == n_blk) commit(q_empty);
                 }
                 nb += n_blk;
             }
-            umma_commit(done);   // nothing is in flight when the tensor memory is freed
+            commit(done);   // nothing is in flight when the tensor memory is freed
             mbar_wait_spin(done, 0, a.c.status, kPagedTimeout);
         }
         __syncwarp();
