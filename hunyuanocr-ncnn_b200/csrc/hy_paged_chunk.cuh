@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
         int blk = 0;           // blocks (index of the scale ring)
         int items = 0, mended = 0;
         bool ok_all = true;
+        const bool leader = elect_one();
         for (;; ++items)
         {
             if (items) ok_all = ok_all && mbar_wait(q_empty, (items - 1) & 1, a.c.status, kPagedTimeout);
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             else
             {
                 // As f16, times the power of two that brings the column's largest magnitude to [2^14, 2^15).
-                constexpr int U = 4;
+                constexpr int U = 8;
 #pragma unroll 1
                 for (int x0 = lt; x0 < 256 * QP; x0 += 128 * U)
                 {
@@ -480,22 +481,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 pg = __ldg(table + x);
             };
             constexpr int CPR = D * static_cast<int>(sizeof(CT)) / 16;   // 16-byte pieces of a row in memory
-            // Page and row: of this thread's key of a block, and (TMA) of the group of 16 that lane / 2 is of.
+            // Page and row: of this thread's key of a block, and (TMA) of the group of 16 keys 2 lw + lane % 2.
             int pg = 0, row = 0, gpg = 0, grow = 0;
-            // Announces and fetches a block by TMA: lane 2 g (+ 1: the upper 64 dimensions of bf16 rows) takes group g.
+            const int group_key = 32 * lw + (lane & 1) * 16;
+            // This warp's two groups of a block by TMA, counted on `bar`.
+            constexpr int WARP_BYTES = 32 * D * static_cast<int>(sizeof(CT));
             auto fetch = [&](int b, int kv, uint32_t dst, uint64_t* bar) {
-                if (lane == 0) mbar_arrive_expect_tx(bar, 128 * D * static_cast<int>(sizeof(CT)));
-                __syncwarp();
-                constexpr int HALVES = (!F16 && D == 128) ? 2 : 1;
-                const int g = lane >> 1, half = lane & 1;
-                if (g < 8 && half < HALVES)
+                const bool ok = b * 128 + group_key < w.it.w.n && gpg >= 0 && gpg < a.c.num_pages;
+                const int page = ok ? gpg : a.c.num_pages;   // (past the last page: zeros)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
                 {
-                    const bool ok = b * 128 + g * 16 < w.it.w.n && gpg >= 0 && gpg < a.c.num_pages;
-                    const int page = ok ? gpg : a.c.num_pages;   // (past the last page: zeros)
-                    const int c1 = tma.row_c == 1 ? grow : tma.head_c == 1 ? w.it.head : page;
-                    const int c2 = tma.row_c == 2 ? grow : tma.head_c == 2 ? w.it.head : page;
-                    const int c3 = tma.row_c == 3 ? grow : tma.head_c == 3 ? w.it.head : page;
-                    tma_load_4d(dst + (F16 ? g * 16 * D : half * 16384 + g * 2048), kv ? &tma.v : &tma.k, half * 64, c1, c2, c3, bar);
+                    const int pgx = __shfl_sync(0xffffffffu, page, x), rwx = __shfl_sync(0xffffffffu, grow, x), g = 2 * lw + x;
+                    const int c1 = tma.row_c == 1 ? rwx : tma.head_c == 1 ? w.it.head : pgx;
+                    const int c2 = tma.row_c == 2 ? rwx : tma.head_c == 2 ? w.it.head : pgx;
+                    const int c3 = tma.row_c == 3 ? rwx : tma.head_c == 3 ? w.it.head : pgx;
+                    if (leader)
+                    {
+                        const CUtensorMap* const map = kv ? &tma.v : &tma.k;
+                        tma_load_4d(dst + (F16 ? g * 16 * D : g * 2048), map, 0, c1, c2, c3, bar);
+                        if constexpr (!F16 && D == 128) tma_load_4d(dst + 16384 + g * 2048, map, 64, c1, c2, c3, bar);
+                    }
                 }
                 __syncwarp();
             };
@@ -503,52 +509,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             {
                 if (tma.on)
                 {
-                    if (lw == 0)
+                    find(w.b0, group_key, gpg, grow);
+                    for (int b = w.b0; b < w.b1 && ok_all; ++b, ++blk)
                     {
-                        find(w.b0, (lane >> 1) * 16, gpg, grow);
-                        for (int b = w.b0; b < w.b1 && ok_all; ++b, ++blk)
-                        {
-                            const int left = w.it.w.n - b * 128;
-                            // live bits: 16 per group, two groups a word
-                            const bool page_ok = gpg >= 0 && gpg < a.c.num_pages;
-                            const int cnt = lane < 16 ? min(max(left - (lane >> 1) * 16, 0), 16) : 0;
-                            if (cnt && !page_ok) paged_status(a.c.status, kPagedBadPage);
-                            const uint32_t bits = page_ok ? (1u << cnt) - 1u : 0u;
-                            const uint32_t b_lo = __shfl_sync(0xffffffffu, bits, (lane & 3) * 4), b_hi = __shfl_sync(0xffffffffu, bits, (lane & 3) * 4 + 2);
-                            if (lane < 4) live_w[(blk & 3) * 4 + lane] = b_lo | (b_hi << 16);
-                            __syncwarp();
-                            const int mend = left < 128 && (left & 15);   // rows behind the last key came along
+                        const int left = w.it.w.n - b * 128;   // keys from this block on
+                        const bool page_ok = gpg >= 0 && gpg < a.c.num_pages;
+                        const int cnt = lane < 2 ? min(max(left - group_key, 0), 16) : 0;
+                        if (cnt && !page_ok) paged_status(a.c.status, kPagedBadPage);
+                        const uint32_t bits = page_ok ? (1u << cnt) - 1u : 0u;
+                        const uint32_t hi = __shfl_sync(0xffffffffu, bits, 1);
+                        if (lane == 0) live_w[(blk & 3) * 4 + lw] = bits | (hi << 16);
+                        __syncwarp();
+                        // Rows behind the last key come along with its group; they may hold anything, and in V they
+                        // become zeros before the products see them: the warp whose group it is announces the block then.
+                        const int mender = (left < 128 && (left & 15)) ? left >> 5 : -1;
 #pragma unroll
-                            for (int kv = 0; kv < 2; ++kv, ++n)
+                        for (int kv = 0; kv < 2; ++kv, ++n)
+                        {
+                            const int slot = n % SLOTS;
+                            if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                            const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
+                            if (kv && mender == lw)
                             {
-                                const int slot = n % SLOTS;
-                                if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
-                                const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
-                                if (kv && mend)
-                                {
-                                    // They may hold anything: zeros before the products see them.
-                                    fetch(b, kv, dst, &st_full[0]);
-                                    ok_all = ok_all && mbar_wait(&st_full[0], mended & 1, a.c.status, kPagedTimeout);
-                                    ++mended;
-                                    constexpr int QP = E::RB / 16;
-                                    for (int x = lane; x < (16 - (left & 15)) * QP; x += 32)
-                                        *reinterpret_cast<uint4*>(smem + E::RING_OFF + slot * E::TILE_B + sw128_at(left + x / QP, x % QP)) = make_uint4(0, 0, 0, 0);
-                                    fence_async_smem();
-                                    __syncwarp();
-                                    if (lane == 0) mbar_arrive(&kv_full[slot]);
-                                }
-                                else
-                                {
-                                    fetch(b, kv, dst, &kv_full[slot]);
-                                }
+                                if (leader) mbar_arrive_expect_tx(&st_full[0], WARP_BYTES);
+                                __syncwarp();
+                                fetch(b, kv, dst, &st_full[0]);
+                                ok_all = ok_all && mbar_wait(&st_full[0], mended & 1, a.c.status, kPagedTimeout);
+                                constexpr int QP = E::RB / 16;
+                                for (int x = lane; x < (16 - (left & 15)) * QP; x += 32)
+                                    *reinterpret_cast<uint4*>(smem + E::RING_OFF + slot * E::TILE_B + sw128_at(left + x / QP, x % QP)) = make_uint4(0, 0, 0, 0);
+                                fence_async_smem();
+                                __syncwarp();
+                                if (leader) mbar_arrive_expect_tx(&kv_full[slot], 3 * WARP_BYTES);
                             }
-                            find(b + 1, (lane >> 1) * 16, gpg, grow);
+                            else
+                            {
+                                if (leader && lw == 0 && !(kv && mender >= 0)) mbar_arrive_expect_tx(&kv_full[slot], 4 * WARP_BYTES);
+                                fetch(b, kv, dst, &kv_full[slot]);
+                            }
+                            if (kv && mender >= 0) ++mended;
                         }
-                    }
-                    else
-                    {
-                        n += 2 * (w.b1 - w.b0);
-                        blk += w.b1 - w.b0;
+                        find(b + 1, group_key, gpg, grow);
                     }
                 }
                 else
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 // Codes to the staging ring two slots ahead, then to the operand ring as f16.
                 const int n0 = n, n1 = n + 2 * (w.b1 - w.b0);
                 int fb = w.b0;   // block of the next fetch
-                if (tma.on) find(fb, (lane >> 1) * 16, gpg, grow);
+                if (tma.on) find(fb, group_key, gpg, grow);
                 else find(fb, lt, pg, row);
                 auto ahead = [&](int x) {   // fetch slot x
                     if (x < n1)
@@ -613,12 +614,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         const int kv = (x - n0) & 1, sg = x % 3;
                         if (tma.on)
                         {
-                            if (lw == 0)
-                            {
-                                if (x >= 3) ok_all = ok_all && mbar_wait(&st_empty[sg], (x / 3 - 1) & 1, a.c.status, kPagedTimeout);
-                                fetch(fb, kv, sm + E::STAGE_OFF + sg * E::CODES_B, &st_full[sg]);
-                            }
-                            if (kv) find(++fb, (lane >> 1) * 16, gpg, grow);
+                            if (x >= 3) ok_all = ok_all && mbar_wait(&st_empty[sg], (x / 3 - 1) & 1, a.c.status, kPagedTimeout);
+                            if (leader && lw == 0) mbar_arrive_expect_tx(&st_full[sg], 4 * WARP_BYTES);
+                            fetch(fb, kv, sm + E::STAGE_OFF + sg * E::CODES_B, &st_full[sg]);
+                            if (kv) find(++fb, group_key, gpg, grow);
                         }
                         else
                         {
@@ -837,28 +836,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t r[128];   // scores, then (packed) weights
-                {
-                    uint32_t(&r0)[32] = *reinterpret_cast<uint32_t(*)[32]>(r);
-                    uint32_t(&r1)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 32);
-                    uint32_t(&r2)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 64);
-                    uint32_t(&r3)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 96);
-                    tmem_ld32(ts, r0);
-                    tmem_ld32(ts + 32, r1);
-                    tmem_ld32(ts + 64, r2);
-                    tmem_ld32(ts + 96, r3);
-                    tmem_ld32_wait(r0);
-                    tmem_ld32_wait(r1);
-                    tmem_ld32_wait(r2);
-                    tmem_ld32_wait(r3);
-                }
+                uint32_t(&r0)[32] = *reinterpret_cast<uint32_t(*)[32]>(r);
+                uint32_t(&r1)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 32);
+                uint32_t(&r2)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 64);
+                uint32_t(&r3)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 96);
+                tmem_ld32(ts, r0);
+                tmem_ld32(ts + 32, r1);
+                tmem_ld32(ts + 64, r2);
+                tmem_ld32(ts + 96, r3);
                 const float4* const sc = reinterpret_cast<const float4*>(smem + E::SCALE_OFF + ring * E::SCALE_B);
                 const int u0 = b * 128, j_first = key(u0), j_last = key(min(u0 + 127, it.keys - 1));
                 uint32_t vis[4];   // what the column sees, a bit per key
-#pragma unroll
-                for (int x = 0; x < 4; ++x) vis[x] = live_w[ring * 4 + x];
+                {
+                    const uint4 x = lds128(sm + E::LIVE_OFF + ring * 16);
+                    vis[0] = x.x; vis[1] = x.y; vis[2] = x.z; vis[3] = x.w;
+                }
                 const bool whole = (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu && p_lo >= 0 &&
                                    (!a.causal || (j_last <= p_lo && (a.window == 0 || j_first > p_hi - a.window || j_last < a.sinks)));
                 bool odd = false;
+                tmem_ld32_wait(r0);
+                tmem_ld32_wait(r1);
+                tmem_ld32_wait(r2);
+                tmem_ld32_wait(r3);
                 if constexpr (F16)
                 {
 #pragma unroll
