@@ -3,6 +3,7 @@
 // the first CUDA call.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <string>
 
@@ -162,16 +163,17 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     if (rc) return rc;
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
-    const PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, krs, khs, vrs, vhs};
-    with_row_type(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
+    PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, krs, khs, vrs, vhs, 1, 0};
+    // Rows of a CTA: one while that leaves the GPU fewer than 8 CTAs per SM, then more; at most 2^16 vectors.
+    a.per_cta = std::min({kRowsPerCta, std::max(1, rows / (8 * 148)), std::max(1, 32768 / cache->num_kv_heads - 1)});
+    a.vectors_inv = static_cast<unsigned>(((1ull << 32) + 2u * cache->num_kv_heads - 1) / (2u * cache->num_kv_heads));
+    const cudaError_t e = with_row_type(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
         using RT = typename decltype(rt)::type;
         using CT = typename decltype(ct)::type;
-        const dim3 grid(rows), block(kRowWarps * 32);
-        const cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (write) paged_write_kernel<RT, CT, decltype(d)::value><<<grid, block, 0, s>>>(a);
-        else paged_read_kernel<RT, CT, decltype(d)::value><<<grid, block, 0, s>>>(a);
+        constexpr int D = decltype(d)::value;
+        return launch_pdl(write ? paged_write_kernel<RT, CT, D> : paged_read_kernel<RT, CT, D>,
+                          dim3((rows + a.per_cta - 1) / a.per_cta), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream), a);
     });
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? HY_OK : cuda_fail(write ? "paged write" : "paged read", e);
 }
 

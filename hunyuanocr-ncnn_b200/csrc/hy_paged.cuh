@@ -250,13 +250,16 @@ __device__ __forceinline__ void store_row(void* base, long long off, const float
 }
 
 // ---------------------------------------------------------------------------
-// Write and read back. One CTA (4 warps) per row; the row's 2 x kv_heads
-// vectors (k, then v) are shared out to groups of lanes that hold 16 bytes of
-// the row tensor each, so that a row's loads are all wide and all in flight at
-// once; the maximum of a vector is taken in registers and its codes leave in
-// the same pass. Bound by memory: each byte moves once.
+// Write and read back. A CTA of 4 warps takes a few consecutive rows (1 to 16, so
+// that small calls spread over the SMs and in large ones a place is looked up
+// once for all that is moved): lane r of every warp finds row r's page, then the
+// rows' 2 x kv_heads vectors (k, then v) are shared out to groups of lanes that
+// hold 16 bytes of the row tensor each, so that all loads are wide and several
+// are in flight per lane. The maximum of a vector is taken in registers and its codes
+// leave in the same pass. Bound by memory: each byte moves once.
 // ---------------------------------------------------------------------------
 constexpr int kRowWarps = 4;
+constexpr int kRowsPerCta = 16;
 
 struct PagedRowArgs {
     PagedCache c;
@@ -264,33 +267,58 @@ struct PagedRowArgs {
     void* k;   // row tensors
     void* v;
     long long k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int per_cta;               // rows of a CTA
+    unsigned vectors_inv;      // ceil(2^32 / (2 kv_heads)): x / (2 kv_heads) = high half of the product, x < 2^16
 };
 
-// Where row r belongs: its page's and row's offsets. False: nowhere.
-__device__ __forceinline__ bool paged_place(const PagedCache& c, const PagedBatch& b, int r, int lane, long long& off,
-                                            long long& s_off)
+// Offsets of row r's page and row in it; off < 0: it has no place. The whole warp calls it, lane i for its own row
+// (r < 0: none); rows of a warp are consecutive.
+__device__ __forceinline__ void paged_places(const PagedCache& c, const PagedBatch& b, int r, int lane, long long& off,
+                                             long long& s_off)
 {
-    const int s = paged_find_seq(b, r, lane);
-    if (s < 0) return false;
+    off = -1;
+    s_off = 0;
+    int s = paged_find_seq(b, __shfl_sync(0xffffffffu, r, 0), lane);   // of the first row
+    if (r < 0 || r >= b.rows) return;
+    s = max(s, 0);
+    while (s < b.num_seqs && __ldg(b.q_start + s + 1) <= r) ++s;       // (rows of short sequences)
+    if (s >= b.num_seqs || r < __ldg(b.q_start + s)) return;
     PagedSeq q;
-    if (!paged_seq(b, s, c.page_size, c.status, q)) return false;
+    if (!paged_seq(b, s, c.page_size, c.status, q)) return;
     if (r < q.row0 || r >= q.row0 + q.n)   // q_start is not ascending
     {
         paged_status(c.status, kPagedBadRows);
-        return false;
+        return;
     }
     const int p = q.kv - q.n + (r - q.row0);
-    if (p < 0) return false;
-    const int pg = __ldg(b.table + s * b.table_stride + p / c.page_size);
-    const int in = p % c.page_size;
+    if (p < 0) return;
+    const int x = p / c.page_size, in = p - x * c.page_size;
+    const int pg = __ldg(b.table + s * b.table_stride + x);
     if (pg < 0 || pg >= c.num_pages)
     {
         paged_status(c.status, kPagedBadPage);
-        return false;
+        return;
     }
     off = pg * c.page_stride + in * c.row_stride;
     s_off = pg * c.s_page_stride + in * c.s_row_stride;
-    return true;
+}
+
+// Vector x of a CTA's rows: row x / (2 kv_heads), k or v, head.
+struct PagedVector {
+    int row, head;
+    bool isv;
+};
+__device__ __forceinline__ PagedVector paged_vector(const PagedRowArgs& a, int x)
+{
+    const int row = static_cast<int>(__umulhi(static_cast<unsigned>(x), a.vectors_inv));
+    const int y = x - row * 2 * a.c.kv_heads;
+    const bool isv = y >= a.c.kv_heads;
+    return {row, isv ? y - a.c.kv_heads : y, isv};
+}
+__device__ __forceinline__ long long paged_row_at(const PagedRowArgs& a, const PagedVector& v, int r0)
+{
+    const long long r = r0 + v.row;
+    return v.isv ? r * a.v_row_stride + v.head * a.v_head_stride : r * a.k_row_stride + v.head * a.k_head_stride;
 }
 
 template <typename RT, typename CT, int D>
@@ -300,71 +328,74 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const Paged
     constexpr int LPV = D / E;                             // lanes per vector: 8, 16 or 32
     constexpr int VPW = 32 / LPV;                          // vectors per warp and step
     constexpr int U = 4;                                   // steps in flight
+    constexpr int STEP = U * kRowWarps * VPW;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r = blockIdx.x;
-    const int nv = 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
-
-    auto load = [&](int v0, float (&x)[U][E]) {
+    const int r0 = blockIdx.x * a.per_cta, n_rows = min(a.per_cta, a.b.rows - r0);
+    const int nv = n_rows * 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+    pdl_wait();
+    uint4 x[U];
+    auto load = [&](int v0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
-            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
-            if (vec >= nv) continue;
-            const bool isv = vec >= a.c.kv_heads;
-            const int h = isv ? vec - a.c.kv_heads : vec;
-            load_row<RT, E>(isv ? a.v : a.k,
-                            isv ? r * a.v_row_stride + h * a.v_head_stride + d
-                                : r * a.k_row_stride + h * a.k_head_stride + d,
-                            x[u]);
+            const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
+            if (i >= nv) continue;
+            const PagedVector v = paged_vector(a, i);
+            x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const RT*>(v.isv ? a.v : a.k) + paged_row_at(a, v, r0) + d));
         }
     };
-    float x[U][E];
-    load(0, x);   // ahead of the look-up of the row's place: a row's values do not depend on it
+    load(0);   // ahead of the look-ups: the values do not depend on them
     long long off, s_off;
-    if (!paged_place(a.c, a.b, r, lane, off, s_off)) return;
-    for (int v0 = 0; v0 < nv; v0 += U * kRowWarps * VPW)
+    paged_places(a.c, a.b, lane < n_rows ? r0 + lane : -1, lane, off, s_off);
+    for (int v0 = 0; v0 < nv; v0 += STEP)
     {
-        if (v0) load(v0, x);
+        if (v0) load(v0);
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
-            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
-            const bool live = vec < nv;
-            const bool isv = vec >= a.c.kv_heads;
-            const int h = isv ? vec - a.c.kv_heads : vec;
-            const long long at = off + h * a.c.head_stride + d;
-            void* const pool = isv ? a.c.v : a.c.k;
+            const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
+            const PagedVector v = paged_vector(a, min(i, nv - 1));
+            const long long o = __shfl_sync(0xffffffffu, off, v.row), so = __shfl_sync(0xffffffffu, s_off, v.row);
+            const bool live = i < nv && o >= 0;
+            const long long at = o + v.head * a.c.head_stride + d;
+            void* const pool = v.isv ? a.c.v : a.c.k;
+            float f[E];
+            const uint32_t w4[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                f[e] = E == 4 ? __uint_as_float(w4[e]) : __uint_as_float((e & 1) ? w4[e >> 1] & 0xFFFF0000u : w4[e >> 1] << 16);
             if constexpr (kCodes<CT>)
             {
                 // The largest magnitude by its bits: an infinity or a NaN comes out on top.
                 uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < E; ++i)
-                    if (live) m = max(m, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                for (int e = 0; e < E; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
 #pragma unroll
-                for (int o = LPV / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                for (int w = LPV / 2; w > 0; w >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, w));
                 const bool finite = m < 0x7f800000u;
                 const float scale =
                     finite ? fmaxf(__fdiv_rn(__uint_as_float(m), kCodeMax<CT>), 1.17549435e-38f) : __int_as_float(0x7fffffff);
-                if (!live) continue;
                 const float inv = __fdiv_rn(1.f, scale);
-                uint32_t w[E / 4];
-#pragma unroll
-                for (int i = 0; i < E / 4; ++i)
+                if (live)
                 {
-                    w[i] = 0;
+                    uint32_t w[E / 4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (finite) w[i] |= quant<CT>(x[u][4 * i + e], scale, inv) << (8 * e);
+                    for (int y = 0; y < E / 4; ++y)
+                    {
+                        w[y] = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (finite) w[y] |= quant<CT>(f[4 * y + e], scale, inv) << (8 * e);
+                    }
+                    uint8_t* p = static_cast<uint8_t*>(pool) + at;
+                    if constexpr (E == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+                    else *reinterpret_cast<uint32_t*>(p) = w[0];
+                    if (lane % LPV == 0) (v.isv ? a.c.v_scale : a.c.k_scale)[so + v.head * a.c.s_head_stride] = scale;
                 }
-                uint8_t* p = static_cast<uint8_t*>(pool) + at;
-                if constexpr (E == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t*>(p) = w[0];
-                if (lane % LPV == 0) (isv ? a.c.v_scale : a.c.k_scale)[s_off + h * a.c.s_head_stride] = scale;
             }
             else
             {
-                if (live) store_row<CT, E>(pool, at, x[u]);
+                if (live) store_row<CT, E>(pool, at, f);
             }
         }
     }
@@ -376,39 +407,60 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
     constexpr int E = 16 / static_cast<int>(sizeof(RT));
     constexpr int LPV = D / E;
     constexpr int VPW = 32 / LPV;
-    constexpr int U = 4;
+    constexpr int U = E * sizeof(CT) > 16 ? 4 : 8;
+    constexpr int STEP = U * kRowWarps * VPW;
+    constexpr int W = E * static_cast<int>(sizeof(CT)) / 4;   // words of the cache that a lane reads
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r = blockIdx.x;
-    const int nv = 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+    const int r0 = blockIdx.x * a.per_cta, n_rows = min(a.per_cta, a.b.rows - r0);
+    const int nv = n_rows * 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+    pdl_wait();
     long long off, s_off;
-    if (!paged_place(a.c, a.b, r, lane, off, s_off)) return;
-    for (int v0 = 0; v0 < nv; v0 += U * kRowWarps * VPW)
+    paged_places(a.c, a.b, lane < n_rows ? r0 + lane : -1, lane, off, s_off);
+    for (int v0 = 0; v0 < nv; v0 += STEP)
     {
-        float x[U][E], scale[U];
+        uint32_t x[U][W];
+        float scale[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
-            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
-            if (vec >= nv) continue;
-            const bool isv = vec >= a.c.kv_heads;
-            const int h = isv ? vec - a.c.kv_heads : vec;
-            load_row<CT, E>(isv ? a.c.v : a.c.k, off + h * a.c.head_stride + d, x[u]);
-            if constexpr (kCodes<CT>) scale[u] = __ldg((isv ? a.c.v_scale : a.c.k_scale) + s_off + h * a.c.s_head_stride);
+            const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
+            const PagedVector v = paged_vector(a, min(i, nv - 1));
+            const long long o = __shfl_sync(0xffffffffu, off, v.row), so = __shfl_sync(0xffffffffu, s_off, v.row);
+            if (i >= nv || o < 0) continue;
+            const CT* const p = static_cast<const CT*>(v.isv ? a.c.v : a.c.k) + o + v.head * a.c.head_stride + d;
+            if constexpr (W == 1) x[u][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            else if constexpr (W == 2)
+            {
+                const uint2 y = __ldg(reinterpret_cast<const uint2*>(p));
+                x[u][0] = y.x; x[u][1] = y.y;
+            }
+            else
+#pragma unroll
+                for (int w = 0; w < W; w += 4)
+                {
+                    const uint4 y = __ldg(reinterpret_cast<const uint4*>(p) + w / 4);
+                    x[u][w] = y.x; x[u][w + 1] = y.y; x[u][w + 2] = y.z; x[u][w + 3] = y.w;
+                }
+            if constexpr (kCodes<CT>) scale[u] = __ldg((v.isv ? a.c.v_scale : a.c.k_scale) + so + v.head * a.c.s_head_stride);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
-            const int vec = v0 + (u * kRowWarps + warp) * VPW + sub;
-            if (vec >= nv) continue;
-            const bool isv = vec >= a.c.kv_heads;
-            const int h = isv ? vec - a.c.kv_heads : vec;
+            const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
+            const PagedVector v = paged_vector(a, min(i, nv - 1));
+            if (__shfl_sync(0xffffffffu, off, v.row) < 0 || i >= nv) continue;
+            float f[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+            {
+                if constexpr (sizeof(CT) == 4) f[e] = __uint_as_float(x[u][e]);
+                else if constexpr (sizeof(CT) == 2) f[e] = __uint_as_float((e & 1) ? x[u][e >> 1] & 0xFFFF0000u : x[u][e >> 1] << 16);
+                else if (e % 4 == 0) decode4<CT>(x[u][e / 4], f + e);
+            }
             if constexpr (kCodes<CT>)
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[u][i] *= scale[u];
-            store_row<RT, E>(isv ? a.v : a.k,
-                             isv ? r * a.v_row_stride + h * a.v_head_stride + d
-                                 : r * a.k_row_stride + h * a.k_head_stride + d,
-                             x[u]);
+                for (int e = 0; e < E; ++e) f[e] *= scale[u];
+            store_row<RT, E>(v.isv ? a.v : a.k, paged_row_at(a, v, r0) + d, f);
         }
     }
 }
