@@ -163,7 +163,11 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     if (rc) return rc;
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
-    PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, krs, khs, vrs, vhs, 1, 0};
+    for (const long long x : {krs, khs, vrs, vhs, static_cast<long long>(cache->head_stride), static_cast<long long>(cache->scale_head_stride)})
+        if (x > INT_MAX) return fail(HY_ERR_CAPACITY, "row and head strides must be below 2^31");
+    PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, static_cast<int>(krs), static_cast<int>(khs),
+                   static_cast<int>(vrs), static_cast<int>(vhs), static_cast<int>(cache->head_stride),
+                   static_cast<int>(cache->scale_head_stride), 1, 0};
     // Rows of a CTA: one while that leaves the GPU fewer than 8 CTAs per SM, then more; at most 2^16 vectors.
     a.per_cta = std::min({kRowsPerCta, std::max(1, rows / (8 * 148)), std::max(1, 32768 / cache->num_kv_heads - 1)});
     a.vectors_inv = static_cast<unsigned>(((1ull << 32) + 2u * cache->num_kv_heads - 1) / (2u * cache->num_kv_heads));

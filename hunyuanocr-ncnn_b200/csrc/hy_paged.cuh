@@ -8,7 +8,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -97,63 +97,79 @@ struct Int8 {
 template <typename CT>
 constexpr bool kCodes = (sizeof(CT) == 1);   // codes with a scale
 
-// x / s rounded to int8, ties to even, for |x| <= 127 s (1 + 2^-23). inv = 1 / s.
-// x * inv is off by a few ulp, so only a quotient that close to a tie needs the
-// exact sign of x - (n + 1/2) s, which the fused multiply-add gives.
-__device__ __forceinline__ uint32_t quant_int8(float x, float s, float inv)
+// x / s rounded to fp32 so that no later rounding to fewer bits can go wrong: where the quotient is not a
+// float, of the two floats around it the one whose last bit is set (it lies on the quotient's side
+// of every tie). The remainder x - q s of the nearest q is exact in a fused multiply-add.
+__device__ __forceinline__ float quotient_odd(float x, float s, float inv)
 {
-    const float q = x * inv;
-    float r = rintf(q);
-    if (fabsf(q - r) > 0.4999f)
-    {
-        const float lo = floorf(q);
-        const float d = fmaf(-(lo + 0.5f), s, x);
-        const bool odd = (static_cast<int>(lo) & 1) != 0;
-        r = (d > 0.f || (d == 0.f && odd)) ? lo + 1.f : lo;
-    }
-    r = fminf(fmaxf(r, -127.f), 127.f);
-    return static_cast<uint32_t>(static_cast<int>(r)) & 0xffu;
+    float q = x * inv;
+    q = fmaf(fmaf(-q, s, x), inv, q);
+    const float r = fmaf(-q, s, x);
+    const int bits = __float_as_int(q);
+    const int away = ((__float_as_int(r) ^ bits) < 0) ? -1 : 1;   // the quotient is the smaller or the larger magnitude
+    return __int_as_float((r == 0.f || (bits & 1) || (bits << 1) == 0) ? bits : bits + away);
 }
 
-// x / s rounded to E4M3 (4 exponent bits, bias 7; 3 fraction bits), ties to
-// even, at most 448: as above, the hardware's rounding of x * inv except near a
-// tie and among the subnormals (|q| < 2^-6), where the sign of a - mid s decides.
-__device__ __forceinline__ uint32_t quant_e4m3(float x, float s, float inv)
-{
-    const float q = x * inv;
-    const uint32_t b = __float_as_uint(q) & 0x7fffffffu;
-    const int off = static_cast<int>(b & 0xFFFFFu) - 0x80000;
-    const bool sub = b < 0x3C800000u;   // 2^-6
-    if ((sub && b != 0) || (off >= -8 && off <= 8))
-    {
-        const float a = fabsf(x), aq = __uint_as_float(b);
-        int lo;
-        float mid;
-        if (sub)
-        {
-            lo = static_cast<int>(aq * 512.f);
-            mid = (static_cast<float>(lo) + 0.5f) * (1.f / 512.f);
-        }
-        else
-        {
-            lo = static_cast<int>(b >> 20) - (120 << 3);
-            mid = __uint_as_float((b & 0xFFF00000u) | 0x80000u);
-        }
-        const float d = fmaf(-mid, s, a);
-        if (d > 0.f || (d == 0.f && (lo & 1))) ++lo;
-        return static_cast<uint32_t>(min(lo, 0x7E)) | ((__float_as_uint(x) >> 24) & 0x80u);
-    }
-    return __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-}
-
+// Four quotients x / s as a word of codes, rounded to nearest, ties to even (inv = 1 / s, off
+// by 2 ulp at most): the hardware's rounding of x * inv, which is off by a few ulp, and where that may
+// matter - next to a tie - of quotient_odd. (bf16 rows meet ties often: one in some 300 quotients of
+// 8-bit significands is within rounding of one.)
 template <typename CT>
-__device__ __forceinline__ uint32_t quant(float x, float s, float inv)
+__device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv)
 {
-    if constexpr (std::is_same_v<CT, E4M3>) return quant_e4m3(x, s, inv);
-    else return quant_int8(x, s, inv);
+    float q[4];
+    if constexpr (std::is_same_v<CT, E4M3>)
+    {
+        // 4 exponent bits, bias 7; 3 fraction bits; at most 448.
+        uint32_t small = 0xffffffffu, tie = 0xffffffffu;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            q[e] = x[e] * inv;
+            const uint32_t b = __float_as_uint(q[e]) & 0x7fffffffu;
+            small = min(small, b);
+            tie = min(tie, (b + (8u - 0x80000u)) & 0xFFFFFu);   // up to 16: within 8 ulp of a tie of the normal codes
+        }
+        if (tie <= 16u || small < 0x3C800000u)   // (below 2^-6: subnormal codes, whose ties lie elsewhere)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = quotient_odd(x[e], s, inv);
+        uint32_t w;
+        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+            "mov.b32 %0, {lo, hi};\n\t}"
+            : "=r"(w)
+            : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+        return w;
+    }
+    else
+    {
+        // To an integer by adding 1.5 * 2^23; magnitudes stay within 127 (1 + 2^-22).
+        float t[4], far = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            q[e] = x[e] * inv;
+            t[e] = q[e] + 12582912.f;
+            far = fmaxf(far, fabsf(q[e] - (t[e] - 12582912.f)));
+        }
+        if (far > 0.4999f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = quotient_odd(x[e], s, inv) + 12582912.f;
+        return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                           __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+    }
 }
 template <typename CT>
 constexpr float kCodeMax = std::is_same_v<CT, E4M3> ? 448.f : 127.f;
+
+// m / kCodeMax correctly rounded, at least 2^-126: the quotient by the rounded reciprocal and its
+// exact remainder once more (Markstein); below 2^-126 kCodeMax, where that could underflow, the bound applies.
+template <typename CT>
+__device__ __forceinline__ float code_scale(float m)
+{
+    constexpr float top = kCodeMax<CT>, inv = 1.f / top;
+    const float q = m * inv;
+    return fmaxf(fmaf(fmaf(-q, top, m), inv, q), 1.17549435e-38f);
+}
 
 // Four codes of a word as fp32.
 template <typename CT>
@@ -161,8 +177,11 @@ __device__ __forceinline__ void decode4(uint32_t w, float* o)
 {
     if constexpr (std::is_same_v<CT, E4M3>)
     {
-        const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(w & 0xffffu, __NV_E4M3)));
-        const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(w >> 16, __NV_E4M3)));
+        uint32_t h0, h1;
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+            : "=r"(h0), "=r"(h1)
+            : "r"(w));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
         o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
     }
     else
@@ -266,18 +285,21 @@ struct PagedRowArgs {
     PagedBatch b;
     void* k;   // row tensors
     void* v;
-    long long k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int page_head_stride, scale_head_stride;   // the cache's
     int per_cta;               // rows of a CTA
     unsigned vectors_inv;      // ceil(2^32 / (2 kv_heads)): x / (2 kv_heads) = high half of the product, x < 2^16
 };
 
-// Offsets of row r's page and row in it; off < 0: it has no place. The whole warp calls it, lane i for its own row
-// (r < 0: none); rows of a warp are consecutive.
-__device__ __forceinline__ void paged_places(const PagedCache& c, const PagedBatch& b, int r, int lane, long long& off,
-                                             long long& s_off)
+// Where a CTA's rows belong: offsets of the page and the row in it, for the elements and for the scales.
+struct PagedPlace {
+    long long off, s_off;   // off < 0: nowhere
+};
+// The place of row r (r < 0: none), by a whole warp, a consecutive row for each of its lanes.
+__device__ __forceinline__ void paged_find_place(const PagedCache& c, const PagedBatch& b, int r, int lane, PagedPlace& o)
 {
-    off = -1;
-    s_off = 0;
+    o.off = -1;
+    o.s_off = 0;
     int s = paged_find_seq(b, __shfl_sync(0xffffffffu, r, 0), lane);   // of the first row
     if (r < 0 || r >= b.rows) return;
     s = max(s, 0);
@@ -299,8 +321,19 @@ __device__ __forceinline__ void paged_places(const PagedCache& c, const PagedBat
         paged_status(c.status, kPagedBadPage);
         return;
     }
-    off = pg * c.page_stride + in * c.row_stride;
-    s_off = pg * c.s_page_stride + in * c.s_row_stride;
+    o.off = pg * c.page_stride + in * c.row_stride;
+    o.s_off = pg * c.s_page_stride + in * c.s_row_stride;
+}
+__device__ __forceinline__ void paged_places(const PagedCache& c, const PagedBatch& b, int r0, int n_rows, PagedPlace* places)
+{
+    if (threadIdx.x < 32)
+    {
+        const int lane = threadIdx.x;
+        PagedPlace o;
+        paged_find_place(c, b, lane < n_rows ? r0 + lane : -1, lane, o);
+        if (lane < kRowsPerCta) places[lane] = o;
+    }
+    __syncthreads();
 }
 
 // Vector x of a CTA's rows: row x / (2 kv_heads), k or v, head.
@@ -315,10 +348,11 @@ __device__ __forceinline__ PagedVector paged_vector(const PagedRowArgs& a, int x
     const bool isv = y >= a.c.kv_heads;
     return {row, isv ? y - a.c.kv_heads : y, isv};
 }
-__device__ __forceinline__ long long paged_row_at(const PagedRowArgs& a, const PagedVector& v, int r0)
+template <typename RT>
+__device__ __forceinline__ RT* paged_row_at(const PagedRowArgs& a, const PagedVector& v, int r0)
 {
-    const long long r = r0 + v.row;
-    return v.isv ? r * a.v_row_stride + v.head * a.v_head_stride : r * a.k_row_stride + v.head * a.k_head_stride;
+    RT* const p = static_cast<RT*>(v.isv ? a.v : a.k) + static_cast<long long>(r0 + v.row) * (v.isv ? a.v_row_stride : a.k_row_stride);
+    return p + static_cast<long long>(v.head) * (v.isv ? a.v_head_stride : a.k_head_stride);
 }
 
 template <typename RT, typename CT, int D>
@@ -332,32 +366,34 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const Paged
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r0 = blockIdx.x * a.per_cta, n_rows = min(a.per_cta, a.b.rows - r0);
     const int nv = n_rows * 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+    __shared__ PagedPlace places[kRowsPerCta];
     pdl_wait();
-    uint4 x[U];
-    auto load = [&](int v0) {
+    uint4 x[U], next[U];
+    auto load = [&](int v0, uint4 (&to)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
             const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
             if (i >= nv) continue;
             const PagedVector v = paged_vector(a, i);
-            x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const RT*>(v.isv ? a.v : a.k) + paged_row_at(a, v, r0) + d));
+            to[u] = __ldg(reinterpret_cast<const uint4*>(paged_row_at<const RT>(a, v, r0) + d));
         }
     };
-    load(0);   // ahead of the look-ups: the values do not depend on them
-    long long off, s_off;
-    paged_places(a.c, a.b, lane < n_rows ? r0 + lane : -1, lane, off, s_off);
+    load(0, next);   // ahead of the look-ups: the values do not depend on them
+    paged_places(a.c, a.b, r0, n_rows, places);
     for (int v0 = 0; v0 < nv; v0 += STEP)
     {
-        if (v0) load(v0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = next[u];
+        if (v0 + STEP < nv) load(v0 + STEP, next);
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
             const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
             const PagedVector v = paged_vector(a, min(i, nv - 1));
-            const long long o = __shfl_sync(0xffffffffu, off, v.row), so = __shfl_sync(0xffffffffu, s_off, v.row);
-            const bool live = i < nv && o >= 0;
-            const long long at = o + v.head * a.c.head_stride + d;
+            const PagedPlace o = places[v.row];
+            const bool live = i < nv && o.off >= 0;
+            const long long at = o.off + static_cast<long long>(v.head) * a.page_head_stride + d;
             void* const pool = v.isv ? a.c.v : a.c.k;
             float f[E];
             const uint32_t w4[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
@@ -368,29 +404,29 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const Paged
             {
                 // The largest magnitude by its bits: an infinity or a NaN comes out on top.
                 uint32_t m = 0;
+                if constexpr (E == 8)   // two bf16 to a word
+                {
 #pragma unroll
-                for (int e = 0; e < E; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
+                    for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w4[e] & 0x7fff7fffu);
+                    m = max(m << 16, m & 0x7fff0000u);
+                }
+                else
+#pragma unroll
+                    for (int e = 0; e < E; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
 #pragma unroll
                 for (int w = LPV / 2; w > 0; w >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, w));
                 const bool finite = m < 0x7f800000u;
-                const float scale =
-                    finite ? fmaxf(__fdiv_rn(__uint_as_float(m), kCodeMax<CT>), 1.17549435e-38f) : __int_as_float(0x7fffffff);
-                const float inv = __fdiv_rn(1.f, scale);
+                const float scale = finite ? code_scale<CT>(__uint_as_float(m)) : __int_as_float(0x7fffffff);
+                const float inv = __fdividef(1.f, scale);   // (scale < 2^126; off by 2 ulp, which quant4 allows for)
                 if (live)
                 {
                     uint32_t w[E / 4];
 #pragma unroll
-                    for (int y = 0; y < E / 4; ++y)
-                    {
-                        w[y] = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (finite) w[y] |= quant<CT>(f[4 * y + e], scale, inv) << (8 * e);
-                    }
+                    for (int y = 0; y < E / 4; ++y) w[y] = finite ? quant4<CT>(f + 4 * y, scale, inv) : 0u;
                     uint8_t* p = static_cast<uint8_t*>(pool) + at;
                     if constexpr (E == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
                     else *reinterpret_cast<uint32_t*>(p) = w[0];
-                    if (lane % LPV == 0) (v.isv ? a.c.v_scale : a.c.k_scale)[so + v.head * a.c.s_head_stride] = scale;
+                    if (lane % LPV == 0) (v.isv ? a.c.v_scale : a.c.k_scale)[o.s_off + static_cast<long long>(v.head) * a.scale_head_stride] = scale;
                 }
             }
             else
@@ -413,9 +449,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r0 = blockIdx.x * a.per_cta, n_rows = min(a.per_cta, a.b.rows - r0);
     const int nv = n_rows * 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
+    __shared__ PagedPlace places[kRowsPerCta];
     pdl_wait();
-    long long off, s_off;
-    paged_places(a.c, a.b, lane < n_rows ? r0 + lane : -1, lane, off, s_off);
+    paged_places(a.c, a.b, r0, n_rows, places);
     for (int v0 = 0; v0 < nv; v0 += STEP)
     {
         uint32_t x[U][W];
@@ -424,10 +460,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
         for (int u = 0; u < U; ++u)
         {
             const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
-            const PagedVector v = paged_vector(a, min(i, nv - 1));
-            const long long o = __shfl_sync(0xffffffffu, off, v.row), so = __shfl_sync(0xffffffffu, s_off, v.row);
-            if (i >= nv || o < 0) continue;
-            const CT* const p = static_cast<const CT*>(v.isv ? a.c.v : a.c.k) + o + v.head * a.c.head_stride + d;
+            if (i >= nv) continue;
+            const PagedVector v = paged_vector(a, i);
+            const PagedPlace o = places[v.row];
+            if (o.off < 0) continue;
+            const CT* const p = static_cast<const CT*>(v.isv ? a.c.v : a.c.k) + o.off + static_cast<long long>(v.head) * a.page_head_stride + d;
             if constexpr (W == 1) x[u][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
             else if constexpr (W == 2)
             {
@@ -441,14 +478,15 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
                     const uint4 y = __ldg(reinterpret_cast<const uint4*>(p) + w / 4);
                     x[u][w] = y.x; x[u][w + 1] = y.y; x[u][w + 2] = y.z; x[u][w + 3] = y.w;
                 }
-            if constexpr (kCodes<CT>) scale[u] = __ldg((v.isv ? a.c.v_scale : a.c.k_scale) + so + v.head * a.c.s_head_stride);
+            if constexpr (kCodes<CT>) scale[u] = __ldg((v.isv ? a.c.v_scale : a.c.k_scale) + o.s_off + static_cast<long long>(v.head) * a.scale_head_stride);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
             const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
-            const PagedVector v = paged_vector(a, min(i, nv - 1));
-            if (__shfl_sync(0xffffffffu, off, v.row) < 0 || i >= nv) continue;
+            if (i >= nv) continue;
+            const PagedVector v = paged_vector(a, i);
+            if (places[v.row].off < 0) continue;
             float f[E];
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -460,7 +498,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
             if constexpr (kCodes<CT>)
 #pragma unroll
                 for (int e = 0; e < E; ++e) f[e] *= scale[u];
-            store_row<RT, E>(v.isv ? a.v : a.k, paged_row_at(a, v, r0) + d, f);
+            store_row<RT, E>(paged_row_at<RT>(a, v, r0), d, f);
         }
     }
 }
