@@ -268,7 +268,7 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     const int group = q_heads / cache->num_kv_heads;
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
-                          power_of_two(cache->page_size), scale * 1.4426950408889634f, workspace_dev};
+                          power_of_two(cache->page_size), power_of_two(group), scale * 1.4426950408889634f, workspace_dev};
     const int cols = tile_columns(batch->max_rows, group, dtype, cache->dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto launch = dtype == HY_DTYPE_F32 ? hy_internal::paged_attention_f32 : hy_internal::paged_attention_bf16;

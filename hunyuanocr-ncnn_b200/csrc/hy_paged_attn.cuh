@@ -22,10 +22,13 @@ struct PagedAttnArgs {
     long long q_row_stride, q_head_stride, o_row_stride, o_head_stride;
     int q_heads, group;   // group = q_heads / kv_heads
     int causal, window, sinks;
-    int page_shift;       // log2(page_size), or -1
+    int page_shift, group_shift;   // log2 of page_size and of group, or -1
     float scale_log2;     // scale * log2(e)
     void* work;           // workspace
 };
+
+// Row of column c.
+__device__ __forceinline__ int paged_row_of(const PagedAttnArgs& a, int c) { return a.group_shift >= 0 ? c >> a.group_shift : c / a.group; }
 
 // The keys that the columns [c0, c0 + cols) of a sequence see. A column is a
 // (row, head of the group) pair: column c is row c / group.
@@ -39,8 +42,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
 {
     PagedSpan o;
     const int last = min(s.n * a.group, c0 + cols) - 1;
-    o.p_first = s.kv - s.n + c0 / a.group;
-    o.p_last = s.kv - s.n + last / a.group;
+    o.p_first = s.kv - s.n + paged_row_of(a, c0);
+    o.p_last = s.kv - s.n + paged_row_of(a, last);
     const int hi = o.p_last < 0 ? 0 : a.causal ? o.p_last + 1 : s.kv;
     o.lo = (a.window > 0) ? min(hi, max(0, o.p_first - a.window + 1)) / ALIGN * ALIGN : 0;
     o.sinks = a.sinks >= o.lo ? o.lo : (a.sinks + ALIGN - 1) / ALIGN * ALIGN;
@@ -223,12 +226,12 @@ __device__ __forceinline__ int split_key(const SplitItem& it, int u) { return u 
 // Row tensor offset of column c of an item.
 __device__ __forceinline__ long long split_q_at(const PagedAttnArgs& a, const SplitItem& it, int tile_cols, int c)
 {
-    const int cc = it.tile * tile_cols + c, row = cc / a.group;
+    const int cc = it.tile * tile_cols + c, row = paged_row_of(a, cc);
     return (it.q.row0 + row) * a.q_row_stride + (it.head * a.group + cc - row * a.group) * a.q_head_stride;
 }
 __device__ __forceinline__ int split_pos(const PagedAttnArgs& a, const SplitItem& it, int tile_cols, int c)
 {
-    return c < it.cols ? it.q.kv - it.q.n + (it.tile * tile_cols + c) / a.group : -1;
+    return c < it.cols ? it.q.kv - it.q.n + paged_row_of(a, it.tile * tile_cols + c) : -1;
 }
 // Every column sees every one of the KEYS keys from u0 on (`live` tells which are there).
 template <int KEYS>
@@ -1177,40 +1180,52 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
         float2* const ml = reinterpret_cast<float2*>(smem + Sh::ML_OFF);   // [warp][COLS]
         eng.put(it.cols, sums + warp * COLS * (D + 4), ml + warp * COLS);
         __syncthreads();
-        if (tid < COLS) colmax[tid] = 0;
         const bool complete = tile0 == 0 && tile1 == it.tiles;
         const int part_slot = 2 * blockIdx.x + (first ? 0 : 1);
         float* const part = parts + static_cast<long long>(part_slot) * Sh::PART;
-        for (int x = tid; x < it.cols * (D / 4); x += kSplitThreads)
+        if (tid < COLS)
         {
-            const int c = x / (D / 4), d = (x % (D / 4)) * 4;
+            colmax[tid] = 0;
+            // A column's joint (m, l), and the warps' factors in the place of their (m, l).
             float2 w[kSplitWarps];
-            float M = -INFINITY, L = 0.f, o[4] = {};
+            float M = -INFINITY, L = 0.f;
 #pragma unroll
             for (int k = 0; k < kSplitWarps; ++k)
             {
-                w[k] = ml[k * COLS + c];
+                w[k] = ml[k * COLS + tid];
                 M = fmaxf(M, w[k].x);
             }
 #pragma unroll
             for (int k = 0; k < kSplitWarps; ++k)
             {
-                const float f = w[k].x == M ? 1.f : ex2(w[k].x - M);
+                w[k].x = w[k].x == M ? 1.f : ex2(w[k].x - M);
+                L += w[k].x * w[k].y;
+            }
+            const float inv = !complete ? 1.f : L == 0.f ? 0.f : E::OUT / L;
+#pragma unroll
+            for (int k = 0; k < kSplitWarps; ++k) ml[k * COLS + tid].x = w[k].x * inv;
+            if (!complete && tid < it.cols) reinterpret_cast<float2*>(part)[tid] = make_float2(M, L);
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int x = tid; x < it.cols * (D / 4); x += kSplitThreads)
+        {
+            const int c = x / (D / 4), d = (x % (D / 4)) * 4;
+            float o[4] = {};
+#pragma unroll
+            for (int k = 0; k < kSplitWarps; ++k)
+            {
+                const float f = ml[k * COLS + c].x;
                 const float4 v = *reinterpret_cast<const float4*>(sums + (k * COLS + c) * (D + 4) + d);
-                L += f * w[k].y;
                 o[0] += f * v.x; o[1] += f * v.y; o[2] += f * v.z; o[3] += f * v.w;
             }
             if (complete)
             {
-                const float inv = L == 0.f ? 0.f : E::OUT / L;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] *= inv;
-                const int cc = it.tile * COLS + c, rw = cc / a.group;
+                const int cc = it.tile * COLS + c, rw = paged_row_of(a, cc);
                 store_row<QT, 4>(a.out, (it.q.row0 + rw) * a.o_row_stride + (it.head * a.group + cc - rw * a.group) * a.o_head_stride + d, o);
             }
             else
             {
-                if (d == 0) reinterpret_cast<float2*>(part)[c] = make_float2(M, L);
                 *reinterpret_cast<float4*>(part + 2 * COLS + c * D + d) = make_float4(o[0], o[1], o[2], o[3]);
             }
         }
@@ -1325,7 +1340,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     }
     const float inv = L == 0.f ? 0.f : E::OUT / L;
     const float r[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    const int cc = j.col0 + c, rw = cc / a.group;
+    const int cc = j.col0 + c, rw = paged_row_of(a, cc);
     store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + d, r);
 }
 
@@ -1395,7 +1410,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_wide_kernel(const Pag
         if (c >= j.cols) continue;
         const float inv = L[x] == 0.f ? 0.f : E::OUT / L[x];
         const float r[4] = {o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv};
-        const int cc = j.col0 + c, rw = cc / a.group;
+        const int cc = j.col0 + c, rw = paged_row_of(a, cc);
         store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + e % LANES * 4, r);
     }
 }

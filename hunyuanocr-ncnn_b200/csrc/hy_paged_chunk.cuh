@@ -245,7 +245,7 @@ struct ItemWalk {
     {
         if (it.cols <= i * 128) return 0;
         const int last = min(it.cols, i * 128 + 128) - 1;
-        const int p = it.q.kv - it.q.n + (it.tile * COLS + last) / a.group;
+        const int p = it.q.kv - it.q.n + paged_row_of(a, it.tile * COLS + last);
         const int hi = p < 0 ? 0 : a.causal ? p + 1 : it.q.kv;
         // (virtual positions below that of key hi)
         const int n = hi <= it.w.sinks ? hi : hi <= it.w.lo ? it.w.sinks : it.w.sinks + hi - it.w.lo;
@@ -820,10 +820,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             const int lim = it.lim[i];
             const bool col = c < it.cols;
             const int p_0 = it.kv - it.n;
-            const int p = col ? p_0 + (it.tile * 256 + c) / a.group : -1;
+            const int p = col ? p_0 + paged_row_of(a, it.tile * 256 + c) : -1;
             // The tile's first and last positions.
-            const int p_lo = p_0 + (it.tile * 256 + i * 128) / a.group;
-            const int p_hi = p_0 + (it.tile * 256 + min(it.cols, i * 128 + 128) - 1) / a.group;
+            const int p_lo = p_0 + paged_row_of(a, it.tile * 256 + i * 128);
+            const int p_hi = p_0 + paged_row_of(a, it.tile * 256 + min(it.cols, i * 128 + 128) - 1);
             auto key = [&](int u) { return u < it.sinks ? u : it.lo + u - it.sinks; };
             float m = -INFINITY, l = 0.f;
             for (int b = it.b0; b < lim && ok; ++b, ++seen)
@@ -1095,7 +1095,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             if (i * 128 < it.cols)
             {
                 if (col && !complete) reinterpret_cast<float2*>(part)[c] = make_float2(m, l);
-                const int cc = it.tile * 256 + c, rw = cc / a.group;
+                const int cc = it.tile * 256 + c, rw = paged_row_of(a, cc);
                 const long long at = (it.row0 + rw) * a.o_row_stride + (it.head * a.group + cc - rw * a.group) * a.o_head_stride;
 #pragma unroll 1
                 for (int x = 0; x < D / 32; ++x)
