@@ -980,6 +980,12 @@ __device__ __forceinline__ int split_row_tiles(const PagedAttnArgs& a, int n)
 template <int TILE>
 __device__ __forceinline__ int split_tiles(int keys) { return max(1, (keys + TILE - 1) / TILE); }
 
+// x / n where the quotient is small; 32-bit arithmetic where it reaches.
+__device__ __forceinline__ int split_div(long long x, int n)
+{
+    return x >> 31 ? static_cast<int>(x / n) : static_cast<int>(x) / n;
+}
+
 // Tiles of sequence s, all its items.
 template <int COLS, int TILE, int ALIGN>
 __device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
@@ -992,13 +998,55 @@ __device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
     return c * a.c.kv_heads;
 }
 
-// The CTA's range of tiles and the sequence of its first tile; every thread returns the same.
+// What the CTA takes of the list, and the sequence it starts in; every thread returns the same.
+// Where a few sequences of one tile of columns each make fewer items than CTAs, the list is counted in units of
+// several tiles of one item, so many that there are no more units than CTAs: every CTA has one unit, and none
+// begins a second item, whose loads would start from nothing (some 5 us). Otherwise the unit is a tile and a CTA
+// takes the next share of them.
 struct SplitStart {
-    long long x0, x1, total;   // the CTA's tiles; of all
-    long long in_seq;          // x0 counted from its sequence's first tile
-    long long share;           // tiles per CTA
+    long long x0, x1, total;   // the CTA's units; of all
+    long long in_seq;          // x0 counted from its sequence's first unit
+    long long share;           // units per CTA (1 where unit > 1)
+    int unit;                  // tiles per unit
     int seq;
 };
+// By every warp for itself; true if the list is of that kind.
+template <int COLS, int TILE, int ALIGN>
+__device__ __forceinline__ bool split_start_few(const PagedAttnArgs& a, SplitStart& o)
+{
+    const int lane = threadIdx.x & 31, ctas = gridDim.x, h = a.c.kv_heads;
+    PagedSeq q = {0, 0, 0};
+    const bool there = lane < a.b.num_seqs && paged_seq(a.b, lane, a.c.page_size, a.c.status, q) && q.n > 0;
+    const int t = there ? split_tiles<TILE>(paged_span<ALIGN>(a, q, 0, COLS).n) : 0;
+    const int all = __reduce_add_sync(0xffffffffu, min(t, 1 << 20));
+    const int items = __popc(__ballot_sync(0xffffffffu, there)) * h;
+    if (__any_sync(0xffffffffu, there && (q.n > COLS || q.n * a.group > COLS)) || items > ctas || all > (1 << 20) / h) return false;
+    int unit = max(1, (all * h + ctas - 1) / ctas), mine = 0, total = 0;
+    for (int tries = 0;; ++tries, ++unit)
+    {
+        if (tries == 6) return false;
+        mine = (t + unit - 1) / unit * h;
+        total = __reduce_add_sync(0xffffffffu, mine);
+        if (total <= ctas) break;
+    }
+    int inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1)
+    {
+        const int v = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += v;
+    }
+    const int x = blockIdx.x;
+    const unsigned in = __ballot_sync(0xffffffffu, x >= inc - mine && x < inc);
+    o.total = total;
+    o.share = 1;
+    o.unit = unit;
+    o.x0 = min(x, total);
+    o.x1 = min(x + 1, total);
+    o.seq = max(__ffs(in) - 1, 0);
+    o.in_seq = x - __shfl_sync(0xffffffffu, inc - mine, o.seq);
+    return true;
+}
 // scan: shared memory for a long long per warp and one more.
 template <int COLS, int TILE, int THREADS, int ALIGN = 1>
 __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long long* scan)
@@ -1007,6 +1055,8 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __shared__ int s_seq;
     SplitStart o;
+    if (a.b.num_seqs <= 32 && split_start_few<COLS, TILE, ALIGN>(a, o)) return o;
+    o.unit = 1;
     o.total = 0;
     const int rounds = (a.b.num_seqs + THREADS - 1) / THREADS;
     long long mine = 0;
@@ -1082,25 +1132,27 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
     // The first item.
     SplitItem it;
     it.seq = st.seq;
-    paged_seq(a.b, it.seq, a.c.page_size, nullptr, it.q);
+    if (!paged_seq(a.b, it.seq, a.c.page_size, nullptr, it.q)) return;   // (the arrays changed under the call)
     long long in = st.in_seq;
+    int units;
     for (it.tile = 0;; ++it.tile)
     {
         it.w = paged_span(a, it.q, it.tile * COLS, COLS);
         it.tiles = split_tiles<TILE>(it.w.n);
-        if (in < static_cast<long long>(it.tiles) * a.c.kv_heads) break;
+        units = (it.tiles + st.unit - 1) / st.unit;
+        if (in < static_cast<long long>(units) * a.c.kv_heads) break;
         if ((it.tile + 1) * COLS >= it.q.n * a.group) return;   // (the arrays changed under the call)
-        in -= static_cast<long long>(it.tiles) * a.c.kv_heads;
+        in -= static_cast<long long>(units) * a.c.kv_heads;
     }
-    it.head = static_cast<int>(in / it.tiles);
-    int tile0 = static_cast<int>(in - static_cast<long long>(it.head) * it.tiles);
+    it.head = split_div(in, units);
+    int tile0 = static_cast<int>(in - static_cast<long long>(it.head) * units) * st.unit;
 
     unsigned char* const ring = smem + warp * S * Sh::STAGE;
     const uint32_t ring_u = smem_u32(ring);
     const uint32_t sc_u = smem_u32(smem + Sh::SC_OFF + warp * S * Sh::SCALES);
     volatile uint32_t* const masks = reinterpret_cast<volatile uint32_t*>(smem + Sh::MASK_OFF) + warp * S;
 
-    long long left = st.x1 - st.x0;
+    long long left = (st.x1 - st.x0) * st.unit;   // tiles
     bool first = true;
     E eng;
     while (true)
@@ -1233,9 +1285,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
         if (!complete && tile0 == 0 && tid == 0)
         {
             // This CTA starts the item: its parts are here and in the CTAs up to the one with the item's last tile.
-            const long long x_last = st.x1 - left - n_tiles + it.tiles - 1;   // (global index of that tile)
             PagedJoin d;
-            d.count = static_cast<int>(x_last / st.share) - static_cast<int>(blockIdx.x) + 1;
+            if (st.unit > 1) d.count = units;
+            else d.count = static_cast<int>((st.x1 - left - n_tiles + it.tiles - 1) / st.share) - static_cast<int>(blockIdx.x) + 1;
             d.first_slot = part_slot;
             d.first_cta = blockIdx.x;
             d.row0 = it.q.row0;
@@ -1245,7 +1297,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
             d.pad = 0;
             *desc = d;
         }
-        if (left == 0) break;
+        if (left == 0 || st.unit > 1) break;
         first = false;
         // The next item: next head, next tile of columns, next sequence.
         tile0 = 0;

@@ -184,12 +184,14 @@ struct ItemWalk {
     SplitItem it;
     long long left;        // blocks of the share not yet walked over
     long long start;       // global index of the item's first block
+    int units;             // (single) CTAs that share the item
     int b0, b1;            // blocks of the item that are this CTA's
-    bool first;
+    bool first, single;    // single: no second item
 
     __device__ __forceinline__ bool open(const PagedAttnArgs& a, const SplitStart& st)
     {
-        left = st.x1 - st.x0;
+        left = (st.x1 - st.x0) * st.unit;
+        single = st.unit > 1;
         first = true;
         if (left <= 0) return false;
         it.seq = st.seq;
@@ -199,15 +201,21 @@ struct ItemWalk {
         {
             it.w = paged_span<16>(a, it.q, it.tile * COLS, COLS);
             it.tiles = split_tiles<TILE>(it.w.n);
-            if (in < static_cast<long long>(it.tiles) * a.c.kv_heads) break;
+            units = (it.tiles + st.unit - 1) / st.unit;
+            if (in < static_cast<long long>(units) * a.c.kv_heads) break;
             if ((it.tile + 1) * COLS >= it.q.n * a.group) return false;   // (the arrays changed under the call)
-            in -= static_cast<long long>(it.tiles) * a.c.kv_heads;
+            in -= static_cast<long long>(units) * a.c.kv_heads;
         }
-        it.head = static_cast<int>(in / it.tiles);
-        b0 = static_cast<int>(in - static_cast<long long>(it.head) * it.tiles);
+        it.head = split_div(in, units);
+        b0 = static_cast<int>(in - static_cast<long long>(it.head) * units) * st.unit;
         start = st.x0 - b0;
         set(a);
         return true;
+    }
+    // The CTA with the item's last block, where the item starts in CTA `cta`.
+    __device__ __forceinline__ int last_cta(const SplitStart& st, int cta) const
+    {
+        return single ? cta + units - 1 : static_cast<int>((start + it.tiles - 1) / max(1ll, st.share));
     }
     __device__ __forceinline__ void set(const PagedAttnArgs& a)
     {
@@ -217,7 +225,7 @@ struct ItemWalk {
     __device__ __forceinline__ bool next(const PagedAttnArgs& a)
     {
         left -= b1 - b0;
-        if (left <= 0) return false;
+        if (left <= 0 || single) return false;
         first = false;
         b0 = 0;
         start += it.tiles;
@@ -408,7 +416,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 d.first = w.first;
                 d.lim[0] = min(w.b1, w.blocks(a, 0));
                 d.lim[1] = min(w.b1, w.blocks(a, 1));
-                d.last_cta = static_cast<int>((w.start + w.it.tiles - 1) / max(1ll, st.share));
+                d.last_cta = w.last_cta(st, blockIdx.x);
                 if (!more || !ok_all) d.b1 = d.b0;
                 items_s[items & 1] = d;
             }
