@@ -51,10 +51,12 @@ struct ChunkEngine {
     static constexpr int SLOTS = F16 ? 3 : 4;              // ring of K and V blocks
     static constexpr int CODES_B = 128 * D, STAGES = F16 ? 3 : 0;   // staging ring of 8-bit blocks
     static constexpr int Q_OFF = 0, RING_OFF = 2 * TILE_B, STAGE_OFF = RING_OFF + SLOTS * TILE_B;
-    // Scales of the last 4 blocks: k, v times the weights' unit, exponent of v's (fp32, 128 each).
+    // Scales of the last 4 blocks: k, v times the weights' unit, exponent of v's (fp32, 128 each), in the order in
+    // which the softmax threads take them: key 16 k + 8 e + 2 t + b at 16 k + 4 t + 2 e + b.
     static constexpr int SCALE_B = 3 * 128 * 4, SCALE_OFF = STAGE_OFF + STAGES * CODES_B;
     static constexpr int LIVE_OFF = SCALE_OFF + (F16 ? 4 * SCALE_B : 0);   // [4 blocks][4] words, a bit for every key
-    static constexpr int QS_OFF = LIVE_OFF + 64;                           // [256] 2^-k of a column's q
+    static constexpr int EV_OFF = LIVE_OFF + 64;                           // [4 blocks][4] largest | smallest exponent << 16
+    static constexpr int QS_OFF = EV_OFF + 64;                           // [256] 2^-k of a column's q
     static constexpr int ITEM_OFF = QS_OFF + 1024;                         // [2] ChunkItem
     static constexpr int BAR_OFF = ITEM_OFF + 2 * 64;
     static constexpr int SMEM = BAR_OFF + 256 + 1024;                      // + alignment of the base to 1024
@@ -76,10 +78,11 @@ struct ChunkItem {
 constexpr int kChunkThreads = 16 * 32;
 constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 12;
 constexpr int kChunkCubic = 1, kChunkCubicOf = 4;   // pairs of weights by the cubic, of so many
-// Registers a thread: 128 at launch; 256 softmax threads take 184, the other 256 keep 72
-// (184 + 72 = 2 x 128: what one half gives up is what the other asks for).
-constexpr int kChunkRegsSoftmax = 184, kChunkRegsOther = 72;
-static_assert(kChunkRegsSoftmax + kChunkRegsOther == 2 * 128, "registers");
+// Registers a thread: 128 at launch; the 256 softmax threads take what the other 256 give up.
+template <bool F16>
+constexpr int kChunkRegsSoftmax = F16 ? 160 : 184;
+template <bool F16>
+constexpr int kChunkRegsOther = 2 * 128 - kChunkRegsSoftmax<F16>;
 template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -161,6 +164,32 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+// 16 lanes x 32 columns as a warp's matrix fragments: register 4 k + j of thread t is (row t / 4 + 8 (j / 2),
+// column 8 k + 2 (t % 4) + j % 2).
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// 16 lanes x 16 columns of packed pairs: register 2 k + j is (row t / 4 + 8 j, column 4 k + t % 4).
+__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int c1, int c2, int c3, uint64_t* bar)
 {
@@ -338,17 +367,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     uint64_t* const kv_empty = kv_full + 4;       // [4] products that read it are done
     uint64_t* const st_full = kv_empty + 4;       // [3] codes are in the staging ring; bf16: [0] a block to be mended
     uint64_t* const st_empty = st_full + 3;       // [3] codes were read (4 warps)
-    uint64_t* const q_full = st_empty + 3;        // q and the item's description are there (128)
+    uint64_t* const q_full = st_empty + 3;        // the item's description is there, and (bf16) q (128)
     uint64_t* const q_empty = q_full + 1;         // products with q are done, the description was read (256)
     uint64_t* const s_full = q_empty + 1;         // [2] scores are there
     uint64_t* const p_full = s_full + 2;          // [2] weights are there (128), output rescaled
     uint64_t* const o_full = p_full + 2;          // [2] weights times values added
-    uint64_t* const done = o_full + 2;            // every product is done
+    uint64_t* const q_ready = o_full + 2;         // 8-bit caches: q is there (256)
+    uint64_t* const done = q_ready + 1;           // every product is done
     int* const pv_skip = reinterpret_cast<int*>(done + 1);   // [2] this block's product was taken by the softmax warps
     uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(pv_skip + 2);
     float* const qscale = reinterpret_cast<float*>(smem + E::QS_OFF);
     ChunkItem* const items_s = reinterpret_cast<ChunkItem*>(smem + E::ITEM_OFF);
     volatile uint32_t* const live_w = reinterpret_cast<volatile uint32_t*>(smem + E::LIVE_OFF);
+    volatile int* const ev_range = reinterpret_cast<volatile int*>(smem + E::EV_OFF);
     __shared__ long long scan[kChunkThreads / 32 + 1];
     static_assert(sizeof(ChunkItem) == 64, "item ring");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -379,6 +410,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             mbar_init(&p_full[i], 128);
             mbar_init(&o_full[i], 1);
         }
+        mbar_init(q_ready, 256);
         mbar_init(done, 1);
         fence_mbar_init();
     }
@@ -394,7 +426,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     if (warp >= kChunkLoadWarp && warp < kChunkMmaWarp)
     {
         // ---------------- loads ----------------
-        regs_dec<kChunkRegsOther>();
+        regs_dec<kChunkRegsOther<F16>>();
         const int lt = tid - kChunkLoadWarp * 32, lw = lt >> 5;
         Walk w;
         bool more = w.open(a, st);
@@ -426,9 +458,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 break;
             }
             // q: rows of the two tiles, 256 columns, zero where there is no column.
-            constexpr int QP = E::RB / 16;   // 16-byte pieces of a row
             if constexpr (!F16)
             {
+                constexpr int QP = E::RB / 16;   // 16-byte pieces of a row
 #pragma unroll 4
                 for (int x = lt; x < 256 * QP; x += 128)
                 {
@@ -440,43 +472,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 cp_commit();
                 cp_wait<0>();
             }
-            else
-            {
-                // As f16, times the power of two that brings the column's largest magnitude to [2^14, 2^15).
-                constexpr int U = 8;
-#pragma unroll 1
-                for (int x0 = lt; x0 < 256 * QP; x0 += 128 * U)
-                {
-                    uint4 raw[U];
-#pragma unroll
-                    for (int y = 0; y < U; ++y)
-                    {
-                        const int c = (x0 + 128 * y) / QP, p = (x0 + 128 * y) % QP;
-                        raw[y] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
-                                                                     split_q_at(a, w.it, 256, min(c, w.it.cols - 1)) + p * 8));
-                        if (c >= w.it.cols) raw[y] = make_uint4(0, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int y = 0; y < U; ++y)
-                    {
-                        const int c = (x0 + 128 * y) / QP, p = (x0 + 128 * y) % QP;
-                        const uint32_t ws[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
-                        uint32_t m = 0, h[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) m = max(m, max((ws[e] << 16) & 0x7fffffffu, ws[e] & 0x7fff0000u));
-#pragma unroll
-                        for (int o = 1; o < QP; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        const uint32_t down = (min(max(m >> 23, 16u), 254u) - 14u) << 23;
-                        const float up = __uint_as_float((254u << 23) - down);
-                        if (p == 0) qscale[c] = __uint_as_float(down);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            h[e] = pack_f16(__uint_as_float(ws[e] << 16) * up, __uint_as_float(ws[e] & 0xFFFF0000u) * up);
-                        *reinterpret_cast<uint4*>(smem + E::Q_OFF + (c >> 7) * E::TILE_B + sw128_at(c & 127, p)) =
-                            make_uint4(h[0], h[1], h[2], h[3]);
-                    }
-                }
-            }
+            // (8-bit caches: the softmax warps write q, as f16)
             fence_async_smem();
             mbar_arrive(q_full);
 
@@ -671,27 +667,39 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             __syncwarp();
                         }
                         if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
-                        const uint32_t src = sm + E::STAGE_OFF + sg * E::CODES_B;
                         unsigned char* const dst = smem + E::RING_OFF + slot * E::TILE_B;
+                        uint4 v[CPR];
+#pragma unroll
+                        for (int x = 0; x < CPR; ++x)
+                        {
+                            const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
+                            v[x] = *reinterpret_cast<const uint4*>(smem + E::STAGE_OFF + sg * E::CODES_B + (lw * 32 + r) * D + c * 16);
+                            if (!((mask >> r) & 1u)) v[x] = make_uint4(0, 0, 0, 0);   // (rows behind the last key)
+                        }
 #pragma unroll
                         for (int x = 0; x < CPR; ++x)
                         {
                             const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR, rr = lw * 32 + r;
-                            uint4 v = lds128(src + rr * D + c * 16);
-                            if (!((mask >> r) & 1u)) v = make_uint4(0, 0, 0, 0);   // (rows behind the last key)
                             *reinterpret_cast<uint4*>(dst + sw128_at(rr, 2 * c)) =
-                                make_uint4(codes_f16<CT>(v.x), codes_f16<CT>(v.x >> 16), codes_f16<CT>(v.y), codes_f16<CT>(v.y >> 16));
+                                make_uint4(codes_f16<CT>(v[x].x), codes_f16<CT>(v[x].x >> 16), codes_f16<CT>(v[x].y), codes_f16<CT>(v[x].y >> 16));
                             *reinterpret_cast<uint4*>(dst + sw128_at(rr, 2 * c + 1)) =
-                                make_uint4(codes_f16<CT>(v.z), codes_f16<CT>(v.z >> 16), codes_f16<CT>(v.w), codes_f16<CT>(v.w >> 16));
+                                make_uint4(codes_f16<CT>(v[x].z), codes_f16<CT>(v[x].z >> 16), codes_f16<CT>(v[x].w), codes_f16<CT>(v[x].w >> 16));
                         }
                         if (kv == 0)
                         {
                             // (entries of a block are written when the one four before it is long used)
                             float* const sc = reinterpret_cast<float*>(smem + E::SCALE_OFF + (blk & 3) * E::SCALE_B);
-                            sc[lt] = ks;
-                            sc[128 + lt] = vs * 64.f;
-                            sc[256 + lt] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(vs) >> 23) - 127, -100), 100));
-                            if (lane == 0) live_w[(blk & 3) * 4 + lw] = mask;
+                            const int at = (lt >> 4) * 16 + ((lt >> 1) & 3) * 4 + ((lt >> 3) & 1) * 2 + (lt & 1);
+                            const int ev = min(max(static_cast<int>(__float_as_uint(vs) >> 23) - 127, -100), 100);
+                            sc[at] = ks;
+                            sc[128 + at] = vs * 64.f;
+                            sc[256 + at] = static_cast<float>(ev);
+                            const int hi = __reduce_max_sync(0xffffffffu, ok ? ev : -100), lo = __reduce_min_sync(0xffffffffu, ok ? ev : 100);
+                            if (lane == 0)
+                            {
+                                live_w[(blk & 3) * 4 + lw] = mask;
+                                ev_range[(blk & 3) * 4 + lw] = (hi & 0xffff) | (lo << 16);
+                            }
                         }
                         fence_async_smem();
                         mbar_arrive(&kv_full[slot]);
@@ -707,7 +715,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     else if (warp >= kChunkMmaWarp)
     {
         // ---------------- products ----------------
-        regs_dec<kChunkRegsOther>();
+        regs_dec<kChunkRegsOther<F16>>();
         if (warp == kChunkMmaWarp)
         {
             // The whole warp walks, waits and computes addresses, so that they stay in uniform registers; one
@@ -760,6 +768,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 const int b0 = __shfl_sync(0xffffffffu, it.b0, 0), n_blk = __shfl_sync(0xffffffffu, it.b1, 0) - b0;
                 const int lim[2] = {__shfl_sync(0xffffffffu, it.lim[0], 0), __shfl_sync(0xffffffffu, it.lim[1], 0)};
                 if (n_blk <= 0) break;
+                if constexpr (F16) ok = __all_sync(0xffffffffu, mbar_wait_spin(q_ready, items & 1, a.c.status, kPagedTimeout));
                 full(2 * nb);
                 if (!ok) break;
 #pragma unroll
@@ -810,7 +819,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     else
     {
         // ---------------- softmax of tile i, one thread per column ----------------
-        regs_inc<kChunkRegsSoftmax>();
+        regs_inc<kChunkRegsSoftmax<F16>>();
         const int i = warp >> 2, c_in = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + E::S_COL + i * 128 + lanes, to = tmem + E::O_COL + i * 128 + lanes;
@@ -822,18 +831,51 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             if (!ok) break;
             const ChunkItem it = items_s[items & 1];
             const int c = i * 128 + c_in;
-            const float fac = F16 ? a.scale_log2 * qscale[c] : a.scale_log2;
             mbar_arrive(q_empty);
             if (it.b1 == it.b0) break;
             const int lim = it.lim[i];
             const bool col = c < it.cols;
             const int p_0 = it.kv - it.n;
-            const int p = col ? p_0 + paged_row_of(a, it.tile * 256 + c) : -1;
             // The tile's first and last positions.
             const int p_lo = p_0 + paged_row_of(a, it.tile * 256 + i * 128);
             const int p_hi = p_0 + paged_row_of(a, it.tile * 256 + min(it.cols, i * 128 + 128) - 1);
             auto key = [&](int u) { return u < it.sinks ? u : it.lo + u - it.sinks; };
             float m = -INFINITY, l = 0.f;
+            // The keys that position pos sees of the 32 from virtual position u on, a bit each. They are (part of) the run
+            // of sinks, then (part of) the window's: of either, the keys from the position's window on, and the sinks, up
+            // to the position itself.
+            auto see_word = [&](int pos, int u) {
+                auto below = [](int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; };   // bits 0 .. x - 1
+                const int split = it.sinks - u;   // keys that belong to the first run
+                const int last = pos < 0 ? -1 : a.causal ? pos : it.kv - 1, from = a.window > 0 ? pos - a.window + 1 : 0;
+                const int k1 = u, k2 = it.lo - split;   // key of bit 0 in the first and in the second run
+                uint32_t in1 = below(last + 1 - k1), in2 = below(last + 1 - k2);
+                if (a.window > 0)
+                {
+                    in1 &= ~below(from - k1) | below(a.sinks - k1);
+                    in2 &= ~below(from - k2) | below(a.sinks - k2);
+                }
+                const uint32_t one = below(split);
+                return (in1 & one) | (in2 & ~one);
+            };
+            // Every column of the tile sees every key of block u0, whose bits are `vis`.
+            auto sees_all = [&](int u0, const uint32_t (&vis)[4]) {
+                const int j_first = key(u0), j_last = key(min(u0 + 127, it.keys - 1));
+                return (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu && p_lo >= 0 &&
+                       (!a.causal || (j_last <= p_lo && (a.window == 0 || j_first > p_hi - a.window || j_last < a.sinks)));
+            };
+            // Of values that are in the fragments' threads, this thread's column's.
+            auto of_row = [&](const float (&v)[4]) {
+                float x[4];
+#pragma unroll
+                for (int f = 0; f < 4; ++f) x[f] = __shfl_sync(0xffffffffu, v[f], (lane & 7) * 4);
+                const int f = lane >> 3;
+                return f == 0 ? x[0] : f == 1 ? x[1] : f == 2 ? x[2] : x[3];
+            };
+            if constexpr (!F16)
+            {
+            const float fac = a.scale_log2;
+            const int p = col ? p_0 + paged_row_of(a, it.tile * 256 + c) : -1;
             for (int b = it.b0; b < lim && ok; ++b, ++seen)
             {
                 const int blk = nb + b - it.b0, ring = blk & 3, vslot = (2 * blk + 1) % SLOTS;
@@ -852,56 +894,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 tmem_ld32(ts + 32, r1);
                 tmem_ld32(ts + 64, r2);
                 tmem_ld32(ts + 96, r3);
-                const float4* const sc = reinterpret_cast<const float4*>(smem + E::SCALE_OFF + ring * E::SCALE_B);
-                const int u0 = b * 128, j_first = key(u0), j_last = key(min(u0 + 127, it.keys - 1));
+                const int u0 = b * 128;
                 uint32_t vis[4];   // what the column sees, a bit per key
                 {
                     const uint4 x = lds128(sm + E::LIVE_OFF + ring * 16);
                     vis[0] = x.x; vis[1] = x.y; vis[2] = x.z; vis[3] = x.w;
                 }
-                const bool whole = (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu && p_lo >= 0 &&
-                                   (!a.causal || (j_last <= p_lo && (a.window == 0 || j_first > p_hi - a.window || j_last < a.sinks)));
+                const bool whole = sees_all(u0, vis);
                 bool odd = false;
                 tmem_ld32_wait(r0);
                 tmem_ld32_wait(r1);
                 tmem_ld32_wait(r2);
                 tmem_ld32_wait(r3);
-                if constexpr (F16)
-                {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                    {
-                        const float4 k = sc[e];
-                        r[4 * e] = __float_as_uint(__uint_as_float(r[4 * e]) * k.x);
-                        r[4 * e + 1] = __float_as_uint(__uint_as_float(r[4 * e + 1]) * k.y);
-                        r[4 * e + 2] = __float_as_uint(__uint_as_float(r[4 * e + 2]) * k.z);
-                        r[4 * e + 3] = __float_as_uint(__uint_as_float(r[4 * e + 3]) * k.w);
-                    }
-                }
                 if (!whole)
                 {
-                    // The block is (part of) the run of sinks, then (part of) the window's: of either, the keys
-                    // from the column's window on, and the sinks, up to the column's own position.
-                    auto below = [](int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; };   // bits 0 .. x - 1
-                    const int split = it.sinks - u0;   // keys of the block that belong to the first run
-                    const int last = p < 0 ? -1 : a.causal ? p : it.kv - 1, from = a.window > 0 ? p - a.window + 1 : 0;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                    {
-                        const int o = 32 * x, k1 = u0 + o, k2 = it.lo - split + o;   // key of bit 0 in the first and in the second run
-                        uint32_t in1 = below(last + 1 - k1), in2 = below(last + 1 - k2);
-                        if (a.window > 0)
-                        {
-                            in1 &= ~below(from - k1) | below(a.sinks - k1);
-                            in2 &= ~below(from - k2) | below(a.sinks - k2);
-                        }
-                        const uint32_t one = below(split - o);
-                        vis[x] &= (in1 & one) | (in2 & ~one);
-                    }
+                    for (int x = 0; x < 4; ++x) vis[x] &= see_word(p, u0 + 32 * x);
 #pragma unroll
                     for (int e = 0; e < 128; ++e)
                         if (!((vis[e >> 5] >> (e & 31)) & 1u)) r[e] = 0xff800000u;   // -inf
-                    if constexpr (!F16)
                     {
                         // 0 times an infinity or NaN is NaN, so a block that some column must not see all of and
                         // that holds such values is not for the tensor cores.
@@ -925,23 +936,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 float top;
                 {
                     float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
-                    auto z = [&](int e, float ev) { return F16 ? fmaf(__uint_as_float(r[e]), fac, ev) : __uint_as_float(r[e]); };
+                    auto z = [&](int e) { return __uint_as_float(r[e]); };
 #pragma unroll
                     for (int e = 0; e < 128; e += 8)
                     {
-                        float4 v0 = make_float4(0, 0, 0, 0), v1 = v0;
-                        if constexpr (F16)
-                        {
-                            v0 = sc[64 + e / 4];
-                            v1 = sc[65 + e / 4];
-                        }
-                        t0 = max3_nan(t0, z(e, v0.x), z(e + 1, v0.y));
-                        t1 = max3_nan(t1, z(e + 2, v0.z), z(e + 3, v0.w));
-                        t2 = max3_nan(t2, z(e + 4, v1.x), z(e + 5, v1.y));
-                        t3 = max3_nan(t3, z(e + 6, v1.z), z(e + 7, v1.w));
+                        t0 = max3_nan(t0, z(e), z(e + 1));
+                        t1 = max3_nan(t1, z(e + 2), z(e + 3));
+                        t2 = max3_nan(t2, z(e + 4), z(e + 5));
+                        t3 = max3_nan(t3, z(e + 6), z(e + 7));
                     }
                     top = max3_nan(max3_nan(t0, t1, t2), t3, t3);
-                    if constexpr (!F16) top *= fac;
+                    top *= fac;
                 }
                 if (top == INFINITY) top = __int_as_float(0x7fffffff);   // inf - inf
                 // A new reference only where the maximum has grown by more than 2^8 (or there was none); a NaN becomes one.
@@ -1002,26 +1007,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         }
                         if (e & 1) sum1 = f2_add(sum1, y);
                         else sum0 = f2_add(sum0, y);
-                        if constexpr (F16)
-                        {
-                            const float2 v = reinterpret_cast<const float2*>(sc)[64 + e];
-                            y = f2_mul(y, f2(v.x, v.y));
-                        }
                         f2_get(y, w0, w1);
-                        if constexpr (F16)
-                        {
-                            // (a scale of NaN must not meet a weight of zero that stands for "not seen")
-                            if constexpr (!PLAIN)
-                            {
-                                if (!((vis[e >> 4] >> (2 * e & 31)) & 1u)) w0 = 0.f;
-                                if (!((vis[e >> 4] >> ((2 * e + 1) & 31)) & 1u)) w1 = 0.f;
-                            }
-                            r[e] = pack_f16(w0, w1);
-                        }
-                        else
-                        {
-                            r[e] = pack_bf16(w0, w1);
-                        }
+                        r[e] = pack_bf16(w0, w1);
                         if (e == 31) tmem_st32(ts + 64, *reinterpret_cast<uint32_t(*)[32]>(r));
                     }
                 };
@@ -1033,7 +1020,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 f2_get(sum1, s2, s3);
                 l += (s0 + s1) + (s2 + s3);
                 tmem_st_wait();
-                if constexpr (!F16)
                 {
                     if (odd)
                     {
@@ -1085,6 +1071,275 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[i]);
+            }
+            }
+            else
+            {
+                // 8-bit caches: every score and weight meets its key's scales. With a column to a thread those
+                // would be 128 loads a thread and array - more shared-memory time than the products take -, so
+                // the scores are taken as matrix fragments: a thread has 32 keys of 4 columns, 8 f + lane / 4.
+                {
+                    // q of this thread's column as f16, times the power of two that brings its largest magnitude to
+                    // [2^14, 2^15). (This tile's products with the last item's q are done: their scores were read.)
+                    constexpr int QP = E::RB / 16;   // 16-byte pieces of a row
+                    const uint4* const src = reinterpret_cast<const uint4*>(
+                        static_cast<const __nv_bfloat16*>(a.q) + (it.row0 + paged_row_of(a, it.tile * 256 + min(c, it.cols - 1))) * a.q_row_stride +
+                        (it.head * a.group + it.tile * 256 + min(c, it.cols - 1) - paged_row_of(a, it.tile * 256 + min(c, it.cols - 1)) * a.group) * a.q_head_stride);
+                    uint4 raw[QP];
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int x = 0; x < QP; ++x) raw[x] = __ldg(src + x);
+#pragma unroll
+                    for (int x = 0; x < QP; ++x)
+                    {
+                        if (!col) raw[x] = make_uint4(0, 0, 0, 0);
+                        top = __vmaxu2(top, __vmaxu2(__vmaxu2(raw[x].x & 0x7fff7fffu, raw[x].y & 0x7fff7fffu),
+                                                     __vmaxu2(raw[x].z & 0x7fff7fffu, raw[x].w & 0x7fff7fffu)));
+                    }
+                    top = max(top << 16, top & 0x7fff0000u);
+                    const uint32_t down = (min(max(top >> 23, 16u), 254u) - 14u) << 23;
+                    const float up = __uint_as_float((254u << 23) - down);
+                    qscale[c] = __uint_as_float(down);
+#pragma unroll
+                    for (int x = 0; x < QP; ++x)
+                    {
+                        auto half = [&](uint32_t w) { return pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xFFFF0000u) * up); };
+                        *reinterpret_cast<uint4*>(smem + E::Q_OFF + i * E::TILE_B + sw128_at(c_in, x)) =
+                            make_uint4(half(raw[x].x), half(raw[x].y), half(raw[x].z), half(raw[x].w));
+                    }
+                    fence_async_smem();
+                    mbar_arrive(q_ready);
+                    __syncwarp();
+                }
+                const int c_0 = i * 128 + (warp & 3) * 32 + (lane >> 2);   // column of f = 0
+                float fac[4], mf[4], lf[4];
+                int pos[4];
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                {
+                    fac[f] = a.scale_log2 * qscale[c_0 + 8 * f];
+                    pos[f] = c_0 + 8 * f < it.cols ? p_0 + paged_row_of(a, it.tile * 256 + c_0 + 8 * f) : -1;
+                    mf[f] = -INFINITY;
+                    lf[f] = 0.f;
+                }
+                for (int b = it.b0; b < lim && ok; ++b, ++seen)
+                {
+                    const int blk = nb + b - it.b0, ring = blk & 3, vslot = (2 * blk + 1) % SLOTS;
+                    ok = mbar_wait(&kv_full[vslot], ((2 * blk + 1) / SLOTS) & 1, a.c.status, kPagedTimeout) &&
+                         mbar_wait(&s_full[i], seen & 1, a.c.status, kPagedTimeout);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float4* const sc = reinterpret_cast<const float4*>(smem + E::SCALE_OFF + ring * E::SCALE_B) + (lane & 3);
+                    uint32_t live[4];
+                    int ev_hi, ev_lo;
+                    {
+                        const uint4 x = lds128(sm + E::LIVE_OFF + ring * 16);
+                        live[0] = x.x; live[1] = x.y; live[2] = x.z; live[3] = x.w;
+                        const uint4 y = lds128(sm + E::EV_OFF + ring * 16);
+                        ev_hi = max(max(static_cast<short>(y.x), static_cast<short>(y.y)), max(static_cast<short>(y.z), static_cast<short>(y.w)));
+                        ev_lo = min(min(static_cast<int>(y.x) >> 16, static_cast<int>(y.y) >> 16), min(static_cast<int>(y.z) >> 16, static_cast<int>(y.w) >> 16));
+                    }
+                    const bool whole = sees_all(b * 128, live);
+                    // The reference takes in the exponents of the values' scales. Where they are close, the block's
+                    // largest serves every key (weights are then smaller by 2^12 at most); it must be of keys that the columns see.
+                    const bool tight = whole && ev_hi - ev_lo <= 12;
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    // First pass, 32 keys at a time (loops, not straight code: four roles' instructions compete for the
+                    // instruction cache): scores times their keys' scales, masked, back to tensor memory; the maxima.
+                    uint32_t r[2][16], next[2][16];   // [h]: columns f = 2 h, 2 h + 1
+                    auto fetch = [&](int x, uint32_t (&to)[2][16]) {
+                        tmem_ld_frag(ts + 32 * x, to[0]);
+                        tmem_ld_frag(ts + 32 * x + (16u << 16), to[1]);
+                    };
+                    auto take = [&]() {
+                        tmem_ld_wait(next[0]);
+                        tmem_ld_wait(next[1]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) r[h][e] = next[h][e];
+                    };
+                    fetch(0, next);
+                    take();
+#pragma unroll 1
+                    for (int x = 0; x < 4; ++x)
+                    {
+                        fetch(min(x + 1, 3), next);   // (the last round's is not used)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                        {
+                            const float4 ks = sc[4 * (2 * x + k)];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                for (int f = 0; f < 4; ++f)
+                                {
+                                    const int at = 8 * k + 4 * e + 2 * (f & 1);
+                                    uint32_t(&q)[16] = r[f >> 1];
+                                    float u, v;
+                                    f2_get(f2_mul(f2(__uint_as_float(q[at]), __uint_as_float(q[at + 1])), e ? f2(ks.z, ks.w) : f2(ks.x, ks.y)), u, v);
+                                    q[at] = __float_as_uint(u);
+                                    q[at + 1] = __float_as_uint(v);
+                                }
+                        }
+                        if (!whole)
+                        {
+                            const uint32_t here = x == 0 ? live[0] : x == 1 ? live[1] : x == 2 ? live[2] : live[3];
+#pragma unroll
+                            for (int f = 0; f < 4; ++f)
+                            {
+                                const uint32_t v = (here & see_word(pos[f], b * 128 + 32 * x)) >> (2 * (lane & 3));
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)   // key 8 (e / 2) + e % 2 + 2 (lane % 4)
+                                    if (!((v >> (8 * (e >> 1) + (e & 1))) & 1u)) r[f >> 1][4 * (e >> 1) + 2 * (f & 1) + (e & 1)] = 0xff800000u;   // -inf
+                            }
+                        }
+                        if (tight)
+                        {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                                for (int f = 0; f < 4; ++f)
+                                    top[f] = max3_nan(top[f], __uint_as_float(r[f >> 1][4 * k + 2 * (f & 1)]), __uint_as_float(r[f >> 1][4 * k + 2 * (f & 1) + 1]));
+                        }
+                        else
+                        {
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                            {
+                                const float4 ev = sc[64 + 4 * (2 * x + k)];
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                    for (int f = 0; f < 4; ++f)
+                                    {
+                                        const int at = 8 * k + 4 * e + 2 * (f & 1);
+                                        top[f] = max3_nan(top[f], fmaf(__uint_as_float(r[f >> 1][at]), fac[f], e ? ev.z : ev.x),
+                                                          fmaf(__uint_as_float(r[f >> 1][at + 1]), fac[f], e ? ev.w : ev.y));
+                                    }
+                            }
+                        }
+                        tmem_st_frag(ts + 32 * x, r[0]);
+                        tmem_st_frag(ts + 32 * x + (16u << 16), r[1]);
+                        take();
+                    }
+                    if (tight)
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) top[f] = fmaf(top[f], fac[f], static_cast<float>(ev_hi));
+                    tmem_st_wait();
+                    fetch(3, next);
+                    take();
+                    bool grew = false, seeing = true;
+                    float corr[4], mm[4];
+                    uint64_t sum[4];
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                    {
+                        top[f] = max3_nan(top[f], __shfl_xor_sync(0xffffffffu, top[f], 1), top[f]);
+                        top[f] = max3_nan(top[f], __shfl_xor_sync(0xffffffffu, top[f], 2), top[f]);
+                        if (top[f] == INFINITY) top[f] = __int_as_float(0x7fffffff);   // inf - inf
+                        const bool grow = !(top[f] <= mf[f] + 8.f) && !(top[f] == -INFINITY);
+                        corr[f] = 1.f;
+                        if (grow)
+                        {
+                            corr[f] = ex2(mf[f] - top[f]);
+                            lf[f] *= corr[f];
+                            mf[f] = top[f];
+                            grew = true;
+                        }
+                        seeing &= mf[f] > -INFINITY;
+                        mm[f] = mf[f] == -INFINITY ? 0.f : -mf[f];
+                        sum[f] = 0;
+                    }
+                    if (b > it.b0 && __any_sync(0xffffffffu, grew))
+                    {
+                        ok = mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
+                        tc_fence_after();
+                        const float mine = of_row(corr);
+#pragma unroll 1
+                        for (int x = 0; x < D / 16; ++x)
+                        {
+                            uint32_t o[16];
+                            tmem_ld16(to + 16 * x, o);
+                            tmem_ld_wait(o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * mine);
+                            tmem_st16(to + 16 * x, o);
+                        }
+                    }
+                    const bool cubic = whole && __all_sync(0xffffffffu, seeing);
+                    // Second pass, from the last keys on: a chunk's weights take the place of scores that are done.
+                    auto weights = [&](auto plain) {
+                        constexpr bool PLAIN = decltype(plain)::value;   // the columns see the whole block
+#pragma unroll 1
+                        for (int x = 3; x >= 0; --x)
+                        {
+                            fetch(max(x - 1, 0), next);
+                            uint32_t out[2][8];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                            {
+                                const float4 vs = sc[32 + 4 * (2 * x + k)];
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                    for (int f = 0; f < 4; ++f)
+                                    {
+                                        const int at = 8 * k + 4 * e + 2 * (f & 1);
+                                        const uint32_t s0 = r[f >> 1][at], s1 = r[f >> 1][at + 1];
+                                        uint64_t y = f2_fma(f2(__uint_as_float(s0), __uint_as_float(s1)), f2(fac[f], fac[f]), f2(mm[f], mm[f]));
+                                        float w0, w1;
+                                        if constexpr (PLAIN)
+                                        {
+                                            if ((f + 2 * k + e) % kChunkCubicOf < kChunkCubic) y = f2_exp2_cubic(y);
+                                            else
+                                            {
+                                                f2_get(y, w0, w1);
+                                                y = f2(ex2(w0), ex2(w1));
+                                            }
+                                        }
+                                        else
+                                        {
+                                            f2_get(y, w0, w1);
+                                            y = f2(ex2(w0), ex2(w1));
+                                        }
+                                        sum[f] = f2_add(sum[f], y);
+                                        f2_get(f2_mul(y, e ? f2(vs.z, vs.w) : f2(vs.x, vs.y)), w0, w1);
+                                        if constexpr (!PLAIN)
+                                        {
+                                            // (a scale of NaN must not meet a weight of zero that stands for "not seen")
+                                            if (s0 == 0xff800000u) w0 = 0.f;
+                                            if (s1 == 0xff800000u) w1 = 0.f;
+                                        }
+                                        out[f >> 1][4 * k + 2 * e + (f & 1)] = pack_f16(w0, w1);
+                                    }
+                            }
+                            tmem_st_pairs(ts + 64 + 16 * x, out[0]);
+                            tmem_st_pairs(ts + 64 + 16 * x + (16u << 16), out[1]);
+                            take();
+                        }
+                    };
+                    if (cubic) weights(std::true_type{});
+                    else weights(std::false_type{});
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                    {
+                        float x, y;
+                        f2_get(sum[f], x, y);
+                        lf[f] += x + y;
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&p_full[i]);
+                }
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                {
+                    lf[f] += __shfl_xor_sync(0xffffffffu, lf[f], 1);
+                    lf[f] += __shfl_xor_sync(0xffffffffu, lf[f], 2);
+                }
+                m = of_row(mf);
+                l = of_row(lf);
             }
             if (!ok) break;
             // ---- the item's output, or this CTA's part of it ----
