@@ -166,20 +166,21 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&o)[T])
     }
 }
 
-// Two 8-bit codes as a pair of f16 (exact for both types). x holds them in its low 16 bits.
-template <typename CT>
+// Two 8-bit codes of x, its low (HIGH: high) 16 bits, as a pair of f16 (exact for both types).
+template <typename CT, bool HIGH = false>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t x)
 {
     if constexpr (std::is_same_v<CT, E4M3>)
     {
         uint32_t y;
-        asm("{.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(y) : "r"(x));
+        if constexpr (HIGH) asm("{.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, u;\n\t}" : "=r"(y) : "r"(x));
+        else asm("{.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(y) : "r"(x));
         return y;
     }
     else
     {
         // 0x6400 | (code ^ 0x80) is 1024 + 128 + code in f16.
-        const uint32_t y = (__byte_perm(x, 0, 0x4140) & 0x00ff00ffu) ^ 0x64806480u;
+        const uint32_t y = __byte_perm(x ^ 0x80808080u, 0x64646464u, HIGH ? 0x4342 : 0x4140);
         const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
         const __half2 z = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
         return *reinterpret_cast<const uint32_t*>(&z);
@@ -494,8 +495,8 @@ struct MmaEngine {
                     const uint32_t y = ks % 4 == 0 ? w1.x : ks % 4 == 1 ? w1.y : ks % 4 == 2 ? w1.z : w1.w;
                     ka[0][0] = codes_f16<CT>(x);
                     ka[0][1] = codes_f16<CT>(y);
-                    ka[0][2] = codes_f16<CT>(x >> 16);
-                    ka[0][3] = codes_f16<CT>(y >> 16);
+                    ka[0][2] = codes_f16<CT, true>(x);
+                    ka[0][3] = codes_f16<CT, true>(y);
                 }
 #pragma unroll
                 for (int j = NQ - 1; j >= 0; --j)

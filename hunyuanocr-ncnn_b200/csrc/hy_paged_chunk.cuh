@@ -77,7 +77,6 @@ struct ChunkItem {
 
 constexpr int kChunkThreads = 16 * 32;
 constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 12;
-constexpr int kChunkCubic = 1, kChunkCubicOf = 4;   // pairs of weights by the cubic, of so many
 // Registers a thread: 128 at launch; the 256 softmax threads take what the other 256 give up.
 template <bool F16>
 constexpr int kChunkRegsSoftmax = F16 ? 160 : 184;
@@ -323,27 +322,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair on the multiply-add units: x = n + f, |f| <= 1/2, and a cubic that
-// is within 7.5e-5 of 2^f (equal ripple of the relative error; the weights it makes
-// are rounded to 2^-8 or 2^-11). For x in [-inf, 126); below -126 it stays at 2^-126.
-__device__ __forceinline__ uint64_t f2_exp2_cubic(uint64_t x)
-{
-    float a, b;
-    f2_get(x, a, b);
-    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const uint64_t magic = f2(12582912.f, 12582912.f);   // 1.5 * 2^23: the sum's low bits are n
-    const uint64_t r = f2_add(x, magic);
-    const uint64_t f = f2_add(x, f2_mul(f2_add(r, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f)));
-    uint64_t y = f2_fma(f, f2(0.05517149f, 0.05517149f), f2(0.24261094f, 0.24261094f));
-    y = f2_fma(y, f, f2(0.69326099f, 0.69326099f));
-    y = f2_fma(y, f, f2(0.99992808f, 0.99992808f));
-    float n0, n1;
-    f2_get(r, n0, n1);
-    f2_get(y, a, b);
-    return f2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23)),
-              __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23)));
-}
-
 // Fetching by TMA: tensor maps of K and V over (dim, page, head, row), the last three in
 // the order of their strides; where[i]: the coordinate (1..3) of row, head and page.
 struct ChunkTma {
@@ -681,9 +659,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         {
                             const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR, rr = lw * 32 + r;
                             *reinterpret_cast<uint4*>(dst + sw128_at(rr, 2 * c)) =
-                                make_uint4(codes_f16<CT>(v[x].x), codes_f16<CT>(v[x].x >> 16), codes_f16<CT>(v[x].y), codes_f16<CT>(v[x].y >> 16));
+                                make_uint4(codes_f16<CT>(v[x].x), codes_f16<CT, true>(v[x].x), codes_f16<CT>(v[x].y), codes_f16<CT, true>(v[x].y));
                             *reinterpret_cast<uint4*>(dst + sw128_at(rr, 2 * c + 1)) =
-                                make_uint4(codes_f16<CT>(v[x].z), codes_f16<CT>(v[x].z >> 16), codes_f16<CT>(v[x].w), codes_f16<CT>(v[x].w >> 16));
+                                make_uint4(codes_f16<CT>(v[x].z), codes_f16<CT, true>(v[x].z), codes_f16<CT>(v[x].w), codes_f16<CT, true>(v[x].w));
                         }
                         if (kv == 0)
                         {
@@ -974,46 +952,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     }
                 }
                 const float mm = m == -INFINITY ? 0.f : m;
-                const bool cubic = whole && __all_sync(0xffffffffu, m > -INFINITY);
                 const uint64_t fac2 = f2(fac, fac), mm2 = f2(-mm, -mm);
                 uint64_t sum0 = 0, sum1 = 0;   // (pairs of zeros)
-                // Weights; some pairs by the cubic: the special-function units make 4 of 2^x a cycle and
-                // quarter of the SM, two tiles' blocks take them 2048 cycles, as long as the products. (The two
-                // cases are whole loops: a branch inside would keep the pairs from overlapping.)
-                auto weights = [&](auto plain) {
-                    constexpr bool PLAIN = decltype(plain)::value;   // the column sees the whole block
 #pragma unroll
-                    for (int e = 0; e < 64; ++e)
-                    {
-                        const uint64_t x = f2_fma(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), fac2, mm2);
-                        uint64_t y;
-                        float w0, w1;
-                        if constexpr (PLAIN)
-                        {
-                            if (e % kChunkCubicOf < kChunkCubic)
-                            {
-                                y = f2_exp2_cubic(x);
-                            }
-                            else
-                            {
-                                f2_get(x, w0, w1);
-                                y = f2(ex2(w0), ex2(w1));
-                            }
-                        }
-                        else
-                        {
-                            f2_get(x, w0, w1);
-                            y = f2(ex2(w0), ex2(w1));
-                        }
-                        if (e & 1) sum1 = f2_add(sum1, y);
-                        else sum0 = f2_add(sum0, y);
-                        f2_get(y, w0, w1);
-                        r[e] = pack_bf16(w0, w1);
-                        if (e == 31) tmem_st32(ts + 64, *reinterpret_cast<uint32_t(*)[32]>(r));
-                    }
-                };
-                if (cubic) weights(std::true_type{});
-                else weights(std::false_type{});
+                for (int e = 0; e < 64; ++e)
+                {
+                    float w0, w1;
+                    f2_get(f2_fma(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), fac2, mm2), w0, w1);
+                    w0 = ex2(w0);
+                    w1 = ex2(w1);
+                    if (e & 1) sum1 = f2_add(sum1, f2(w0, w1));
+                    else sum0 = f2_add(sum0, f2(w0, w1));
+                    r[e] = pack_bf16(w0, w1);
+                    if (e == 31) tmem_st32(ts + 64, *reinterpret_cast<uint32_t(*)[32]>(r));
+                }
                 tmem_st32(ts + 96, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
                 float s0, s1, s2, s3;
                 f2_get(sum0, s0, s1);
@@ -1229,7 +1181,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     tmem_st_wait();
                     fetch(3, next);
                     take();
-                    bool grew = false, seeing = true;
+                    bool grew = false;
                     float corr[4], mm[4];
                     uint64_t sum[4];
 #pragma unroll
@@ -1247,7 +1199,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             mf[f] = top[f];
                             grew = true;
                         }
-                        seeing &= mf[f] > -INFINITY;
                         mm[f] = mf[f] == -INFINITY ? 0.f : -mf[f];
                         sum[f] = 0;
                     }
@@ -1267,7 +1218,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             tmem_st16(to + 16 * x, o);
                         }
                     }
-                    const bool cubic = whole && __all_sync(0xffffffffu, seeing);
                     // Second pass, from the last keys on: a chunk's weights take the place of scores that are done.
                     auto weights = [&](auto plain) {
                         constexpr bool PLAIN = decltype(plain)::value;   // the columns see the whole block
@@ -1289,20 +1239,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                                         const uint32_t s0 = r[f >> 1][at], s1 = r[f >> 1][at + 1];
                                         uint64_t y = f2_fma(f2(__uint_as_float(s0), __uint_as_float(s1)), f2(fac[f], fac[f]), f2(mm[f], mm[f]));
                                         float w0, w1;
-                                        if constexpr (PLAIN)
-                                        {
-                                            if ((f + 2 * k + e) % kChunkCubicOf < kChunkCubic) y = f2_exp2_cubic(y);
-                                            else
-                                            {
-                                                f2_get(y, w0, w1);
-                                                y = f2(ex2(w0), ex2(w1));
-                                            }
-                                        }
-                                        else
-                                        {
-                                            f2_get(y, w0, w1);
-                                            y = f2(ex2(w0), ex2(w1));
-                                        }
+                                        f2_get(y, w0, w1);
+                                        y = f2(ex2(w0), ex2(w1));
                                         sum[f] = f2_add(sum[f], y);
                                         f2_get(f2_mul(y, e ? f2(vs.z, vs.w) : f2(vs.x, vs.y)), w0, w1);
                                         if constexpr (!PLAIN)
@@ -1319,7 +1257,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             take();
                         }
                     };
-                    if (cubic) weights(std::true_type{});
+                    if (whole) weights(std::true_type{});
                     else weights(std::false_type{});
 #pragma unroll
                     for (int f = 0; f < 4; ++f)
