@@ -53,6 +53,7 @@ EXPORTED_SYMBOLS = (
     "hy_ctx_set_wait_limit", "hy_debug_wait_probe", "hy_ctx_create_from_package", "hy_draft_load_package",
     "hy_package_inspect", "hy_package_read_tensor", "hy_debug_step_trace",
     "hy_paged_kv_write", "hy_paged_kv_read", "hy_paged_attention", "hy_paged_attention_workspace",
+    "hy_kv_device_rows",
 )
 TOKEN_CALLBACK = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.c_void_p)
 DFLASH_MASK_TOKEN = 120817
@@ -157,6 +158,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "hy_attention": ([_P, _I, _P, _I, _P, _P, _P], _I),
         "hy_kv_write": ([_P, _I, _I, _I, _P, _P], _I),
         "hy_kv_read": ([_P, _I, _I, _I, _P, _P], _I),
+        "hy_kv_device_rows": ([_P, _I, ctypes.POINTER(_P), ctypes.POINTER(_P), ctypes.POINTER(_I),
+                               ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)], _I),
         "hy_bench_ar_steps": ([_P, _I, ctypes.POINTER(_F)], _I),
         "hy_bench_kernel": ([_P, _I, _I, ctypes.POINTER(_F)], _I),
         "hy_ctx_set_ar_path": ([_P, _I], _I),
@@ -538,6 +541,23 @@ class TextRuntime:
         v = np.empty((8, rows, HEAD_DIM), np.float32)
         _check(_LIB.hy_kv_read(self._ctx, layer, start, rows, _ptr(k), _ptr(v)))
         return k, v
+
+    def kv_device_rows(self, layer: int):
+        """hy_kv_device_rows: (k pointer, v pointer, dtype, row stride, head stride) of a layer's KV cache."""
+        k, v, dt = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_int()
+        rs, hs = ctypes.c_int64(), ctypes.c_int64()
+        _check(_LIB.hy_kv_device_rows(self._ctx, layer, ctypes.byref(k), ctypes.byref(v), ctypes.byref(dt),
+                                      ctypes.byref(rs), ctypes.byref(hs)))
+        return k.value, v.value, dt.value, rs.value, hs.value
+
+    def store_kv_pages(self, layer: int, cache, batch, rows: int) -> None:
+        """Rows [0, rows) of a layer's KV cache into the pages of a paged.PagedKVCache, quantised as its type is
+        (hy_paged_kv_write on the context's stream, in order with torch's current stream)."""
+        cache.with_runtime(self, layer, batch, rows, write=True)
+
+    def load_kv_pages(self, layer: int, cache, batch, rows: int) -> None:
+        """Rows [0, rows) of a layer's KV cache back from pages (hy_paged_kv_read); set_length follows."""
+        cache.with_runtime(self, layer, batch, rows, write=False)
 
     # -- timing -------------------------------------------------------------
     def last_timing(self) -> TextDecodeTiming:

@@ -3688,6 +3688,20 @@ int hy_kv_read(hy_ctx* c, int layer, int start, int rows, float* k, float* v)
     return kv_copy(c, layer, start, rows, nullptr, nullptr, k, v);
 }
 
+int hy_kv_device_rows(hy_ctx* c, int layer, void** k_dev, void** v_dev, int* dtype, int64_t* row_stride,
+                      int64_t* head_stride)
+{
+    if (!c || !k_dev || !v_dev || !dtype || !row_stride || !head_stride)
+        return fail(HY_ERR_INVALID_ARGUMENT, "null argument");
+    if (layer < 0 || layer >= c->cfg.num_layers) return fail(HY_ERR_INVALID_ARGUMENT, "invalid layer");
+    *k_dev = c->kc_layer(layer);
+    *v_dev = c->vc_layer(layer);
+    *dtype = c->cfg.kv_dtype;
+    *row_stride = kHeadDim;
+    *head_stride = static_cast<int64_t>(c->cfg.max_context) * kHeadDim;
+    return HY_OK;
+}
+
 int hy_bench_ar_steps(hy_ctx* c, int count, float* ms)
 {
     if (!c || !ms || count < 1) return fail(HY_ERR_INVALID_ARGUMENT, "invalid arguments");

@@ -130,10 +130,7 @@ class PagedKVCache:
             raise HyError(HY_ERR_INVALID_ARGUMENT, f"{name} requires a gradient: these calls have none")
         return dtype
 
-    def _pair(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, fn) -> None:
-        dtype = self._rows(k, self._heads, "k")
-        if self._rows(v, self._heads, "v") != dtype or v.shape != k.shape:
-            raise HyError(HY_ERR_INVALID_ARGUMENT, "k and v must have one shape and type")
+    def _call(self, fn, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, dtype: int) -> None:
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
         k0, k1, _ = k.stride()
@@ -143,21 +140,29 @@ class PagedKVCache:
         if rc:
             _check(rc)
 
+    def _pair(self, k: torch.Tensor, v: torch.Tensor) -> int:
+        dtype = self._rows(k, self._heads, "k")
+        if self._rows(v, self._heads, "v") != dtype or v.shape != k.shape:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "k and v must have one shape and type")
+        return dtype
+
     def write(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Writes rows k, v [rows, kv heads, head_dim] at their positions (hy_paged_kv_write)."""
-        self._pair(batch, k, v, self._lib.hy_paged_kv_write)
+        self._call(self._lib.hy_paged_kv_write, batch, k, v, self._pair(k, v))
 
     def read(self, batch: PagedBatch, rows: int, dtype: torch.dtype = torch.float32,
              out: tuple[torch.Tensor, torch.Tensor] | None = None):
         """The batch's positions as rows k, v [rows, kv heads, head_dim] (hy_paged_kv_read). Rows of `out` that
         belong to no sequence are left as they were; without `out` they hold anything."""
         if out is None:
-            shape = (rows, self._heads, self._dim)
-            k = torch.empty(shape, dtype=dtype, device=self.device)
+            code = _ROW_DTYPES.get(dtype)
+            _need(code is not None, "rows are read as float32 or bfloat16")
+            k = torch.empty((rows, self._heads, self._dim), dtype=dtype, device=self.device)
             out = (k, torch.empty_like(k))
         else:
             _need(out[0].shape[0] == rows and out[0].dtype == dtype, "out must hold `rows` rows of `dtype`")
-        self._pair(batch, *out, self._lib.hy_paged_kv_read)
+            code = self._pair(*out)
+        self._call(self._lib.hy_paged_kv_read, batch, *out, code)
         return out
 
     def attention(self, batch: PagedBatch, q: torch.Tensor, scale: float, *, causal: bool = True, window: int = 0,
@@ -167,7 +172,7 @@ class PagedKVCache:
         false. The workspace comes from torch's allocator, one for each call."""
         dtype = self._rows(q, 0, "q")
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         elif self._rows(out, q.shape[1], "out") != dtype or out.shape != q.shape:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "q and out must have one shape and type")
         if batch.index != self._index:
@@ -191,6 +196,20 @@ class PagedKVCache:
         if rc:
             _check(rc)
         return out
+
+    def with_runtime(self, runtime, layer: int, batch: PagedBatch, rows: int, write: bool) -> None:
+        """Moves rows [0, rows) of a TextRuntime's layer into (write) or out of the batch's positions, on the
+        runtime's stream, ordered after and before torch's current stream."""
+        k, v, dtype, rs, hs = runtime.kv_device_rows(layer)
+        _need(runtime.cfg.device == self._index and batch.index == self._index,
+              "the runtime, the cache and the batch must be on one device")
+        _need(self._heads == 8 and self._dim == 128, "the runtime has 8 KV heads of 128")
+        _need(0 <= rows <= runtime.cfg.max_context, "rows exceed the runtime's KV capacity")
+        ours, theirs = torch.cuda.current_stream(self.device), torch.cuda.ExternalStream(runtime.stream, self.device)
+        theirs.wait_stream(ours)
+        fn = self._lib.hy_paged_kv_write if write else self._lib.hy_paged_kv_read
+        _check(fn(self._ref, batch._ref, rows, dtype, k, rs, hs, v, rs, hs, runtime.stream))
+        ours.wait_stream(theirs)
 
     def check(self) -> None:
         """Raises what the calls since the last check met on the device (waits for them), and clears it."""

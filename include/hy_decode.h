@@ -416,6 +416,15 @@ int hy_attention(hy_ctx* ctx, int layer, const float* qkv, int rows, const float
 int hy_kv_write(hy_ctx* ctx, int layer, int start, int rows, const float* k, const float* v);
 int hy_kv_read(hy_ctx* ctx, int layer, int start, int rows, float* k, float* v);
 int hy_seq_set_length(hy_ctx* ctx, int rows);
+/* One layer's KV cache where it lies on the device, as row tensors for
+ * hy_paged_kv_write / hy_paged_kv_read (hy_paged.h): element d of (row, head) is
+ * at row * row_stride + head * head_stride + d of k_dev and v_dev, of `dtype`;
+ * 8 heads of 128, max_context rows. With those calls on hy_ctx_stream a
+ * sequence's rows go to pages (a prefix that other contexts start from) and
+ * come back, followed by hy_seq_set_length. The pointers hold for the
+ * context's life. */
+int hy_kv_device_rows(hy_ctx* ctx, int layer, void** k_dev, void** v_dev, int* dtype, int64_t* row_stride,
+                      int64_t* head_stride);
 
 /* Raw stream handle (cudaStream_t): the context's calls run on it; a caller
  * orders its own work before or after them with events on this stream. */

@@ -568,3 +568,49 @@ def test_prompt_then_tokens(paged, cache):
     step([30, 0], 0, F32)
     for i in range(12):
         step([1, 1], 32 if i % 2 else 0, BF16 if i % 3 else F32)
+
+
+def test_prefix_moves_between_contexts_by_pages(paged, pkg):
+    """A context's prefilled KV rows into pages and from there into another context, which then decodes the same
+    tokens (fp32 pages are exact); 8-bit pages bring back code * scale of the same rows."""
+    cfg = dict(num_layers=2, vocab_size=4096, max_context=256, max_prefill=192, max_tokens=64)
+    rng = np.random.default_rng(5)
+    seq = 150
+    embeds = rng.standard_normal((seq, 1024)).astype(np.float32) * 0.02
+    cos, sin = pkg.rope_rows(0, seq, True), pkg.rope_rows(0, seq, False)
+    table = torch.randperm(12, generator=torch.Generator().manual_seed(1)).int().to(DEV)[None]
+    batch = paged.PagedBatch(torch.tensor([0, seq], dtype=torch.int32, device=DEV),
+                             torch.tensor([seq], dtype=torch.int32, device=DEV), table, seq)
+    with pkg.TextRuntime.synthetic(seed=3, norm_std=0.1, **cfg) as a, pkg.TextRuntime.synthetic(seed=3, norm_std=0.1, **cfg) as b:
+        a.prefill(embeds, cos, sin)
+        rows = [a.kv_read(layer, 0, seq) for layer in range(2)]
+        pages = [paged.PagedKVCache.allocate(12, 8, 16, 128, F32) for _ in range(2)]
+        for layer in range(2):
+            a.store_kv_pages(layer, pages[layer], batch, seq)
+        a.set_history([])
+        want, _ = a.generate(7, 7, 24, 1.08)
+        b.reset()
+        for layer in range(2):
+            b.load_kv_pages(layer, pages[layer], batch, seq)
+        b.prefill(embeds[:1], cos[:1], sin[:1])   # any sequence of its own: the length is set below
+        for layer in range(2):
+            b.load_kv_pages(layer, pages[layer], batch, seq)
+            pages[layer].check()
+            k, v = b.kv_read(layer, 0, seq)
+            assert np.array_equal(k, rows[layer][0]) and np.array_equal(v, rows[layer][1])
+        b.set_length(seq)
+        b.set_history([])
+        got, _ = b.generate(7, 7, 24, 1.08)
+        assert got == want
+        small = paged.PagedKVCache.allocate(12, 8, 16, 128, INT8)
+        a.store_kv_pages(1, small, batch, seq)
+        b.load_kv_pages(1, small, batch, seq)
+        small.check()
+        back = b.kv_read(1, 0, seq)
+        for x, y in zip(rows[1], back):
+            code, scale = R.quantise(torch.from_numpy(x), INT8)
+            assert np.array_equal(y, (code.float() * scale.float()[..., None]).numpy())
+        with pytest.raises(pkg.HyError, match="capacity"):
+            a.store_kv_pages(0, pages[0], batch, 257)
+        with pytest.raises(pkg.HyError, match="layer"):
+            a.store_kv_pages(2, pages[0], batch, seq)

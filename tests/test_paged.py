@@ -105,3 +105,11 @@ def test_workspace_is_checked(paged):
     c, b = _cache(paged), _batch(paged)
     assert lib.hy_paged_attention_workspace(ctypes.byref(c), ctypes.byref(b), 2, 4, 1, None) == 1
     assert lib.hy_paged_attention_workspace(ctypes.byref(c), ctypes.byref(b), 2, 3, 1, ctypes.byref(n)) == 1
+
+
+def test_device_rows_need_a_context(paged):
+    lib = paged._library()
+    k, v, d, r, h = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_int(), ctypes.c_int64(), ctypes.c_int64()
+    assert lib.hy_kv_device_rows(None, 0, ctypes.byref(k), ctypes.byref(v), ctypes.byref(d), ctypes.byref(r),
+                                 ctypes.byref(h)) == 1
+    assert b"null" in lib.hy_last_error()
