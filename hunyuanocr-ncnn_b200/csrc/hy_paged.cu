@@ -184,6 +184,10 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
 // Columns of a tile: as many as a sequence's rows need, up to 32, in the split
 // kernels (fp32 caches have tiles of 2 and 4 too, FmaEngine), else 256, for which
 // bf16 rows take the tcgen05 kernel; fp32 rows and fp32 caches stay at 32.
+// The border, in us with tiles of 32 / 256 columns (16 sequences at 8192 keys, 8 KV heads
+// of 128): 24 columns 114 / 134, 32 columns 117 / 135, 40 columns 201 / 135 (bf16 cache);
+// 32 columns 152 / 221, 40 columns 269 / 222 (INT8); one sequence at 2048 keys: 32 columns
+// 17.8 / 18.6, 40 columns 18.9 / 18.8 (bf16), 18.1 / 22.5 and 19.9 / 23.1 (INT8).
 int tile_columns(int max_rows, int group, int dtype, int cache_dtype)
 {
     const long long cols = static_cast<long long>(max_rows) * group;
