@@ -788,6 +788,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             if (ok) qk(i, blk + 1);
                         }
                     }
+                    // (an item whose columns see nothing uses neither: their slots are free when they have arrived)
+                    if (ok && !v_there) full(2 * blk + 1);
+                    if (ok && more && !k_there) full(2 * blk + 2);
                     if (!ok) break;
                     commit(&kv_empty[(2 * blk + 1) % SLOTS]);
                     if (more) commit(&kv_empty[(2 * blk + 2) % SLOTS]);

@@ -287,6 +287,23 @@ def test_rows_that_see_nothing(paged, rows, cache):
         assert bool((out[:n0] == 0).all()) and bool((out[st.starts[1]:st.starts[2]] == 0).all())
 
 
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_items_that_see_nothing_between_others(paged, cache):
+    """Wide tiles of padding rows only, several to a CTA and between real ones, with and without whole pages of 16;
+    repeated, and the same bits every time."""
+    for page in (16, 24):
+        seqs = [(0, 70), (400, 300), (0, 130), (5, 200), (1000, 129), (0, 40), (257, 64)] * 6
+        st = Setup(paged, cache, seqs, kv_heads=4, page=page, seed=18)
+        st.fill()
+        out = st.check_attention(8, BF16)
+        q = torch.randn(st.rows, 8, 128, generator=st.gen).to(BF16).to(DEV)
+        first = st.cache.attention(st.batch, q, 0.1)
+        for _ in range(20):
+            assert torch.equal(st.cache.attention(st.batch, q, 0.1), first)
+        st.cache.check()
+        assert bool((out[:70] == 0).all())
+
+
 @pytest.mark.parametrize("seqs", [[(50, 16)], [(300, 200)], [(700, 300)]], ids=["block", "chunk", "long"])
 @pytest.mark.parametrize("rows,cache", [(F32, F32), (BF16, BF16), (F32, BF16), (BF16, F32), (BF16, E4M3)])
 @pytest.mark.parametrize("value", [math.inf, math.nan])
