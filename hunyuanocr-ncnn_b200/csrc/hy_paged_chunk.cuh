@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + E::BAR_OFF);
     uint64_t* const kv_full = bars;               // [4] the block is in operand layout
     uint64_t* const kv_empty = kv_full + 4;       // [4] products that read it are done
-    uint64_t* const st_full = kv_empty + 4;       // [3] codes are in the staging ring; bf16: [0] a block to be mended
-    uint64_t* const st_empty = st_full + 3;       // [3] codes were read (4 warps)
+    uint64_t* const st_full = kv_empty + 4;       // [3] codes are in the staging ring; bf16: [4] a warp's rows to be mended
+    uint64_t* const st_empty = st_full + 4;       // [3] codes were read (4 warps)
     uint64_t* const q_full = st_empty + 3;        // the item's description is there, and (bf16) q (128)
     uint64_t* const q_empty = q_full + 1;         // products with q are done, the description was read (256)
     uint64_t* const s_full = q_empty + 1;         // [2] scores are there
@@ -381,11 +381,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             mbar_init(&kv_full[i], (!F16 && tma.on) ? 1 : 128);
             mbar_init(&kv_empty[i], 1);
         }
-        for (int i = 0; i < 3; ++i)
-        {
-            mbar_init(&st_full[i], 1);
-            mbar_init(&st_empty[i], 4);
-        }
+        for (int i = 0; i < 4; ++i) mbar_init(&st_full[i], 1);
+        for (int i = 0; i < 3; ++i) mbar_init(&st_empty[i], 4);
         mbar_init(q_full, 128);
         mbar_init(q_empty, 1 + 256);
         for (int i = 0; i < 2; ++i)
@@ -519,10 +516,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
                             if (kv && mender == lw)
                             {
-                                if (leader) mbar_arrive_expect_tx(&st_full[0], WARP_BYTES);
+                                if (leader) mbar_arrive_expect_tx(&st_full[lw], WARP_BYTES);
                                 __syncwarp();
-                                fetch(b, kv, dst, &st_full[0]);
-                                ok_all = ok_all && mbar_wait(&st_full[0], mended & 1, a.c.status, kPagedTimeout);
+                                fetch(b, kv, dst, &st_full[lw]);
+                                ok_all = ok_all && mbar_wait(&st_full[lw], mended & 1, a.c.status, kPagedTimeout);
+                                ++mended;   // (of this warp)
                                 constexpr int QP = E::RB / 16;
                                 for (int x = lane; x < (16 - (left & 15)) * QP; x += 32)
                                     *reinterpret_cast<uint4*>(smem + E::RING_OFF + slot * E::TILE_B + sw128_at(left + x / QP, x % QP)) = make_uint4(0, 0, 0, 0);
@@ -535,7 +533,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                                 if (leader && lw == 0 && !(kv && mender >= 0)) mbar_arrive_expect_tx(&kv_full[slot], 4 * WARP_BYTES);
                                 fetch(b, kv, dst, &kv_full[slot]);
                             }
-                            if (kv && mender >= 0) ++mended;
                         }
                         find(b + 1, group_key, gpg, grow);
                     }
