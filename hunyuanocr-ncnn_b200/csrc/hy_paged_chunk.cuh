@@ -1075,7 +1075,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
 #pragma unroll
                 for (int f = 0; f < 4; ++f)
                 {
-                    fac[f] = a.scale_log2 * qscale[c_0 + 8 * f];
+                    fac[f] = fmaxf(a.scale_log2 * qscale[c_0 + 8 * f], 1e-45f);   // (0 times a masked -inf is NaN)
                     pos[f] = c_0 + 8 * f < it.cols ? p_0 + paged_row_of(a, it.tile * 256 + c_0 + 8 * f) : -1;
                     mf[f] = -INFINITY;
                     lf[f] = 0.f;

@@ -77,13 +77,22 @@ def attention(q, keys, values, positions_, scale, causal=True, window=0, sinks=0
     return out, mass, reach
 
 
-def tolerance(out, mass, reach, length, dim, dtype):
+def tolerance(out, mass, reach, length, dim, dtype, codes=False):
     """What the kernel's arithmetic allows at every output. Scores: products exact to 2^-22, dim of them summed in
     fp32, so off by at most reach * (2^-22 + dim 2^-24), which is the relative error of a weight and counts twice
     (weight and sum); exp2 and its argument 2^-20; length additions of 2^-24. bf16 rows: weights rounded to half a
-    step, 2^-8, and the output once more."""
+    step, 2^-8, and the output once more.
+
+    8-bit caches (codes): a weight times its value's scale is an f16 number (fp32 rows: two of them), off by at most
+    2^-25 below 2^-14 besides. In that unit the row's largest such product t is at least 2^14 (the maximum is taken
+    over score plus the scale's exponent, the scale's fraction is at least 1, the factor is 2^14); in tiles of 256
+    columns, bf16 rows only, at least 2^-6 (factor 2^6, and 2^12 lost where one exponent stands for a block's). So
+    every key's product is off by at most 2^-39 t or 2^-19 t, and its code times t at most that share of the row's
+    largest mass (the largest code of a row of values is the type's largest)."""
     rel = 2 * reach * (2.0 ** -22 + dim * 2.0 ** -24) + 2.0 ** -20 + length * 2.0 ** -24
     tol = mass * rel + 2.0 ** -126
+    if codes:
+        tol = tol + length * 2.0 ** (-19 if dtype == torch.bfloat16 else -39) * mass.amax(dim=-1, keepdim=True)
     if dtype == torch.bfloat16:
         tol = tol + mass * 2.0 ** -8 + out.abs() * 2.0 ** -8 + tol * 2.0 ** -8
     return tol

@@ -62,11 +62,14 @@ class Setup:
         self.d_table = table.to(DEV)
         self.batch = paged.PagedBatch(self.d_starts, self.d_kv, self.d_table, max(self.n + [0]))
 
-    def fill(self, spread=1.0):
-        """Writes every position of every sequence; keeps what the cache then stands for in 64 bits."""
+    def fill(self, spread=1.0, octaves=0):
+        """Writes every position of every sequence (values times a power of two of the position, up to 2^octaves
+        either way); keeps what the cache then stands for in 64 bits."""
         total = sum(self.kv)
         k = torch.randn(total, self.kv_heads, self.dim, generator=self.gen) * spread
         v = torch.randn(total, self.kv_heads, self.dim, generator=self.gen)
+        if octaves:
+            v = v * 2.0 ** torch.randint(-octaves, octaves + 1, (total, 1, 1), generator=self.gen)
         starts = torch.tensor(np.concatenate([[0], np.cumsum(self.kv)]), dtype=torch.int32, device=DEV)
         whole = self.paged.PagedBatch(starts, self.d_kv, self.d_table, max(self.kv + [0]))
         self.cache.write(whole, k.to(DEV), v.to(DEV))
@@ -102,7 +105,7 @@ class Setup:
                 want, mass, reach = R.attention(q[r0 + a:r0 + b].double(), self.keys[s], self.values[s], pos[a:b],
                                                 scale, causal, window, sinks)
                 have = out[r0 + a:r0 + b].double()
-                tol = R.tolerance(want, mass, reach, kv, self.dim, q.dtype)
+                tol = R.tolerance(want, mass, reach, kv, self.dim, q.dtype, self.dtype in R.LARGEST)
                 off = torch.nan_to_num((have - want).abs() - tol, nan=0.0)
                 assert torch.equal(torch.isnan(have), torch.isnan(want)), s
                 assert float(off.max()) <= 0, (s, float((have - want).abs().max()), float(tol.min()))
@@ -341,6 +344,16 @@ def test_large_scores(paged, rows, seqs):
     assert bool(torch.isfinite(out).all())
 
 
+@pytest.mark.parametrize("scale", [1e-45, 1e-30, 1e30])
+@pytest.mark.parametrize("seqs", [RAGGED, BLOCKS, CHUNKS], ids=["tokens", "blocks", "chunks"])
+def test_queries_of_zeros(paged, seqs, scale):
+    """Every score is zero at any scale: the mean of the visible values."""
+    for rows, cache in ((F32, F32), (F32, E4M3), (BF16, BF16), (BF16, INT8)):
+        st = Setup(paged, cache, seqs, seed=23)
+        st.fill()
+        st.check_attention(4, rows, scale=scale, window=50, sinks=2, q=torch.zeros(st.rows, 4, 128, dtype=rows, device=DEV))
+
+
 def test_long_sequence_few_rows(paged):
     """The keys of one sequence split over the whole GPU and joined."""
     for rows, cache, seqs, heads in ((F32, F32, [(20001, 1)], (2, 1)), (BF16, E4M3, [(33333, 2)], (8, 1)),
@@ -360,6 +373,67 @@ def test_many_sequences(paged):
         st = Setup(paged, cache, seqs, kv_heads=1, dim=64, page=16, seed=10)
         st.fill()
         st.check_attention(2, rows)
+
+
+def test_many_blocks(paged):
+    """More sequences than a CTA's threads look at in one round, tiles of 256 columns."""
+    rng = np.random.default_rng(2)
+    for cache in (BF16, E4M3):
+        seqs = [(int(rng.integers(0, 90)), int(rng.integers(0, 40))) for _ in range(900)]
+        st = Setup(paged, cache, seqs, kv_heads=1, dim=64, page=16, seed=19, extra_rows=4)
+        st.fill()
+        st.check_attention(4, BF16)
+
+
+@pytest.mark.parametrize("octaves", [5, 6, 7, 30])
+@pytest.mark.parametrize("cache", [E4M3, INT8])
+def test_values_of_many_sizes(paged, cache, octaves):
+    """8-bit caches whose value scales lie close together and far apart within a block of keys."""
+    for seqs in (RAGGED, BLOCKS, CHUNKS):
+        for rows in (F32, BF16):
+            st = Setup(paged, cache, seqs, seed=20)
+            st.fill(octaves=octaves)
+            st.check_attention(4, rows)
+            st.check_attention(4, rows, window=100, sinks=3)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(64, 1), (1024, 1), (1024, 1024), (99, 3)])
+def test_many_heads(paged, q_heads, kv_heads):
+    """Groups of more heads than a tile has columns; as many KV heads as there may be."""
+    for rows, cache in ((BF16, BF16), (BF16, INT8), (F32, E4M3)):
+        st = Setup(paged, cache, [(300, 1), (0, 0), (20, 2)], kv_heads=kv_heads, dim=64, page=16, seed=21)
+        st.fill()
+        st.check_attention(q_heads, rows)
+
+
+@pytest.mark.parametrize("cache", TYPES)
+def test_shared_pages_and_interleaved_pools(paged, cache):
+    """Sequences that share the pages of a prefix, and keys and values that alternate page by page in one tensor,
+    give the same bits as separate ones."""
+    for n, page in ((1, 16), (5, 16), (90, 16), (90, 24)):
+        st = Setup(paged, cache, [(400, n), (400, n), (400, n)], page=page, seed=22)
+        rows = [torch.randn(400, 2, 128, generator=st.gen).to(DEV) for _ in range(2)]
+        starts = torch.tensor([0, 400, 800, 1200], dtype=torch.int32, device=DEV)
+        whole = paged.PagedBatch(starts, st.d_kv, st.d_table, 400)
+        st.cache.write(whole, *(t.repeat(3, 1, 1) for t in rows))
+        for q_dtype in (F32, BF16):
+            q = torch.randn(3 * n, 4, 128, generator=st.gen).to(q_dtype).to(DEV)
+            want = st.cache.attention(st.batch, q, 0.1)
+            shared = paged.PagedBatch(st.d_starts, st.d_kv, st.d_table[:1].expand(3, -1), n)
+            assert torch.equal(st.cache.attention(shared, q, 0.1), want)
+            c = st.cache
+
+            def alternate(x, y):
+                return [t.view(x.dtype) for t in torch.stack((x.view(torch.uint8) if cache.itemsize == 1 else x,
+                                                              y.view(torch.uint8) if cache.itemsize == 1 else y), 1).unbind(1)]
+
+            k, v = alternate(c.k, c.v)
+            scales = torch.stack((c.k_scale, c.v_scale), -1).unbind(-1) if cache.itemsize == 1 else (None, None)
+            other = paged.PagedKVCache(k, v, *scales)
+            assert not k.is_contiguous()
+            assert torch.equal(other.attention(st.batch, q, 0.1), want)
+            other.check()
+        st.cache.check()
 
 
 def test_offsets_past_32_bits(paged):
