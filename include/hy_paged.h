@@ -110,9 +110,15 @@ int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, i
  *   causal == 0: every j < kv_len (window must be 0).
  * A row that sees nothing gives zeros. Positions that a row does not see do
  * not reach its output, whatever they hold (infinities and NaN included).
- * scale must be positive. q and out have the same dtype and must not overlap. Products and softmax
- * sums are in fp32. F32 rows: every product is exact to 2^-22 or better. BF16
- * rows: probabilities are rounded to bf16 before they multiply v. */
+ * scale must be finite and positive. q and out have the same dtype and must
+ * not overlap. Products and softmax sums are in fp32. F32 rows: every product
+ * is exact to 2^-22 or better. BF16 rows: probabilities are rounded to bf16
+ * before they multiply v, over 8-bit caches (times v's scale) to f16; there,
+ * scales of v beyond 2^100 overflow and those below 2^-100 lose bits. An
+ * infinity that a row does see may give NaN.
+ * Limits: q_heads and num_kv_heads 1024, num_seqs 65535, rows * q_heads 2^31,
+ * table_width * page_size 2^30; writes and reads take row and head strides
+ * (the cache's head strides too) below 2^31. */
 int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
                        const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, void* out_dev,
                        int64_t out_row_stride, int64_t out_head_stride, float scale, int causal, int window,
