@@ -110,53 +110,77 @@ __device__ __forceinline__ float quotient_odd(float x, float s, float inv)
     return __int_as_float((r == 0.f || (bits & 1) || (bits << 1) == 0) ? bits : bits + away);
 }
 
-// Four quotients x / s as a word of codes, rounded to nearest, ties to even (inv = 1 / s, off
-// by 2 ulp at most): the hardware's rounding of x * inv, which is off by a few ulp, and where that may
-// matter - next to a tie - of quotient_odd. (bf16 rows meet ties often: one in some 300 quotients of
-// 8-bit significands is within rounding of one.)
+// Two fp32 at once.
+__device__ __forceinline__ uint64_t f2(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Four quotients x / s as a word of codes, rounded to nearest, ties to even (inv = 1 / s, off by 2 ulp at
+// most): the hardware's rounding of a product that is surely a little below the quotient and of one that is a
+// little above (lo and hi: inv (1 -+ 2^-20)). Rounding is monotone, so equal codes are the quotient's; else a tie may lie between, and
+// quotient_odd decides. (bf16 rows meet ties often: one in some 300 quotients of 8-bit significands is within
+// rounding of one. Looking for ties in the quotient's bits took three times the integer instructions, which bound it.)
 template <typename CT>
 __device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv)
 {
-    float q[4];
-    if constexpr (std::is_same_v<CT, E4M3>)
-    {
-        // 4 exponent bits, bias 7; 3 fraction bits; at most 448.
-        uint32_t small = 0xffffffffu, tie = 0xffffffffu;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-        {
-            q[e] = x[e] * inv;
-            const uint32_t b = __float_as_uint(q[e]) & 0x7fffffffu;
-            small = min(small, b);
-            tie = min(tie, (b + (8u - 0x80000u)) & 0xFFFFFu);   // up to 16: within 8 ulp of a tie of the normal codes
-        }
-        if (tie <= 16u || small < 0x3C800000u)   // (below 2^-6: subnormal codes, whose ties lie elsewhere)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = quotient_odd(x[e], s, inv);
+    const float lo = inv * (1.f - 0x1p-20f), hi = inv * (1.f + 0x1p-20f);
+    auto codes = [](const float* q) {
         uint32_t w;
-        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
-            "mov.b32 %0, {lo, hi};\n\t}"
-            : "=r"(w)
-            : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+        if constexpr (std::is_same_v<CT, E4M3>)
+            asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+                "mov.b32 %0, {lo, hi};\n\t}"
+                : "=r"(w)
+                : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+        else   // (q holds integers plus 1.5 * 2^23)
+            w = __byte_perm(__byte_perm(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x0040),
+                            __byte_perm(__float_as_uint(q[2]), __float_as_uint(q[3]), 0x0040), 0x5410);
         return w;
-    }
-    else
+    };
+    // x times f; INT8: to an integer by adding 1.5 * 2^23 in the same rounding; magnitudes stay within 127 (1 + 2^-19).
+    auto times = [&](float f, float* q) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+            f2_get(std::is_same_v<CT, E4M3> ? f2_mul(f2(x[e], x[e + 1]), f2(f, f))
+                                            : f2_fma(f2(x[e], x[e + 1]), f2(f, f), f2(12582912.f, 12582912.f)),
+                   q[e], q[e + 1]);
+    };
+    float q[4], p[4];
+    times(lo, q);
+    times(hi, p);
+    uint32_t w = codes(q);
+    if (w != codes(p))
     {
-        // To an integer by adding 1.5 * 2^23; magnitudes stay within 127 (1 + 2^-22).
-        float t[4], far = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            q[e] = x[e] * inv;
-            t[e] = q[e] + 12582912.f;
-            far = fmaxf(far, fabsf(q[e] - (t[e] - 12582912.f)));
+            q[e] = quotient_odd(x[e], s, inv);
+            if constexpr (!std::is_same_v<CT, E4M3>) q[e] += 12582912.f;
         }
-        if (far > 0.4999f)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = quotient_odd(x[e], s, inv) + 12582912.f;
-        return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
-                           __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+        w = codes(q);
     }
+    return w;
 }
 template <typename CT>
 constexpr float kCodeMax = std::is_same_v<CT, E4M3> ? 448.f : 127.f;
