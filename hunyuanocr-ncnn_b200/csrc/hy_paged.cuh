@@ -384,25 +384,28 @@ __device__ __forceinline__ RT* paged_row_at(const PagedRowArgs& a, const PagedVe
 template <typename RT, typename CT, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const PagedRowArgs a)
 {
-    constexpr int E = 16 / static_cast<int>(sizeof(RT));   // elements per lane
-    constexpr int LPV = D / E;                             // lanes per vector: 8, 16 or 32
+    constexpr int E = 16 / static_cast<int>(sizeof(RT));   // elements of a piece
+    constexpr int P = 2;                                   // pieces per lane, D / P elements apart
+    constexpr int LPV = D / (E * P);                       // lanes per vector: 4, 8 or 16
     constexpr int VPW = 32 / LPV;                          // vectors per warp and step
-    constexpr int U = 4;                                   // steps in flight
+    constexpr int U = 2;                                   // steps in flight
     constexpr int STEP = U * kRowWarps * VPW;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r0 = blockIdx.x * a.per_cta, n_rows = min(a.per_cta, a.b.rows - r0);
     const int nv = n_rows * 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
     __shared__ PagedPlace places[kRowsPerCta];
     pdl_wait();
-    uint4 x[U], next[U];
-    auto load = [&](int v0, uint4 (&to)[U]) {
+    uint4 x[U][P], next[U][P];
+    auto load = [&](int v0, uint4 (&to)[U][P]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
             const int i = v0 + (u * kRowWarps + warp) * VPW + sub;
             if (i >= nv) continue;
             const PagedVector v = paged_vector(a, i);
-            to[u] = __ldg(reinterpret_cast<const uint4*>(paged_row_at<const RT>(a, v, r0) + d));
+            const RT* const p = paged_row_at<const RT>(a, v, r0) + d;
+#pragma unroll
+            for (int c = 0; c < P; ++c) to[u][c] = __ldg(reinterpret_cast<const uint4*>(p + c * (D / P)));
         }
     };
     load(0, next);   // ahead of the look-ups: the values do not depend on them
@@ -410,7 +413,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const Paged
     for (int v0 = 0; v0 < nv; v0 += STEP)
     {
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = next[u];
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < P; ++c) x[u][c] = next[u][c];
         if (v0 + STEP < nv) load(v0 + STEP, next);
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -421,24 +426,26 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const Paged
             const bool live = i < nv && o.off >= 0;
             const long long at = o.off + static_cast<long long>(v.head) * a.page_head_stride + d;
             void* const pool = v.isv ? a.c.v : a.c.k;
-            float f[E];
-            const uint32_t w4[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+            auto piece = [&](int c, float (&f)[E]) {   // as fp32
+                const uint32_t w4[4] = {x[u][c].x, x[u][c].y, x[u][c].z, x[u][c].w};
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                f[e] = E == 4 ? __uint_as_float(w4[e]) : __uint_as_float((e & 1) ? w4[e >> 1] & 0xFFFF0000u : w4[e >> 1] << 16);
+                for (int e = 0; e < E; ++e)
+                    f[e] = E == 4 ? __uint_as_float(w4[e]) : __uint_as_float((e & 1) ? w4[e >> 1] & 0xFFFF0000u : w4[e >> 1] << 16);
+            };
             if constexpr (kCodes<CT>)
             {
                 // The largest magnitude by its bits: an infinity or a NaN comes out on top.
                 uint32_t m = 0;
-                if constexpr (E == 8)   // two bf16 to a word
+#pragma unroll
+                for (int c = 0; c < P; ++c)
                 {
+                    const uint32_t w4[4] = {x[u][c].x, x[u][c].y, x[u][c].z, x[u][c].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w4[e] & 0x7fff7fffu);
-                    m = max(m << 16, m & 0x7fff0000u);
+                    for (int e = 0; e < 4; ++e)
+                        if constexpr (E == 8) m = __vmaxu2(m, w4[e] & 0x7fff7fffu);   // two bf16 to a word
+                        else m = max(m, w4[e] & 0x7fffffffu);
                 }
-                else
-#pragma unroll
-                    for (int e = 0; e < E; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
+                if constexpr (E == 8) m = max(m << 16, m & 0x7fff0000u);
 #pragma unroll
                 for (int w = LPV / 2; w > 0; w >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, w));
                 const bool finite = m < 0x7f800000u;
@@ -446,18 +453,31 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_write_kernel(const Paged
                 const float inv = __fdividef(1.f, scale);   // (scale < 2^126; off by 2 ulp, which quant4 allows for)
                 if (live)
                 {
-                    uint32_t w[E / 4];
+                    uint8_t* const p = static_cast<uint8_t*>(pool) + at;
 #pragma unroll
-                    for (int y = 0; y < E / 4; ++y) w[y] = finite ? quant4<CT>(f + 4 * y, scale, inv) : 0u;
-                    uint8_t* p = static_cast<uint8_t*>(pool) + at;
-                    if constexpr (E == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-                    else *reinterpret_cast<uint32_t*>(p) = w[0];
+                    for (int c = 0; c < P; ++c)
+                    {
+                        float f[E];
+                        piece(c, f);
+                        uint32_t w[E / 4];
+#pragma unroll
+                        for (int y = 0; y < E / 4; ++y) w[y] = finite ? quant4<CT>(f + 4 * y, scale, inv) : 0u;
+                        if constexpr (E == 8) *reinterpret_cast<uint2*>(p + c * (D / P)) = make_uint2(w[0], w[1]);
+                        else *reinterpret_cast<uint32_t*>(p + c * (D / P)) = w[0];
+                    }
                     if (lane % LPV == 0) (v.isv ? a.c.v_scale : a.c.k_scale)[o.s_off + static_cast<long long>(v.head) * a.scale_head_stride] = scale;
                 }
             }
             else
             {
-                if (live) store_row<CT, E>(pool, at, f);
+                if (live)
+#pragma unroll
+                    for (int c = 0; c < P; ++c)
+                    {
+                        float f[E];
+                        piece(c, f);
+                        store_row<CT, E>(pool, at + c * (D / P), f);
+                    }
             }
         }
     }
