@@ -487,11 +487,12 @@ template <typename RT, typename CT, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedRowArgs a)
 {
     constexpr int E = 16 / static_cast<int>(sizeof(RT));
-    constexpr int LPV = D / E;
+    constexpr int P = 2;                                      // pieces per lane, as in the write
+    constexpr int LPV = D / (E * P);
     constexpr int VPW = 32 / LPV;
-    constexpr int U = E * sizeof(CT) > 16 ? 4 : 8;
+    constexpr int U = E * sizeof(CT) > 16 ? 2 : 4;
     constexpr int STEP = U * kRowWarps * VPW;
-    constexpr int W = E * static_cast<int>(sizeof(CT)) / 4;   // words of the cache that a lane reads
+    constexpr int W = E * static_cast<int>(sizeof(CT)) / 4;   // words of a piece in the cache
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r0 = blockIdx.x * a.per_cta, n_rows = min(a.per_cta, a.b.rows - r0);
     const int nv = n_rows * 2 * a.c.kv_heads, sub = lane / LPV, d = (lane % LPV) * E;
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
     paged_places(a.c, a.b, r0, n_rows, places);
     for (int v0 = 0; v0 < nv; v0 += STEP)
     {
-        uint32_t x[U][W];
+        uint32_t x[U][P][W];
         float scale[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -511,19 +512,24 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
             const PagedPlace o = places[v.row];
             if (o.off < 0) continue;
             const CT* const p = static_cast<const CT*>(v.isv ? a.c.v : a.c.k) + o.off + static_cast<long long>(v.head) * a.page_head_stride + d;
-            if constexpr (W == 1) x[u][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-            else if constexpr (W == 2)
-            {
-                const uint2 y = __ldg(reinterpret_cast<const uint2*>(p));
-                x[u][0] = y.x; x[u][1] = y.y;
-            }
-            else
 #pragma unroll
-                for (int w = 0; w < W; w += 4)
+            for (int c = 0; c < P; ++c)
+            {
+                const CT* const pc = p + c * (D / P);
+                if constexpr (W == 1) x[u][c][0] = __ldg(reinterpret_cast<const uint32_t*>(pc));
+                else if constexpr (W == 2)
                 {
-                    const uint4 y = __ldg(reinterpret_cast<const uint4*>(p) + w / 4);
-                    x[u][w] = y.x; x[u][w + 1] = y.y; x[u][w + 2] = y.z; x[u][w + 3] = y.w;
+                    const uint2 y = __ldg(reinterpret_cast<const uint2*>(pc));
+                    x[u][c][0] = y.x; x[u][c][1] = y.y;
                 }
+                else
+#pragma unroll
+                    for (int w = 0; w < W; w += 4)
+                    {
+                        const uint4 y = __ldg(reinterpret_cast<const uint4*>(pc) + w / 4);
+                        x[u][c][w] = y.x; x[u][c][w + 1] = y.y; x[u][c][w + 2] = y.z; x[u][c][w + 3] = y.w;
+                    }
+            }
             if constexpr (kCodes<CT>) scale[u] = __ldg((v.isv ? a.c.v_scale : a.c.k_scale) + o.s_off + static_cast<long long>(v.head) * a.scale_head_stride);
         }
 #pragma unroll
@@ -533,18 +539,23 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_read_kernel(const PagedR
             if (i >= nv) continue;
             const PagedVector v = paged_vector(a, i);
             if (places[v.row].off < 0) continue;
-            float f[E];
+            RT* const to = paged_row_at<RT>(a, v, r0);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
+            for (int c = 0; c < P; ++c)
             {
-                if constexpr (sizeof(CT) == 4) f[e] = __uint_as_float(x[u][e]);
-                else if constexpr (sizeof(CT) == 2) f[e] = __uint_as_float((e & 1) ? x[u][e >> 1] & 0xFFFF0000u : x[u][e >> 1] << 16);
-                else if (e % 4 == 0) decode4<CT>(x[u][e / 4], f + e);
-            }
-            if constexpr (kCodes<CT>)
+                float f[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) f[e] *= scale[u];
-            store_row<RT, E>(paged_row_at<RT>(a, v, r0), d, f);
+                for (int e = 0; e < E; ++e)
+                {
+                    if constexpr (sizeof(CT) == 4) f[e] = __uint_as_float(x[u][c][e]);
+                    else if constexpr (sizeof(CT) == 2) f[e] = __uint_as_float((e & 1) ? x[u][c][e >> 1] & 0xFFFF0000u : x[u][c][e >> 1] << 16);
+                    else if (e % 4 == 0) decode4<CT>(x[u][c][e / 4], f + e);
+                }
+                if constexpr (kCodes<CT>)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) f[e] *= scale[u];
+                store_row<RT, E>(to, d + c * (D / P), f);
+            }
         }
     }
 }
