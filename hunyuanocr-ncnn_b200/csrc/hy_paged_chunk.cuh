@@ -65,7 +65,7 @@ struct ChunkEngine {
     static constexpr int QS_OFF = EV_OFF + 64;                           // [256] 2^-k of a column's q
     static constexpr int ITEM_OFF = QS_OFF + 1024;                         // [2] ChunkItem
     static constexpr int BAR_OFF = ITEM_OFF + 2 * 64;
-    static constexpr int SMEM = BAR_OFF + 256 + 1024;                      // + alignment of the base to 1024
+    static constexpr int SMEM = BAR_OFF + 320 + 1024;                      // + alignment of the base to 1024
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static constexpr int S_COL = 0, O_COL = 256;           // tensor memory columns of tile 0; tile 1: + 128
 };
@@ -332,8 +332,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     uint64_t* const o_full = p_full + 2;          // [2] weights times values added
     uint64_t* const q_ready = o_full + 2;         // 8-bit caches: q is there (256)
     uint64_t* const done = q_ready + 1;           // every product is done
-    int* const pv_skip = reinterpret_cast<int*>(done + 1);   // [2] this block's product was taken by the softmax warps
-    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(pv_skip + 2);
+    uint64_t* const agreed = done + 1;            // [2] bf16: every thread of the tile looked for odd values (128)
+    int* const pv_skip = reinterpret_cast<int*>(agreed + 2);   // [2] this block's product was taken by the softmax warps
+    int* const odd_s = pv_skip + 2;                          // [2] the last block (1 + its number) in which a thread found some
+    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(odd_s + 2);
     float* const qscale = reinterpret_cast<float*>(smem + E::QS_OFF);
     ChunkItem* const items_s = reinterpret_cast<ChunkItem*>(smem + E::ITEM_OFF);
     volatile uint32_t* const live_w = reinterpret_cast<volatile uint32_t*>(smem + E::LIVE_OFF);
@@ -364,6 +366,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
             mbar_init(&o_full[i], 1);
+            mbar_init(&agreed[i], 128);
+            odd_s[i] = 0;
         }
         mbar_init(q_ready, 256);
         mbar_init(done, 1);
@@ -782,6 +786,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + E::S_COL + i * 128 + lanes, to = tmem + E::O_COL + i * 128 + lanes;
         int nb = 0, seen = 0;   // blocks of earlier items; blocks of this tile
+        int masked = 0;         // bf16: those that not every column sees all of
         bool ok = true;
         for (int items = 0;; ++items)
         {
@@ -882,13 +887,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
 #pragma unroll
                             for (int e = 0; e < 4; ++e) bad |= (ws[e] & 0x7f800000u) == 0x7f800000u || (ws[e] & 0x7f80u) == 0x7f80u;
                         }
-                        uint32_t any;
-                        asm volatile(
-                            "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                            : "=r"(any)
-                            : "r"(bad), "r"(1 + i)
-                            : "memory");
-                        odd = any != 0;
+                        // (the mark of this block stands until the tile's weights are out)
+                        if (bad) *reinterpret_cast<volatile int*>(&odd_s[i]) = seen + 1;
+                        mbar_arrive(&agreed[i]);
+                        ok = mbar_wait(&agreed[i], masked & 1, a.c.status, kPagedTimeout);
+                        ++masked;
+                        odd = *reinterpret_cast<volatile int*>(&odd_s[i]) == seen + 1;
                     }
                 }
                 float top;
