@@ -28,7 +28,8 @@
 // 4 sequences of ~1012 rows over 6000-8192 bf16 keys (213 GFLOP): 238 us, 893 TFLOP/s; the
 // tensor cores are busy 45% of the time and the special-function units 46%: a tile's softmax
 // and its products follow one another, and only two tiles fit tensor memory. Over 8-bit
-// keys the softmax threads' products with the scales bound it (406-418 us). Pages of 24 rows
+// keys the softmax threads' products with the scales bound it (406-418 us; 16 softmax warps or 8 loading
+// warps instead of 8 and 4 changed nothing: the windowed INT8 chunks take 236 and 240 us with them, 230 without). Pages of 24 rows
 // instead of 32, copied by threads: 183 instead of 139 us (windowed chunks, bf16).
 //
 // Tensor memory (512 columns): scores of the two tiles (128 each; the
