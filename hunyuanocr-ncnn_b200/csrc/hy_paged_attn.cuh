@@ -1128,6 +1128,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
     float* const parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.work) + kSplitDescBytes);
     uint32_t* const colmax = reinterpret_cast<uint32_t*>(smem + Sh::MAX_OFF);
     if (tid < COLS) colmax[tid] = 0;
+    if constexpr (E::F16) __syncthreads();   // before any warp's maxima (split_start may hold no barrier)
     pdl_wait();
     pdl_launch();
 
