@@ -352,10 +352,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     }
     if (tid == 0)
     {
-        // (bf16 blocks by TMA: one arrival, of the thread that announces the bytes)
+        // (bf16 blocks by TMA: an arrival of each loading warp, with its own bytes; it also publishes the warp's
+        // word of key-present bits)
         for (int i = 0; i < 4; ++i)
         {
-            mbar_init(&kv_full[i], (!F16 && tma.on) ? 1 : 128);
+            mbar_init(&kv_full[i], (!F16 && tma.on) ? 4 : 128);
             mbar_init(&kv_empty[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&st_full[i], 1);
@@ -485,7 +486,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         if (lane == 0) live_w[(blk & 3) * 4 + lw] = bits | (hi << 16);
                         __syncwarp();
                         // Rows behind the last key come along with its group; they may hold anything, and in V they
-                        // become zeros before the products see them: the warp whose group it is announces the block then.
+                        // become zeros before the products see them: the warp whose group it is arrives then.
                         const int mender = (left < 128 && (left & 15)) ? left >> 5 : -1;
 #pragma unroll
                         for (int kv = 0; kv < 2; ++kv, ++n)
@@ -505,11 +506,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                                     *reinterpret_cast<uint4*>(smem + E::RING_OFF + slot * E::TILE_B + sw128_at(left + x / QP, x % QP)) = make_uint4(0, 0, 0, 0);
                                 fence_async_smem();
                                 __syncwarp();
-                                if (leader) mbar_arrive_expect_tx(&kv_full[slot], 3 * WARP_BYTES);
+                                if (leader) mbar_arrive(&kv_full[slot]);
                             }
                             else
                             {
-                                if (leader && lw == 0 && !(kv && mender >= 0)) mbar_arrive_expect_tx(&kv_full[slot], 4 * WARP_BYTES);
+                                if (leader) mbar_arrive_expect_tx(&kv_full[slot], WARP_BYTES);
+                                __syncwarp();
                                 fetch(b, kv, dst, &kv_full[slot]);
                             }
                         }

@@ -26,3 +26,29 @@ def test_few_sequences_repeat_themselves(paged, cache, rows):
     for _ in range(200):
         assert torch.equal(st.cache.attention(st.batch, q, 1.0 / math.sqrt(128)), first)
     st.cache.check()
+
+
+@pytest.mark.parametrize("page", [16, 24, 64])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_scattered_bad_pages_in_chunks(paged, pkg, cache, page):
+    """Pages that are none, scattered over the blocks of keys so that every loading warp's bits differ from block to
+    block and end inside one: those keys are not seen, the others are, the same bits every time."""
+    kv, n = 2011, 150
+    st = Setup(paged, cache, [(kv, n)], kv_heads=4, page=page, seed=32)
+    st.fill()
+    gone = torch.rand(st.table.shape[1], generator=st.gen) < 0.4
+    gone[-1] = False
+    st.d_table[0, gone.to(DEV)] = -1
+    there = np.repeat(~gone.numpy(), page)[:kv]
+    sel = torch.from_numpy(np.flatnonzero(there)).to(DEV)
+    before = np.cumsum(there)   # keys that are there up to a position
+    q = torch.randn(n, 8, 128, generator=st.gen).to(BF16).to(DEV)
+    first = st.cache.attention(st.batch, q, 0.1)
+    want, mass, reach = R.attention(q.double(), st.keys[0][sel], st.values[0][sel],
+                                    [int(before[p]) - 1 for p in range(kv - n, kv)], 0.1)
+    tol = R.tolerance(want, mass, reach, kv, 128, BF16, cache in R.LARGEST)
+    assert bool(((first.double() - want).abs() <= tol).all())
+    for _ in range(30):
+        assert torch.equal(st.cache.attention(st.batch, q, 0.1), first)
+    with pytest.raises(pkg.HyError, match="page number"):
+        st.cache.check()
