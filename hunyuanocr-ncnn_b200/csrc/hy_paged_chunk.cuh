@@ -204,6 +204,20 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
         : "memory");
 }
+// Bounded waits of a whole (converged) warp: true in all its threads or in none, so that what comes next
+// may be of the whole warp whichever way a wait ends.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, kPagedTimeout));
+}
+__device__ __forceinline__ bool warp_wait_spin(uint64_t* bar, uint32_t parity, int* status)
+{
+    return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, status, kPagedTimeout));
+}
+__device__ __forceinline__ bool warp_try_wait(uint64_t* bar, uint32_t parity)
+{
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Byte offset of 16-byte piece c of row r in a 128-row tile: 64 dimensions (128 bytes) to a
@@ -394,11 +408,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
         int n = 0;             // slots filled
         int blk = 0;           // blocks (index of the scale ring)
         int items = 0, mended = 0;
+        int staged = 0;        // slots of the staging ring fetched
         bool ok_all = true;
         const bool leader = elect_one();
         for (;; ++items)
         {
-            if (items) ok_all = ok_all && mbar_wait(q_empty, (items - 1) & 1, a.c.status, kPagedTimeout);
+            if (items) ok_all = ok_all && warp_wait(q_empty, (items - 1) & 1, a.c.status);
             if (lt == 0)
             {
                 ChunkItem d;
@@ -492,15 +507,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         for (int kv = 0; kv < 2; ++kv, ++n)
                         {
                             const int slot = n % SLOTS;
-                            if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                            if (n >= SLOTS) ok_all = ok_all && warp_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status);
+                            if (!ok_all) break;
                             const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
                             if (kv && mender == lw)
                             {
                                 if (leader) mbar_arrive_expect_tx(&st_full[lw], WARP_BYTES);
                                 __syncwarp();
                                 fetch(b, kv, dst, &st_full[lw]);
-                                ok_all = ok_all && mbar_wait(&st_full[lw], mended & 1, a.c.status, kPagedTimeout);
+                                ok_all = warp_wait(&st_full[lw], mended & 1, a.c.status);
                                 ++mended;   // (of this warp)
+                                if (!ok_all) break;
                                 constexpr int QP = E::RB / 16;
                                 for (int x = lane; x < (16 - (left & 15)) * QP; x += 32)
                                     *reinterpret_cast<uint4*>(smem + E::RING_OFF + slot * E::TILE_B + sw128_at(left + x / QP, x % QP)) = make_uint4(0, 0, 0, 0);
@@ -541,10 +558,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         {
                             const int slot = n % SLOTS;
                             const CT* const base = static_cast<const CT*>(kv ? a.c.v : a.c.k);
-                            if (n >= SLOTS && !mbar_try_wait(&kv_empty[slot], (n / SLOTS - 1) & 1))
+                            if (n >= SLOTS && !warp_try_wait(&kv_empty[slot], (n / SLOTS - 1) & 1))
                             {
                                 drain();   // what was fetched is on its way before this waits
-                                ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                                ok_all = ok_all && warp_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status);
+                                if (!ok_all) break;
                             }
                             const uint32_t dst = sm + E::RING_OFF + slot * E::TILE_B;
 #pragma unroll 8
@@ -580,10 +598,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         const int kv = (x - n0) & 1, sg = x % 3;
                         if (tma.on)
                         {
-                            if (x >= 3) ok_all = ok_all && mbar_wait(&st_empty[sg], (x / 3 - 1) & 1, a.c.status, kPagedTimeout);
-                            if (leader && lw == 0) mbar_arrive_expect_tx(&st_full[sg], 4 * WARP_BYTES);
-                            fetch(fb, kv, sm + E::STAGE_OFF + sg * E::CODES_B, &st_full[sg]);
-                            if (kv) find(++fb, group_key, gpg, grow);
+                            if (x >= 3) ok_all = ok_all && warp_wait(&st_empty[sg], (x / 3 - 1) & 1, a.c.status);
+                            if (ok_all)
+                            {
+                                if (leader && lw == 0) mbar_arrive_expect_tx(&st_full[sg], 4 * WARP_BYTES);
+                                fetch(fb, kv, sm + E::STAGE_OFF + sg * E::CODES_B, &st_full[sg]);
+                                staged = x + 1;
+                                if (kv) find(++fb, group_key, gpg, grow);
+                            }
                         }
                         else
                         {
@@ -622,13 +644,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     {
                         const int slot = n % SLOTS, sg = n % 3;
                         ahead(n + 2);
-                        if (tma.on) ok_all = ok_all && mbar_wait(&st_full[sg], (n / 3) & 1, a.c.status, kPagedTimeout);
+                        if (tma.on) ok_all = ok_all && warp_wait(&st_full[sg], (n / 3) & 1, a.c.status);
                         else
                         {
                             cp_wait<2>();
                             __syncwarp();
                         }
-                        if (n >= SLOTS) ok_all = ok_all && mbar_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status, kPagedTimeout);
+                        if (n >= SLOTS) ok_all = ok_all && warp_wait(&kv_empty[slot], (n / SLOTS - 1) & 1, a.c.status);
+                        if (!ok_all) break;
                         unsigned char* const dst = smem + E::RING_OFF + slot * E::TILE_B;
                         uint4 v[CPR];
 #pragma unroll
@@ -672,6 +695,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 cp_wait<0>();
             }
             more = w.next(a);
+        }
+        if (!ok_all && tma.on)
+        {
+            // After a wait that gave up: the block does not end before this warp's copies have landed (or as many
+            // waits have given up again).
+            if constexpr (F16)
+                for (int x = max(0, staged - 3); x < staged; ++x) warp_wait(&st_full[x % 3], (x / 3) & 1, a.c.status);
+            else
+                for (int x = max(0, n - SLOTS); x < n; ++x) warp_wait(&kv_full[x % SLOTS], (x / SLOTS) & 1, a.c.status);
         }
     }
     else if (warp >= kChunkMmaWarp)
@@ -718,19 +750,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 __syncwarp();
             };
             auto full = [&](int slot_n) {
-                ok = ok && mbar_wait_spin(&kv_full[slot_n % SLOTS], (slot_n / SLOTS) & 1, a.c.status, kPagedTimeout);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = ok && warp_wait_spin(&kv_full[slot_n % SLOTS], (slot_n / SLOTS) & 1, a.c.status);
                 tc_fence_after();
             };
             for (int items = 0; ok; ++items)
             {
-                ok = __all_sync(0xffffffffu, mbar_wait_spin(q_full, items & 1, a.c.status, kPagedTimeout));
+                ok = warp_wait_spin(q_full, items & 1, a.c.status);
                 if (!ok) break;
                 const ChunkItem it = items_s[items & 1];
                 const int b0 = __shfl_sync(0xffffffffu, it.b0, 0), n_blk = __shfl_sync(0xffffffffu, it.b1, 0) - b0;
                 const int lim[2] = {__shfl_sync(0xffffffffu, it.lim[0], 0), __shfl_sync(0xffffffffu, it.lim[1], 0)};
                 if (n_blk <= 0) break;
-                if constexpr (F16) ok = __all_sync(0xffffffffu, mbar_wait_spin(q_ready, items & 1, a.c.status, kPagedTimeout));
+                if constexpr (F16) ok = warp_wait_spin(q_ready, items & 1, a.c.status);
                 full(2 * nb);
                 if (!ok) break;
 #pragma unroll
@@ -748,7 +779,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     {
                         if (ok && b0 + j < lim[i])
                         {
-                            ok = __all_sync(0xffffffffu, mbar_wait_spin(&p_full[i], p_seen[i] & 1, a.c.status, kPagedTimeout));
+                            ok = warp_wait_spin(&p_full[i], p_seen[i] & 1, a.c.status);
                             ++p_seen[i];
                             if (!v_there) full(2 * blk + 1);
                             v_there = true;
@@ -777,7 +808,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 nb += n_blk;
             }
             commit(done);   // nothing is in flight when the tensor memory is freed
-            mbar_wait_spin(done, 0, a.c.status, kPagedTimeout);
+            warp_wait_spin(done, 0, a.c.status);
         }
         __syncwarp();
     }
@@ -793,7 +824,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
         bool ok = true;
         for (int items = 0;; ++items)
         {
-            ok = mbar_wait(q_full, items & 1, a.c.status, kPagedTimeout);
+            ok = warp_wait(q_full, items & 1, a.c.status);
             if (!ok) break;
             const ChunkItem it = items_s[items & 1];
             const int c = i * 128 + c_in;
@@ -847,8 +878,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 const int blk = nb + b - it.b0, ring = blk & 3, vslot = (2 * blk + 1) % SLOTS;
                 // (the values' barrier tells that the block's scales and bits are there too, and its slot
                 // cannot be filled anew before this tile's weights are out)
-                ok = mbar_wait(&kv_full[vslot], ((2 * blk + 1) / SLOTS) & 1, a.c.status, kPagedTimeout) &&
-                     mbar_wait(&s_full[i], seen & 1, a.c.status, kPagedTimeout);
+                ok = warp_wait(&kv_full[vslot], ((2 * blk + 1) / SLOTS) & 1, a.c.status) &&
+                     warp_wait(&s_full[i], seen & 1, a.c.status);
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t r[128];   // scores, then (packed) weights
@@ -893,8 +924,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                         // (the mark of this block stands until the tile's weights are out)
                         if (bad) *reinterpret_cast<volatile int*>(&odd_s[i]) = seen + 1;
                         mbar_arrive(&agreed[i]);
-                        ok = mbar_wait(&agreed[i], masked & 1, a.c.status, kPagedTimeout);
+                        ok = warp_wait(&agreed[i], masked & 1, a.c.status);
                         ++masked;
+                        if (!ok) break;
                         odd = *reinterpret_cast<volatile int*>(&odd_s[i]) == seen + 1;
                     }
                 }
@@ -925,7 +957,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 }
                 if (b > it.b0 && __any_sync(0xffffffffu, grow))
                 {
-                    ok = mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
+                    ok = warp_wait(&o_full[i], (seen - 1) & 1, a.c.status);
+                    if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int x = 0; x < D / 16; ++x)
@@ -963,7 +996,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     if (odd)
                     {
                         // o += p v, key by key, for what the column sees.
-                        if (b > it.b0) ok = ok && mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
+                        if (b > it.b0) ok = warp_wait(&o_full[i], (seen - 1) & 1, a.c.status);
+                        if (!ok) break;
                         tc_fence_after();
                         const uint32_t vbase = sm + E::RING_OFF + vslot * E::TILE_B;
                         auto vis_at = [&](int x) { return x == 0 ? vis[0] : x == 1 ? vis[1] : x == 2 ? vis[2] : vis[3]; };
@@ -1064,8 +1098,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                 for (int b = it.b0; b < lim && ok; ++b, ++seen)
                 {
                     const int blk = nb + b - it.b0, ring = blk & 3, vslot = (2 * blk + 1) % SLOTS;
-                    ok = mbar_wait(&kv_full[vslot], ((2 * blk + 1) / SLOTS) & 1, a.c.status, kPagedTimeout) &&
-                         mbar_wait(&s_full[i], seen & 1, a.c.status, kPagedTimeout);
+                    ok = warp_wait(&kv_full[vslot], ((2 * blk + 1) / SLOTS) & 1, a.c.status) &&
+                         warp_wait(&s_full[i], seen & 1, a.c.status);
                     if (!ok) break;
                     tc_fence_after();
                     const float4* const sc = reinterpret_cast<const float4*>(smem + E::SCALE_OFF + ring * E::SCALE_B) + (lane & 3);
@@ -1191,7 +1225,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     }
                     if (b > it.b0 && __any_sync(0xffffffffu, grew))
                     {
-                        ok = mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
+                        ok = warp_wait(&o_full[i], (seen - 1) & 1, a.c.status);
+                        if (!ok) break;
                         tc_fence_after();
                         const float mine = of_row(corr);
 #pragma unroll 1
@@ -1271,7 +1306,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             const bool any = lim > it.b0;
             if (any)
             {
-                ok = mbar_wait(&o_full[i], (seen - 1) & 1, a.c.status, kPagedTimeout);
+                ok = warp_wait(&o_full[i], (seen - 1) & 1, a.c.status);
                 if (!ok) break;
                 tc_fence_after();
             }

@@ -1,0 +1,18 @@
+"""CPU checks of the paged cache at the edges of what its calls allow."""
+
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hunyuanocr-ncnn_b200", "csrc")
+
+
+def test_waits_of_the_wide_kernel_end_alike_in_a_whole_warp():
+    """What follows a wait there is of the whole warp (tensor memory, shuffles), so a wait's outcome has to be too:
+    every one goes through a vote."""
+    with open(os.path.join(CSRC, "hy_paged_chunk.cuh")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    waits = re.findall(r"[^\n;{]*\bmbar_(?:try_)?wait(?:_spin)?\(", text)
+    assert len(waits) == 3
+    assert all("__all_sync(0xffffffffu, mbar_" in w for w in waits), waits
+    uses = re.findall(r"[^\n;{]*\bwarp_wait(?:_spin)?\([^;]*;", text)
+    assert len(uses) > 20
