@@ -270,6 +270,9 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     const int group = q_heads / cache->num_kv_heads;
+    // Positions lie below 2^30: wider windows and more sinks change nothing, and sums with these stay within 32 bits.
+    window = std::min(window, 1 << 30);
+    sinks = std::min(sinks, 1 << 30);
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
                           power_of_two(cache->page_size), power_of_two(group), scale * 1.4426950408889634f, workspace_dev};

@@ -45,7 +45,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
     o.p_first = s.kv - s.n + paged_row_of(a, c0);
     o.p_last = s.kv - s.n + paged_row_of(a, last);
     const int hi = o.p_last < 0 ? 0 : a.causal ? o.p_last + 1 : s.kv;
-    o.lo = (a.window > 0) ? min(hi, max(0, o.p_first - a.window + 1)) / ALIGN * ALIGN : 0;
+    // (rows before position 0 see nothing: the first that may see something stands at 0 or later)
+    o.lo = (a.window > 0) ? min(hi, max(0, max(0, o.p_first) - a.window + 1)) / ALIGN * ALIGN : 0;
     o.sinks = a.sinks >= o.lo ? o.lo : (a.sinks + ALIGN - 1) / ALIGN * ALIGN;
     o.n = o.sinks + hi - o.lo;
     return o;

@@ -52,3 +52,15 @@ def test_scattered_bad_pages_in_chunks(paged, pkg, cache, page):
         assert torch.equal(st.cache.attention(st.batch, q, 0.1), first)
     with pytest.raises(pkg.HyError, match="page number"):
         st.cache.check()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30])
+@pytest.mark.parametrize("rows,cache", [(F32, F32), (BF16, BF16), (BF16, E4M3)])
+def test_window_without_end_and_padding(paged, rows, cache, window):
+    """The largest windows and sinks there are, beside rows that lie far before position 0."""
+    for seqs in ([(3, 9), (0, 4), (20, 1)], [(100, 150), (0, 70), (300, 40)]):
+        for page in (16, 24):
+            for sinks in (0, 3, 2 ** 31 - 1):
+                st = Setup(paged, cache, seqs, extra_rows=1, page=page, seed=33)
+                st.fill()
+                st.check_attention(4, rows, window=window, sinks=sinks)
