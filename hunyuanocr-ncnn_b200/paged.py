@@ -23,6 +23,7 @@ _STATUS = {1: "a page number lies outside the cache", 2: "a kv_len does not fit 
            4: "q_start is not ascending or leaves the rows", 8: "a bounded wait inside a kernel gave up"}
 
 _I, _L, _P = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
+_INT_MAX = 2 ** 31 - 1
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the handle alone, without building a torch.cuda.Stream
 
 
@@ -190,6 +191,7 @@ class PagedKVCache:
         work = torch.empty(need, dtype=torch.uint8, device=self.device)
         q0, q1, _ = q.stride()
         o0, o1, _ = out.stride()
+        window, sinks = max(min(window, _INT_MAX), -1), max(min(sinks, _INT_MAX), -1)   # (a C int would wrap)
         rc = self._lib.hy_paged_attention(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), q0, q1,
                                           out.data_ptr(), o0, o1, scale, causal, window, sinks, work.data_ptr(), need,
                                           _raw_stream(self._index))

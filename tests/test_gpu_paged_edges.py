@@ -64,3 +64,17 @@ def test_window_without_end_and_padding(paged, rows, cache, window):
                 st = Setup(paged, cache, seqs, extra_rows=1, page=page, seed=33)
                 st.fill()
                 st.check_attention(4, rows, window=window, sinks=sinks)
+
+
+def test_window_and_sinks_of_any_size(paged, pkg):
+    """Numbers past 32 bits are no other numbers: they see what any window as long as the cache sees."""
+    st = Setup(paged, BF16, [(300, 5), (90, 1)], seed=38)
+    st.fill()
+    q = torch.randn(st.rows, 4, 128, generator=st.gen).to(BF16).to(DEV)
+    want = st.cache.attention(st.batch, q, 0.1)
+    for window, sinks in ((2 ** 31, 0), (2 ** 32 + 5, 2), (10 ** 18, 0), (3, 2 ** 32 + 1), (3, 2 ** 31)):
+        out = st.check_attention(4, BF16, scale=0.1, window=window, sinks=sinks, q=q)
+        assert torch.equal(out, want)
+    for over in (dict(window=-2 ** 32 - 5), dict(window=-1), dict(window=3, sinks=-2 ** 32 + 7)):
+        with pytest.raises(pkg.HyError, match="negative"):
+            st.cache.attention(st.batch, q, 0.1, **over)
