@@ -129,6 +129,11 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Exponent of a scale of values, of either sign, kept within 100 octaves.
+__device__ __forceinline__ int scale_exponent(float v)
+{
+    return min(max(static_cast<int>((__float_as_uint(v) >> 23) & 0xffu) - 127, -100), 100);
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
 {
     const __half2 v = __floats2half2_rn(lo, hi);
@@ -543,7 +548,7 @@ struct MmaEngine {
                     const float v = lds_f32(at + KEYS * 4);
                     // The maximum is taken over the score plus the exponent of the value's scale, so that
                     // a weight times its scale is below 2 and fits f16 (times 2^14).
-                    ev[hv][r] = static_cast<float>(min(max(static_cast<int>(__float_as_uint(v) >> 23) - 127, -100), 100));
+                    ev[hv][r] = static_cast<float>(scale_exponent(v));
                     vs[hv][r] = v * 16384.f;
                 }
             }

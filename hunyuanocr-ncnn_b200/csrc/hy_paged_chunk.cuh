@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                             // (entries of a block are written when the one four before it is long used)
                             float* const sc = reinterpret_cast<float*>(smem + E::SCALE_OFF + (blk & 3) * E::SCALE_B);
                             const int at = (lt >> 4) * 16 + ((lt >> 1) & 3) * 4 + ((lt >> 3) & 1) * 2 + (lt & 1);
-                            const int ev = min(max(static_cast<int>(__float_as_uint(vs) >> 23) - 127, -100), 100);
+                            const int ev = scale_exponent(vs);
                             sc[at] = ks;
                             sc[128 + at] = vs * 64.f;
                             sc[256 + at] = static_cast<float>(ev);

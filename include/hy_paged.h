@@ -29,7 +29,8 @@ extern "C" {
 #endif
 
 /* Cache types beside HY_DTYPE_F32 and HY_DTYPE_BF16, with one fp32 scale per
- * row and head: a value is code * scale. */
+ * row and head: a value is code * scale (a caller's own scales may have
+ * either sign). */
 enum hy_paged_dtype { HY_DTYPE_E4M3 = 2, HY_DTYPE_INT8 = 3 };
 
 /* Bits that the kernels set in *status_dev (never cleared by the library) when

@@ -78,3 +78,26 @@ def test_window_and_sinks_of_any_size(paged, pkg):
     for over in (dict(window=-2 ** 32 - 5), dict(window=-1), dict(window=3, sinks=-2 ** 32 + 7)):
         with pytest.raises(pkg.HyError, match="negative"):
             st.cache.attention(st.batch, q, 0.1, **over)
+
+
+@pytest.mark.parametrize("cache", [E4M3, INT8])
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("seqs", [RAGGED, BLOCKS, CHUNKS], ids=["tokens", "blocks", "chunks"])
+def test_scales_of_either_sign(paged, rows, cache, seqs):
+    """A caller's own scales may be negative: a value is code * scale, in attention as in what is read back."""
+    st = Setup(paged, cache, seqs, seed=34)
+    st.fill()
+    for which, held in (("k_scale", st.keys), ("v_scale", st.values)):
+        scale = getattr(st.cache, which)
+        sign = torch.where(torch.rand(scale.shape, generator=st.gen) < 0.3, -1.0, 1.0)
+        scale *= sign.to(DEV)
+        for s, kv in enumerate(st.kv):
+            p = torch.arange(kv)
+            held[s] *= sign[st.table[s, p // st.page].long(), :, p % st.page][..., None].double().to(DEV)
+    st.check_attention(4, rows)
+    st.check_attention(4, rows, window=100, sinks=3)
+    for s, kv in enumerate(st.kv):   # and the same values are read back
+        if kv:
+            one = paged.PagedBatch(torch.tensor([0, kv], dtype=torch.int32, device=DEV), st.d_kv[s:s + 1], st.d_table[s:s + 1], kv)
+            k, v = st.cache.read(one, kv, F32)
+            assert torch.equal(k, st.keys[s].float()) and torch.equal(v, st.values[s].float())
