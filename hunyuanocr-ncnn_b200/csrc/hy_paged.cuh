@@ -99,9 +99,15 @@ constexpr bool kCodes = (sizeof(CT) == 1);   // codes with a scale
 
 // x / s rounded to fp32 so that no later rounding to fewer bits can go wrong: where the quotient is not a
 // float, of the two floats around it the one whose last bit is set (it lies on the quotient's side
-// of every tie). The remainder x - q s of the nearest q is exact in a fused multiply-add.
+// of every tie). The remainder x - q s of the nearest q is exact in a fused multiply-add as long as it is no
+// smaller than the smallest number: scales below 2^-60 and their x are first taken 2^80 times (exactly; a
+// quotient next to a tie is at least 2^-10, so its remainder is a multiple of 2^(-33 - 23 - 60)).
 __device__ __forceinline__ float quotient_odd(float x, float s, float inv)
 {
+    const bool tiny = s < 0x1p-60f;
+    x *= tiny ? 0x1p80f : 1.f;
+    s *= tiny ? 0x1p80f : 1.f;
+    inv *= tiny ? 0x1p-80f : 1.f;
     float q = x * inv;
     q = fmaf(fmaf(-q, s, x), inv, q);
     const float r = fmaf(-q, s, x);

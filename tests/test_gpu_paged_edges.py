@@ -101,3 +101,30 @@ def test_scales_of_either_sign(paged, rows, cache, seqs):
             one = paged.PagedBatch(torch.tensor([0, kv], dtype=torch.int32, device=DEV), st.d_kv[s:s + 1], st.d_table[s:s + 1], kv)
             k, v = st.cache.read(one, kv, F32)
             assert torch.equal(k, st.keys[s].float()) and torch.equal(v, st.values[s].float())
+
+
+@pytest.mark.parametrize("cache", [E4M3, INT8])
+def test_quantisation_near_ties_at_tiny_scales(paged, cache):
+    """Scales from the smallest, 2^-126, up: quotients just below, at and just above a tie, where the remainder of a
+    division lies below the smallest normal number."""
+    rng = np.random.default_rng(5)
+    rows, dim, top = 4096, 128, R.LARGEST[cache]
+    grid = R.e4m3_values() if cache == E4M3 else np.arange(128.0)
+    mids = (grid[1:] + grid[:-1]) / 2
+    amax = (rng.uniform(1.0, 2.0, rows) * top * 2.0 ** rng.integers(-128, -20, rows)).astype(np.float32)
+    scale = np.maximum((amax.astype(np.float64) / top).astype(np.float32), np.float32(2.0 ** -126)).astype(np.float64)
+    x = (rng.choice(mids, (rows, dim)) * scale[:, None]).astype(np.float32)
+    x = np.nextafter(x, rng.choice([-np.inf, 0, np.inf], (rows, dim)).astype(np.float32), dtype=np.float32)
+    x *= rng.choice([-1, 1], (rows, dim)).astype(np.float32)
+    x = np.clip(x, -amax[:, None], amax[:, None])
+    x[:, 0] = amax
+    t = torch.from_numpy(x)[:, None, :].contiguous()
+    st = Setup(paged, cache, [(rows, rows)], kv_heads=1)
+    st.cache.write(st.batch, t.to(DEV), t.to(DEV))
+    st.cache.check()
+    code, s = R.quantise(t, cache)
+    p = torch.arange(rows)
+    at = (st.table[0, p // st.page].long(), slice(None), p % st.page)
+    for pool, scales in ((st.cache.k, st.cache.k_scale), (st.cache.v, st.cache.v_scale)):
+        assert torch.equal(scales.cpu()[at], s.float())
+        assert torch.equal(pool.float().cpu()[at].double(), code)
