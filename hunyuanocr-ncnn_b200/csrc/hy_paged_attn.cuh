@@ -7,7 +7,8 @@
 //
 // What a tile of rows sees is one run of "virtual" positions: the sinks before
 // its window, then the window's positions up to the last row's; neither the
-// gap between them nor what lies behind the last row is ever loaded.
+// gap between them nor what lies behind the last row is ever looked up. (The wide kernel of
+// hy_paged_chunk.cuh fetches pages 16 rows at a time where they hold a multiple of 16.)
 #pragma once
 
 #include "hy_paged.cuh"
@@ -36,9 +37,9 @@ struct PagedSpan {
     int p_first, p_last;   // positions of the first and last row
     int sinks, lo, n;      // virtual position u < sinks: u, else lo + u - sinks; n of them
 };
-// ALIGN: the run's parts start and the sinks end at multiples of it (what that adds is masked).
-template <int ALIGN = 1>
-__device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const PagedSeq& s, int c0, int cols)
+// align (a power of two): the run's parts start and the sinks end at multiples of it (what that adds is masked).
+// Above 1 only where it divides the page size: then what it adds lies in pages that hold visible keys too.
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const PagedSeq& s, int c0, int cols, int align = 1)
 {
     PagedSpan o;
     const int last = min(s.n * a.group, c0 + cols) - 1;
@@ -46,8 +47,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
     o.p_last = s.kv - s.n + paged_row_of(a, last);
     const int hi = o.p_last < 0 ? 0 : a.causal ? o.p_last + 1 : s.kv;
     // (rows before position 0 see nothing: the first that may see something stands at 0 or later)
-    o.lo = (a.window > 0) ? min(hi, max(0, max(0, o.p_first) - a.window + 1)) / ALIGN * ALIGN : 0;
-    o.sinks = a.sinks >= o.lo ? o.lo : (a.sinks + ALIGN - 1) / ALIGN * ALIGN;
+    o.lo = (a.window > 0) ? min(hi, max(0, max(0, o.p_first) - a.window + 1)) & -align : 0;
+    o.sinks = a.sinks >= o.lo ? o.lo : (a.sinks + align - 1) & -align;
     o.n = o.sinks + hi - o.lo;
     return o;
 }
@@ -999,14 +1000,14 @@ __device__ __forceinline__ int split_div(long long x, int n)
 }
 
 // Tiles of sequence s, all its items.
-template <int COLS, int TILE, int ALIGN>
-__device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s)
+template <int COLS, int TILE>
+__device__ __forceinline__ long long split_cost(const PagedAttnArgs& a, int s, int align)
 {
     PagedSeq q;
     if (s >= a.b.num_seqs || !paged_seq(a.b, s, a.c.page_size, a.c.status, q)) return 0;
     long long c = 0;
     const int rt = split_row_tiles<COLS>(a, q.n);
-    for (int t = 0; t < rt; ++t) c += split_tiles<TILE>(paged_span<ALIGN>(a, q, t * COLS, COLS).n);
+    for (int t = 0; t < rt; ++t) c += split_tiles<TILE>(paged_span(a, q, t * COLS, COLS, align).n);
     return c * a.c.kv_heads;
 }
 
@@ -1023,13 +1024,13 @@ struct SplitStart {
     int seq;
 };
 // By every warp for itself; true if the list is of that kind.
-template <int COLS, int TILE, int ALIGN>
-__device__ __forceinline__ bool split_start_few(const PagedAttnArgs& a, SplitStart& o)
+template <int COLS, int TILE>
+__device__ __forceinline__ bool split_start_few(const PagedAttnArgs& a, int align, SplitStart& o)
 {
     const int lane = threadIdx.x & 31, ctas = gridDim.x, h = a.c.kv_heads;
     PagedSeq q = {0, 0, 0};
     const bool there = lane < a.b.num_seqs && paged_seq(a.b, lane, a.c.page_size, a.c.status, q) && q.n > 0;
-    const int t = there ? split_tiles<TILE>(paged_span<ALIGN>(a, q, 0, COLS).n) : 0;
+    const int t = there ? split_tiles<TILE>(paged_span(a, q, 0, COLS, align).n) : 0;
     const int all = __reduce_add_sync(0xffffffffu, min(t, 1 << 20));
     const int items = __popc(__ballot_sync(0xffffffffu, there)) * h;
     if (__any_sync(0xffffffffu, there && (q.n > COLS || q.n * a.group > COLS)) || items > ctas || all > (1 << 20) / h) return false;
@@ -1060,21 +1061,21 @@ __device__ __forceinline__ bool split_start_few(const PagedAttnArgs& a, SplitSta
     return true;
 }
 // scan: shared memory for a long long per warp and one more.
-template <int COLS, int TILE, int THREADS, int ALIGN = 1>
-__device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long long* scan)
+template <int COLS, int TILE, int THREADS>
+__device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long long* scan, int align = 1)
 {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __shared__ int s_seq;
     SplitStart o;
-    if (a.b.num_seqs <= 32 && split_start_few<COLS, TILE, ALIGN>(a, o)) return o;
+    if (a.b.num_seqs <= 32 && split_start_few<COLS, TILE>(a, align, o)) return o;
     o.unit = 1;
     o.total = 0;
     const int rounds = (a.b.num_seqs + THREADS - 1) / THREADS;
     long long mine = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        mine = split_cost<COLS, TILE, ALIGN>(a, r * THREADS + tid);
+        mine = split_cost<COLS, TILE>(a, r * THREADS + tid, align);
         o.total += mine;
     }
 #pragma unroll
@@ -1092,7 +1093,7 @@ __device__ __forceinline__ SplitStart split_start(const PagedAttnArgs& a, long l
     long long base = 0;
     for (int r = 0; r < rounds; ++r)
     {
-        if (rounds > 1) mine = split_cost<COLS, TILE, ALIGN>(a, r * THREADS + tid);
+        if (rounds > 1) mine = split_cost<COLS, TILE>(a, r * THREADS + tid, align);
         long long inc = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1)

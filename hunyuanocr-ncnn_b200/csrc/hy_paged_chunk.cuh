@@ -236,9 +236,11 @@ struct ItemWalk {
     int units;             // (single) CTAs that share the item
     int b0, b1;            // blocks of the item that are this CTA's
     bool first, single;    // single: no second item
+    int align;             // of the spans
 
-    __device__ __forceinline__ bool open(const PagedAttnArgs& a, const SplitStart& st)
+    __device__ __forceinline__ bool open(const PagedAttnArgs& a, const SplitStart& st, int span_align)
     {
+        align = span_align;
         left = (st.x1 - st.x0) * st.unit;
         single = st.unit > 1;
         first = true;
@@ -248,7 +250,7 @@ struct ItemWalk {
         long long in = st.in_seq;
         for (it.tile = 0;; ++it.tile)
         {
-            it.w = paged_span<16>(a, it.q, it.tile * COLS, COLS);
+            it.w = paged_span(a, it.q, it.tile * COLS, COLS, align);
             it.tiles = split_tiles<TILE>(it.w.n);
             units = (it.tiles + st.unit - 1) / st.unit;
             if (in < static_cast<long long>(units) * a.c.kv_heads) break;
@@ -290,7 +292,7 @@ struct ItemWalk {
                 } while (it.seq < a.b.num_seqs && (!paged_seq(a.b, it.seq, a.c.page_size, nullptr, it.q) || it.q.n == 0));
                 if (it.seq >= a.b.num_seqs) return false;   // (the arrays changed under the call)
             }
-            it.w = paged_span<16>(a, it.q, it.tile * COLS, COLS);
+            it.w = paged_span(a, it.q, it.tile * COLS, COLS, align);
             it.tiles = split_tiles<TILE>(it.w.n);
         }
         set(a);
@@ -397,14 +399,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     pdl_launch();
     if (tid == 0) static_cast<PagedJoin*>(a.work)[blockIdx.x].count = 0;   // (rewritten below by the same thread)
 
-    const SplitStart st = split_start<256, 128, kChunkThreads, 16>(a, scan);
+    const int align = tma.on ? 16 : 1;   // (copied row by row, a block may start anywhere)
+    const SplitStart st = split_start<256, 128, kChunkThreads>(a, scan, align);
     if (warp >= kChunkLoadWarp && warp < kChunkMmaWarp)
     {
         // ---------------- loads ----------------
         regs_dec<kChunkRegsOther<F16>>();
         const int lt = tid - kChunkLoadWarp * 32, lw = lt >> 5;
         Walk w;
-        bool more = w.open(a, st);
+        bool more = w.open(a, st, align);
         int n = 0;             // slots filled
         int blk = 0;           // blocks (index of the scale ring)
         int items = 0, mended = 0;

@@ -128,3 +128,19 @@ def test_quantisation_near_ties_at_tiny_scales(paged, cache):
     for pool, scales in ((st.cache.k, st.cache.k_scale), (st.cache.v, st.cache.v_scale)):
         assert torch.equal(scales.cpu()[at], s.float())
         assert torch.equal(pool.float().cpu()[at].double(), code)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 40, 64])
+@pytest.mark.parametrize("window,sinks", [(1024, 4), (1000, 0), (300, 17), (7, 33)])
+def test_pages_that_no_row_sees_may_be_unmapped(paged, page, window, sinks):
+    """Pages wholly behind the window of a sequence's first row and past the sinks are given back (-1): no row sees
+    them, nothing is reported and the outputs are right."""
+    for rows, cache, seqs in ((BF16, BF16, [(5000, 300), (2000, 40), (64, 64)]), (BF16, E4M3, [(5000, 300), (2011, 17)]),
+                              (F32, BF16, [(3000, 20), (1500, 1)]), (BF16, INT8, [(3001, 1), (1200, 1)])):
+        st = Setup(paged, cache, seqs, page=page, seed=35)
+        st.fill()
+        for s, (kv, n) in enumerate(seqs):
+            for x in range(-(-kv // page)):
+                if x * page >= sinks and (x + 1) * page - 1 <= kv - n - window:
+                    st.d_table[s, x] = -1
+        st.check_attention(4, rows, window=window, sinks=sinks)
