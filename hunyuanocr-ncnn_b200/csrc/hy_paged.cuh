@@ -70,7 +70,8 @@ __device__ __forceinline__ bool paged_seq(const PagedBatch& b, int s, int page_s
 }
 
 // The sequence that holds row r (the last one whose q_start is <= r), by the
-// whole warp: 32 starts per round, counted by a ballot. -1: no sequence does.
+// whole warp: 32 starts per round, counted by a ballot. -1: r lies before the first sequence;
+// num_seqs: behind the last.
 __device__ __forceinline__ int paged_find_seq(const PagedBatch& b, int r, int lane)
 {
     int below = 0;
@@ -82,7 +83,7 @@ __device__ __forceinline__ int paged_find_seq(const PagedBatch& b, int r, int la
         below += c;
         if (c < 32) break;
     }
-    return (below == 0 || below > b.num_seqs) ? -1 : below - 1;
+    return below - 1;
 }
 
 // ---------------------------------------------------------------------------

@@ -144,3 +144,34 @@ def test_pages_that_no_row_sees_may_be_unmapped(paged, page, window, sinks):
                 if x * page >= sinks and (x + 1) * page - 1 <= kv - n - window:
                     st.d_table[s, x] = -1
         st.check_attention(4, rows, window=window, sinks=sinks)
+
+
+def test_rows_behind_the_last_sequence_cost_no_walk(paged):
+    """Padding rows of a call with many sequences are found to be nobody's about as fast as rows are found."""
+    n, rows = 60000, 4096
+    kv = torch.zeros(n, dtype=torch.int32, device=DEV)
+    kv[-1] = rows
+    table = torch.arange(rows // 16, dtype=torch.int32, device=DEV)[None].expand(n, -1)
+    starts = torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    cache = paged.PagedKVCache.allocate(rows // 16, 1, 16, 64, BF16)
+    k = torch.randn(rows, 1, 64, device=DEV)
+    padded = paged.PagedBatch(starts.clone(), kv, table, 1)      # every row lies behind the last sequence
+    starts[-1] = rows
+    owned = paged.PagedBatch(starts, kv, table, rows)            # every row is the last sequence's
+
+    def time(batch):
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(4):
+                cache.write(batch, k, k)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    time(owned)
+    t_owned, t_padded = time(owned), time(padded)
+    cache.check()
+    assert t_padded < 2.5 * t_owned, (t_padded, t_owned)
