@@ -51,7 +51,9 @@ struct ChunkEngine {
     using CT = CT_;
     static constexpr int D = D_, COLS = 256, KEYS = 128;
     static constexpr bool F16 = kCodes<CT>;
-    // f16 weights carry 2^6: below 2^(6 + 8 + 1), and exact to 11 bits down to 2^-20 of the largest.
+    // f16 weights (times their values' scales) carry 2^6: below 2^(6 + 8 + 1), and rounded to 11 bits down to
+    // 2^-20 of a row's largest, 2^-16 where one exponent stands for a block's scales; smaller ones lose bits, and below
+    // 2^-27 nothing of them is left.
     static constexpr float OUT = F16 ? 1.f / 64.f : 1.f;
     static constexpr int RB = D * 2;                       // bytes of a row in operand layout
     static constexpr int TILE_B = 128 * RB;                // a block of K or V, a tile of q
@@ -1117,8 +1119,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
                     }
                     const bool whole = sees_all(b * 128, live);
                     // The reference takes in the exponents of the values' scales. Where they are close, the block's
-                    // largest serves every key (weights are then smaller by 2^12 at most); it must be of keys that the columns see.
-                    const bool tight = whole && ev_hi - ev_lo <= 12;
+                    // largest serves every key; it must be of keys that the columns see. Weights are then smaller by up to
+                    // 2^4: with 2^12 a row of 16000 light keys beside a heavy one lost them all.
+                    const bool tight = whole && ev_hi - ev_lo <= 4;
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     // First pass, 32 keys at a time (loops, not straight code: four roles' instructions compete for the
                     // instruction cache): scores times their keys' scales, masked, back to tensor memory; the maxima.

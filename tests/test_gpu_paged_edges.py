@@ -175,3 +175,40 @@ def test_rows_behind_the_last_sequence_cost_no_walk(paged):
     t_owned, t_padded = time(owned), time(padded)
     cache.check()
     assert t_padded < 2.5 * t_owned, (t_padded, t_owned)
+
+
+@pytest.mark.parametrize("cache", [E4M3, INT8])
+def test_many_light_keys_beside_a_heavy_one(paged, cache):
+    """A key with nearly all the weight, some 16000 light ones of 2^-20 each that make up a 64th, and among those, one
+    in 128, keys of next to no weight whose values' scale is 2^12 times the others'. In the wide kernel one exponent may
+    stand for the scales of a block; the light keys' products must not fall below f16's smallest number for it.
+
+    A key's f16 product carries 2^6, is off by half a step, 2^-11 of it, and at least 2^-25; the running maximum is at most
+    2^4 above the row's largest weight times scale (T). So a key adds at most 2^(-25 - 6 + 4) |code| T to the error."""
+    seqs, kv, n, dim = 160, 16384, 40, 64   # (more items than CTAs, so that a CTA meets the heavy key and the light ones)
+    top = R.LARGEST[cache]
+    k, v = torch.zeros(kv, 1, dim), torch.zeros(kv, 1, dim)
+    k[:, :, 0] = 100.0
+    k[0::128, :, 0] = 80.0
+    k[1, :, 0] = 120.0
+    v[:, :, 0], v[:, :, 1] = top, 0.5 * top
+    v[1], v[0::128] = 0.0, 0.0
+    v[1, :, 2], v[0::128, :, 3] = top, top * 2.0 ** 12
+    st = Setup(paged, cache, [(kv, kv)], kv_heads=1, dim=dim, page=16, seed=36)
+    st.cache.write(st.batch, k.to(DEV), v.to(DEV))
+    keys, values = st.stand_for(k), st.stand_for(v)
+    scales = R.quantise(v, cache)[1][:, 0].to(DEV)
+    q = torch.zeros(seqs * n, 1, dim, dtype=BF16, device=DEV)
+    q[:, :, 0] = 1.0
+    batch = paged.PagedBatch(torch.arange(0, seqs * n + 1, n, dtype=torch.int32, device=DEV),
+                             st.d_kv.expand(seqs).contiguous(), st.d_table.expand(seqs, -1), n)
+    scale = math.log(2.0)   # a score is a power of two's exponent
+    out = st.cache.attention(batch, q, scale).view(seqs, n, 1, dim).double()
+    st.cache.check()
+    want, mass, _ = R.attention(q[:n].double(), keys, values, list(range(kv - n, kv)), scale)
+    weight = torch.exp2(keys[:, 0, 0] - 120.0)
+    weight /= weight.sum()
+    codes = (values[:, 0] / scales[:, None]).abs().sum(dim=0)
+    tol = 2.0 ** -27 * float((weight * scales).max()) * codes + mass * (2.0 ** -11 + 2.0 ** -16) + want.abs() * 2.0 ** -8
+    assert float((tol / want.abs())[..., :2].max()) < 2.0 ** -6   # (nothing like the outputs themselves)
+    assert bool(((out - want).abs() <= tol).all()), (out[0, 0, 0, :4], want[0, 0, :4])
