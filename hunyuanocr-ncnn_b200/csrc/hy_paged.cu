@@ -49,6 +49,9 @@ int power_of_two(int n)
     return s;
 }
 
+// A stride of a dimension with one entry is never taken.
+bool off16(long long stride, int elem, int entries) { return entries > 1 && stride * elem % 16 != 0; }
+
 int elem_size(int dtype) { return dtype == HY_DTYPE_F32 ? 4 : dtype == HY_DTYPE_BF16 ? 2 : 1; }
 
 int check_cache(const hy_paged_cache* c)
@@ -63,8 +66,8 @@ int check_cache(const hy_paged_cache* c)
     if (c->num_kv_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "num_kv_heads must be at most 1024");
     if (!c->k_dev || !c->v_dev) return fail(HY_ERR_INVALID_ARGUMENT, "cache memory is null");
     const int e = elem_size(c->dtype);
-    if (!aligned16(c->k_dev) || !aligned16(c->v_dev) || c->page_stride * e % 16 || c->head_stride * e % 16 ||
-        c->row_stride * e % 16)
+    if (!aligned16(c->k_dev) || !aligned16(c->v_dev) || off16(c->page_stride, e, c->num_pages) ||
+        off16(c->head_stride, e, c->num_kv_heads) || off16(c->row_stride, e, c->page_size))
         return fail(HY_ERR_INVALID_ARGUMENT, "cache rows must start on 16 bytes");
     if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->scale_page_stride < 0 ||
         c->scale_head_stride < 0 || c->scale_row_stride < 0)
@@ -93,13 +96,13 @@ int check_batch(const hy_paged_batch* b, const hy_paged_cache* c)
     return HY_OK;
 }
 
-int check_rows(const char* name, const void* p, long long row_stride, long long head_stride, int dtype)
+int check_rows(const char* name, const void* p, int rows, int heads, long long row_stride, long long head_stride, int dtype)
 {
     char msg[96];
     const int e = elem_size(dtype);
     const char* what = !p                                                                      ? "%s is null"
                        : row_stride < 0 || head_stride < 0                                     ? "%s strides must not be negative"
-                       : !aligned16(p) || row_stride * e % 16 || head_stride * e % 16          ? "%s rows must start on 16 bytes"
+                       : !aligned16(p) || off16(row_stride, e, rows) || off16(head_stride, e, heads) ? "%s rows must start on 16 bytes"
                                                                                                : nullptr;
     if (!what) return HY_OK;
     snprintf(msg, sizeof msg, what, name);
@@ -158,8 +161,8 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     if (!rc) rc = check_dtype(rows, dtype);
     if (rc) return rc;
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
-    rc = check_rows("k", k, krs, khs, dtype);
-    if (!rc) rc = check_rows("v", v, vrs, vhs, dtype);
+    rc = check_rows("k", k, rows, cache->num_kv_heads, krs, khs, dtype);
+    if (!rc) rc = check_rows("v", v, rows, cache->num_kv_heads, vrs, vhs, dtype);
     if (rc) return rc;
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
@@ -259,8 +262,8 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     if (!(scale > 0.f) || scale - scale != 0.f)
         return fail(HY_ERR_INVALID_ARGUMENT, "scale must be finite and positive");
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
-    rc = check_rows("q", q_dev, q_row_stride, q_head_stride, dtype);
-    if (!rc) rc = check_rows("out", out_dev, out_row_stride, out_head_stride, dtype);
+    rc = check_rows("q", q_dev, rows, q_heads, q_row_stride, q_head_stride, dtype);
+    if (!rc) rc = check_rows("out", out_dev, rows, q_heads, out_row_stride, out_head_stride, dtype);
     if (rc) return rc;
     if (q_dev == out_dev) return fail(HY_ERR_INVALID_ARGUMENT, "q and out must not overlap");
     if (!workspace_dev || !aligned16(workspace_dev))

@@ -212,3 +212,26 @@ def test_many_light_keys_beside_a_heavy_one(paged, cache):
     tol = 2.0 ** -27 * float((weight * scales).max()) * codes + mass * (2.0 ** -11 + 2.0 ** -16) + want.abs() * 2.0 ** -8
     assert float((tol / want.abs())[..., :2].max()) < 2.0 ** -6   # (nothing like the outputs themselves)
     assert bool(((out - want).abs() <= tol).all()), (out[0, 0, 0, :4], want[0, 0, :4])
+
+
+@pytest.mark.parametrize("cache", TYPES)
+@pytest.mark.parametrize("rows", [F32, BF16])
+def test_strides_of_single_entries_do_not_matter(paged, cache, rows):
+    """One row, one head, one page: what its stride is has no meaning, so it need not be a multiple of 16 bytes."""
+    kv, dim, page = 40, 128, 48
+    mem = [torch.zeros(page * dim, dtype=torch.uint8 if cache.itemsize == 1 else cache, device=DEV) for _ in range(2)]
+    k, v = (torch.as_strided(m, (1, 1, page, dim), (7, 3, dim, 1)).view(cache) for m in mem)
+    scales = [torch.full((1, 1, page), math.nan, device=DEV) for _ in range(2)] if cache.itemsize == 1 else (None, None)
+    st = Setup(paged, cache, [(kv, 1)], kv_heads=1, dim=dim, page=page, seed=45, spare_pages=0)
+    st.cache = paged.PagedKVCache(k, v, *scales)
+    st.fill()
+    for heads in (1, 4, 40):
+        wide = torch.randn(heads * dim, generator=st.gen).to(rows).to(DEV)
+        q = torch.as_strided(wide, (1, heads, dim), (5, dim if heads > 1 else 9, 1))
+        out = torch.as_strided(torch.full_like(wide, 77.0), (1, heads, dim), (11, dim if heads > 1 else 1, 1))
+        st.check_attention(heads, rows, q=q, out=out)
+        st.check_attention(heads, rows, window=9, sinks=2, q=q, out=out)
+    back = [torch.as_strided(torch.zeros(dim, device=DEV), (1, 1, dim), (3, 5, 1)) for _ in range(2)]
+    st.cache.read(st.batch, 1, F32, out=tuple(back))
+    st.cache.check()
+    assert torch.equal(back[0][0], st.keys[0][-1].float()) and torch.equal(back[1][0], st.values[0][-1].float())
