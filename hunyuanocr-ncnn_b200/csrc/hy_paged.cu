@@ -259,8 +259,9 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     if (rc) return rc;
     if (window < 0 || sinks < 0) return fail(HY_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
     if (!causal && window > 0) return fail(HY_ERR_UNSUPPORTED, "a window needs causal attention");
-    if (!(scale > 0.f) || scale - scale != 0.f)
-        return fail(HY_ERR_INVALID_ARGUMENT, "scale must be finite and positive");
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!(scale > 0.f) || scale_log2 - scale_log2 != 0.f)
+        return fail(HY_ERR_INVALID_ARGUMENT, "scale must be positive, and finite times log2(e) too");
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
     rc = check_rows("q", q_dev, rows, q_heads, q_row_stride, q_head_stride, dtype);
     if (!rc) rc = check_rows("out", out_dev, rows, q_heads, out_row_stride, out_head_stride, dtype);
@@ -278,7 +279,7 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     sinks = std::min(sinks, 1 << 30);
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
-                          power_of_two(cache->page_size), power_of_two(group), scale * 1.4426950408889634f, workspace_dev};
+                          power_of_two(cache->page_size), power_of_two(group), scale_log2, workspace_dev};
     const int cols = tile_columns(batch->max_rows, group, dtype, cache->dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto launch = dtype == HY_DTYPE_F32 ? hy_internal::paged_attention_f32 : hy_internal::paged_attention_bf16;

@@ -111,7 +111,7 @@ int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, i
  *   causal == 0: every j < kv_len (window must be 0).
  * A row that sees nothing gives zeros. Positions that a row does not see do
  * not reach its output, whatever they hold (infinities and NaN included).
- * scale must be finite and positive. q and out have the same dtype and must
+ * scale must be positive, and scale * log2(e) finite. q and out have the same dtype and must
  * not overlap. Products and softmax sums are in fp32. F32 rows: every product
  * is exact to 2^-22 or better. BF16 rows: probabilities are rounded to bf16
  * before they multiply v, over 8-bit caches (times v's scale) to f16; there,
