@@ -109,6 +109,15 @@ int check_rows(const char* name, const void* p, int rows, int heads, long long r
     return fail(HY_ERR_INVALID_ARGUMENT, msg);
 }
 
+// Rows that a call writes: entries of a dimension whose stride is below head_dim share elements for certain.
+int check_apart(const char* name, int rows, int heads, int head_dim, long long row_stride, long long head_stride)
+{
+    if ((rows < 2 || row_stride >= head_dim) && (heads < 2 || head_stride >= head_dim)) return HY_OK;
+    char msg[96];
+    snprintf(msg, sizeof msg, "%s rows must not overlap", name);
+    return fail(HY_ERR_INVALID_ARGUMENT, msg);
+}
+
 int check_dtype(int rows, int dtype)
 {
     if (rows < 0) return fail(HY_ERR_INVALID_ARGUMENT, "rows must not be negative");
@@ -163,7 +172,10 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
     rc = check_rows("k", k, rows, cache->num_kv_heads, krs, khs, dtype);
     if (!rc) rc = check_rows("v", v, rows, cache->num_kv_heads, vrs, vhs, dtype);
+    if (!rc && !write) rc = check_apart("k", rows, cache->num_kv_heads, cache->head_dim, krs, khs);
+    if (!rc && !write) rc = check_apart("v", rows, cache->num_kv_heads, cache->head_dim, vrs, vhs);
     if (rc) return rc;
+    if (!write && k == v) return fail(HY_ERR_INVALID_ARGUMENT, "k and v must not overlap");
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     for (const long long x : {krs, khs, vrs, vhs, static_cast<long long>(cache->head_stride), static_cast<long long>(cache->scale_head_stride)})
@@ -265,6 +277,7 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
     rc = check_rows("q", q_dev, rows, q_heads, q_row_stride, q_head_stride, dtype);
     if (!rc) rc = check_rows("out", out_dev, rows, q_heads, out_row_stride, out_head_stride, dtype);
+    if (!rc) rc = check_apart("out", rows, q_heads, cache->head_dim, out_row_stride, out_head_stride);
     if (rc) return rc;
     if (q_dev == out_dev) return fail(HY_ERR_INVALID_ARGUMENT, "q and out must not overlap");
     if (!workspace_dev || !aligned16(workspace_dev))

@@ -86,7 +86,7 @@ typedef struct hy_paged_batch {
 /* Row tensors: `rows` rows of num_kv_heads (k, v) or q_heads (q, out) heads of
  * head_dim elements of `dtype` (HY_DTYPE_F32 or HY_DTYPE_BF16), element d of
  * (row, head) at row * row_stride + head * head_stride + d; every (row, head)
- * starts on 16 bytes. */
+ * starts on 16 bytes, and those that a call writes share no memory. */
 
 /* Writes k and v of every row at its position. F32 and BF16 caches: rounded to
  * nearest. 8-bit caches: scale = max(max|x| / M, 2^-126) in fp32 with M = 448

@@ -1,12 +1,13 @@
 """CPU checks of the paged cache at the edges of what its calls allow."""
 
+import ctypes
 import importlib
 import os
 import re
 
 import pytest
 
-from test_paged import _batch, _cache, _calls
+from test_paged import FAKE, _batch, _cache, _calls
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hunyuanocr-ncnn_b200", "csrc")
 
@@ -34,3 +35,24 @@ def test_scales_whose_multiple_overflows_are_refused(paged, scale):
     rc = list(_calls(paged, _cache(paged), _batch(paged), scale=scale))[2]
     assert rc == 1
     assert b"finite" in paged._library().hy_last_error()
+
+
+@pytest.mark.parametrize("strides", [(0, 128), (512, 0), (64, 512), (512, 120)])
+def test_outputs_that_overlap_themselves_are_refused(paged, strides):
+    """Rows or heads of an output that share memory would be written by several blocks at once."""
+    lib = paged._library()
+    c, b = _cache(paged), _batch(paged)
+    ref = [ctypes.byref(x) for x in (c, b)]
+    assert lib.hy_paged_kv_read(*ref, 2, 1, FAKE, *strides, 2 * FAKE, 512, 128, None) == 1
+    assert b"k rows must not overlap" in lib.hy_last_error()
+    assert lib.hy_paged_kv_read(*ref, 2, 1, FAKE, 512, 128, 2 * FAKE, *strides, None) == 1
+    assert b"v rows must not overlap" in lib.hy_last_error()
+    assert lib.hy_paged_attention(*ref, 2, 4, 1, FAKE, 512, 128, 2 * FAKE, *strides, 0.1, 1, 0, 0, None, 0, None) == 1
+    assert b"out rows must not overlap" in lib.hy_last_error()
+
+
+def test_one_output_for_keys_and_values_is_refused(paged):
+    lib = paged._library()
+    c, b = _cache(paged), _batch(paged)
+    assert lib.hy_paged_kv_read(ctypes.byref(c), ctypes.byref(b), 2, 1, FAKE, 512, 128, FAKE, 512, 128, None) == 1
+    assert b"overlap" in lib.hy_last_error()
