@@ -289,9 +289,9 @@ struct SplitShape {
 // lies in the same lane for the scores and for the output.
 //
 // bf16 and fp32 caches multiply in bf16 (an fp32 number as three terms, products
-// of terms i + j <= 2: exact to 2^-23); 8-bit caches in f16, where their codes and
-// the query (each row times a power of two) are exact, fp32 queries as two f16
-// terms. Which dimensions a lane takes from a row is free as long as q
+// of terms i + j <= 2: the three left out are below 2^-21 together); 8-bit caches in f16, where their codes are
+// exact and so is a bf16 query (each row times a power of two; what is below 2^-31 of its largest loses bits), fp32
+// queries as two f16 terms. Which dimensions a lane takes from a row is free as long as q
 // agrees, so 8-bit and fp32 keys are read from shared memory in 16-byte pieces.
 //
 // Decode steps are bound by memory; with 32 columns of fp32 queries the 192 products a

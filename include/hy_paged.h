@@ -111,12 +111,18 @@ int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, i
  *   causal == 0: every j < kv_len (window must be 0).
  * A row that sees nothing gives zeros. Positions that a row does not see do
  * not reach its output, whatever they hold (infinities and NaN included).
- * scale must be positive, and scale * log2(e) finite. q and out have the same dtype and must
- * not overlap. Products and softmax sums are in fp32. F32 rows: every product
- * is exact to 2^-22 or better. BF16 rows: probabilities are rounded to bf16
- * before they multiply v, over 8-bit caches (times v's scale) to f16; there,
- * scales of v beyond 2^100 overflow and those below 2^-100 lose bits. An
- * infinity that a row does see may give NaN.
+ * scale must be positive, and scale * log2(e) finite. q and out have the same
+ * dtype and must not overlap. Products and softmax sums are in fp32; the tensor
+ * cores cut sums instead of rounding them.
+ * F32 rows: products are exact to 2^-21. Over 8-bit caches q and the weights
+ * (probabilities times v's scale) are off by 2^-22 of themselves, or by 2^-39 of
+ * a row's largest where that is more.
+ * BF16 rows: probabilities are rounded to bf16 before they multiply v; over
+ * 8-bit caches they are multiplied by v's scale and rounded to f16, off by 2^-11
+ * of themselves, or by 2^-39 of the row's largest such product (2^-27 where
+ * max_rows times q_heads / num_kv_heads is above 32) where that is more.
+ * Over 8-bit caches scales of v beyond 2^100 overflow and those below 2^-100
+ * lose bits. An infinity that a row does see may give NaN.
  * Limits: q_heads and num_kv_heads 1024, num_seqs 65535, rows * q_heads 2^31,
  * table_width * page_size 2^30; writes and reads take row and head strides
  * (the cache's head strides too) below 2^31. */

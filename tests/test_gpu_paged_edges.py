@@ -2,6 +2,7 @@
 either sign and of every size, windows without end, unmapped pages, padded batches, singleton strides."""
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -235,3 +236,33 @@ def test_strides_of_single_entries_do_not_matter(paged, cache, rows):
     st.cache.read(st.batch, 1, F32, out=tuple(back))
     st.cache.check()
     assert torch.equal(back[0][0], st.keys[0][-1].float()) and torch.equal(back[1][0], st.values[0][-1].float())
+
+
+def test_threads_call_at_once(paged):
+    """Calls of four threads on streams of their own overlap: the same bits as alone."""
+    sts, qs, want = [], [], []
+    for i, (cache, seqs) in enumerate([(BF16, RAGGED), (E4M3, CHUNKS), (F32, BLOCKS), (INT8, [(4000, 1)] * 5)]):
+        st = Setup(paged, cache, seqs, kv_heads=2, seed=40 + i)
+        st.fill()
+        sts.append(st)
+        qs.append(torch.randn(st.rows, 4, 128, generator=st.gen).to(F32 if cache == F32 else BF16).to(DEV))
+        want.append(st.cache.attention(st.batch, qs[-1], 0.1))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for r in range(50):
+                got = sts[i].cache.attention(sts[i].batch, qs[i], 0.1)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    bad.append((i, r))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for st in sts:
+        st.cache.check()
+    assert not bad
