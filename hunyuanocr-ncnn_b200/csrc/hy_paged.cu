@@ -176,10 +176,10 @@ int paged_rows(bool write, const hy_paged_cache* cache, const hy_paged_batch* ba
     if (!rc && !write) rc = check_apart("v", rows, cache->num_kv_heads, cache->head_dim, vrs, vhs);
     if (rc) return rc;
     if (!write && k == v) return fail(HY_ERR_INVALID_ARGUMENT, "k and v must not overlap");
-    DeviceGuard guard(cache->device);
-    if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     for (const long long x : {krs, khs, vrs, vhs, static_cast<long long>(cache->head_stride), static_cast<long long>(cache->scale_head_stride)})
         if (x > INT_MAX) return fail(HY_ERR_CAPACITY, "row and head strides must be below 2^31");
+    DeviceGuard guard(cache->device);
+    if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     PagedRowArgs a{device_cache(cache), device_batch(batch, rows), k, v, static_cast<int>(krs), static_cast<int>(khs),
                    static_cast<int>(vrs), static_cast<int>(vhs), static_cast<int>(cache->head_stride),
                    static_cast<int>(cache->scale_head_stride), 1, 0};

@@ -2,6 +2,7 @@
 
 import ctypes
 import importlib
+import itertools
 import os
 import re
 
@@ -56,3 +57,12 @@ def test_one_output_for_keys_and_values_is_refused(paged):
     c, b = _cache(paged), _batch(paged)
     assert lib.hy_paged_kv_read(ctypes.byref(c), ctypes.byref(b), 2, 1, FAKE, 512, 128, FAKE, 512, 128, None) == 1
     assert b"overlap" in lib.hy_last_error()
+
+
+@pytest.mark.parametrize("rows_stride,cache_stride", [((1 << 31, 128), 2048), ((512, 1 << 31), 2048), ((512, 128), 1 << 31)])
+def test_long_strides_are_refused_before_any_device_call(paged, rows_stride, cache_stride):
+    lib = paged._library()
+    calls = _calls(paged, _cache(paged, head_stride=cache_stride), _batch(paged), strides=rows_stride)
+    for rc in itertools.islice(calls, 2):
+        assert rc == 4
+        assert b"2^31" in lib.hy_last_error()
