@@ -306,10 +306,10 @@ __device__ __forceinline__ void store_row(void* base, long long off, const float
 // rows' 2 x kv_heads vectors (k, then v) are shared out to groups of lanes that
 // hold two pieces of 16 bytes of the row tensor each, so that all loads are wide, several
 // are in flight per lane and the index arithmetic serves 32 bytes (with one piece both calls
-// on the 38.6k rows below took 113 us, with two 97). The maximum of a vector is taken in registers and its codes
+// on the 38.6k rows below took 113 us, with two 99). The maximum of a vector is taken in registers and its codes
 // leave in the same pass. Each byte moves once: reading 264k rows of 8 heads of 128 (INT8
-// to bf16) takes 289 us, 6.1 TB/s; writing 38.6k such rows (bf16 to E4M3) 60 us, reading them
-// back 43 us; the write is bound by its instructions (68% of the issue slots, integer units 64%
+// to bf16) takes 290 us, 6.0 TB/s; writing 38.6k such rows (bf16 to E4M3) 62 us, reading them
+// back 42 us; the write is bound by its instructions (69% of the issue slots, integer units 63%
 // busy) rather than by its 237 MB.
 // ---------------------------------------------------------------------------
 constexpr int kRowWarps = 4;

@@ -204,7 +204,8 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x)
 // (a key is used by the group's heads only), so all that matters is that loads
 // never pause: every warp owns a quarter of a tile's keys and a cp.async ring of its
 // own, and the warps meet only at the end of an item. 64 tokens over 1024-8192 E4M3
-// keys each (613 MB): 109 us, 5.6 TB/s; one token over 2048 fp32 keys: 11 us, of which the
+// keys each (613 MB): 109 us, 5.6 TB/s, in a run of a few calls, 117 us, 5.2 TB/s, back to back (the power
+// limit holds the SM clock at 1.78 GHz); one token over 2048 fp32 keys: 11 us, of which the
 // keys take 2.5 and the look-ups and joins around them the rest.
 //
 // A CTA's first and last items may be shared with its neighbours: those leave
@@ -295,7 +296,10 @@ struct SplitShape {
 // agrees, so 8-bit and fp32 keys are read from shared memory in 16-byte pieces.
 //
 // Decode steps are bound by memory; with 32 columns of fp32 queries the 192 products a
-// warp's 16 keys take bound it (8 cycles each): 4 verify blocks of 16 rows at 2048 keys 26.5 us.
+// warp's 16 keys take bound it (8 cycles each): 4 verify blocks of 16 rows at 2048 keys 26.5 us. Chunks of fp32
+// rows, and of any rows over fp32 pages, stay here too, every 32 columns reading the keys anew: 4 x ~1012 rows over
+// 6000-8192 keys take 2.0 ms (fp32 rows, BF16 pages), 1.8 (fp32, E4M3), 3.5 (bf16, F32) and 5.2 (fp32, F32).
+// (fp32 rows over fp32 pages of 128 dimensions, 32 columns: 216 bytes of spills a thread.)
 // ---------------------------------------------------------------------------
 template <typename QT_, typename CT_, int D_, int NT>
 struct MmaEngine {

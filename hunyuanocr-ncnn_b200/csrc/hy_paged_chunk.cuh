@@ -23,19 +23,22 @@
 //
 // Where pages hold a multiple of 16 rows, blocks are fetched by TMA, 16 rows of a
 // page at a time (the window's start is rounded down to 16, masks do the rest);
-// for other page sizes the loading warps copy row by row.
+// for other page sizes the loading warps copy row by row, from the very first key.
 //
-// 4 sequences of ~1012 rows over 6000-8192 bf16 keys (213 GFLOP): 238 us, 893 TFLOP/s; the
-// tensor cores are busy 45% of the time and the special-function units 46%: a tile's softmax
+// 4 sequences of ~1012 rows over 6000-8192 bf16 keys (213 GFLOP): 243 us, 873 TFLOP/s, in a run of a few
+// calls; 274 us, 777 TFLOP/s, back to back, where the power limit (990 W drawn) holds the SM clock at 1.74 GHz. The
+// tensor cores are busy 45% of the time and the special-function units 45%: a tile's softmax
 // and its products follow one another, and only two tiles fit tensor memory. Over 8-bit
-// keys the softmax threads' products with the scales bound it (406-418 us; 16 softmax warps or 8 loading
+// keys the softmax threads' products with the scales bound it (422 us; 16 softmax warps or 8 loading
 // warps instead of 8 and 4 changed nothing: the windowed INT8 chunks take 236 and 240 us with them, 230 without). Pages of 24 rows
-// instead of 32, copied by threads: 183 instead of 139 us (windowed chunks, bf16).
+// instead of 32, copied by threads: 181 instead of 144 us (windowed chunks, bf16).
+// ptxas spills 72 bytes a thread (BF16, 128 dimensions), 110 (BF16, 64), 118 and 130 (INT8 and E4M3, 128), 12 and 28
+// (64); it does not say in which role.
 //
 // Tensor memory (512 columns): scores of the two tiles (128 each; the
 // weights, 16 bits, in the upper 64 of them), outputs of the two tiles (128 each).
-// Every wait is bounded; a wait that gives up sets a status bit, and the CTA
-// runs on to free its tensor memory.
+// Every wait is bounded and ends alike in a whole warp; a wait that gives up sets a status bit, the warp
+// leaves its role, and the CTA runs on to free its tensor memory.
 #pragma once
 
 #include <cuda.h>

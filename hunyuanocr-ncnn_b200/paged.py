@@ -61,7 +61,7 @@ class PagedBatch:
     """The sequences of a call: q_start [n + 1] and kv_len [n] int32, block_table [n, width] int32 (rows may be
     strided), on the cache's device. Sequence s has the rows q_start[s] .. q_start[s + 1] - 1 of the row tensors,
     standing at the last positions of its kv_len[s]. max_rows: about the most rows of a sequence (attention is laid
-    out for it). The arrays may be changed in place between calls, and between replays of a captured call."""
+    out for it, all sequences alike: tokens beside long chunks are faster in a call of their own). The arrays may be changed in place between calls, and between replays of a captured call."""
 
     def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor, max_rows: int):
         for t, name in ((q_start, "q_start"), (kv_len, "kv_len"), (block_table, "block_table")):
@@ -170,7 +170,8 @@ class PagedKVCache:
                   sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of rows q [rows, q heads, head_dim] over the cache (hy_paged_attention): the row at position p
         sees the positions j <= p, with a window those with p - j < window or j < sinks; all of them where causal is
-        false. The workspace comes from torch's allocator, one for each call."""
+        false. Rows of `out` that belong to no sequence are left as they were; without `out` they hold anything. The
+        workspace comes from torch's allocator, one for each call."""
         dtype = self._rows(q, 0, "q")
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)

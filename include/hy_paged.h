@@ -75,7 +75,9 @@ typedef struct hy_paged_cache {
 typedef struct hy_paged_batch {
     int num_seqs;
     int max_rows;              /* about the most rows of a sequence: attention is laid out for
-                                  it (another number costs time, not correctness) */
+                                  it, all sequences alike (another number costs time, not
+                                  correctness; tokens beside long chunks are faster in a
+                                  call of their own) */
     int table_width;
     int64_t table_stride;
     const int* q_start_dev;    /* [num_seqs + 1] */
