@@ -296,10 +296,11 @@ struct SplitShape {
 // agrees, so 8-bit and fp32 keys are read from shared memory in 16-byte pieces.
 //
 // Decode steps are bound by memory; with 32 columns of fp32 queries the 192 products a
-// warp's 16 keys take bound it (8 cycles each): 4 verify blocks of 16 rows at 2048 keys 26.5 us. Chunks of fp32
+// warp's 16 keys take bound it (8 cycles each): 4 verify blocks of 16 rows at 2048 keys 26.8 us. Chunks of fp32
 // rows, and of any rows over fp32 pages, stay here too, every 32 columns reading the keys anew: 4 x ~1012 rows over
-// 6000-8192 keys take 2.0 ms (fp32 rows, BF16 pages), 1.8 (fp32, E4M3), 3.5 (bf16, F32) and 5.2 (fp32, F32).
-// (fp32 rows over fp32 pages of 128 dimensions, 32 columns: 216 bytes of spills a thread.)
+// 6000-8192 keys take 2.1 ms (fp32 rows, BF16 pages), 1.9 (fp32, E4M3), 3.5 (bf16, F32) and 5.6 (fp32, F32).
+// (Spills: 116 bytes a thread for fp32 rows over fp32 pages of 128 dimensions and 32 columns, 100 and fewer for fp32 rows over
+// 8-bit pages of 128 dimensions.)
 // ---------------------------------------------------------------------------
 template <typename QT_, typename CT_, int D_, int NT>
 struct MmaEngine {
@@ -704,7 +705,16 @@ struct MmaEngine {
                     pb[nt][1][j] = movmatrix(p1[j]);
                 }
             }
+            // The tensor cores cut sums, so that many of them one after another pull a sum toward zero: fp32 rows add up
+            // a step's products by themselves and the steps by rounded additions (error where a warp adds up 250 steps:
+            // 1.6e-5 -> 1.1e-6 over fp32 pages; verify blocks 26.0 -> 26.8 us, chunks over fp32 pages 5.2 -> 5.6 ms).
             auto pv = [&](int mt, const uint32_t (&va)[MG][NK][4]) {   // m tiles mt .. mt + MG - 1
+                float sum[NQ > 1 ? MG : 1][NQ > 1 ? NT : 1][4];
+                if constexpr (NQ > 1)
+#pragma unroll
+                    for (int x = 0; x < MG; ++x)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) sum[x][nt][0] = sum[x][nt][1] = sum[x][nt][2] = sum[x][nt][3] = 0.f;
 #pragma unroll
                 for (int j = NQ - 1; j >= 0; --j)
 #pragma unroll
@@ -713,7 +723,18 @@ struct MmaEngine {
                         for (int x = 0; x < MG; ++x)
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
-                                if (n + j <= 2) mma16816<F16>(acc[nt][mt + x], va[x][n], pb[nt][0][j], pb[nt][1][j]);
+                                if (n + j <= 2)
+                                {
+                                    if constexpr (NQ > 1) mma16816<F16>(sum[x][nt], va[x][n], pb[nt][0][j], pb[nt][1][j]);
+                                    else mma16816<F16>(acc[nt][mt + x], va[x][n], pb[nt][0][j], pb[nt][1][j]);
+                                }
+                if constexpr (NQ > 1)
+#pragma unroll
+                    for (int x = 0; x < MG; ++x)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[nt][mt + x][e] += sum[x][nt][e];
             };
             if constexpr (sizeof(CT) == 2)
             {

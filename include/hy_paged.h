@@ -114,8 +114,8 @@ int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, i
  * A row that sees nothing gives zeros. Positions that a row does not see do
  * not reach its output, whatever they hold (infinities and NaN included).
  * scale must be positive, and scale * log2(e) finite. q and out have the same
- * dtype and must not overlap. Products and softmax sums are in fp32; the tensor
- * cores cut sums instead of rounding them.
+ * dtype and must not overlap. Products and sums are in fp32 (BF16 rows: as the
+ * tensor cores add, which cut sums instead of rounding them).
  * F32 rows: products are exact to 2^-21. Over 8-bit caches q and the weights
  * (probabilities times v's scale) are off by 2^-22 of themselves, or by 2^-39 of
  * a row's largest where that is more.
