@@ -296,11 +296,11 @@ struct SplitShape {
 // agrees, so 8-bit and fp32 keys are read from shared memory in 16-byte pieces.
 //
 // Decode steps are bound by memory; with 32 columns of fp32 queries the 192 products a
-// warp's 16 keys take bound it (8 cycles each): 4 verify blocks of 16 rows at 2048 keys 26.8 us. Chunks of fp32
+// warp's 16 keys take bound it (8 cycles each): 4 verify blocks of 16 rows at 2048 keys 27.3 us. Chunks of fp32
 // rows, and of any rows over fp32 pages, stay here too, every 32 columns reading the keys anew: 4 x ~1012 rows over
-// 6000-8192 keys take 2.1 ms (fp32 rows, BF16 pages), 1.9 (fp32, E4M3), 3.5 (bf16, F32) and 5.6 (fp32, F32).
-// (Spills: 116 bytes a thread for fp32 rows over fp32 pages of 128 dimensions and 32 columns, 100 and fewer for fp32 rows over
-// 8-bit pages of 128 dimensions.)
+// 6000-8192 keys take 2.2 ms (fp32 rows, BF16 pages), 1.9 (fp32, E4M3), 3.5 (bf16, F32) and 5.8 (fp32, F32).
+// (Spills: 52 bytes a thread for fp32 rows over fp32 pages of 128 dimensions and 32 columns, 44 over BF16 pages, 48 to 100
+// over 8-bit pages.)
 // ---------------------------------------------------------------------------
 template <typename QT_, typename CT_, int D_, int NT>
 struct MmaEngine {
@@ -319,7 +319,10 @@ struct MmaEngine {
     static constexpr int Q_SMEM = KS * NT * NQ * 256;
     static constexpr int QI = KS * NT / kSplitWarps;                           // q fragments that a thread makes
     static constexpr bool QREG = KS * NT * 2 * NQ <= 32;                       // q stays in registers
-    static constexpr int NA = NT >= 4 ? 1 : NQ * NK == 1 ? 2 : NQ > NK ? NQ : NK;   // chains of products per score
+    // Chains of products per score. The tensor cores cut a sum at every product, so the products of the second and third
+    // terms, which hardly change it, have chains of their own (verify blocks over fp32 pages with loud dimensions: off by
+    // 7.3e-7 instead of 4.1e-6, over BF16 pages 6.7e-7 instead of 2.0e-6; 27.1 -> 27.3 us).
+    static constexpr int NA = NT >= 4 ? (NQ == 3 ? 2 : 1) : NQ * NK == 1 ? 2 : NQ > NK ? NQ : NK;
     static constexpr int MG = NT >= 4 ? 1 : 2;                                      // m tiles whose products alternate
     static constexpr float OUT = F16 ? 1.f / 16384.f : 1.f;                         // the sums' unit
 
@@ -524,7 +527,7 @@ struct MmaEngine {
 #pragma unroll
                         for (int n = NK - 1; n >= 0; --n)
                             if (n + j <= 2)
-                                mma16816<F16>(part[NA == 1 ? 0 : NQ * NK == 1 ? ks % NA : (n + j) % NA][nt], ka[n], b.x, b.y);
+                                mma16816<F16>(part[NQ * NK == 1 ? ks % NA : n + j < NA ? n + j : NA - 1][nt], ka[n], b.x, b.y);
                     }
             }
 #pragma unroll

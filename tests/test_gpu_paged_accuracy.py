@@ -108,3 +108,29 @@ def test_long_chains_of_additions(paged, cache):
         err += float((out[a:b].double() - want).square().sum())
         ref += float(want.square().sum())
     assert math.sqrt(err / ref) <= ordinary_bound(F32), math.sqrt(err / ref)
+
+
+@pytest.mark.parametrize("cache", TYPES)
+def test_scores_of_loud_dimensions(paged, cache):
+    """fp32 rows in tiles of 32 columns over keys with four dimensions eight times the others: scores of some 2 units,
+    up to 10. The tensor cores cut a sum at every product (by 2^-24 of it on average): through all 24 of a score over BF16
+    pages (48 over F32) the same arithmetic on the CPU is off by 1.8e-6 in the outputs, through the 8 that matter by
+    6e-7; the bound leaves a factor of 2 over that."""
+    seqs = [(1500, 16), (2600, 16), (1800, 16), (2111, 16)]
+    st = Setup(paged, cache, seqs, kv_heads=8, seed=47)
+    loud = torch.ones(128)
+    loud[[3, 40, 77, 126]] = 8.0
+    k, v = (torch.randn(sum(st.kv), 8, 128, generator=st.gen) * loud for _ in range(2))
+    starts = torch.tensor([0, 1500, 4100, 5900, 8011], dtype=torch.int32, device=DEV)
+    st.cache.write(paged.PagedBatch(starts, st.d_kv, st.d_table, 2600), k.to(DEV), v.to(DEV))
+    keys, values = (st.stand_for(x).split(st.kv) for x in (k, v))
+    q = torch.randn(st.rows, 16, 128, generator=st.gen).to(DEV)
+    out = st.cache.attention(st.batch, q, 0.0883883)
+    st.cache.check()
+    err = ref = 0.0
+    for s, (kv, n) in enumerate(seqs):
+        a, b = st.starts[s], st.starts[s + 1]
+        want, _, _ = R.attention(q[a:b].double(), keys[s], values[s], list(range(kv - n, kv)), 0.0883883)
+        err += float((out[a:b].double() - want).square().sum())
+        ref += float(want.square().sum())
+    assert math.sqrt(err / ref) <= 1.25 * 2.0 ** -20, math.sqrt(err / ref)
