@@ -53,7 +53,7 @@ EXPORTED_SYMBOLS = (
     "hy_ctx_set_wait_limit", "hy_debug_wait_probe", "hy_ctx_create_from_package", "hy_draft_load_package",
     "hy_package_inspect", "hy_package_read_tensor", "hy_debug_step_trace",
     "hy_paged_kv_write", "hy_paged_kv_read", "hy_paged_attention", "hy_paged_attention_workspace",
-    "hy_kv_device_rows",
+    "hy_kv_device_rows", "hy_norm_rotate", "hy_paged_kv_write_rotated", "hy_token_logprobs", "hy_lm_head_logprobs",
 )
 TOKEN_CALLBACK = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.c_void_p)
 DFLASH_MASK_TOKEN = 120817
@@ -148,6 +148,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "hy_decoder_step": ([_P, _P, _I, _P, _P, _P, _P], _I),
         "hy_lm_head_select": ([_P, _P, _I, _P, _F, _P, _P, _P], _I),
         "hy_lm_head_select_noalloc": ([_P, _P, _I, _F, _P, _P], _I),
+        "hy_lm_head_logprobs": ([_P, _P, _I, _P, _I, _P, _P, _P, _P], _I),
         "hy_generate": ([_P, _I, _I, _I, _F, _P, _I, _P, _P, ctypes.POINTER(_I)], _I),
         "hy_verify_block": ([_P, _P, _I, _F, _P, _I, _P, ctypes.POINTER(_I), ctypes.POINTER(_I),
                              ctypes.POINTER(_I)], _I),
@@ -517,6 +518,23 @@ class TextRuntime:
         _check(_LIB.hy_lm_head_select(self._ctx, _ptr(h), rows, _ptr(pre), penalty, _ptr(tok), _ptr(raw),
                                       _ptr(logits)))
         return tok, raw, logits
+
+    def lm_head_logprobs(self, hidden: np.ndarray, tokens=None, top: int = 0):
+        """Log probabilities behind the LM head (hy_lm_head_logprobs) for final-normed hidden rows [rows, 1024]:
+        (log probabilities of `tokens`, one a row, or None; entropies; ids and log probabilities of the `top` most
+        likely tokens [rows, top], or None). No repetition penalty."""
+        h = _f32(hidden).reshape(-1, HIDDEN)
+        rows = h.shape[0]
+        tok = None if tokens is None else _i32(tokens).reshape(-1)
+        if tok is not None and tok.size != rows:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "lm_head_logprobs takes a token for every hidden row")
+        lp = None if tok is None else np.empty(rows, np.float32)
+        entropy = np.empty(rows, np.float32)
+        ids = np.empty((rows, max(top, 0)), np.int32) if top else None
+        alt = np.empty((rows, max(top, 0)), np.float32) if top else None
+        _check(_LIB.hy_lm_head_logprobs(self._ctx, _ptr(h), rows, _ptr(tok), top, _ptr(lp), _ptr(entropy), _ptr(ids),
+                                        _ptr(alt)))
+        return lp, entropy, ids, alt
 
     def select_logit_rows_noalloc(self, hidden_dev: int, rows: int, penalty: float, tokens_dev: int,
                                   raw_top1_dev: int) -> None:

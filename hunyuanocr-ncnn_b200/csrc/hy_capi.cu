@@ -12,6 +12,7 @@
 
 #include "hy_decode.h"
 #include "hy_debug.h"
+#include "hy_logprobs.h"
 
 #include <cuda_runtime.h>
 
@@ -134,6 +135,7 @@ struct hy_ctx {
     int* feat_idx = nullptr;    // [max_prefill]
     float* feats = nullptr;     // vision features [max_prefill x 1024]
     float* logits = nullptr;    // [16 x V] (lazily)
+    float* logprobs = nullptr;  // hy_lm_head_logprobs' inputs and outputs (lazily)
     // Prompt prefill in passes of up to pf_rows rows (the residual stream is ctx->prompt).
     // GEMM operands are split (hi / lo) and tiled for the tensor core (hy_umma.cuh);
     // activation buffers hold pf_pad = pf_rows rounded up to 128 rows.
@@ -1269,6 +1271,7 @@ void free_ctx(hy_ctx* c)
     if (c->h_bstate) cudaFreeHost(c->h_bstate);
     for (void* p : c->allocs) cudaFree(p);
     if (c->logits) cudaFree(c->logits);
+    if (c->logprobs) cudaFree(c->logprobs);
     if (c->h_st) cudaFreeHost(c->h_st);
     if (c->h_stage) cudaFreeHost(c->h_stage);
     if (c->h_hist) cudaFreeHost(c->h_hist);
@@ -2837,6 +2840,44 @@ int hy_lm_head_select_noalloc(hy_ctx* c, const float* hidden_dev, int rows, floa
         e = rows == 1 ? enqueue_lm_select_scratch_t<float, 1>(c, rows, hidden_dev, penalty, scratch, tokens_dev, raw_top1_dev)
                       : enqueue_lm_select_scratch_t<float, 16>(c, rows, hidden_dev, penalty, scratch, tokens_dev, raw_top1_dev);
     if (e != cudaSuccess) return fail(HY_ERR_CUDA, std::string("LM head launch: ") + cudaGetErrorString(e));
+    return check_device_error(c);
+}
+
+int hy_lm_head_logprobs(hy_ctx* c, const float* hidden, int rows, const int* tokens, int top, float* logprobs,
+                        float* entropy, int* top_ids, float* top_logprobs)
+{
+    if (!c || !hidden) return fail(HY_ERR_INVALID_ARGUMENT, "null argument");
+    if (rows < 1 || rows > kMaxStepRows) return fail(HY_ERR_INVALID_ARGUMENT, "rows must be in 1..16");
+    if ((tokens == nullptr) != (logprobs == nullptr)) return fail(HY_ERR_INVALID_ARGUMENT, "tokens and logprobs belong together");
+    if (top < 0 || top > HY_LOGPROBS_MAX_TOP || top > c->cfg.vocab_size)
+        return fail(HY_ERR_INVALID_ARGUMENT, "top must be in 0..64 and at most vocab");
+    if (top > 0 && (!top_ids || !top_logprobs)) return fail(HY_ERR_INVALID_ARGUMENT, "null argument");
+    int rc = set_device(c);
+    if (rc) return rc;
+    // Beside the logits: [16] tokens, log probabilities and entropies, [16 x 64] ids and their log probabilities.
+    constexpr int kTop = kMaxStepRows * HY_LOGPROBS_MAX_TOP;
+    if (!c->logits) HY_CUDA(cudaMalloc(reinterpret_cast<void**>(&c->logits), sizeof(float) * kMaxStepRows * c->cfg.vocab_size));
+    if (!c->logprobs) HY_CUDA(cudaMalloc(reinterpret_cast<void**>(&c->logprobs), sizeof(float) * (3 * kMaxStepRows + 2 * kTop)));
+    int* const d_tokens = reinterpret_cast<int*>(c->logprobs);
+    float* const d_lp = c->logprobs + kMaxStepRows;
+    float* const d_entropy = d_lp + kMaxStepRows;
+    int* const d_ids = reinterpret_cast<int*>(d_entropy + kMaxStepRows);
+    float* const d_top = reinterpret_cast<float*>(d_ids + kTop);
+    HY_CUDA(cudaMemcpyAsync(c->hidden, hidden, sizeof(float) * rows * kHidden, cudaMemcpyHostToDevice, c->stream));
+    if (tokens) HY_CUDA(cudaMemcpyAsync(d_tokens, tokens, sizeof(int) * rows, cudaMemcpyHostToDevice, c->stream));
+    t_next_plain = true;
+    const cudaError_t e = enqueue_lm_select(c, rows, c->hidden, 1.f, false, c->logits);
+    if (e != cudaSuccess) return fail(HY_ERR_CUDA, std::string("LM head launch: ") + cudaGetErrorString(e));
+    rc = hy_token_logprobs(c->logits, rows, c->cfg.vocab_size, c->cfg.vocab_size, HY_DTYPE_F32, c->cfg.device, d_tokens,
+                           tokens ? 1 : 0, top, d_lp, d_entropy, d_ids, d_top, c->stream);
+    if (rc) return rc;
+    if (logprobs) HY_CUDA(cudaMemcpyAsync(logprobs, d_lp, sizeof(float) * rows, cudaMemcpyDeviceToHost, c->stream));
+    if (entropy) HY_CUDA(cudaMemcpyAsync(entropy, d_entropy, sizeof(float) * rows, cudaMemcpyDeviceToHost, c->stream));
+    if (top > 0)
+    {
+        HY_CUDA(cudaMemcpyAsync(top_ids, d_ids, sizeof(int) * rows * top, cudaMemcpyDeviceToHost, c->stream));
+        HY_CUDA(cudaMemcpyAsync(top_logprobs, d_top, sizeof(float) * rows * top, cudaMemcpyDeviceToHost, c->stream));
+    }
     return check_device_error(c);
 }
 

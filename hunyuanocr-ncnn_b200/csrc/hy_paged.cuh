@@ -21,6 +21,7 @@ constexpr int kPagedBadPage = 1;
 constexpr int kPagedBadLength = 2;
 constexpr int kPagedBadRows = 4;
 constexpr int kPagedTimeout = 8;
+constexpr int kPagedBadPosition = 16;
 
 struct PagedCache {
     void* k;
@@ -327,8 +328,9 @@ struct PagedRowArgs {
 };
 
 // Where a CTA's rows belong: offsets of the page and the row in it, for the elements and for the scales.
+constexpr long long kPlaceLost = -2;
 struct PagedPlace {
-    long long off, s_off;   // off < 0: nowhere
+    long long off, s_off;   // off < 0: nowhere (kPlaceLost: a row of a sequence, but its page is not one)
 };
 // The place of row r (r < 0: none), by a whole warp, a consecutive row for each of its lanes.
 __device__ __forceinline__ void paged_find_place(const PagedCache& c, const PagedBatch& b, int r, int lane, PagedPlace& o)
@@ -354,6 +356,7 @@ __device__ __forceinline__ void paged_find_place(const PagedCache& c, const Page
     if (pg < 0 || pg >= c.num_pages)
     {
         paged_status(c.status, kPagedBadPage);
+        o.off = kPlaceLost;
         return;
     }
     o.off = pg * c.page_stride + in * c.row_stride;

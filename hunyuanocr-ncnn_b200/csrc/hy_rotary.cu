@@ -1,0 +1,168 @@
+// C ABI of the norms with rotation (include/hy_rotary.h, hy_paged_kv_write_rotated
+// of include/hy_paged.h): checks of arguments, launches.
+#include <algorithm>
+#include <cmath>
+
+#include "hy_call.cuh"
+#include "hy_paged_launch.cuh"
+#include "hy_rotary.cuh"
+
+using namespace hy;
+
+namespace {
+
+int check_rotation(const hy_rotation* t)
+{
+    if (!t) return fail(HY_ERR_INVALID_ARGUMENT, "rotation is null");
+    if (!t->q_weight_dev || !t->k_weight_dev || !t->cos_dev || !t->sin_dev)
+        return fail(HY_ERR_INVALID_ARGUMENT, "norm weights or angles are null");
+    if (!aligned16(t->q_weight_dev) || !aligned16(t->k_weight_dev) || !aligned16(t->cos_dev) || !aligned16(t->sin_dev) ||
+        off16(t->table_stride, 4, t->table_rows))
+        return fail(HY_ERR_INVALID_ARGUMENT, "norm weights and rows of angles must start on 16 bytes");
+    if (t->table_rows < 0 || t->table_stride < 0)
+        return fail(HY_ERR_INVALID_ARGUMENT, "table_rows and table_stride must not be negative");
+    if (!(t->eps >= 0.f) || !std::isfinite(t->eps)) return fail(HY_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+    return HY_OK;
+}
+
+// An output is the input itself or lies elsewhere.
+int check_output(const char* name, const void* out, long long row, long long head, const void* in, long long in_row,
+                 long long in_head, int rows, int heads)
+{
+    if (out != in || ((rows < 2 || row == in_row) && (heads < 2 || head == in_head))) return HY_OK;
+    char msg[96];
+    snprintf(msg, sizeof msg, "%s in place of its input needs the input's strides", name);
+    return fail(HY_ERR_INVALID_ARGUMENT, msg);
+}
+
+int check_heads(int rows, int q_heads, int kv_heads)
+{
+    if (q_heads < 1 || kv_heads < 1) return fail(HY_ERR_INVALID_ARGUMENT, "q_heads and kv_heads must be positive");
+    if (q_heads > 1024 || kv_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "q_heads and kv_heads must be at most 1024");
+    if (static_cast<long long>(rows) * std::max(q_heads, kv_heads) > INT_MAX)
+        return fail(HY_ERR_CAPACITY, "rows * heads must be below 2^31");
+    return HY_OK;
+}
+
+RotateArgs rotate_args(const hy_rotation* t, int rows, int q_heads, int kv_heads, int head_dim)
+{
+    RotateArgs a{};
+    a.q_weight = t->q_weight_dev;
+    a.k_weight = t->k_weight_dev;
+    a.cos = t->cos_dev;
+    a.sin = t->sin_dev;
+    a.positions = t->positions_dev;
+    a.table_stride = t->table_stride;
+    a.table_rows = t->table_rows;
+    a.eps = t->eps;
+    a.inv_dim = 1.f / static_cast<float>(head_dim);
+    a.rotate_first = t->rotate_first != 0;
+    a.rows = rows;
+    a.q_heads = q_heads;
+    a.kv_heads = kv_heads;
+    return a;
+}
+
+template <typename RT, typename CT, int D, bool CACHE>
+cudaError_t launch_rotate(RotateArgs a, cudaStream_t s)
+{
+    constexpr int VPW = 32 / (D / (2 * (16 / static_cast<int>(sizeof(RT)))));
+    const int heads = a.q_heads + (CACHE ? 2 : 1) * a.kv_heads;
+    a.whole = a.rows >= 4 * 148;
+    int parts = 1;
+    if (a.whole)
+        a.per_cta = std::min(kRowsPerCta, std::max(4, a.rows / (8 * 148) / 4 * 4));
+    else
+    {
+        a.per_cta = 1;
+        parts = std::min((heads + kRowWarps * VPW - 1) / (kRowWarps * VPW), std::max(1, 4 * 148 / a.rows));
+    }
+    return launch_pdl(rotate_kernel<RT, CT, D, CACHE>, dim3((a.rows + a.per_cta - 1) / a.per_cta, parts), kRowWarps * 32, 0, s, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int hy_norm_rotate(const hy_rotation* rotation, int rows, int q_heads, int kv_heads, int head_dim, int dtype,
+                   int device, const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, const void* k_dev,
+                   int64_t k_row_stride, int64_t k_head_stride, void* q_out_dev, int64_t q_out_row_stride,
+                   int64_t q_out_head_stride, void* k_out_dev, int64_t k_out_row_stride, int64_t k_out_head_stride,
+                   int* status_dev, void* stream)
+{
+    int rc = check_rotation(rotation);
+    if (!rc) rc = check_dtype(rows, dtype);
+    if (rc) return rc;
+    if (head_dim != 64 && head_dim != 128) return fail(HY_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (device < 0) return fail(HY_ERR_INVALID_ARGUMENT, "device must not be negative");
+    rc = check_heads(rows, q_heads, kv_heads);
+    if (rc || rows == 0) return rc;
+    rc = check_rows("q", q_dev, rows, q_heads, q_row_stride, q_head_stride, dtype);
+    if (!rc) rc = check_rows("k", k_dev, rows, kv_heads, k_row_stride, k_head_stride, dtype);
+    if (!rc) rc = check_rows("q_out", q_out_dev, rows, q_heads, q_out_row_stride, q_out_head_stride, dtype);
+    if (!rc) rc = check_rows("k_out", k_out_dev, rows, kv_heads, k_out_row_stride, k_out_head_stride, dtype);
+    if (!rc) rc = check_apart("q_out", rows, q_heads, head_dim, q_out_row_stride, q_out_head_stride);
+    if (!rc) rc = check_apart("k_out", rows, kv_heads, head_dim, k_out_row_stride, k_out_head_stride);
+    if (!rc) rc = check_output("q_out", q_out_dev, q_out_row_stride, q_out_head_stride, q_dev, q_row_stride, q_head_stride, rows, q_heads);
+    if (!rc) rc = check_output("k_out", k_out_dev, k_out_row_stride, k_out_head_stride, k_dev, k_row_stride, k_head_stride, rows, kv_heads);
+    if (rc) return rc;
+    if (q_out_dev == k_out_dev || q_out_dev == k_dev || k_out_dev == q_dev)
+        return fail(HY_ERR_INVALID_ARGUMENT, "q_out and k_out must not overlap, nor each the other's input");
+    DeviceGuard guard(device);
+    if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
+    RotateArgs a = rotate_args(rotation, rows, q_heads, kv_heads, head_dim);
+    a.q = q_dev; a.q_row = q_row_stride; a.q_head = q_head_stride;
+    a.k = k_dev; a.k_row = k_row_stride; a.k_head = k_head_stride;
+    a.q_out = q_out_dev; a.qo_row = q_out_row_stride; a.qo_head = q_out_head_stride;
+    a.k_out = k_out_dev; a.ko_row = k_out_row_stride; a.ko_head = k_out_head_stride;
+    a.status = status_dev;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e =
+        dtype == HY_DTYPE_F32
+            ? (head_dim == 64 ? launch_rotate<float, float, 64, false>(a, s) : launch_rotate<float, float, 128, false>(a, s))
+            : (head_dim == 64 ? launch_rotate<__nv_bfloat16, __nv_bfloat16, 64, false>(a, s)
+                              : launch_rotate<__nv_bfloat16, __nv_bfloat16, 128, false>(a, s));
+    return e == cudaSuccess ? HY_OK : cuda_fail("norm and rotation", e);
+}
+
+int hy_paged_kv_write_rotated(const hy_paged_cache* cache, const hy_paged_batch* batch, const hy_rotation* rotation,
+                              int rows, int q_heads, int dtype, const void* q_dev, int64_t q_row_stride,
+                              int64_t q_head_stride, const void* k_dev, int64_t k_row_stride, int64_t k_head_stride,
+                              const void* v_dev, int64_t v_row_stride, int64_t v_head_stride, void* q_out_dev,
+                              int64_t q_out_row_stride, int64_t q_out_head_stride, void* stream)
+{
+    int rc = check_cache(cache);
+    if (!rc) rc = check_batch(batch, cache);
+    if (!rc) rc = check_rotation(rotation);
+    if (!rc) rc = check_dtype(rows, dtype);
+    if (!rc) rc = check_heads(rows, q_heads, cache->num_kv_heads);
+    if (rc) return rc;
+    if (rows == 0 || batch->num_seqs == 0) return HY_OK;
+    const int kv_heads = cache->num_kv_heads;
+    rc = check_rows("q", q_dev, rows, q_heads, q_row_stride, q_head_stride, dtype);
+    if (!rc) rc = check_rows("k", k_dev, rows, kv_heads, k_row_stride, k_head_stride, dtype);
+    if (!rc) rc = check_rows("v", v_dev, rows, kv_heads, v_row_stride, v_head_stride, dtype);
+    if (!rc) rc = check_rows("q_out", q_out_dev, rows, q_heads, q_out_row_stride, q_out_head_stride, dtype);
+    if (!rc) rc = check_apart("q_out", rows, q_heads, cache->head_dim, q_out_row_stride, q_out_head_stride);
+    if (!rc) rc = check_output("q_out", q_out_dev, q_out_row_stride, q_out_head_stride, q_dev, q_row_stride, q_head_stride, rows, q_heads);
+    if (rc) return rc;
+    if (q_out_dev == k_dev || q_out_dev == v_dev)
+        return fail(HY_ERR_INVALID_ARGUMENT, "q_out must not overlap k or v");
+    DeviceGuard guard(cache->device);
+    if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
+    RotateArgs a = rotate_args(rotation, rows, q_heads, kv_heads, cache->head_dim);
+    a.q = q_dev; a.q_row = q_row_stride; a.q_head = q_head_stride;
+    a.k = k_dev; a.k_row = k_row_stride; a.k_head = k_head_stride;
+    a.v = v_dev; a.v_row = v_row_stride; a.v_head = v_head_stride;
+    a.q_out = q_out_dev; a.qo_row = q_out_row_stride; a.qo_head = q_out_head_stride;
+    a.status = cache->status_dev;
+    a.c = device_cache(cache);
+    a.b = device_batch(batch, rows);
+    const cudaError_t e = with_row_type(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
+        return launch_rotate<typename decltype(rt)::type, typename decltype(ct)::type, decltype(d)::value, true>(
+            a, static_cast<cudaStream_t>(stream));
+    });
+    return e == cudaSuccess ? HY_OK : cuda_fail("rotated paged write", e);
+}
+
+}  // extern "C"

@@ -14,13 +14,15 @@ import ctypes
 import torch
 
 from . import HY_ERR_INVALID_ARGUMENT, HyError, _check, load_library
+from .rotary import Rotation, _Rotation
 
 DTYPE_F32, DTYPE_BF16, DTYPE_E4M3, DTYPE_INT8 = range(4)
 _CACHE_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float8_e4m3fn: DTYPE_E4M3,
                  torch.int8: DTYPE_INT8}
 _ROW_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 _STATUS = {1: "a page number lies outside the cache", 2: "a kv_len does not fit its row of the block table",
-           4: "q_start is not ascending or leaves the rows", 8: "a bounded wait inside a kernel gave up"}
+           4: "q_start is not ascending or leaves the rows", 8: "a bounded wait inside a kernel gave up",
+           16: "a row's angles lie outside their table"}
 
 _I, _L, _P = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _INT_MAX = 2 ** 31 - 1
@@ -48,6 +50,9 @@ def _library():
                                            _L, _L, ctypes.c_float, _I, _I, _I, _P, ctypes.c_size_t, _P]
         lib.hy_paged_attention_workspace.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I,
                                                      ctypes.POINTER(ctypes.c_size_t)]
+        lib.hy_paged_kv_write_rotated.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch),
+                                                  ctypes.POINTER(_Rotation), _I, _I, _I, _P, _L, _L, _P, _L, _L, _P,
+                                                  _L, _L, _P, _L, _L, _P]
         lib.hy_paged_kv_write.argtypes = rows
     return lib
 
@@ -150,6 +155,36 @@ class PagedKVCache:
     def write(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Writes rows k, v [rows, kv heads, head_dim] at their positions (hy_paged_kv_write)."""
         self._call(self._lib.hy_paged_kv_write, batch, k, v, self._pair(k, v))
+
+    def write_rotated(self, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                      positions: torch.Tensor | None = None, *, eps: float = 1e-5, rotate_first: bool = True,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+        """`write` with the norms and the rotation of rotary.norm_rotate on the way (hy_paged_kv_write_rotated): k is
+        normed, rotated and written, v written as it is, and the normed and rotated q [rows, q heads, head_dim] comes
+        back (in `out`, which may be q itself). A row takes the angles of its `positions` (int32 [rows]), which are the
+        caller's: after an eviction they are not its place in the cache."""
+        dtype = self._pair(k, v)
+        if self._rows(q, 0, "q") != dtype or q.shape[0] != k.shape[0]:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "q must have the rows and type of k")
+        if out is None:
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+        elif self._rows(out, q.shape[1], "out") != dtype or out.shape != q.shape:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "q and out must have one shape and type")
+        if batch.index != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
+        turn = Rotation(q.shape[0], self._dim, self._index, q_weight, k_weight, cos, sin, positions, eps, rotate_first)
+        rows, heads, _ = q.shape
+        q0, q1, _ = q.stride()
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        o0, o1, _ = out.stride()
+        rc = self._lib.hy_paged_kv_write_rotated(self._ref, batch._ref, turn.ref, rows, heads, dtype, q.data_ptr(), q0,
+                                                 q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, out.data_ptr(), o0,
+                                                 o1, _raw_stream(self._index))
+        if rc:
+            _check(rc)
+        return out
 
     def read(self, batch: PagedBatch, rows: int, dtype: torch.dtype = torch.float32,
              out: tuple[torch.Tensor, torch.Tensor] | None = None):

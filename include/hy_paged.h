@@ -23,6 +23,7 @@
 #define HY_PAGED_H
 
 #include "hy_decode.h"
+#include "hy_rotary.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -40,7 +41,8 @@ enum hy_paged_status {
                                 in what is read back, and are not seen by attention */
     HY_PAGED_BAD_LENGTH = 2, /* kv_len negative or beyond table_width * page_size: the sequence is left out */
     HY_PAGED_BAD_ROWS = 4,   /* q_start not ascending or outside the rows: the sequence is left out */
-    HY_PAGED_TIMEOUT = 8     /* a bounded wait inside a kernel gave up */
+    HY_PAGED_TIMEOUT = 8,    /* a bounded wait inside a kernel gave up */
+    HY_PAGED_BAD_POSITION = 16 /* a row's angles lie outside their table: it comes out as NaN */
 };
 
 /* Element d of (page, head, row) is at page * page_stride + head * head_stride
@@ -104,6 +106,18 @@ int hy_paged_kv_write(const hy_paged_cache* cache, const hy_paged_batch* batch, 
 int hy_paged_kv_read(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int dtype, void* k_dev,
                      int64_t k_row_stride, int64_t k_head_stride, void* v_dev, int64_t v_row_stride,
                      int64_t v_head_stride, void* stream);
+
+/* hy_paged_kv_write with the norms and the rotation of hy_rotary.h on the way: k
+ * is normed and rotated in fp32 and written at its positions (rounded or quantised
+ * once, straight from fp32), v is written as it is, and q_out gets the normed and
+ * rotated q [rows x q_heads] of the same dtype (q_out may be q itself, with the
+ * same strides; otherwise it shares no memory with the inputs). Rows of q_out
+ * that are padding or outside every sequence are left as they were. */
+int hy_paged_kv_write_rotated(const hy_paged_cache* cache, const hy_paged_batch* batch, const hy_rotation* rotation,
+                              int rows, int q_heads, int dtype, const void* q_dev, int64_t q_row_stride,
+                              int64_t q_head_stride, const void* k_dev, int64_t k_row_stride, int64_t k_head_stride,
+                              const void* v_dev, int64_t v_row_stride, int64_t v_head_stride, void* q_out_dev,
+                              int64_t q_out_row_stride, int64_t q_out_head_stride, void* stream);
 
 /* Attention of the batch's rows over the cache, which holds the rows' own keys
  * and values already: out = softmax(scale * q k^T) v over the visible
