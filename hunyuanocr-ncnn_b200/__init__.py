@@ -54,6 +54,7 @@ EXPORTED_SYMBOLS = (
     "hy_package_inspect", "hy_package_read_tensor", "hy_debug_step_trace",
     "hy_paged_kv_write", "hy_paged_kv_read", "hy_paged_attention", "hy_paged_attention_workspace",
     "hy_kv_device_rows", "hy_norm_rotate", "hy_paged_kv_write_rotated", "hy_token_logprobs", "hy_lm_head_logprobs",
+    "hy_paged_attention_lse", "hy_paged_add_weights", "hy_paged_evict",
 )
 TOKEN_CALLBACK = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.c_void_p)
 DFLASH_MASK_TOKEN = 120817

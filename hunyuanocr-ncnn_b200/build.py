@@ -20,8 +20,8 @@ REPO = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libhy_decode.so")
 RECORD = os.path.join(HERE, "libhy_decode.build.json")   # what the last in-tree build compiled, and how
 SOURCES = [os.path.join(HERE, "csrc", f) for f in (
-    "hy_capi.cu", "hy_paged.cu", "hy_paged_attn_f32.cu", "hy_paged_attn_bf16.cu", "hy_rotary.cu", "hy_logprobs.cu",
-    "hy_package.cpp")]
+    "hy_capi.cu", "hy_paged.cu", "hy_paged_attn_f32.cu", "hy_paged_attn_bf16.cu", "hy_paged_weigh.cu", "hy_rotary.cu",
+    "hy_logprobs.cu",     "hy_package.cpp")]
 DEPS = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))] + [
     os.path.join(REPO, "include", f) for f in ("hy_decode.h", "hy_paged.h", "hy_rotary.h", "hy_logprobs.h")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

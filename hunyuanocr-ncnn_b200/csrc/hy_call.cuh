@@ -160,4 +160,49 @@ inline PagedBatch device_batch(const hy_paged_batch* b, int rows)
     return {b->q_start_dev, b->kv_len_dev, b->block_table_dev, b->table_stride, b->table_width, b->num_seqs, rows};
 }
 
+inline int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype)
+{
+    int rc = check_cache(cache);
+    if (!rc) rc = check_batch(batch, cache);
+    if (!rc) rc = check_dtype(rows, dtype);
+    if (rc) return rc;
+    if (q_heads < 1 || q_heads % cache->num_kv_heads)
+        return fail(HY_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of num_kv_heads");
+    if (q_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "q_heads must be at most 1024");
+    if (static_cast<long long>(rows) * q_heads > INT_MAX)
+        return fail(HY_ERR_CAPACITY, "rows * q_heads must be below 2^31");
+    return HY_OK;
+}
+
+// Scale, window and sinks of a call.
+inline int check_view(float scale, int causal, int window, int sinks)
+{
+    if (window < 0 || sinks < 0) return fail(HY_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
+    if (!causal && window > 0) return fail(HY_ERR_UNSUPPORTED, "a window needs causal attention");
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!(scale > 0.f) || scale_log2 - scale_log2 != 0.f)
+        return fail(HY_ERR_INVALID_ARGUMENT, "scale must be positive, and finite times log2(e) too");
+    return HY_OK;
+}
+
+// The lse of a call's rows.
+inline int check_lse(const float* lse, int rows, int q_heads, long long row_stride, long long head_stride)
+{
+    if (row_stride < 0 || head_stride < 0) return fail(HY_ERR_INVALID_ARGUMENT, "lse strides must not be negative");
+    if (reinterpret_cast<uintptr_t>(lse) % 4 != 0) return fail(HY_ERR_INVALID_ARGUMENT, "lse must be aligned to 4 bytes");
+    return check_apart("lse", rows, q_heads, 1, row_stride, head_stride);
+}
+
+// Weights of the cache's positions. (A dimension with one entry is not stepped over.)
+inline int check_weights(const hy_paged_weights* w, const hy_paged_cache* c)
+{
+    if (!w || !w->weights_dev) return fail(HY_ERR_INVALID_ARGUMENT, "weights are null");
+    if (reinterpret_cast<uintptr_t>(w->weights_dev) % 4 != 0) return fail(HY_ERR_INVALID_ARGUMENT, "weights must be aligned to 4 bytes");
+    if (w->page_stride < 0 || w->head_stride < 0 || w->row_stride < 0)
+        return fail(HY_ERR_INVALID_ARGUMENT, "weight strides must not be negative");
+    if ((c->num_pages > 1 && w->page_stride == 0) || (c->num_kv_heads > 1 && w->head_stride == 0) || (c->page_size > 1 && w->row_stride == 0))
+        return fail(HY_ERR_INVALID_ARGUMENT, "weights must not overlap");
+    return HY_OK;
+}
+
 }  // namespace hy

@@ -61,20 +61,6 @@ int tile_columns(int max_rows, int group, int dtype, int cache_dtype)
     return cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
 }
 
-int check_attention(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype)
-{
-    int rc = check_cache(cache);
-    if (!rc) rc = check_batch(batch, cache);
-    if (!rc) rc = check_dtype(rows, dtype);
-    if (rc) return rc;
-    if (q_heads < 1 || q_heads % cache->num_kv_heads)
-        return fail(HY_ERR_INVALID_ARGUMENT, "q_heads must be a positive multiple of num_kv_heads");
-    if (q_heads > 1024) return fail(HY_ERR_UNSUPPORTED, "q_heads must be at most 1024");
-    if (static_cast<long long>(rows) * q_heads > INT_MAX)
-        return fail(HY_ERR_CAPACITY, "rows * q_heads must be below 2^31");
-    return HY_OK;
-}
-
 // Descriptions and two parts for every CTA.
 size_t attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int q_heads, int dtype)
 {
@@ -117,19 +103,33 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
                        int64_t out_row_stride, int64_t out_head_stride, float scale, int causal, int window, int sinks,
                        void* workspace_dev, size_t workspace_bytes, void* stream)
 {
+    return hy_paged_attention_lse(cache, batch, rows, q_heads, dtype, q_dev, q_row_stride, q_head_stride, out_dev,
+                                  out_row_stride, out_head_stride, nullptr, 0, 0, scale, causal, window, sinks,
+                                  workspace_dev, workspace_bytes, stream);
+}
+
+int hy_paged_attention_lse(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
+                           const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, void* out_dev,
+                           int64_t out_row_stride, int64_t out_head_stride, float* lse_dev, int64_t lse_row_stride,
+                           int64_t lse_head_stride, float scale, int causal, int window, int sinks,
+                           void* workspace_dev, size_t workspace_bytes, void* stream)
+{
     int rc = check_attention(cache, batch, rows, q_heads, dtype);
     if (rc) return rc;
-    if (window < 0 || sinks < 0) return fail(HY_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
-    if (!causal && window > 0) return fail(HY_ERR_UNSUPPORTED, "a window needs causal attention");
-    const float scale_log2 = scale * 1.4426950408889634f;
-    if (!(scale > 0.f) || scale_log2 - scale_log2 != 0.f)
-        return fail(HY_ERR_INVALID_ARGUMENT, "scale must be positive, and finite times log2(e) too");
+    rc = check_view(scale, causal, window, sinks);
+    if (rc) return rc;
     if (rows == 0 || batch->num_seqs == 0) return HY_OK;
     rc = check_rows("q", q_dev, rows, q_heads, q_row_stride, q_head_stride, dtype);
     if (!rc) rc = check_rows("out", out_dev, rows, q_heads, out_row_stride, out_head_stride, dtype);
     if (!rc) rc = check_apart("out", rows, q_heads, cache->head_dim, out_row_stride, out_head_stride);
     if (rc) return rc;
     if (q_dev == out_dev) return fail(HY_ERR_INVALID_ARGUMENT, "q and out must not overlap");
+    if (lse_dev)
+    {
+        rc = check_lse(lse_dev, rows, q_heads, lse_row_stride, lse_head_stride);
+        if (rc) return rc;
+        if (lse_dev == out_dev || lse_dev == q_dev) return fail(HY_ERR_INVALID_ARGUMENT, "lse must not overlap q or out");
+    }
     if (!workspace_dev || !aligned16(workspace_dev))
         return fail(HY_ERR_INVALID_ARGUMENT, "the workspace is null or not on 16 bytes");
     if (workspace_bytes < attention_workspace(cache, batch, q_heads, dtype))
@@ -142,7 +142,8 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
     sinks = std::min(sinks, 1 << 30);
     const PagedAttnArgs a{device_cache(cache), device_batch(batch, rows), q_dev, out_dev, q_row_stride, q_head_stride,
                           out_row_stride, out_head_stride, q_heads, group, causal != 0, window, window > 0 ? sinks : 0,
-                          power_of_two(cache->page_size), power_of_two(group), scale_log2, workspace_dev};
+                          power_of_two(cache->page_size), power_of_two(group), scale * 1.4426950408889634f, workspace_dev,
+                          lse_dev, lse_row_stride, lse_head_stride};
     const int cols = tile_columns(batch->max_rows, group, dtype, cache->dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto launch = dtype == HY_DTYPE_F32 ? hy_internal::paged_attention_f32 : hy_internal::paged_attention_bf16;

@@ -26,10 +26,20 @@ struct PagedAttnArgs {
     int page_shift, group_shift;   // log2 of page_size and of group, or -1
     float scale_log2;     // scale * log2(e)
     void* work;           // workspace
+    float* lse;           // null, or where the logarithms of the sums go
+    long long lse_row_stride, lse_head_stride;
 };
 
 // Row of column c.
 __device__ __forceinline__ int paged_row_of(const PagedAttnArgs& a, int c) { return a.group_shift >= 0 ? c >> a.group_shift : c / a.group; }
+
+// Logarithm of a column's sum of exponentials: l times 2^m. Column cc (row and head of the group) of KV head `head`.
+__device__ __forceinline__ void paged_put_lse(const PagedAttnArgs& a, int row0, int head, int cc, float m, float l)
+{
+    const int row = paged_row_of(a, cc);
+    a.lse[(row0 + row) * a.lse_row_stride + (head * a.group + cc - row * a.group) * a.lse_head_stride] =
+        l == 0.f ? -INFINITY : fmaf(m, 0.6931471805599453f, logf(l));
+}
 
 // The keys that the columns [c0, c0 + cols) of a sequence see. A column is a
 // (row, head of the group) pair: column c is row c / group.
@@ -1299,6 +1309,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitShape<E>::OCC) paged_split
 #pragma unroll
             for (int k = 0; k < kSplitWarps; ++k) ml[k * COLS + tid].x = w[k].x * inv;
             if (!complete && tid < it.cols) reinterpret_cast<float2*>(part)[tid] = make_float2(M, L);
+            if (complete && a.lse && tid < it.cols) paged_put_lse(a, it.q.row0, it.head, it.tile * COLS + tid, M, L);
         }
         __syncthreads();
 #pragma unroll 2
@@ -1435,6 +1446,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     const float inv = L == 0.f ? 0.f : E::OUT / L;
     const float r[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     const int cc = j.col0 + c, rw = paged_row_of(a, cc);
+    if (d == 0 && a.lse) paged_put_lse(a, j.row0, j.head, cc, top, L);
     store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + d, r);
 }
 
@@ -1505,6 +1517,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_wide_kernel(const Pag
         const float inv = L[x] == 0.f ? 0.f : E::OUT / L[x];
         const float r[4] = {o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv};
         const int cc = j.col0 + c, rw = paged_row_of(a, cc);
+        if (e % LANES == 0 && a.lse) paged_put_lse(a, j.row0, j.head, cc, M[x], L[x]);
         store_row<typename E::QT, 4>(a.out, (j.row0 + rw) * a.o_row_stride + (j.head * a.group + cc - rw * a.group) * a.o_head_stride + e % LANES * 4, r);
     }
 }

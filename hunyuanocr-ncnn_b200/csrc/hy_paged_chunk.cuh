@@ -1327,6 +1327,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             if (i * 128 < it.cols)
             {
                 if (col && !complete) reinterpret_cast<float2*>(part)[c] = make_float2(m, l);
+                if (col && complete && a.lse) paged_put_lse(a, it.row0, it.head, it.tile * 256 + c, m, l);
                 const int cc = it.tile * 256 + c, rw = paged_row_of(a, cc);
                 const long long at = (it.row0 + rw) * a.o_row_stride + (it.head * a.group + cc - rw * a.group) * a.o_head_stride;
 #pragma unroll 1

@@ -41,6 +41,10 @@ class _Batch(ctypes.Structure):
                 ("kv_len_dev", _P), ("block_table_dev", _P)]
 
 
+class _Weights(ctypes.Structure):
+    _fields_ = [("weights_dev", _P), ("page_stride", _L), ("head_stride", _L), ("row_stride", _L)]
+
+
 def _library():
     lib = load_library()
     if lib.hy_paged_kv_write.argtypes is None:
@@ -48,6 +52,13 @@ def _library():
         lib.hy_paged_kv_read.argtypes = rows
         lib.hy_paged_attention.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I, _P, _L, _L, _P,
                                            _L, _L, ctypes.c_float, _I, _I, _I, _P, ctypes.c_size_t, _P]
+        lib.hy_paged_attention_lse.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I, _P, _L, _L,
+                                               _P, _L, _L, _P, _L, _L, ctypes.c_float, _I, _I, _I, _P, ctypes.c_size_t,
+                                               _P]
+        lib.hy_paged_add_weights.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I, _P, _L, _L, _P,
+                                             _L, _L, ctypes.c_float, _I, _I, _I, ctypes.POINTER(_Weights), _P]
+        lib.hy_paged_evict.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I,
+                                       ctypes.POINTER(_Weights), _P, _P, _P]
         lib.hy_paged_attention_workspace.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I,
                                                      ctypes.POINTER(ctypes.c_size_t)]
         lib.hy_paged_kv_write_rotated.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch),
@@ -202,11 +213,13 @@ class PagedKVCache:
         return out
 
     def attention(self, batch: PagedBatch, q: torch.Tensor, scale: float, *, causal: bool = True, window: int = 0,
-                  sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+                  sinks: int = 0, out: torch.Tensor | None = None, return_lse: bool = False):
         """Attention of rows q [rows, q heads, head_dim] over the cache (hy_paged_attention): the row at position p
         sees the positions j <= p, with a window those with p - j < window or j < sinks; all of them where causal is
         false. Rows of `out` that belong to no sequence are left as they were; without `out` they hold anything. The
-        workspace comes from torch's allocator, one for each call."""
+        workspace comes from torch's allocator, one for each call. With return_lse (out, lse): lse [rows, q heads]
+        float32, the logarithm of the sum of exponentials of every row and head (hy_paged_attention_lse), as add_weights
+        takes it."""
         dtype = self._rows(q, 0, "q")
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
@@ -228,12 +241,72 @@ class PagedKVCache:
         q0, q1, _ = q.stride()
         o0, o1, _ = out.stride()
         window, sinks = max(min(window, _INT_MAX), -1), max(min(sinks, _INT_MAX), -1)   # (a C int would wrap)
+        if return_lse:
+            lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device)
+            rc = self._lib.hy_paged_attention_lse(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), q0, q1,
+                                                  out.data_ptr(), o0, o1, lse.data_ptr(), heads, 1, scale, causal,
+                                                  window, sinks, work.data_ptr(), need, _raw_stream(self._index))
+            if rc:
+                _check(rc)
+            return out, lse
         rc = self._lib.hy_paged_attention(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), q0, q1,
                                           out.data_ptr(), o0, o1, scale, causal, window, sinks, work.data_ptr(), need,
                                           _raw_stream(self._index))
         if rc:
             _check(rc)
         return out
+
+    def allocate_weights(self) -> torch.Tensor:
+        """Attention weights of every position, zeros [pages, kv heads, page rows] float32, for add_weights and evict."""
+        return torch.zeros(self.k.shape[:3], dtype=torch.float32, device=self.device)
+
+    def _weights(self, weights: torch.Tensor) -> _Weights:
+        if weights.dtype != torch.float32 or weights.shape != self.k.shape[:3] or weights.get_device() != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "weights must be a float32 tensor [pages, kv heads, page rows] beside the cache")
+        return _Weights(weights.data_ptr(), *weights.stride())
+
+    def add_weights(self, batch: PagedBatch, q: torch.Tensor, lse: torch.Tensor, scale: float, weights: torch.Tensor, *,
+                    causal: bool = True, window: int = 0, sinks: int = 0) -> None:
+        """Adds what the rows' attention gave to every position that they see to `weights` (any strides): per KV head, the
+        sum of the probabilities over the rows and the head's query heads (hy_paged_add_weights). q, scale, window and sinks
+        are those of the attention call, lse [rows, q heads] float32 what it returned. The rows' own positions start
+        anew; positions that no row sees stay as they are."""
+        dtype = self._rows(q, 0, "q")
+        rows, heads, _ = q.shape
+        if lse.dtype != torch.float32 or lse.shape != (rows, heads) or lse.get_device() != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "lse must be a float32 tensor [rows, q heads] on the cache's device")
+        if batch.index != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
+        w = self._weights(weights)
+        q0, q1, _ = q.stride()
+        window, sinks = max(min(window, _INT_MAX), -1), max(min(sinks, _INT_MAX), -1)   # (a C int would wrap)
+        rc = self._lib.hy_paged_add_weights(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), q0, q1,
+                                            lse.data_ptr(), *lse.stride(), scale, causal, window, sinks, ctypes.byref(w),
+                                            _raw_stream(self._index))
+        if rc:
+            _check(rc)
+
+    def evict(self, batch: PagedBatch, keep: int, weights: torch.Tensor, *, recent: int = 0, first: int = 0,
+              kept: torch.Tensor | None = None) -> torch.Tensor:
+        """Cuts every sequence that has more than `keep` positions to `keep`, each KV head to its own (hy_paged_evict):
+        the `first` first and `recent` last ones stay, and of the others those of the largest weights, of equal ones the
+        lower. Their rows, scales and weights move to the positions 0 .. keep - 1 in the order they had, and batch.kv_len
+        becomes `keep`; the pages behind are free. Returns the former positions [seqs, kv heads, keep] int32 (in `kept`),
+        -1 past the end of a shorter sequence. Keys keep their rotation: positions of later rows count on."""
+        if batch.index != self._index:
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
+        shape = (batch.num_seqs, self._heads, max(keep, 0))
+        if kept is None:
+            kept = torch.empty(shape, dtype=torch.int32, device=self.device)
+        else:
+            _need(kept.dtype == torch.int32 and kept.shape == shape and kept.is_contiguous() and
+                  kept.get_device() == self._index, "kept must be a contiguous int32 tensor [seqs, kv heads, keep]")
+        w = self._weights(weights)
+        rc = self._lib.hy_paged_evict(self._ref, batch._ref, keep, first, recent, ctypes.byref(w),
+                                      batch.kv_len.data_ptr(), kept.data_ptr(), _raw_stream(self._index))
+        if rc:
+            _check(rc)
+        return kept
 
     def with_runtime(self, runtime, layer: int, batch: PagedBatch, rows: int, write: bool) -> None:
         """Moves rows [0, rows) of a TextRuntime's layer into (write) or out of the batch's positions, on the

@@ -146,10 +146,57 @@ int hy_paged_attention(const hy_paged_cache* cache, const hy_paged_batch* batch,
                        const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, void* out_dev,
                        int64_t out_row_stride, int64_t out_head_stride, float scale, int causal, int window,
                        int sinks, void* workspace_dev, size_t workspace_bytes, void* stream);
-/* Bytes of workspace_dev (16-byte aligned, any contents) that the call needs.
+/* The same, and in lse_dev [rows x q_heads] (fp32; nullable) the logarithm of the
+ * sum of exponentials that a row's probabilities were divided by: log sum over the
+ * visible positions of exp(scale * q k), -infinity where a row sees nothing. Rows
+ * outside every sequence are left as they were. hy_paged_add_weights takes it. */
+int hy_paged_attention_lse(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
+                           const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, void* out_dev,
+                           int64_t out_row_stride, int64_t out_head_stride, float* lse_dev, int64_t lse_row_stride,
+                           int64_t lse_head_stride, float scale, int causal, int window, int sinks,
+                           void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Bytes of workspace_dev (16-byte aligned, any contents) that either call needs.
  * They do not depend on the sequences' lengths. */
 int hy_paged_attention_workspace(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads,
                                  int dtype, size_t* bytes);
+
+/* What the cached positions have got of attention so far, one fp32 number for every
+ * position and KV head: (page, head, row) at page * page_stride + head *
+ * head_stride + row * row_stride of weights_dev (strides in elements, not
+ * negative, no two numbers in one place). */
+typedef struct hy_paged_weights {
+    float* weights_dev;
+    int64_t page_stride, head_stride, row_stride;
+} hy_paged_weights;
+
+/* Adds the attention weights of the batch's rows to those of the positions that
+ * they see: position j of KV head h gets the sum over the rows i that see it
+ * (hy_paged_attention's rule) and h's query heads of exp(scale * q_i k_j - lse_i),
+ * the probabilities that hy_paged_attention_lse gave them with its lse. The rows'
+ * own positions start anew: theirs are set, others' added to. So one call for
+ * every attention call, with its q, lse, scale, window and sinks, keeps the
+ * weights. Positions that no row sees stay as they are. fp32 throughout (products
+ * as in hy_paged_attention); the same call gives the same bits. */
+int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
+                         const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, const float* lse_dev,
+                         int64_t lse_row_stride, int64_t lse_head_stride, float scale, int causal, int window,
+                         int sinks, const hy_paged_weights* weights, void* stream);
+
+/* Cuts every sequence that has more than `keep` positions to `keep`, for each KV
+ * head its own: the first `first` and the last `recent` positions stay (first +
+ * recent <= keep), and of the others those of the largest weights, of equal ones
+ * the lower positions (a NaN counts least). The rows that stay, with their scales
+ * and weights, move to the positions 0 .. keep - 1 in the order they had, and
+ * kv_len_dev[s] (the batch's own array) becomes `keep`; what lies behind is left as it was, and
+ * its pages are the caller's again. kept_dev [num_seqs x num_kv_heads x keep] gets the
+ * former positions, -1 past the end of a shorter sequence and throughout where a
+ * length or a page does not hold (that sequence is left as it was). Keys keep the
+ * rotation they have: positions of later rows are counted on by the caller, not
+ * taken from kv_len, and a window then counts places in the cache. The batch's q_start is not
+ * read. Pages of a sequence that is cut must be its own; scale strides must not be 0 where
+ * there is more than one entry. */
+int hy_paged_evict(const hy_paged_cache* cache, const hy_paged_batch* batch, int keep, int first, int recent,
+                   const hy_paged_weights* weights, int* kv_len_dev, int* kept_dev, void* stream);
 
 #ifdef __cplusplus
 }
