@@ -88,14 +88,12 @@ cudaError_t launch_split(const PagedAttnArgs& a, int device, cudaStream_t s)
     return e;
 }
 
-// Tensor maps of K and V for blocks fetched 16 rows of a page at a time. Pages that do not
-// hold a multiple of 16 rows, and layouts that the maps cannot express, are copied row by row.
-template <typename CT, int D>
-ChunkTma chunk_tma(const PagedAttnArgs& a)
+// cuTensorMapEncodeTiled, or null.
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeFn tensor_map_encoder()
 {
-    using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static const EncodeFn encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q{};
@@ -104,6 +102,15 @@ ChunkTma chunk_tma(const PagedAttnArgs& a)
             fn = nullptr;
         return reinterpret_cast<EncodeFn>(fn);
     }();
+    return encode;
+}
+
+// Tensor maps of K and V for blocks fetched 16 rows of a page at a time. Pages that do not
+// hold a multiple of 16 rows, and layouts that the maps cannot express, are copied row by row.
+template <typename CT, int D>
+ChunkTma chunk_tma(const PagedAttnArgs& a)
+{
+    const auto encode = tensor_map_encoder();
     ChunkTma t;
     std::memset(&t, 0, sizeof t);
     if (!encode || a.c.page_size % 16 != 0) return t;

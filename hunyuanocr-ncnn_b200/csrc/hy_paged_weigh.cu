@@ -7,6 +7,7 @@
 #include "hy_paged_evict.cuh"
 #include "hy_paged_launch.cuh"
 #include "hy_paged_weigh.cuh"
+#include "hy_paged_weigh_chunk.cuh"
 
 using namespace hy;
 
@@ -24,6 +25,33 @@ cudaError_t launch_weigh_wide(const PagedWeighArgs& w, int device, cudaStream_t 
     using E = WeighWide<QT, CT, D>;
     const cudaError_t e = allow_smem<paged_weigh_wide_kernel<E>>(E::SMEM, device);
     return e != cudaSuccess ? e : launch_pdl(paged_weigh_wide_kernel<E>, dim3(148), kWeighWideWarps * 32, E::SMEM, s, w);
+}
+
+// Tensor map of q, whose boxes are tiles of 128 columns: groups that divide 128, and rows a whole number of heads apart.
+template <int D>
+WeighTma weigh_tma(const PagedAttnArgs& a)
+{
+    WeighTma t;
+    std::memset(&t, 0, sizeof t);
+    const auto encode = tensor_map_encoder();
+    const long long head = (a.q_heads > 1 ? a.q_head_stride : D) * 2, row = a.b.rows > 1 ? a.q_row_stride * 2 : head * a.q_heads;
+    if (!encode || 128 % a.group != 0 || head < 16 || row < head || row % head != 0 || row >= (1ll << 40)) return t;
+    const cuuint64_t size[3] = {D, static_cast<cuuint64_t>(a.q_heads), static_cast<cuuint64_t>(a.b.rows)};
+    const cuuint64_t stride[2] = {static_cast<cuuint64_t>(head), static_cast<cuuint64_t>(row)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(128 / a.group)}, step[3] = {1, 1, 1};
+    t.on = encode(&t.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), size, stride, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return t;
+}
+
+template <typename CT, int D>
+cudaError_t launch_weigh_chunk(const PagedWeighArgs& w, int device, cudaStream_t s)
+{
+    using E = WeighChunk<CT, D>;
+    const WeighTma tma = weigh_tma<D>(w.a);
+    const cudaError_t e = allow_smem<paged_weigh_chunk_kernel<CT, D>>(E::SMEM, device);
+    return e != cudaSuccess ? e : launch_pdl(paged_weigh_chunk_kernel<CT, D>, dim3(148), kWeighChunkThreads, E::SMEM, s, w, tma);
 }
 
 }  // namespace
@@ -73,6 +101,8 @@ int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batc
             if (cols <= 4) return launch_weigh<WeighFma<RT, D, 4>>(w, s);
         }
         else if (cols <= 8) return launch_weigh<WeighMma<RT, CT, D>>(w, s);
+        if constexpr (std::is_same_v<RT, __nv_bfloat16> && !std::is_same_v<CT, float>)
+            if (cols > 32) return launch_weigh_chunk<CT, D>(w, cache->device, s);
         return launch_weigh_wide<RT, CT, D>(w, cache->device, s);
     });
     return e == cudaSuccess ? HY_OK : cuda_fail("attention weights", e);
