@@ -7,12 +7,14 @@
 // all scores of its key, one tile after another, and nothing is ever reduced across
 // threads. Two blocks to an item, so that q is fetched (from L2) half as often.
 //
-// Roles of a CTA's 13 warps, which meet at mbarriers only:
-//   warps 0-3, 4-7: exponentials and sums of block 0 and 1, a thread per key;
-//   warps 8-11: loads, and the walk over the list. Each fetches a quarter of an item's keys (8-bit ones become
+// Roles of a CTA's 21 warps, which meet at mbarriers only:
+//   warps 0-15: exponentials and sums. Four warps (128 keys) take the even tiles for block 0, four for block 1, and
+//     eight the odd tiles; the two sums of a key are added up when its columns are through. So a tile's hand-over and
+//     products (some 1600 cycles) run under the other tile's exponentials (2048).
+//   warps 16-19: loads, and the walk over the list. Each fetches a quarter of an item's keys (8-bit ones become
 //     bf16 on the way, exactly), and every fourth tile of q alone, so that four fetches are under way: by TMA
 //     where a tile is a box of q (group a power of two), else by cp.async, column by column;
-//   warp 12: the products.
+//   warp 20: the products.
 //
 // Tensor memory: scores of two tiles for each of the two blocks, 4 x 128 columns, so that
 // the products of a tile run under the exponentials of the one before. Every wait is bounded, as in hy_paged_chunk.cuh.
@@ -25,9 +27,9 @@
 
 namespace hy {
 
-constexpr int kWeighChunkWarps = 13;
+constexpr int kWeighChunkWarps = 21;
 constexpr int kWeighChunkThreads = kWeighChunkWarps * 32;
-constexpr int kWeighLoadWarp = 8, kWeighMmaWarp = 12;
+constexpr int kWeighLoadWarp = 16, kWeighMmaWarp = 20;
 
 template <typename CT_, int D_>
 struct WeighChunk {
@@ -39,7 +41,8 @@ struct WeighChunk {
     static constexpr int INFO_OFF = Q_OFF + 4 * BLOCK_B;             // [8 tiles] -lse and position of 128 columns
     static constexpr int INFO_B = 2 * 128 * 4;
     static constexpr int ITEM_OFF = INFO_OFF + 8 * INFO_B;           // WeighItem
-    static constexpr int BAR_OFF = ITEM_OFF + 64;
+    static constexpr int PART_OFF = ITEM_OFF + 64;                   // [2 items][2 blocks][128] sums of the odd tiles
+    static constexpr int BAR_OFF = PART_OFF + 4 * 128 * 4;
     static constexpr int SMEM = BAR_OFF + 256 + 1024;                // + alignment of the base to 1024
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -59,12 +62,25 @@ struct WeighItem {
     int pad[4];
 };
 
+// Bytes to come in the barrier's phase, without an arrival.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar)
 {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
+}
+
+// One arrival for a whole warp, after what all its lanes did. (256 arrivals of threads at one barrier are taken one after
+// another, and cost a tile more than its products.)
+__device__ __forceinline__ void warp_arrive(uint64_t* bar)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // The columns that see any of the keys of blocks [b, b + blocks) of a sequence: from column c0 on, in tiles of 128.
@@ -192,15 +208,16 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
     unsigned char* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     const uint32_t sm = smem_u32(smem);
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + E::BAR_OFF);
-    uint64_t* const k_full = bars;          // an item's keys and description are there (128)
+    uint64_t* const k_full = bars;          // an item's keys and description are there (4 warps)
     uint64_t* const k_empty = bars + 1;     // its products are done
-    uint64_t* const d_read = bars + 2;      // its description was read (256)
-    uint64_t* const q_full = bars + 4;      // [4] a tile of q and its columns' numbers are there (32)
+    uint64_t* const d_read = bars + 2;      // its description was read (16 warps)
+    uint64_t* const q_full = bars + 4;      // [4] a tile of q and its columns' numbers are there (a warp; by TMA also the bytes)
     uint64_t* const q_empty = bars + 8;     // [4] its products are done
     uint64_t* const s_full = bars + 12;     // [2 tiles][2 blocks] scores are there (the products, and their thread)
-    uint64_t* const s_empty = bars + 16;    // [2 tiles][2 blocks] they were read (128)
-    uint64_t* const done = bars + 20;
-    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 21);
+    uint64_t* const s_empty = bars + 16;    // [2 tiles][2 blocks] they were read (4 warps)
+    uint64_t* const part_full = bars + 20;  // [2 items][2 blocks] sums of the odd tiles are there (4 warps)
+    uint64_t* const done = bars + 24;
+    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 25);
     WeighItem* const items = reinterpret_cast<WeighItem*>(smem + E::ITEM_OFF);
     __shared__ long long scan[kWeighChunkWarps + 1];
     static_assert(sizeof(WeighItem) == 64, "description");
@@ -214,15 +231,16 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
     }
     if (tid == 0)
     {
-        mbar_init(k_full, 128);
+        mbar_init(k_full, 4);
         mbar_init(k_empty, 1);
-        mbar_init(d_read, 256);
+        mbar_init(d_read, 16);
         for (int i = 0; i < 4; ++i)
         {
-            mbar_init(&q_full[i], 32);
+            mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 2);
-            mbar_init(&s_empty[i], 128);
+            mbar_init(&s_empty[i], 4);
+            mbar_init(&part_full[i], 4);
         }
         mbar_init(done, 1);
         fence_mbar_init();
@@ -320,7 +338,7 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
             if (lw == 0 && lane == 0) *items = d;
             if (d.blocks == 0)
             {
-                mbar_arrive(k_full);
+                warp_arrive(k_full);
                 break;
             }
             if (kb < d.blocks)
@@ -361,7 +379,7 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
                 }
                 fence_async_smem();
             }
-            mbar_arrive(k_full);
+            warp_arrive(k_full);
 
             // ---- this warp's tiles of q ----
             for (int x = (lw - tile_no) & 3; x < d.tiles && ok; x += 4)
@@ -376,7 +394,7 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
                 {
                     if (leader)
                     {
-                        mbar_arrive_expect_tx(&q_full[lw], E::BLOCK_B);
+                        mbar_expect_tx(&q_full[lw], E::BLOCK_B);
                         const int y = it.head * a.group, z = it.q.row0 + paged_row_of(a, c0);
                         tma_load_3d(sm + qdst, &tma.q, 0, y, z, &q_full[lw]);
                         if constexpr (D == 128) tma_load_3d(sm + qdst + 16384, &tma.q, 64, y, z, &q_full[lw]);
@@ -418,8 +436,7 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
                     cp_wait<0>();
                     fence_async_smem();
                 }
-                if (!tma.on || !leader) mbar_arrive(&q_full[lw]);   // (the leader has, with the bytes to come)
-                __syncwarp();
+                warp_arrive(&q_full[lw]);
                 ++fetched;
             }
             tile_no += d.tiles;
@@ -485,8 +502,8 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
     }
     else
     {
-        // ---------------- exponentials and sums of block i, one thread per key ----------------
-        const int i = warp >> 2, key = tid & 127;
+        // ---------------- exponentials and sums of block i, a thread for every other tile of a key ----------------
+        const int i = (warp >> 2) & 1, odd = warp >> 3, key = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         bool ok = true;
         int no = 0;
@@ -495,7 +512,7 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
             ok = warp_wait(k_full, item & 1, a.c.status);
             if (!ok) break;
             const WeighItem it = *items;
-            mbar_arrive(d_read);
+            warp_arrive(d_read);
             if (it.blocks == 0) break;
             // This thread's key: its place, what it has.
             const int u = (it.block + i) * 128 + key;
@@ -508,35 +525,40 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
                 const int x = a.page_shift >= 0 ? j >> a.page_shift : j / a.c.page_size, row = j - x * a.c.page_size;
                 const int pg = __ldg(a.b.table + it.seq * a.b.table_stride + x);
                 live = pg >= 0 && pg < a.c.num_pages;
-                if (live)
+                if (live && (CODES || !odd))
                 {
                     at = w.weights + pg * w.w_page_stride + row * w.w_row_stride + it.head * w.w_head_stride;
-                    if (j < p_0) old = *at;
+                    if (!odd && j < p_0) old = *at;
                     if constexpr (CODES) kf = __ldg(a.c.k_scale + pg * a.c.s_page_stride + row * a.c.s_row_stride + it.head * a.c.s_head_stride);
                 }
             }
             // Rows that see the key stand at see_lo .. see_lo + see_n (columns that are not there at -1).
             const unsigned see_lo = a.causal ? j : 0, see_n = a.window > 0 && j >= a.sinks ? a.window - 1 : INT_MAX - see_lo;
-            // Whether every key of the block is there, and its first and last.
-            const bool full = (it.block + i + 1) * 128 <= it.keys;
-            const int u0 = (it.block + i) * 128, u1 = u0 + 127;
-            const int j_first = u0 < it.sinks ? u0 : it.lo + u0 - it.sinks, j_last = u1 < it.sinks ? u1 : it.lo + u1 - it.sinks;
-            for (int x = 0; x < it.tiles; ++x, ++no)
+            // Tiles [whole_a, whole_b) of the item whose columns are all there and see every key of the block: their rows
+            // stand at its last key or later and (window) at most window - 1 behind its first.
+            int whole_a = 0, whole_b = 0;
+            if (i < it.blocks && (it.block + i + 1) * 128 <= it.keys)
             {
-                const int slot = no & 1;
-                ok = warp_wait(&s_full[slot * 2 + i], (no / 2) & 1, a.c.status);
+                const int u0 = (it.block + i) * 128, u1 = u0 + 127;
+                const int j_first = u0 < it.sinks ? u0 : it.lo + u0 - it.sinks, j_last = u1 < it.sinks ? u1 : it.lo + u1 - it.sinks;
+                const int row_a = max(0, (a.causal ? j_last : 0) - p_0);
+                const long long row_b = a.window > 0 && j_last >= a.sinks ? static_cast<long long>(j_first) + a.window - p_0 : it.n;
+                whole_a = max(0, (row_a * a.group - it.c0 + 127) / 128);
+                whole_b = static_cast<int>((max(0ll, min(row_b, static_cast<long long>(it.n))) * a.group - it.c0) / 128);
+            }
+            for (int x = (no + odd) & 1; x < it.tiles; x += 2)
+            {
+                const int tile = no + x;
+                ok = warp_wait(&s_full[odd * 2 + i], (tile / 2) & 1, a.c.status);
                 if (!ok) break;
                 tc_fence_after();
                 if (i < it.blocks)
                 {
-                    const uint32_t ts = tmem + (slot * 2 + i) * 128 + lanes;
-                    const float* const info = reinterpret_cast<const float*>(smem + E::INFO_OFF + (no & 7) * E::INFO_B);
-                    const int c0 = it.c0 + x * 128, c1 = min(c0 + 128, it.n * a.group) - 1;
-                    const int p_first = p_0 + paged_row_of(a, c0), p_last = p_0 + paged_row_of(a, c1);
-                    const bool whole = full && c1 == c0 + 127 && p_first >= 0 &&
-                                       (!a.causal || (j_last <= p_first && (a.window == 0 || j_first > p_last - a.window || j_last < a.sinks)));
+                    const uint32_t ts = tmem + (odd * 2 + i) * 128 + lanes;
+                    const float* const info = reinterpret_cast<const float*>(smem + E::INFO_OFF + (tile & 7) * E::INFO_B);
+                    const bool whole = x >= whole_a && x < whole_b;
                     uint64_t total = 0;   // (a pair of zeros)
-                    // In a loop that the instruction caches hold: 32 columns, while the next 32 are on their way.
+                    // In a loop that the instruction caches hold (straight code for all columns waited for instructions).
                     auto columns = [&](auto masked) {
                         const uint64_t log2e = f2(kLog2e, kLog2e), kf2 = f2(kf, kf), scale2 = f2(w.scale, w.scale);
                         auto add = [&](const uint32_t (&r)[32], int q) {
@@ -566,17 +588,13 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
                                 total = f2_add(total, f2_add(f2(p[0], p[1]), f2(p[2], p[3])));
                             }
                         };
-                        uint32_t r0[32], r1[32];
-                        tmem_ld32(ts, r0);
 #pragma unroll 1
-                        for (int q = 0; q < 128; q += 64)
+                        for (int q = 0; q < 128; q += 32)
                         {
-                            tmem_ld32_wait(r0);
-                            tmem_ld32(ts + q + 32, r1);
-                            add(r0, q);
-                            tmem_ld32_wait(r1);
-                            if (q == 0) tmem_ld32(ts + 64, r0);
-                            add(r1, q + 32);
+                            uint32_t r[32];
+                            tmem_ld32(ts + q, r);
+                            tmem_ld32_wait(r);
+                            add(r, q);
                         }
                     };
                     if (whole) columns(std::false_type{});
@@ -586,9 +604,22 @@ __global__ void __launch_bounds__(kWeighChunkThreads, 1) paged_weigh_chunk_kerne
                     sum += t0 + t1;
                     tc_fence_before();
                 }
-                mbar_arrive(&s_empty[slot * 2 + i]);
+                warp_arrive(&s_empty[odd * 2 + i]);
             }
-            if (live && ok) *at = old + sum;
+            no += it.tiles;
+            // ---- the two sums of a key ----
+            float* const part = reinterpret_cast<float*>(smem + E::PART_OFF) + ((item & 1) * 2 + i) * 128 + key;
+            uint64_t* const there = &part_full[(item & 1) * 2 + i];
+            if (odd)
+            {
+                *part = sum;
+                warp_arrive(there);
+            }
+            else
+            {
+                ok = ok && warp_wait(there, (item / 2) & 1, a.c.status);
+                if (live && ok) *at = old + (sum + *part);
+            }
         }
     }
     __syncwarp();
