@@ -10,11 +10,11 @@ using namespace hy;
 
 namespace {
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, int THREADS>
 cudaError_t launch_logprobs(const LogprobArgs& a, int device, cudaStream_t s)
 {
-    const int smem = TOP ? a.iters * kLogprobThreads * static_cast<int>(sizeof(float)) : 0;
-    cudaError_t e = allow_smem<logprob_kernel<T, TOP>>(160 * 1024, device);
+    const int smem = TOP ? (a.iters + kLogprobRun - 1) / kLogprobRun * THREADS * static_cast<int>(sizeof(float)) : 0;
+    cudaError_t e = allow_smem<logprob_kernel<T, TOP, THREADS>>(16 * 1024, device);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -24,12 +24,28 @@ cudaError_t launch_logprobs(const LogprobArgs& a, int device, cudaStream_t s)
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.rows * a.split);
-    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, logprob_kernel<T, TOP>, a);
+    return cudaLaunchKernelEx(&cfg, logprob_kernel<T, TOP, THREADS>, a);
+}
+
+template <typename T>
+cudaError_t launch_logprobs(LogprobArgs a, int device, cudaStream_t s)
+{
+    // CTAs of a row: more while the rows leave SMs without work, of at least 4096 logits each (1024 rows of 120818: 75 us
+    // with one, 85 with four; 200 rows 27 and 19).
+    while (a.split < kLogprobMaxCluster && ((a.rows * a.split < 4 * 148 && a.vocab / a.split > 4096) || a.vocab / a.split > (1 << 18))) a.split *= 2;
+    constexpr int EV = 16 / static_cast<int>(sizeof(T));
+    const bool few = a.rows * a.split < 148;
+    const int vectors = (a.vocab + 2 * EV - 2) / EV;   // (a row may start anywhere in its first vector)
+    const int step = (few ? kLogprobFewThreads : kLogprobManyThreads) * (32 / EV);
+    a.iters = (vectors + a.split * step - 1) / (a.split * step);
+    if (few)
+        return a.top ? launch_logprobs<T, true, kLogprobFewThreads>(a, device, s) : launch_logprobs<T, false, kLogprobFewThreads>(a, device, s);
+    return a.top ? launch_logprobs<T, true, kLogprobManyThreads>(a, device, s) : launch_logprobs<T, false, kLogprobManyThreads>(a, device, s);
 }
 
 }  // namespace
@@ -59,15 +75,8 @@ int hy_token_logprobs(const void* logits_dev, int rows, int vocab, int64_t row_s
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     LogprobArgs a{logits_dev, row_stride, rows, vocab, tokens_dev, tokens_per_row, top, logprobs_dev, entropy_dev,
                   top_ids_dev, top_logprobs_dev, 1, 1};
-    // CTAs of a row: more while the rows leave SMs without one, of at least 4096 logits each.
-    while (a.split < kLogprobMaxCluster && ((rows * a.split < 4 * 148 && vocab / a.split > 4096) || vocab / a.split > (1 << 18))) a.split *= 2;
-    const int ev = 16 / elem_size(dtype), vectors = (vocab + 2 * ev - 2) / ev;   // (a row may start anywhere in its first vector)
-    const int step = kLogprobThreads * (32 / ev);
-    a.iters = (vectors + a.split * step - 1) / (a.split * step);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e;
-    if (dtype == HY_DTYPE_F32) e = top ? launch_logprobs<float, true>(a, device, s) : launch_logprobs<float, false>(a, device, s);
-    else e = top ? launch_logprobs<__nv_bfloat16, true>(a, device, s) : launch_logprobs<__nv_bfloat16, false>(a, device, s);
+    const cudaError_t e = dtype == HY_DTYPE_F32 ? launch_logprobs<float>(a, device, s) : launch_logprobs<__nv_bfloat16>(a, device, s);
     return e == cudaSuccess ? HY_OK : cuda_fail("log probabilities", e);
 }
 

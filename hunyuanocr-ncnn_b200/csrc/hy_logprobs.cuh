@@ -5,14 +5,15 @@
 //   log prob of x = (x - M) - log(c + s),   entropy = log(c + s) + t / (c + s).
 // s and t hold no term of the largest logit, so that what is left beside a probability
 // near 1 keeps its relative precision (log(1 + s) is taken as log1p), and no large terms
-// cancel. One pass: every thread keeps (m, c, s, t) of its own elements, rescaled when m
-// grows; they are joined at the end.
+// cancel. One pass: every thread keeps (c, s, t) of its own elements against the largest m that
+// its warp has met, rescaled when that grows; they are joined at the end. (With a largest of
+// its own for every thread some lane has a new one in nearly every step, and the whole warp pays for it.)
 //
-// The alternatives come from the same pass: what is stored of every group of 32
+// The alternatives come from the same pass: what is stored of every group of 128
 // elements is its maximum (in shared memory). The n-th largest of the threads' maxima
 // is a lower bound of the row's n-th largest element, so the groups whose maximum
 // reaches it - hardly more than n - hold all that is looked for, and only they are read
-// again. A list that overflows (thousands of equal logits) is left aside for n
+// again, a vector to a thread. A list that overflows (thousands of equal logits) is left aside for n
 // passes that take one element each.
 //
 // A row belongs to a cluster of 1 to 8 CTAs, which meet in the shared memory of the first.
@@ -24,7 +25,10 @@
 
 namespace hy {
 
-constexpr int kLogprobThreads = 256;
+constexpr int kLogprobManyThreads = 128;   // of a CTA, eight to an SM: while some are in their last steps, others load
+constexpr int kLogprobFewThreads = 512;    // where there are fewer CTAs than SMs: a row's loads are all on their way at once
+constexpr int kLogprobRun = 4;         // steps of a group: 128 elements
+constexpr int kLogprobGroups = 256;    // groups that are read again by all threads together
 constexpr int kLogprobList = 512;      // candidates of a CTA
 constexpr int kLogprobMaxTop = 64;
 constexpr int kLogprobMaxCluster = 8;
@@ -54,6 +58,13 @@ __device__ __forceinline__ float max_nan(float a, float b)
 {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Largest of a warp's; a NaN among them comes out.
+__device__ __forceinline__ float warp_max_nan(float x)
+{
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float exp2_approx(float x)
@@ -132,7 +143,8 @@ struct LogprobRow {
     }
 };
 
-// Block-wide maximum (a NaN comes out) and sum; red: shared memory of 3 * 8 floats.
+// Block-wide maximum (a NaN comes out); red: shared memory of a float per warp.
+template <int kLogprobThreads>
 __device__ __forceinline__ float logprob_block_max(float x, float* red)
 {
 #pragma unroll
@@ -146,29 +158,35 @@ __device__ __forceinline__ float logprob_block_max(float x, float* red)
     return x;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobArgs a)
+template <typename T, bool TOP, int kLogprobThreads>
+__global__ void __launch_bounds__(kLogprobThreads, 1024 / kLogprobThreads) logprob_kernel(const LogprobArgs a)
 {
     namespace cg = cooperative_groups;
     using Row = LogprobRow<T>;
     constexpr int EV = Row::EV, U = 32 / EV, NW = kLogprobThreads / 32;
-    extern __shared__ __align__(16) float group_max[];   // [iters][threads]
-    __shared__ float red[3 * NW], thread_max[kLogprobThreads];
+    extern __shared__ __align__(16) float group_max[];   // [groups of a thread][threads]
+    __shared__ float red[3 * NW];
+    __shared__ __align__(16) float thread_max[kLogprobThreads];
     __shared__ LogprobState parts[kLogprobMaxCluster];             // (the first CTA's are used)
     __shared__ unsigned long long list[TOP ? kLogprobList : 1];    // candidates
-    __shared__ unsigned long long tops[TOP ? kLogprobMaxCluster * kLogprobMaxTop : 1];   // (the first CTA's) sorted lists
+    __shared__ __align__(16) unsigned long long tops[TOP ? kLogprobMaxCluster * kLogprobMaxTop : 1];   // (the first CTA's) sorted lists
     __shared__ unsigned long long mine[TOP ? kLogprobMaxTop : 1], best[NW];
-    __shared__ int count;
+    __shared__ int group_list[TOP ? kLogprobGroups : 1];           // groups that may hold some of the top
+    __shared__ int count, groups;
     __shared__ float bound;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x % a.split, r = blockIdx.x / a.split;
-    cg::this_cluster().barrier_arrive();   // (the first CTA runs before the others write to its shared memory)
+    if (a.split > 1) cg::this_cluster().barrier_arrive();   // (the first CTA runs before the others write to its shared memory)
     pdl_wait();
     const Row row(static_cast<const T*>(a.logits) + r * a.row_stride, a.vocab);
     const int nv = row.vectors(), per = a.iters * kLogprobThreads * U;
     const int v0 = rank * per, v1 = min(nv, v0 + per);   // this CTA's vectors
 
     LogprobState st = {-INFINITY, 0.f, 0.f, 0.f};
+    float own_max = -INFINITY, run_max = -INFINITY;
+    // (the first token's logit, ahead of the row's)
+    const int token0 = rank == 0 && tid < a.tokens_per_row ? __ldg(a.tokens + static_cast<long long>(r) * a.tokens_per_row + tid) : -1;
+    const float logit0 = token0 >= 0 && token0 < a.vocab ? to_f32<T>(static_cast<const T*>(a.logits)[r * a.row_stride + token0]) : 0.f;
     for (int it = 0; it < a.iters; ++it)
     {
         const int v = v0 + it * kLogprobThreads * U + tid;
@@ -187,8 +205,18 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
             m1 = max_nan(m1, f[e + 2], f[e + 3]);
         }
         const float top = max_nan(m0, m1);
-        if constexpr (TOP) group_max[it * kLogprobThreads + tid] = top;
-        if (top < st.m)
+        if constexpr (TOP)
+        {
+            run_max = max_nan(run_max, top);
+            if (it % kLogprobRun == kLogprobRun - 1 || it == a.iters - 1)
+            {
+                group_max[it / kLogprobRun * kLogprobThreads + tid] = run_max;
+                own_max = max_nan(own_max, run_max);
+                run_max = -INFINITY;
+            }
+        }
+        const float most = warp_max_nan(top);   // (what follows is alike in the whole warp)
+        if (most < st.m)
         {
             // x - m, its exponential, the sums; -1000 stands for less (the exponential is 0: 0 times infinity is not taken).
             const uint64_t neg = f2(-st.m, -st.m), log2e = f2(1.4426950408889634f, 1.4426950408889634f);
@@ -212,9 +240,9 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
             f2_get(t2, y0, y1);
             st.t -= y0 + y1;
         }
-        else if (top != -INFINITY)   // the first finite ones, a new maximum, one more like it, a NaN
+        else if (most != -INFINITY)   // the first finite ones, a new maximum, one more like it, a NaN
         {
-            if (!(top <= st.m) && st.m == st.m) logprob_raise(st, top);   // (a NaN stays one)
+            if (!(most <= st.m) && st.m == st.m) logprob_raise(st, most);   // (a NaN stays one)
             float s = 0.f, t = 0.f;
 #pragma unroll
             for (int e = 0; e < U * EV; ++e)
@@ -231,8 +259,17 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
     }
 
     // ---- the CTA's state ----
-    if constexpr (TOP) thread_max[tid] = st.m;
-    const float M = logprob_block_max(st.m, red);   // (also makes group_max and thread_max visible)
+    if constexpr (TOP)
+    {
+        if (a.top > kLogprobThreads / 16) thread_max[tid] = own_max;
+        else
+        {
+            float x = max_nan(own_max, __shfl_xor_sync(0xffffffffu, own_max, 1));
+            x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            if ((tid & 3) == 0) thread_max[tid >> 2] = x;
+        }
+    }
+    const float M = logprob_block_max<kLogprobThreads>(st.m, red);   // (also makes group_max and thread_max visible)
     if (st.m != M) logprob_raise(st, M);
     float sum[3] = {st.c, st.s, st.t};
 #pragma unroll
@@ -241,21 +278,27 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
         sum[i] = warp_sum(sum[i]);
         if (lane == 0) red[i * NW + warp] = sum[i];
     }
-    if (tid == 0) count = 0;
+    if (tid == 0) count = groups = 0;
     if constexpr (TOP)
     {
-        // The threads' n-th largest maximum.
-        int above = 0;
-#pragma unroll 8
-        for (int j = 0; j < kLogprobThreads; ++j)
+        // The n-th largest of the maxima of runs of 4 threads (of single threads where n is large).
+        const int many = a.top > kLogprobThreads / 16 ? kLogprobThreads : kLogprobThreads / 4;
+        if (tid < many)
         {
-            const float o = thread_max[j], own = thread_max[tid];
-            above += o > own || (o == own && j < tid);
+            const float own = thread_max[tid];
+            int above = 0;
+#pragma unroll 4
+            for (int j = 0; j < many; j += 4)
+            {
+                const float4 o = *reinterpret_cast<const float4*>(thread_max + j);
+                above += (o.x > own || (o.x == own && j < tid)) + (o.y > own || (o.y == own && j + 1 < tid)) +
+                         (o.z > own || (o.z == own && j + 2 < tid)) + (o.w > own || (o.w == own && j + 3 < tid));
+            }
+            if (above == a.top - 1) bound = own;
         }
-        if (above == a.top - 1) bound = thread_max[tid];
     }
     __syncthreads();
-    cg::this_cluster().barrier_wait();
+    if (a.split > 1) cg::this_cluster().barrier_wait();
     if (tid == 0)
     {
         LogprobState p = {M, 0.f, 0.f, 0.f};
@@ -272,25 +315,42 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
         // (with a NaN in the row nothing below is used; `bound` may then hold anything)
         const bool usable = M == M && M != -INFINITY && M != INFINITY;
         const float low = usable ? bound : INFINITY;
+        const int all_groups = (a.iters + kLogprobRun - 1) / kLogprobRun * kLogprobThreads;
+        auto look = [&](int g, int x, auto&& take) {   // vector x of group g
+            const int it = g / kLogprobThreads * kLogprobRun + x / U, v = v0 + (it * U + x % U) * kLogprobThreads + g % kLogprobThreads;
+            if (it >= a.iters || v >= v1) return;
+            float f[EV];
+            Row::unpack(row.raw(v), f);
+#pragma unroll
+            for (int e = 0; e < EV; ++e)
+                if (f[e] >= low && f[e] != -INFINITY) take(logprob_key(f[e], v * EV + e - row.skip));
+        };
         auto each = [&](auto&& take) {   // every element of this CTA's that may be among the top
-            for (int g = tid; g < a.iters * kLogprobThreads; g += kLogprobThreads)
+            for (int g = tid; g < all_groups; g += kLogprobThreads)
             {
                 if (!(group_max[g] >= low) || group_max[g] == -INFINITY) continue;
-                const int v = v0 + (g / kLogprobThreads) * kLogprobThreads * U + tid;
-                for (int u = 0; u < U && v + u * kLogprobThreads < v1; ++u)
-                {
-                    float f[EV];
-                    Row::unpack(row.raw(v + u * kLogprobThreads), f);
-#pragma unroll
-                    for (int e = 0; e < EV; ++e)
-                        if (f[e] >= low && f[e] != -INFINITY) take(logprob_key(f[e], (v + u * kLogprobThreads) * EV + e - row.skip));
-                }
+#pragma unroll 1
+                for (int x = 0; x < U * kLogprobRun; ++x) look(g, x, take);
             }
         };
-        each([&](unsigned long long key) {
+        auto note = [&](unsigned long long key) {
             const int i = atomicAdd(&count, 1);
             if (i < kLogprobList) list[i] = key;
-        });
+        };
+        for (int g = tid; g < all_groups; g += kLogprobThreads)
+            if (group_max[g] >= low && group_max[g] != -INFINITY)
+            {
+                const int i = atomicAdd(&groups, 1);
+                if (i < kLogprobGroups) group_list[i] = g;
+            }
+        __syncthreads();
+        if (groups <= kLogprobGroups)
+        {
+            // A vector of a group to a thread, so that all loads are on their way at once.
+#pragma unroll 4
+            for (int x = tid; x < groups * U * kLogprobRun; x += kLogprobThreads) look(group_list[x / (U * kLogprobRun)], x % (U * kLogprobRun), note);
+        }
+        else each(note);
         if (tid < kLogprobMaxTop) mine[tid] = 0;
         __syncthreads();
         const int n = count;
@@ -328,9 +388,10 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
                 __syncthreads();
             }
         }
-        if (tid < a.top) cg::this_cluster().map_shared_rank(tops, 0)[rank * kLogprobMaxTop + tid] = mine[tid];
+        if (tid < a.top) cg::this_cluster().map_shared_rank(tops, 0)[rank * a.top + tid] = mine[tid];
     }
-    cg::this_cluster().sync();
+    if (a.split > 1) cg::this_cluster().sync();
+    else __syncthreads();
     if (rank != 0) return;
 
     // ---- the row's answer, by its first CTA ----
@@ -351,10 +412,10 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
     if (tid == 0 && a.entropy) a.entropy[r] = usable ? less + t / (c + s) : nan;
     for (int i = tid; i < a.tokens_per_row; i += kLogprobThreads)
     {
-        const int token = __ldg(a.tokens + static_cast<long long>(r) * a.tokens_per_row + i);
+        const int token = i == tid ? token0 : __ldg(a.tokens + static_cast<long long>(r) * a.tokens_per_row + i);
         float lp = nan;
         if (usable && token >= 0 && token < a.vocab)
-            lp = (to_f32<T>(static_cast<const T*>(a.logits)[r * a.row_stride + token]) - top) - less;
+            lp = ((i == tid ? logit0 : to_f32<T>(static_cast<const T*>(a.logits)[r * a.row_stride + token])) - top) - less;
         a.logprobs[static_cast<long long>(r) * a.tokens_per_row + i] = lp;
     }
     if constexpr (TOP)
@@ -366,18 +427,24 @@ __global__ void __launch_bounds__(kLogprobThreads) logprob_kernel(const LogprobA
             a.top_logprobs[at] = there ? (logprob_key_value(key) - top) - less : usable ? -INFINITY : nan;
         };
         // The CTAs' sorted lists into one: an entry's place is the number of larger ones.
+        const int n = a.split * a.top;
         int total = 0;
-        for (int i = tid; i < a.split * a.top; i += kLogprobThreads)
+        for (int i0 = 0; i0 < n; i0 += kLogprobThreads)
         {
-            const unsigned long long key = tops[(i / a.top) * kLogprobMaxTop + i % a.top];
+            const int i = i0 + tid;
+            const unsigned long long key = i < n ? tops[i] : 0;
+            total += __syncthreads_count(key != 0);
             if (key == 0) continue;
-            int above = 0;
-            for (int p = 0; p < a.split; ++p)
-                for (int j = 0; j < a.top; ++j) above += tops[p * kLogprobMaxTop + j] > key;
+            int above = 0, j = 0;
+#pragma unroll 4
+            for (; j + 2 <= n; j += 2)
+            {
+                const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(tops + j);
+                above += (o.x > key) + (o.y > key);
+            }
+            if (j < n) above += tops[j] > key;
             if (above < a.top) put(above, key);
         }
-        for (int p = 0; p < a.split; ++p)
-            for (int j = 0; j < a.top; ++j) total += tops[p * kLogprobMaxTop + j] != 0;
         for (int i = (usable ? total : 0) + tid; i < a.top; i += kLogprobThreads) put(i, 0);
     }
 }

@@ -28,11 +28,16 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor | None
 
 
+_LIB = None
+
+
 def _library():
-    lib = load_library()
-    if lib.hy_token_logprobs.argtypes is None:
+    global _LIB
+    if _LIB is None:
+        lib = load_library()
         lib.hy_token_logprobs.argtypes = [_P, _I, _I, _L, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P]
-    return lib
+        _LIB = lib
+    return _LIB
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
@@ -42,30 +47,29 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     ordered by the lower token. Logits of -infinity (masked tokens) have probability 0 and are no alternatives (-1 and
     -infinity where too few are left). A token outside the vocabulary (padding) gives NaN, as does all of a row that
     holds a NaN, +infinity or nothing above -infinity (its top_ids are -1)."""
-    dtype, index = _ROW_DTYPES.get(logits.dtype), logits.get_device()
-    if dtype is None or index < 0 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise HyError(HY_ERR_INVALID_ARGUMENT, "logits must be a float32 or bfloat16 CUDA tensor [rows, vocab] with contiguous rows")
+    dtype, index, shape = _ROW_DTYPES.get(logits.dtype), logits.get_device(), logits.shape
+    if dtype is None or index < 0 or len(shape) != 2:
+        raise HyError(HY_ERR_INVALID_ARGUMENT, "logits must be a float32 or bfloat16 CUDA tensor [rows, vocab]")
+    rows, vocab = shape
+    stride, one = logits.stride()
+    if one != 1 and vocab > 1:
+        raise HyError(HY_ERR_INVALID_ARGUMENT, "the rows of logits must be contiguous")
     if logits.requires_grad and torch.is_grad_enabled():
         raise HyError(HY_ERR_INVALID_ARGUMENT, "logits require a gradient: this call has none")
-    rows, vocab = logits.shape
-    if (tokens.dtype != torch.int32 or tokens.get_device() != index or tokens.dim() not in (1, 2) or
-            tokens.shape[0] != rows or not tokens.is_contiguous()):
+    tshape = tokens.shape
+    if (tokens.dtype is not torch.int32 or tokens.get_device() != index or len(tshape) not in (1, 2) or tshape[0] != rows or
+            not tokens.is_contiguous()):
         raise HyError(HY_ERR_INVALID_ARGUMENT, "tokens must be a contiguous int32 tensor [rows] or [rows, n] beside the logits")
     if not 0 <= top <= 64:
         raise HyError(HY_ERR_INVALID_ARGUMENT, "top must be in 0..64 and at most vocab")
-    per_row = 1 if tokens.dim() == 1 else tokens.shape[1]
-    # One allocation: log probabilities, entropies, top ids, their log probabilities.
-    n = rows * per_row
-    held = torch.empty(n + rows + 2 * rows * top, dtype=torch.float32, device=logits.device)
-    lp, entropy = held[:n].view(tokens.shape), held[n:n + rows]
-    at = held.data_ptr()
-    ids = alternatives = None
+    per_row = 1 if len(tshape) == 1 else tshape[1]
+    lp, entropy = logits.new_empty(tshape, dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32)
+    ids = alternatives = at = ids_at = None
     if top:
-        ids = held[n + rows:n + rows + rows * top].view(torch.int32).view(rows, top)
-        alternatives = held[n + rows + rows * top:].view(rows, top)
-    rc = _library().hy_token_logprobs(logits.data_ptr(), rows, vocab, logits.stride(0), dtype, index, tokens.data_ptr(),
-                                      per_row, top, at, at + 4 * n, at + 4 * (n + rows), at + 4 * (n + rows + rows * top),
-                                      _raw_stream(index))
+        ids, alternatives = tokens.new_empty((rows, top)), logits.new_empty((rows, top), dtype=torch.float32)
+        ids_at, at = ids.data_ptr(), alternatives.data_ptr()
+    rc = (_LIB or _library()).hy_token_logprobs(logits.data_ptr(), rows, vocab, stride, dtype, index, tokens.data_ptr(), per_row,
+                                                top, lp.data_ptr(), entropy.data_ptr(), ids_at, at, _raw_stream(index))
     if rc:
         _check(rc)
     return TokenLogprobs(lp, entropy, ids, alternatives)

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import HY_ERR_INVALID_ARGUMENT, HyError, _check, load_library
-from .rotary import Rotation, _Rotation
+from .rotary import rotation
 
 DTYPE_F32, DTYPE_BF16, DTYPE_E4M3, DTYPE_INT8 = range(4)
 _CACHE_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float8_e4m3fn: DTYPE_E4M3,
@@ -62,8 +62,7 @@ def _library():
         lib.hy_paged_attention_workspace.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), _I, _I, _I,
                                                      ctypes.POINTER(ctypes.c_size_t)]
         lib.hy_paged_kv_write_rotated.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch),
-                                                  ctypes.POINTER(_Rotation), _I, _I, _I, _P, _L, _L, _P, _L, _L, _P,
-                                                  _L, _L, _P, _L, _L, _P]
+                                                  _P, _I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P]
         lib.hy_paged_kv_write.argtypes = rows
     return lib
 
@@ -178,21 +177,21 @@ class PagedKVCache:
         dtype = self._pair(k, v)
         if self._rows(q, 0, "q") != dtype or q.shape[0] != k.shape[0]:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "q must have the rows and type of k")
+        rows, heads, dim = q.shape
         if out is None:
-            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
-        elif self._rows(out, q.shape[1], "out") != dtype or out.shape != q.shape:
+            out = q.new_empty((rows, heads, dim))
+        elif self._rows(out, heads, "out") != dtype or out.shape != q.shape:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "q and out must have one shape and type")
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
-        turn = Rotation(q.shape[0], self._dim, self._index, q_weight, k_weight, cos, sin, positions, eps, rotate_first)
-        rows, heads, _ = q.shape
+        turn = rotation(rows, dim, self._index, q_weight, k_weight, cos, sin, positions, eps, rotate_first)
         q0, q1, _ = q.stride()
         k0, k1, _ = k.stride()
         v0, v1, _ = v.stride()
         o0, o1, _ = out.stride()
-        rc = self._lib.hy_paged_kv_write_rotated(self._ref, batch._ref, turn.ref, rows, heads, dtype, q.data_ptr(), q0,
-                                                 q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, out.data_ptr(), o0,
-                                                 o1, _raw_stream(self._index))
+        rc = self._lib.hy_paged_kv_write_rotated(self._ref, batch._ref, turn, rows, heads, dtype, q.data_ptr(), q0, q1,
+                                                 k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, out.data_ptr(), o0, o1,
+                                                 _raw_stream(self._index))
         if rc:
             _check(rc)
         return out
@@ -261,7 +260,8 @@ class PagedKVCache:
         return torch.zeros(self.k.shape[:3], dtype=torch.float32, device=self.device)
 
     def _weights(self, weights: torch.Tensor) -> _Weights:
-        if weights.dtype != torch.float32 or weights.shape != self.k.shape[:3] or weights.get_device() != self._index:
+        if (weights.dtype != torch.float32 or weights.shape != self.k.shape[:3] or weights.get_device() != self._index or
+                weights.requires_grad and torch.is_grad_enabled()):
             raise HyError(HY_ERR_INVALID_ARGUMENT, "weights must be a float32 tensor [pages, kv heads, page rows] beside the cache")
         return _Weights(weights.data_ptr(), *weights.stride())
 
@@ -273,7 +273,8 @@ class PagedKVCache:
         anew; positions that no row sees stay as they are."""
         dtype = self._rows(q, 0, "q")
         rows, heads, _ = q.shape
-        if lse.dtype != torch.float32 or lse.shape != (rows, heads) or lse.get_device() != self._index:
+        if (lse.dtype != torch.float32 or lse.shape != (rows, heads) or lse.get_device() != self._index or
+                lse.requires_grad and torch.is_grad_enabled()):
             raise HyError(HY_ERR_INVALID_ARGUMENT, "lse must be a float32 tensor [rows, q heads] on the cache's device")
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
