@@ -14,9 +14,10 @@ using namespace hy;
 namespace {
 
 template <typename E>
-cudaError_t launch_weigh(const PagedWeighArgs& w, cudaStream_t s)
+cudaError_t launch_weigh(const PagedWeighArgs& w, int device, cudaStream_t s)
 {
-    return launch_pdl(paged_weigh_kernel<E>, dim3(148 * kWeighCtas), kSplitThreads, 0, s, w);
+    const cudaError_t e = allow_smem<paged_weigh_kernel<E>>(WeighShape<E>::SMEM, device);
+    return e != cudaSuccess ? e : launch_pdl(paged_weigh_kernel<E>, dim3(148 * kWeighCtas), kSplitThreads, WeighShape<E>::SMEM, s, w);
 }
 
 template <typename QT, typename CT, int D>
@@ -97,10 +98,10 @@ int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batc
         constexpr int D = decltype(d)::value;
         if constexpr (std::is_same_v<CT, float>)
         {
-            if (cols <= 2) return launch_weigh<WeighFma<RT, D, 2>>(w, s);
-            if (cols <= 4) return launch_weigh<WeighFma<RT, D, 4>>(w, s);
+            if (cols <= 2) return launch_weigh<WeighFma<RT, D, 2>>(w, cache->device, s);
+            if (cols <= 4) return launch_weigh<WeighFma<RT, D, 4>>(w, cache->device, s);
         }
-        else if (cols <= 8) return launch_weigh<WeighMma<RT, CT, D>>(w, s);
+        else if (cols <= 8) return launch_weigh<WeighMma<RT, CT, D>>(w, cache->device, s);
         if constexpr (std::is_same_v<RT, __nv_bfloat16> && !std::is_same_v<CT, float>)
             if (cols > 32) return launch_weigh_chunk<CT, D>(w, cache->device, s);
         return launch_weigh_wide<RT, CT, D>(w, cache->device, s);

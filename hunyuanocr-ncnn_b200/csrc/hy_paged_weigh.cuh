@@ -100,16 +100,15 @@ __device__ __forceinline__ int weigh_pos(const PagedAttnArgs& a, const SplitItem
 // What a column has of a key, from their product; d's rounding is relative to d.
 __device__ __forceinline__ float weigh_exp(float s, float fac, float lse) { return ex2(fmaf(s, fac, -lse) * kLog2e); }
 
-// A key of a warp's step, held by the lane that has its number: where its weight is and what it had.
+// Keys of a warp's step: a key's scale in the lane that has its number, and which keys are there.
 struct WeighKey {
-    long long at;   // of its weight
-    float old;      // what it has, 0 for a new row's
-    float scale;    // of its codes
-    uint32_t mask;  // (of the warp) keys that are there
+    float scale;
+    uint32_t mask;
 };
 
 // ---------------------------------------------------------------------------
-// Few columns. Every warp streams its keys through registers, a step (4 KB) ahead, with q in registers.
+// Few columns. Every warp streams its keys through a cp.async ring of its own, three steps of 4 KB ahead (with the next
+// step in registers 64 tokens over 1024-8192 E4M3 keys took 103 us), with q in registers.
 // ---------------------------------------------------------------------------
 template <typename QT_, typename CT_, int D_>
 struct WeighMma {
@@ -306,15 +305,27 @@ struct WeighFma {
 };
 
 constexpr int kWeighCtas = 3;   // per SM
+constexpr int kWeighRing = 4;   // steps of a warp's ring
+// A step in the ring: the lanes' pieces, then by key where its weight is, what it has (0 for a new row's), its scale; the mask.
+template <typename E>
+struct WeighShape {
+    static constexpr int AT = E::RAW * 512, OLD = AT + 256, SCALE = OLD + 128, MASK = SCALE + 128, STAGE = MASK + 16;
+    static constexpr int SMEM = kSplitWarps * kWeighRing * STAGE;
+    static_assert(SMEM * kWeighCtas <= 224 * 1024, "shared memory");
+};
 
 template <typename E>
 __global__ void __launch_bounds__(kSplitThreads, kWeighCtas) paged_weigh_kernel(const PagedWeighArgs w)
 {
     using CT = typename E::CT;
     constexpr int KEYS = E::KEYS, TILE = kSplitWarps * KEYS, PIECE = 16 / static_cast<int>(sizeof(CT));
+    using Sh = WeighShape<E>;
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan[kSplitWarps + 1];
     const PagedAttnArgs& a = w.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kr = lane % KEYS;
+    unsigned char* const ring = smem + warp * kWeighRing * Sh::STAGE;
+    const uint32_t ring_u = smem_u32(ring);
     pdl_wait();
     pdl_launch();
     const SplitStart st = split_start<kWeighAll, TILE, kSplitThreads>(a, scan);
@@ -345,45 +356,67 @@ __global__ void __launch_bounds__(kSplitThreads, kWeighCtas) paged_weigh_kernel(
                 row = j - x * a.c.page_size;
                 pg = __ldg(table + x);
             };
-            uint4 raw[E::RAW], next[E::RAW];
-            WeighKey key, key_next = {0, 0.f, 0.f, 0u};
             auto load = [&](int i, int pg, int row) {
-                const int u = (tile0 + i) * TILE + warp * KEYS + kr;
-                const bool live = i < n_tiles && u < it.w.n, ok = live && pg >= 0 && pg < a.c.num_pages;
-                if (live && !ok) paged_status(a.c.status, kPagedBadPage);
-                key_next.mask = __ballot_sync(0xffffffffu, ok);
-                if constexpr (KEYS < 32) key_next.mask &= (1u << KEYS) - 1u;
-                const long long off = ok ? pg * a.c.page_stride + row * a.c.row_stride + it.head * a.c.head_stride : 0;
-#pragma unroll
-                for (int x = 0; x < E::RAW; ++x)
+                if (i < n_tiles)
                 {
-                    const int r = E::row_of(lane, x);
-                    const long long o = __shfl_sync(0xffffffffu, off, r) + E::piece_of(lane, x) * PIECE;
-                    next[x] = (key_next.mask >> r) & 1u ? __ldg(reinterpret_cast<const uint4*>(static_cast<const CT*>(a.c.k) + o)) : make_uint4(0, 0, 0, 0);
+                    const int u = (tile0 + i) * TILE + warp * KEYS + kr, slot = i % kWeighRing;
+                    const bool live = u < it.w.n, ok = live && pg >= 0 && pg < a.c.num_pages;
+                    if (live && !ok) paged_status(a.c.status, kPagedBadPage);
+                    uint32_t mask = __ballot_sync(0xffffffffu, ok);
+                    if constexpr (KEYS < 32) mask &= (1u << KEYS) - 1u;
+                    const long long off = ok ? pg * a.c.page_stride + row * a.c.row_stride + it.head * a.c.head_stride : 0;
+                    const uint32_t to = ring_u + slot * Sh::STAGE;
+#pragma unroll
+                    for (int x = 0; x < E::RAW; ++x)
+                    {
+                        const int r = E::row_of(lane, x);
+                        const long long o = __shfl_sync(0xffffffffu, off, r) + E::piece_of(lane, x) * PIECE;
+                        cp_async16_zfill(to + x * 512 + lane * 16, static_cast<const CT*>(a.c.k) + o, (mask >> r) & 1u);
+                    }
+                    const long long at = ok ? pg * w.w_page_stride + row * w.w_row_stride + it.head * w.w_head_stride : 0;
+                    // (the first columns' pass sets the weights of new rows)
+                    cp_async4_zfill(to + Sh::OLD + lane * 4, w.weights + at, ok && !(c0 == 0 && split_key(it, u) >= it.q.kv - it.q.n));
+                    if constexpr (E::F16)
+                        cp_async4_zfill(to + Sh::SCALE + lane * 4, a.c.k_scale + (ok ? pg * a.c.s_page_stride + row * a.c.s_row_stride + it.head * a.c.s_head_stride : 0), ok);
+                    reinterpret_cast<volatile long long*>(ring + slot * Sh::STAGE + Sh::AT)[lane] = at;
+                    if (lane == 0) *reinterpret_cast<volatile uint32_t*>(ring + slot * Sh::STAGE + Sh::MASK) = mask;
                 }
-                if (!ok) return;
-                if constexpr (E::F16) key_next.scale = __ldg(a.c.k_scale + pg * a.c.s_page_stride + row * a.c.s_row_stride + it.head * a.c.s_head_stride);
-                key_next.at = pg * w.w_page_stride + row * w.w_row_stride + it.head * w.w_head_stride;
-                // (the first columns' pass sets the weights of new rows)
-                key_next.old = (c0 == 0 && split_key(it, u) >= it.q.kv - it.q.n) ? 0.f : w.weights[key_next.at];
+                cp_commit();
             };
-            int pg = -1, row = 0, pg1 = -1, row1 = 0;
-            look_up(0, pg, row);
-            look_up(1, pg1, row1);
-            load(0, pg, row);
+            int pg[kWeighRing], row[kWeighRing];
+#pragma unroll
+            for (int i = 0; i < kWeighRing; ++i)
+            {
+                pg[i] = -1;
+                row[i] = 0;
+                look_up(i, pg[i], row[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < kWeighRing - 1; ++i) load(i, pg[i], row[i]);
+            int pg1 = pg[kWeighRing - 1], row1 = row[kWeighRing - 1];
             eng.columns(w, it, c0);
             for (int i = 0; i < n_tiles; ++i)
             {
-#pragma unroll
-                for (int x = 0; x < E::RAW; ++x) raw[x] = next[x];
-                key = key_next;
-                load(i + 1, pg1, row1);
-                look_up(i + 2, pg1, row1);
+                cp_wait<kWeighRing - 2>();
+                __syncwarp();
+                load(i + kWeighRing - 1, pg1, row1);
+                look_up(i + kWeighRing, pg1, row1);
                 const int u0 = (tile0 + i) * TILE + warp * KEYS;
                 if (u0 >= it.w.n) continue;   // (uniform)
+                const unsigned char* const from = ring + i % kWeighRing * Sh::STAGE;
+                uint4 raw[E::RAW];
+#pragma unroll
+                for (int x = 0; x < E::RAW; ++x) raw[x] = *reinterpret_cast<const uint4*>(from + x * 512 + lane * 16);
+                WeighKey key;
+                key.mask = *reinterpret_cast<const volatile uint32_t*>(from + Sh::MASK);
+                key.scale = E::F16 ? reinterpret_cast<const volatile float*>(from + Sh::SCALE)[lane] : 0.f;
                 const float sum = eng.step(a, it, u0, raw, key);
-                if (lane < KEYS && ((key.mask >> lane) & 1u)) w.weights[key.at] = key.old + sum;
+                if (lane < KEYS && ((key.mask >> lane) & 1u))
+                    w.weights[reinterpret_cast<const volatile long long*>(from + Sh::AT)[lane]] =
+                        reinterpret_cast<const volatile float*>(from + Sh::OLD)[lane] + sum;
             }
+            cp_wait<0>();
+            __syncwarp();   // the ring was read
         }
         left -= n_tiles;
         if (left <= 0 || st.unit > 1) break;

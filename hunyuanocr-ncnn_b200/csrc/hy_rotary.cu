@@ -56,7 +56,6 @@ RotateArgs rotate_args(const hy_rotation* t, int rows, int q_heads, int kv_heads
     a.table_rows = t->table_rows;
     a.eps = t->eps;
     a.inv_dim = 1.f / static_cast<float>(head_dim);
-    a.rotate_first = t->rotate_first != 0;
     a.rows = rows;
     a.q_heads = q_heads;
     a.kv_heads = kv_heads;
@@ -64,20 +63,20 @@ RotateArgs rotate_args(const hy_rotation* t, int rows, int q_heads, int kv_heads
 }
 
 template <typename RT, typename CT, int D, bool CACHE>
-cudaError_t launch_rotate(RotateArgs a, cudaStream_t s)
+cudaError_t launch_rotate(RotateArgs a, bool first, cudaStream_t s)
 {
     constexpr int VPW = 32 / (D / (2 * (16 / static_cast<int>(sizeof(RT)))));
     const int heads = a.q_heads + (CACHE ? 2 : 1) * a.kv_heads;
     a.whole = a.rows >= 4 * 148;
     int parts = 1;
     if (a.whole)
-        a.per_cta = std::min(kRowsPerCta, std::max(4, a.rows / (8 * 148) / 4 * 4));
+        a.per_cta = std::min(kRowsPerCta, std::max(8, a.rows / (8 * 148) / 4 * 4));
     else
     {
         a.per_cta = 1;
         parts = std::min((heads + kRowWarps * VPW - 1) / (kRowWarps * VPW), std::max(1, 4 * 148 / a.rows));
     }
-    return launch_pdl(rotate_kernel<RT, CT, D, CACHE>, dim3((a.rows + a.per_cta - 1) / a.per_cta, parts), kRowWarps * 32, 0, s, a);
+    return launch_pdl(first ? rotate_kernel<RT, CT, D, CACHE, true> : rotate_kernel<RT, CT, D, CACHE, false>, dim3((a.rows + a.per_cta - 1) / a.per_cta, parts), kRowWarps * 32, 0, s, a);
 }
 
 }  // namespace
@@ -117,11 +116,12 @@ int hy_norm_rotate(const hy_rotation* rotation, int rows, int q_heads, int kv_he
     a.k_out = k_out_dev; a.ko_row = k_out_row_stride; a.ko_head = k_out_head_stride;
     a.status = status_dev;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool first = rotation->rotate_first != 0;
     const cudaError_t e =
         dtype == HY_DTYPE_F32
-            ? (head_dim == 64 ? launch_rotate<float, float, 64, false>(a, s) : launch_rotate<float, float, 128, false>(a, s))
-            : (head_dim == 64 ? launch_rotate<__nv_bfloat16, __nv_bfloat16, 64, false>(a, s)
-                              : launch_rotate<__nv_bfloat16, __nv_bfloat16, 128, false>(a, s));
+            ? (head_dim == 64 ? launch_rotate<float, float, 64, false>(a, first, s) : launch_rotate<float, float, 128, false>(a, first, s))
+            : (head_dim == 64 ? launch_rotate<__nv_bfloat16, __nv_bfloat16, 64, false>(a, first, s)
+                              : launch_rotate<__nv_bfloat16, __nv_bfloat16, 128, false>(a, first, s));
     return e == cudaSuccess ? HY_OK : cuda_fail("norm and rotation", e);
 }
 
@@ -160,7 +160,7 @@ int hy_paged_kv_write_rotated(const hy_paged_cache* cache, const hy_paged_batch*
     a.b = device_batch(batch, rows);
     const cudaError_t e = with_row_type(dtype, cache->dtype, cache->head_dim, [&](auto rt, auto ct, auto d) {
         return launch_rotate<typename decltype(rt)::type, typename decltype(ct)::type, decltype(d)::value, true>(
-            a, static_cast<cudaStream_t>(stream));
+            a, rotation->rotate_first != 0, static_cast<cudaStream_t>(stream));
     });
     return e == cudaSuccess ? HY_OK : cuda_fail("rotated paged write", e);
 }
