@@ -110,9 +110,22 @@ __global__ void __launch_bounds__(kEvictThreads, 2) paged_evict_kernel(const Pag
             return evict_order(*weight_at(place(j)));
         };
         // Position i * T + tid of a run of CHUNK; those of the first run are held, others read again whenever they are needed.
+        // (All look-ups, then all weights, so that they are on their way together.)
         uint32_t held[R];
+        {
+            EvictPlace at[R];
+            float wt[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) held[i] = i * T < kv ? key(i * T + tid) : 0;
+            for (int i = 0; i < R; ++i) at[i] = i * T < kv ? place(min(i * T + tid, kv - 1)) : EvictPlace{0, 0};
+#pragma unroll
+            for (int i = 0; i < R; ++i) wt[i] = i * T < kv ? *weight_at(at[i]) : 0.f;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+            {
+                const int j = i * T + tid;
+                held[i] = j >= kv ? 0 : j < a.first || j >= kv - a.recent ? 0xffffffffu : evict_order(wt[i]);
+            }
+        }
         auto reach = [&](uint32_t least) {   // how many keys reach `least` (not 0)
             int n = 0;
 #pragma unroll
