@@ -16,7 +16,9 @@
 // again, a vector to a thread. A list that overflows (thousands of equal logits) is left aside for n
 // passes that take one element each.
 //
-// A row belongs to a cluster of 1 to 8 CTAs, which meet in the shared memory of the first.
+// A row belongs to a cluster of 1 to 8 CTAs, which meet in the shared memory of the first. Memory bounds it where
+// there are many rows: 1024 of 120818 fp32 logits take 75 us without alternatives, 6.6 TB/s, 81 with 8; bf16 56 and 62 (bound by
+// instructions). One row with 20 alternatives: 9 us, one latency after another.
 #pragma once
 
 #include <cooperative_groups.h>

@@ -17,7 +17,9 @@
 //   warp 20: the products.
 //
 // Tensor memory: scores of two tiles for each of the two blocks, 4 x 128 columns, so that
-// the products of a tile run under the exponentials of the one before. Every wait is bounded, as in hy_paged_chunk.cuh.
+// the products of a tile run under the exponentials of the one before. 4 sequences of ~1012 rows over 6000-8192 bf16
+// keys (111 GFLOP): 163 us, 683 TFLOP/s; the special-function units are busy 70% of the time (101 us of exponentials),
+// the tensor cores 35%, and the CTAs' shares, whole blocks, differ by 12%.  Every wait is bounded, as in hy_paged_chunk.cuh.
 #pragma once
 
 #include <climits>

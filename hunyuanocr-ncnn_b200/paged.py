@@ -270,7 +270,7 @@ class PagedKVCache:
         """Adds what the rows' attention gave to every position that they see to `weights` (any strides): per KV head, the
         sum of the probabilities over the rows and the head's query heads (hy_paged_add_weights). q, scale, window and sinks
         are those of the attention call, lse [rows, q heads] float32 what it returned. The rows' own positions start
-        anew; positions that no row sees stay as they are."""
+        anew; positions that no row sees stay as they are. Sequences of a call must not share pages."""
         dtype = self._rows(q, 0, "q")
         rows, heads, _ = q.shape
         if (lse.dtype != torch.float32 or lse.shape != (rows, heads) or lse.get_device() != self._index or
@@ -288,11 +288,13 @@ class PagedKVCache:
             _check(rc)
 
     def evict(self, batch: PagedBatch, keep: int, weights: torch.Tensor, *, recent: int = 0, first: int = 0,
-              kept: torch.Tensor | None = None) -> torch.Tensor:
+              kept: torch.Tensor | None = None, set_lengths: bool = True) -> torch.Tensor:
         """Cuts every sequence that has more than `keep` positions to `keep`, each KV head to its own (hy_paged_evict):
         the `first` first and `recent` last ones stay, and of the others those of the largest weights, of equal ones the
         lower. Their rows, scales and weights move to the positions 0 .. keep - 1 in the order they had, and batch.kv_len
-        becomes `keep`; the pages behind are free. Returns the former positions [seqs, kv heads, keep] int32 (in `kept`),
+        becomes `keep` (with set_lengths; caches that share a batch, a layer's each, are cut with set_lengths=False but for
+        the last, since all have to be cut at the same length); the pages behind are free. A sequence's pages must be its
+        own. Returns the former positions [seqs, kv heads, keep] int32 (in `kept`),
         -1 past the end of a shorter sequence. Keys keep their rotation: positions of later rows count on."""
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
@@ -304,7 +306,8 @@ class PagedKVCache:
                   kept.get_device() == self._index, "kept must be a contiguous int32 tensor [seqs, kv heads, keep]")
         w = self._weights(weights)
         rc = self._lib.hy_paged_evict(self._ref, batch._ref, keep, first, recent, ctypes.byref(w),
-                                      batch.kv_len.data_ptr(), kept.data_ptr(), _raw_stream(self._index))
+                                      batch.kv_len.data_ptr() if set_lengths else None, kept.data_ptr(),
+                                      _raw_stream(self._index))
         if rc:
             _check(rc)
         return kept

@@ -175,8 +175,9 @@ typedef struct hy_paged_weights {
  * the probabilities that hy_paged_attention_lse gave them with its lse. The rows'
  * own positions start anew: theirs are set, others' added to. So one call for
  * every attention call, with its q, lse, scale, window and sinks, keeps the
- * weights. Positions that no row sees stay as they are. fp32 throughout (products
- * as in hy_paged_attention); the same call gives the same bits. */
+ * weights. Positions that no row sees stay as they are. Sequences of a call must
+ * not share pages (a position's number would be written by both). fp32 throughout
+ * (products as in hy_paged_attention); the same call gives the same bits. */
 int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
                          const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, const float* lse_dev,
                          int64_t lse_row_stride, int64_t lse_head_stride, float scale, int causal, int window,
@@ -186,15 +187,17 @@ int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batc
  * head its own: the first `first` and the last `recent` positions stay (first +
  * recent <= keep), and of the others those of the largest weights, of equal ones
  * the lower positions (a NaN counts least). The rows that stay, with their scales
- * and weights, move to the positions 0 .. keep - 1 in the order they had, and
- * kv_len_dev[s] (the batch's own array) becomes `keep`; what lies behind is left as it was, and
- * its pages are the caller's again. kept_dev [num_seqs x num_kv_heads x keep] gets the
- * former positions, -1 past the end of a shorter sequence and throughout where a
- * length or a page does not hold (that sequence is left as it was). Keys keep the
- * rotation they have: positions of later rows are counted on by the caller, not
- * taken from kv_len, and a window then counts places in the cache. The batch's q_start is not
- * read. Pages of a sequence that is cut must be its own; scale strides must not be 0 where
- * there is more than one entry. */
+ * and weights, move to the positions 0 .. keep - 1 in the order they had; what lies
+ * behind is left as it was, and its pages are the caller's again. kv_len_dev is the
+ * batch's own array, where lengths above `keep` become `keep`, or NULL: the lengths
+ * are left to the caller (for all caches but the last that share a batch, say a
+ * layer's each: they have to be cut at the same length). kept_dev [num_seqs x
+ * num_kv_heads x keep] gets the former positions, -1 past the end of a shorter
+ * sequence and throughout where a length or a page does not hold (that sequence is
+ * left as it was). Keys keep the rotation they have: positions of later rows are
+ * counted on by the caller, not taken from kv_len, and a window then counts places
+ * in the cache. The batch's q_start is not read. A sequence's pages must be its
+ * own; scale strides must not be 0 where there is more than one entry. */
 int hy_paged_evict(const hy_paged_cache* cache, const hy_paged_batch* batch, int keep, int first, int recent,
                    const hy_paged_weights* weights, int* kv_len_dev, int* kept_dev, void* stream);
 

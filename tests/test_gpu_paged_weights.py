@@ -305,7 +305,7 @@ def _check_evict(s, keep, first=0, recent=0):
 @pytest.mark.parametrize("kv,kv_heads,dim,page,keep,first,recent", [
     ([2], 1, 64, 16, 1, 0, 0), ([5, 3, 4], 2, 64, 2, 3, 1, 1), ([700, 100, 64], 3, 128, 24, 64, 4, 16),
     ([1100] * 20 + [900], 8, 128, 16, 1024, 4, 256), ([9000, 200], 2, 64, 100, 5000, 0, 7), ([513], 16, 128, 7, 512, 0, 512),
-    ([20000], 1, 128, 64, 300, 1, 0), ([600], 8, 64, 64, 500, 500, 0)])
+    ([20000], 1, 128, 64, 300, 1, 0), ([600], 8, 64, 64, 500, 500, 0), ([40000, 33000], 1, 64, 64, 900, 1, 5)])
 def test_evict(paged, cache, kv, kv_heads, dim, page, keep, first, recent):
     s = Setup(paged, cache, BF16, kv, [1] * len(kv), kv_heads, kv_heads, dim, page, keep)
     _check_evict(s, keep, first, recent)
@@ -352,6 +352,20 @@ def test_sequences_that_do_not_hold_are_left(paged, pkg):
     others = torch.ones(s.pages, dtype=torch.bool)
     others[s.table[2].cpu().long()] = False
     assert torch.equal(s.c.k[others], held[others])
+
+
+def test_layers_that_share_a_batch(paged):
+    """Every layer's cache is cut at the same lengths, which change with the last."""
+    layers = [Setup(paged, BF16, BF16, [400, 90, 250], [1] * 3, 2, 2, 64, 16, 50 + i) for i in range(3)]
+    batch = layers[0].batch
+    for s in layers:
+        s.table, s.batch = layers[0].table, batch
+    for s in layers:
+        want, kept, lengths = _evicted(s, 100, 2, 10)
+        last = s is layers[-1]
+        assert torch.equal(s.c.evict(batch, 100, s.weights, recent=10, first=2, set_lengths=last).cpu(), kept)
+        assert batch.kv_len.tolist() == (lengths if last else s.kv)
+        assert all(torch.equal(a, b) for a, b in zip((s.c.k, s.c.v, s.weights), want))
 
 
 def test_other_layouts_and_capture(paged):

@@ -61,7 +61,7 @@ def test_weights_refusals(paged, call, over, message):
 
 @pytest.mark.parametrize("over,message", [
     (dict(keep=0), "keep"), (dict(first=-1), "keep"), (dict(recent=-1), "keep"), (dict(keep=4, first=2, recent=3), "keep"),
-    (dict(first=2 ** 31 - 1, recent=2 ** 31 - 1), "keep"), (dict(kv_len=None), "null"), (dict(kept=None), "null"),
+    (dict(first=2 ** 31 - 1, recent=2 ** 31 - 1), "keep"), (dict(kept=None), "null"),
     (dict(kv_len=2 * FAKE), "own"), (dict(kept=FAKE), "overlap"),
 ])
 def test_evict_refusals(paged, over, message):
