@@ -454,7 +454,9 @@ struct WeighWide {
     static constexpr int NQ = std::is_same_v<QT, float> ? (F16 ? 2 : 3) : 1;
     static constexpr int NK = std::is_same_v<CT, float> ? 3 : 1;
     static constexpr int RB = D * static_cast<int>(sizeof(CT)), KS = D / 16, PIECES = RB / 64;
-    static constexpr int HV = NK == 1 ? 2 : 1, KEYS = 16 * HV, TILE = kWeighWideWarps * KEYS;
+    // Keys of a warp, in 16s: 32 over 8-bit caches (4 x ~1012 fp32 rows over 6000-8192 E4M3 keys: 1.0 ms, 1.5 with 16; 2 x 350
+    // rows and keys 59 us, 44 with 16), 16 over others (BF16: 1.68 ms, 1.83 with 32; 48 us, 98 with 32).
+    static constexpr int HV = F16 ? 2 : 1, KEYS = 16 * HV, TILE = kWeighWideWarps * KEYS;
     static constexpr int FRAGS = NQ * KS * NT * 32;                       // uint2s of a tile of columns
     static constexpr int SMEM = 2 * (FRAGS * 8 + 3 * COLS * 4);           // two tiles: fragments, lse, factor, position
     static constexpr int QI = KS / 2;                                     // fragments that a thread makes
