@@ -2,6 +2,8 @@
 
 import ctypes
 import importlib
+import os
+import re
 
 import pytest
 
@@ -102,3 +104,15 @@ def test_lse_refusals_of_the_attention(paged, over, message):
     rc = lib.hy_paged_attention_lse(ctypes.byref(c), ctypes.byref(b), 2, 4, 1, FAKE, 512, 128, 2 * FAKE, 512, 128,
                                     f["lse"], *f["strides"], 0.1, 1, 0, 0, None, 0, None)
     assert rc == 1 and _says(paged, message or "workspace")
+
+
+def test_waits_of_the_tensor_core_kernel_end_alike_in_a_whole_warp():
+    """What follows a wait there is of the whole warp (tensor memory, shuffles, barriers that a warp arrives at once), so
+    every wait is one of those that vote; and every arrival of a thread alone is the products' leader's."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hunyuanocr-ncnn_b200", "csrc",
+                        "hy_paged_weigh_chunk.cuh")
+    with open(path) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.findall(r"\bmbar_(?:try_)?wait(?:_spin)?\(", text)
+    assert len(re.findall(r"\bwarp_wait(?:_spin)?\(", text)) >= 10
+    assert len(re.findall(r"\bmbar_arrive\(", text)) == 2   # warp_arrive's own, and the leader's
