@@ -298,7 +298,9 @@ class PagedKVCache:
         -1 past the end of a shorter sequence. Keys keep their rotation: positions of later rows count on."""
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
-        shape = (batch.num_seqs, self._heads, max(keep, 0))
+        _need(1 <= keep <= 2 ** 30 and first >= 0 and recent >= 0 and first + recent <= keep,   # (a C int would wrap)
+              "keep must be in 1..2^30, first and recent not negative and together at most keep")
+        shape = (batch.num_seqs, self._heads, keep)
         if kept is None:
             kept = torch.empty(shape, dtype=torch.int32, device=self.device)
         else:

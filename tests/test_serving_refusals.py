@@ -1,0 +1,53 @@
+"""CPU checks of the calls around the paged cache and behind the LM head: numbers past 32 bits, which a C int would wrap,
+are refused before the library is called."""
+
+import importlib
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def paged(pkg):
+    return importlib.import_module("hy_b200.paged")
+
+
+class Reached(Exception):
+    pass
+
+
+class NoLibrary:
+    """Stands for the library: a call that gets there was not refused."""
+
+    def __getattr__(self, name):
+        raise Reached(name)
+
+
+def _cache(paged, dtype=torch.float32):
+    """A cache of host memory without a library behind it: only the checks before a call can run."""
+    c = object.__new__(paged.PagedKVCache)
+    c._lib, c.k, c.device, c._index, c._heads, c._dim = NoLibrary(), torch.zeros(4, 2, 8, 64, dtype=dtype), "cpu", -1, 2, 64
+    c._ref = None
+    return c
+
+
+def _batch(paged):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)   # noqa: E731
+    return paged.PagedBatch(i32(0, 1), i32(20), torch.zeros(1, 3, dtype=torch.int32), 1)
+
+
+@pytest.mark.parametrize("over", [
+    dict(recent=2 ** 32), dict(first=2 ** 32), dict(recent=2 ** 32 + 3), dict(first=-2 ** 32), dict(recent=-1),
+    dict(first=5, recent=5), dict(keep=0), dict(keep=-2 ** 32 + 8), dict(keep=2 ** 32 + 8), dict(keep=2 ** 31),
+])
+def test_evict_sizes(paged, pkg, over):
+    c, f = _cache(paged), dict(keep=8, first=1, recent=2)
+    f.update(over)
+    with pytest.raises(pkg.HyError, match="keep"):
+        c.evict(_batch(paged), f["keep"], torch.zeros(4, 2, 8), first=f["first"], recent=f["recent"])
+
+
+def test_evict_sizes_that_hold_reach_the_library(paged):
+    for keep, first, recent in ((8, 0, 0), (8, 3, 5), (1, 0, 1)):
+        with pytest.raises(Reached, match="hy_paged_evict"):
+            _cache(paged).evict(_batch(paged), keep, torch.zeros(4, 2, 8), first=first, recent=recent)
