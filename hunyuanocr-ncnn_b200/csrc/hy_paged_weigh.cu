@@ -118,6 +118,8 @@ int hy_paged_evict(const hy_paged_cache* cache, const hy_paged_batch* batch, int
     if (rc) return rc;
     if (keep < 1 || first < 0 || recent < 0 || static_cast<long long>(first) + recent > keep)
         return fail(HY_ERR_INVALID_ARGUMENT, "keep must be positive, first and recent not negative and together at most keep");
+    // (positions lie below 2^30; the kernel's index over the list, a step of threads ahead of it, stays within 32 bits)
+    if (keep > 1 << 30) return fail(HY_ERR_INVALID_ARGUMENT, "keep must be at most 2^30");
     if (static_cast<long long>(batch->num_seqs) * cache->num_kv_heads * kEvictMaxCluster > INT_MAX)
         return fail(HY_ERR_CAPACITY, "num_seqs * num_kv_heads must be below 2^28");
     const int e = elem_size(cache->dtype);

@@ -185,7 +185,7 @@ int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batc
 
 /* Cuts every sequence that has more than `keep` positions to `keep`, for each KV
  * head its own: the first `first` and the last `recent` positions stay (first +
- * recent <= keep), and of the others those of the largest weights, of equal ones
+ * recent <= keep <= 2^30), and of the others those of the largest weights, of equal ones
  * the lower positions (a NaN counts least). The rows that stay, with their scales
  * and weights, move to the positions 0 .. keep - 1 in the order they had; what lies
  * behind is left as it was, and its pages are the caller's again. kv_len_dev is the

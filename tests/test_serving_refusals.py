@@ -6,6 +6,9 @@ import importlib
 import pytest
 import torch
 
+import test_paged
+import test_paged_weights
+
 
 @pytest.fixture(scope="module")
 def paged(pkg):
@@ -51,3 +54,11 @@ def test_evict_sizes_that_hold_reach_the_library(paged):
     for keep, first, recent in ((8, 0, 0), (8, 3, 5), (1, 0, 1)):
         with pytest.raises(Reached, match="hy_paged_evict"):
             _cache(paged).evict(_batch(paged), keep, torch.zeros(4, 2, 8), first=first, recent=recent)
+
+
+@pytest.mark.parametrize("keep", [2 ** 30 + 1, 2 ** 31 - 512, 2 ** 31 - 1])
+def test_eviction_to_more_than_positions_reach(paged, keep):
+    """The list of what stays is walked in steps of a CTA's threads, by a C int that must not pass its largest."""
+    assert test_paged_weights._evict(paged, keep=keep) == 1
+    assert "2^30" in paged._library().hy_last_error().decode()
+    assert test_paged_weights._evict(paged, keep=2 ** 30, batch=test_paged._batch(paged, num_seqs=0)) == 0
