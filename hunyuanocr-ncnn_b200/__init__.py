@@ -529,10 +529,12 @@ class TextRuntime:
         tok = None if tokens is None else _i32(tokens).reshape(-1)
         if tok is not None and tok.size != rows:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "lm_head_logprobs takes a token for every hidden row")
+        if not 0 <= top <= 64:   # (a C int would wrap)
+            raise HyError(HY_ERR_INVALID_ARGUMENT, "top must be in 0..64 and at most vocab")
         lp = None if tok is None else np.empty(rows, np.float32)
         entropy = np.empty(rows, np.float32)
-        ids = np.empty((rows, max(top, 0)), np.int32) if top else None
-        alt = np.empty((rows, max(top, 0)), np.float32) if top else None
+        ids = np.empty((rows, top), np.int32) if top else None
+        alt = np.empty((rows, top), np.float32) if top else None
         _check(_LIB.hy_lm_head_logprobs(self._ctx, _ptr(h), rows, _ptr(tok), top, _ptr(lp), _ptr(entropy), _ptr(ids),
                                         _ptr(alt)))
         return lp, entropy, ids, alt

@@ -62,3 +62,16 @@ def test_eviction_to_more_than_positions_reach(paged, keep):
     assert test_paged_weights._evict(paged, keep=keep) == 1
     assert "2^30" in paged._library().hy_last_error().decode()
     assert test_paged_weights._evict(paged, keep=2 ** 30, batch=test_paged._batch(paged, num_seqs=0)) == 0
+
+
+@pytest.mark.parametrize("top", [2 ** 32, 2 ** 32 + 3, -2 ** 32, -1, 65])
+def test_alternatives_behind_the_lm_head(pkg, monkeypatch, top):
+    """(2^32 came to the library as 0, and arrays that nobody had written came back.)"""
+    monkeypatch.setattr(pkg, "_LIB", NoLibrary())
+    rt = object.__new__(pkg.TextRuntime)
+    rt._ctx = None
+    with pytest.raises(pkg.HyError, match="top"):
+        rt.lm_head_logprobs(torch.zeros(2, 1024).numpy(), top=top)
+    with pytest.raises(Reached, match="hy_lm_head_logprobs"):
+        rt.lm_head_logprobs(torch.zeros(2, 1024).numpy(), top=64)
+    del rt._ctx
