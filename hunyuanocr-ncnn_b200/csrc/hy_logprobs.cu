@@ -66,6 +66,8 @@ int hy_token_logprobs(const void* logits_dev, int rows, int vocab, int64_t row_s
     if (device < 0) return fail(HY_ERR_INVALID_ARGUMENT, "device must not be negative");
     if (static_cast<long long>(rows) * std::max({tokens_per_row, top, kLogprobMaxCluster}) > INT_MAX)
         return fail(HY_ERR_CAPACITY, "rows * max(tokens_per_row, top, 8) must be below 2^31");
+    // (the kernel's index of a token, a step of threads ahead of the last, stays within 32 bits)
+    if (tokens_per_row > 1 << 30) return fail(HY_ERR_CAPACITY, "tokens_per_row must be at most 2^30");
     if (rows == 0) return HY_OK;
     if (!logits_dev || (tokens_per_row > 0 && (!tokens_dev || !logprobs_dev)) || (top > 0 && (!top_ids_dev || !top_logprobs_dev)))
         return fail(HY_ERR_INVALID_ARGUMENT, "logits, tokens or an output is null");

@@ -63,6 +63,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not 0 <= top <= 64:
         raise HyError(HY_ERR_INVALID_ARGUMENT, "top must be in 0..64 and at most vocab")
     per_row = 1 if len(tshape) == 1 else tshape[1]
+    if rows >= 2 ** 31 or vocab >= 2 ** 31 or per_row >= 2 ** 31:   # (a C int would wrap)
+        raise HyError(HY_ERR_INVALID_ARGUMENT, "rows, vocab and the tokens of a row must be below 2^31")
     lp, entropy = logits.new_empty(tshape, dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32)
     ids = alternatives = at = ids_at = None
     if top:

@@ -31,8 +31,8 @@ extern "C" {
  * Logits of -infinity (masked tokens) have probability 0. A row that holds a NaN or
  * +infinity, or nothing above -infinity, gives NaN throughout and tokens of -1. All
  * in fp32; what is left beside a probability near 1 keeps its relative precision.
- * 0 <= top <= HY_LOGPROBS_MAX_TOP, top <= vocab, vocab <= 2^20,
- * rows * max(tokens_per_row, top) < 2^31. */
+ * 0 <= top <= HY_LOGPROBS_MAX_TOP, top <= vocab, vocab <= 2^20, tokens_per_row <=
+ * 2^30, rows * max(tokens_per_row, top, 8) < 2^31 (a row has up to 8 blocks). */
 int hy_token_logprobs(const void* logits_dev, int rows, int vocab, int64_t row_stride, int dtype, int device,
                       const int* tokens_dev, int tokens_per_row, int top, float* logprobs_dev, float* entropy_dev,
                       int* top_ids_dev, float* top_logprobs_dev, void* stream);

@@ -75,3 +75,50 @@ def test_alternatives_behind_the_lm_head(pkg, monkeypatch, top):
     with pytest.raises(Reached, match="hy_lm_head_logprobs"):
         rt.lm_head_logprobs(torch.zeros(2, 1024).numpy(), top=64)
     del rt._ctx
+
+
+class Shape:
+    """Stands for a tensor on a device: what the checks before a call read of it."""
+    requires_grad = False
+
+    def __init__(self, *shape, dtype=torch.float32):
+        self.shape, self.dtype = torch.Size(shape), dtype
+
+    def get_device(self):
+        return 0
+
+    def stride(self):
+        return (self.shape[1], 1)
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 1 << 20
+
+    def new_empty(self, shape, dtype=None):
+        return Shape(*(shape if isinstance(shape, tuple) else (shape,)), dtype=dtype or self.dtype)
+
+
+@pytest.mark.parametrize("rows,vocab,tokens", [
+    (2 ** 32, 1, (2 ** 32,)), (2 ** 32 + 2, 5, (2 ** 32 + 2,)), (1, 2 ** 32 + 100, (1,)), (1, 9, (1, 2 ** 32)),
+    (2, 9, (2, 2 ** 32 + 1)),
+])
+def test_log_probabilities_past_32_bits(pkg, monkeypatch, rows, vocab, tokens):
+    """(A C int would wrap, and arrays that nobody had written would come back.)"""
+    logprobs = importlib.import_module("hy_b200.logprobs")
+    monkeypatch.setattr(logprobs, "_LIB", NoLibrary())
+    monkeypatch.setattr(logprobs, "_raw_stream", lambda index: 0)
+    with pytest.raises(Reached):
+        logprobs.token_logprobs(Shape(2, 9), Shape(2, dtype=torch.int32))
+    with pytest.raises(pkg.HyError, match="2.31"):
+        logprobs.token_logprobs(Shape(rows, vocab), Shape(*tokens, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("per_row", [2 ** 30 + 1, 2 ** 31 - 1])
+def test_more_tokens_of_a_row_than_its_threads_can_count(pkg, per_row):
+    """A CTA walks a row's tokens in steps of its threads, by a C int that must not pass its largest."""
+    import test_logprobs
+    lib = importlib.import_module("hy_b200.logprobs")._library()
+    assert test_logprobs._call(lib, rows=1, per_row=per_row, top=0) == 4
+    assert "2^30" in lib.hy_last_error().decode()
