@@ -2,7 +2,7 @@
 CUDA tensors. Behind a runtime's own LM head: TextRuntime.lm_head_logprobs.
 
 The calls run asynchronously on torch's current stream of the logits' device and can be captured into a CUDA graph.
-They have no backward pass: logits that require a gradient are refused.
+They have no backward pass and no forward-mode derivative: logits that require a gradient or carry a tangent are refused.
 """
 
 from __future__ import annotations
@@ -11,8 +11,10 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import HY_ERR_INVALID_ARGUMENT, HyError, _check, load_library
+from .rotary import refuse_tangents
 
 _I, _L, _P = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -56,6 +58,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise HyError(HY_ERR_INVALID_ARGUMENT, "the rows of logits must be contiguous")
     if logits.requires_grad and torch.is_grad_enabled():
         raise HyError(HY_ERR_INVALID_ARGUMENT, "logits require a gradient: this call has none")
+    if forward_ad._current_level >= 0:
+        refuse_tangents(logits)
     tshape = tokens.shape
     if (tokens.dtype is not torch.int32 or tokens.get_device() != index or len(tshape) not in (1, 2) or tshape[0] != rows or
             not tokens.is_contiguous()):

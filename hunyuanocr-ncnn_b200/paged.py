@@ -12,9 +12,10 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import HY_ERR_INVALID_ARGUMENT, HyError, _check, load_library
-from .rotary import rotation
+from .rotary import refuse_tangents, rotation
 
 DTYPE_F32, DTYPE_BF16, DTYPE_E4M3, DTYPE_INT8 = range(4)
 _CACHE_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float8_e4m3fn: DTYPE_E4M3,
@@ -144,6 +145,8 @@ class PagedKVCache:
                           f"{self._dim}] on {self.device} with contiguous heads")
         if t.requires_grad and torch.is_grad_enabled():
             raise HyError(HY_ERR_INVALID_ARGUMENT, f"{name} requires a gradient: these calls have none")
+        if forward_ad._current_level >= 0:
+            refuse_tangents(t)
         return dtype
 
     def _call(self, fn, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, dtype: int) -> None:
@@ -263,6 +266,8 @@ class PagedKVCache:
         if (weights.dtype != torch.float32 or weights.shape != self.k.shape[:3] or weights.get_device() != self._index or
                 weights.requires_grad and torch.is_grad_enabled()):
             raise HyError(HY_ERR_INVALID_ARGUMENT, "weights must be a float32 tensor [pages, kv heads, page rows] beside the cache")
+        if forward_ad._current_level >= 0:
+            refuse_tangents(weights)
         return _Weights(weights.data_ptr(), *weights.stride())
 
     def add_weights(self, batch: PagedBatch, q: torch.Tensor, lse: torch.Tensor, scale: float, weights: torch.Tensor, *,
@@ -276,6 +281,8 @@ class PagedKVCache:
         if (lse.dtype != torch.float32 or lse.shape != (rows, heads) or lse.get_device() != self._index or
                 lse.requires_grad and torch.is_grad_enabled()):
             raise HyError(HY_ERR_INVALID_ARGUMENT, "lse must be a float32 tensor [rows, q heads] on the cache's device")
+        if forward_ad._current_level >= 0:
+            refuse_tangents(lse)
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
         w = self._weights(weights)

@@ -3,7 +3,7 @@ decoder (rotation first) and the DFlash draft (norm first) have them, on torch C
 cache: paged.PagedKVCache.write_rotated.
 
 The calls run asynchronously on torch's current stream of the rows' device and can be captured into a CUDA graph. They
-have no backward pass: rows that require a gradient are refused.
+have no backward pass and no forward-mode derivative: rows that require a gradient or carry a tangent are refused.
 """
 
 from __future__ import annotations
@@ -12,6 +12,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import HY_ERR_INVALID_ARGUMENT, HyError, _check, load_library
 
@@ -42,6 +43,12 @@ def _refuse(message: str):
     raise HyError(HY_ERR_INVALID_ARGUMENT, message)
 
 
+def refuse_tangents(*tensors: torch.Tensor) -> None:
+    """Dual tensors (forward mode): these calls would drop their tangents. For where forward_ad._current_level >= 0."""
+    if torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse("a tensor carries a forward-mode tangent: these calls have no derivative")
+
+
 def rotation(rows: int, dim: int, index: int, q_weight, k_weight, cos, sin, positions, eps, rotate_first) -> bytes:
     """A call's norms and angles, checked, as the bytes of a hy_rotation: weights [head_dim], cos and sin [table rows,
     head_dim] of one layout, all float32, and positions [rows] int32 (or None: row r takes the table's row r)."""
@@ -49,6 +56,8 @@ def rotation(rows: int, dim: int, index: int, q_weight, k_weight, cos, sin, posi
     shape = cos.shape
     if torch.is_grad_enabled() and (q_weight.requires_grad or k_weight.requires_grad or cos.requires_grad or sin.requires_grad):
         _refuse("weights or angles that require a gradient: these calls have none")
+    if forward_ad._current_level >= 0:
+        refuse_tangents(q_weight, k_weight, cos, sin)
     if not (q_weight.dtype is f32 and k_weight.dtype is f32 and cos.dtype is f32 and sin.dtype is f32 and
             q_weight.get_device() == k_weight.get_device() == cos.get_device() == sin.get_device() == index):
         _refuse("weights, cos and sin must be float32 tensors on the rows' device")
@@ -95,6 +104,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weig
                 "CUDA device")
     if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
         _refuse("rows that require a gradient: this call has none")
+    if forward_ad._current_level >= 0:
+        refuse_tangents(q, k, *(out or ()))
     rows, heads, dim = shape
     if out is None:
         a, b = q.new_empty(shape), k.new_empty(kshape)

@@ -1,0 +1,46 @@
+"""Calls of the norms, the paged cache and the log probabilities that are refused, and ones beside them that are not, on the
+GPU."""
+
+import importlib
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mods(pkg):
+    return [importlib.import_module("hy_b200." + m) for m in ("paged", "rotary", "logprobs")]
+
+
+def _projection(rows, heads, dim, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(rows, heads, dim, generator=gen, device="cuda").to(dtype)
+
+
+def _angles(rows, dim):
+    a = torch.arange(rows, device="cuda")[:, None] * (1 + torch.arange(dim, device="cuda") % (dim // 2)) * 0.01
+    return a.cos(), a.sin()
+
+
+def test_forward_mode_tangents(mods, pkg):
+    _, rotary, logprobs = mods
+    x = _projection(3, 6, 64, torch.float32, 1)
+    cos, sin = _angles(3, 64)
+    w = torch.ones(64, device="cuda")
+    q, k = x[:, :4], x[:, 4:]
+    logits, tokens = _projection(3, 1, 100, torch.float32, 2)[:, 0], torch.zeros(3, dtype=torch.int32, device="cuda")
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(q, q), k), (q, forward_ad.make_dual(k, k))):
+            with pytest.raises(pkg.HyError, match="tangent"):
+                rotary.norm_rotate(*args, w, w, cos, sin)
+        out = forward_ad.make_dual(torch.empty_like(q), torch.empty_like(q))
+        with pytest.raises(pkg.HyError, match="tangent"):
+            rotary.norm_rotate(q, k, w, w, cos, sin, out=(out, torch.empty_like(k)))
+        with pytest.raises(pkg.HyError, match="tangent"):
+            logprobs.token_logprobs(forward_ad.make_dual(logits, logits), tokens)
+        got = rotary.norm_rotate(q, k, w, w, cos, sin)   # (a level alone refuses nothing)
+    assert all(torch.equal(a, b) for a, b in zip(got, rotary.norm_rotate(q, k, w, w, cos, sin)))
+    assert logprobs.token_logprobs(logits, tokens).logprob.shape == (3,)

@@ -23,14 +23,16 @@ class NoLibrary:
     """Stands for the library: a call that gets there was not refused."""
 
     def __getattr__(self, name):
-        raise Reached(name)
+        def call(*args):
+            raise Reached(name)
+        return call
 
 
 def _cache(paged, dtype=torch.float32):
     """A cache of host memory without a library behind it: only the checks before a call can run."""
     c = object.__new__(paged.PagedKVCache)
     c._lib, c.k, c.device, c._index, c._heads, c._dim = NoLibrary(), torch.zeros(4, 2, 8, 64, dtype=dtype), "cpu", -1, 2, 64
-    c._ref = None
+    c._ref, c._workspace = None, {}
     return c
 
 
@@ -122,3 +124,34 @@ def test_more_tokens_of_a_row_than_its_threads_can_count(pkg, per_row):
     lib = importlib.import_module("hy_b200.logprobs")._library()
     assert test_logprobs._call(lib, rows=1, per_row=per_row, top=0) == 4
     assert "2^30" in lib.hy_last_error().decode()
+
+
+def test_forward_mode_tangents(paged, pkg):
+    """The calls have no derivative of either mode: a tangent would be lost without a word."""
+    import torch.autograd.forward_ad as forward_ad
+    rotary = importlib.import_module("hy_b200.rotary")
+    c, batch = _cache(paged), _batch(paged)
+    q, k, v, lse, weights = torch.zeros(1, 4, 64), torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), torch.zeros(1, 4), torch.zeros(4, 2, 8)
+    norm, table, pos = torch.ones(64), torch.ones(5, 64), torch.zeros(1, dtype=torch.int32)
+
+    def turn(*args):
+        return rotary.rotation(1, 64, -1, *args, pos, 1e-5, True)
+
+    calls = [
+        (lambda q, k, v: c.write_rotated(batch, q, k, v, norm, norm, table, table, pos), (q, k, v)),
+        (lambda q: c.attention(batch, q, 0.1), (q,)), (lambda out: c.attention(batch, q, 0.1, out=out), (torch.zeros(1, 4, 64),)),
+        (lambda k, v: c.write(batch, k, v), (k, v)), (lambda k, v: c.read(batch, 1, out=(k, v)), (k, v)),
+        (lambda q, lse, weights: c.add_weights(batch, q, lse, 0.1, weights), (q, lse, weights)),
+        (lambda weights: c.evict(batch, 4, weights), (weights,)), (turn, (norm, norm, table, table)),
+    ]
+    for call, args in calls:
+        for i in range(len(args)):
+            with forward_ad.dual_level():
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                with pytest.raises(pkg.HyError, match="tangent"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(pkg.HyError, match="tangent"):   # (that turns off the other mode alone)
+                    call(*dual)
+                if call is not turn:
+                    with pytest.raises(Reached):
+                        call(*args)
