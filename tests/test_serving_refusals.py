@@ -52,7 +52,12 @@ def test_evict_sizes(paged, pkg, over):
         c.evict(_batch(paged), f["keep"], torch.zeros(4, 2, 8), first=f["first"], recent=f["recent"])
 
 
-def test_evict_sizes_that_hold_reach_the_library(paged):
+@pytest.fixture
+def no_stream(paged, monkeypatch):
+    monkeypatch.setattr(paged, "_raw_stream", lambda index: 0)
+
+
+def test_evict_sizes_that_hold_reach_the_library(paged, no_stream):
     for keep, first, recent in ((8, 0, 0), (8, 3, 5), (1, 0, 1)):
         with pytest.raises(Reached, match="hy_paged_evict"):
             _cache(paged).evict(_batch(paged), keep, torch.zeros(4, 2, 8), first=first, recent=recent)
@@ -126,7 +131,7 @@ def test_more_tokens_of_a_row_than_its_threads_can_count(pkg, per_row):
     assert "2^30" in lib.hy_last_error().decode()
 
 
-def test_forward_mode_tangents(paged, pkg):
+def test_forward_mode_tangents(paged, pkg, no_stream):
     """The calls have no derivative of either mode: a tangent would be lost without a word."""
     import torch.autograd.forward_ad as forward_ad
     rotary = importlib.import_module("hy_b200.rotary")
