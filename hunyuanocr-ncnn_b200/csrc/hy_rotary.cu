@@ -25,13 +25,62 @@ int check_rotation(const hy_rotation* t)
     return HY_OK;
 }
 
-// An output is the input itself or lies elsewhere.
-int check_output(const char* name, const void* out, long long row, long long head, const void* in, long long in_row,
-                 long long in_head, int rows, int heads)
+// Row tensors of one type and as many rows.
+struct RowTensor {
+    const char* name;
+    const void* p;
+    int heads;
+    long long row, head;   // strides
+};
+
+// Whether two of them share elements. Interleaved ones, views of one projection, are told apart exactly; only those whose
+// ranges meet and whose rows lie differently far apart (in one buffer, that is) are not looked into.
+bool rows_meet(const RowTensor& a, const RowTensor& b, int rows, int dim, int elem)
 {
-    if (out != in || ((rows < 2 || row == in_row) && (heads < 2 || head == in_head))) return HY_OK;
+    using Wide = __int128;   // (strides may be anything)
+    const Wide apart = (static_cast<Wide>(reinterpret_cast<uintptr_t>(b.p)) - static_cast<Wide>(reinterpret_cast<uintptr_t>(a.p))) / elem;
+    auto extent = [&](const RowTensor& t) { return static_cast<Wide>(rows - 1) * t.row + static_cast<Wide>(t.heads - 1) * t.head + dim; };
+    if (apart >= extent(a) || -apart >= extent(b)) return false;
+    if (rows > 1 && a.row != b.row) return false;
+    // Head i of a and j of b, rows d apart: |apart + j b.head - i a.head - d row| < dim for a d of at most rows - 1.
+    auto heads_meet = [&](Wide i, Wide j) {
+        const Wide x = apart + j * b.head - i * a.head;
+        if (rows == 1 || a.row == 0) return x < dim && -x < dim;
+        const Wide r = a.row, y = x < 0 ? -x : x;
+        const Wide low = y / r, d = low < rows - 1 ? low : rows - 1;   // the nearest rows
+        return y - d * r < dim || (d + 1 < rows && (d + 1) * r - y < dim);
+    };
+    if (a.head == b.head || a.heads == 1 || b.heads == 1)   // the heads' distance alone counts
+    {
+        for (int j = 0; j < b.heads; ++j)
+            if (heads_meet(0, j)) return true;
+        for (int i = 1; i < a.heads; ++i)
+            if (heads_meet(i, 0)) return true;
+        return false;
+    }
+    for (int i = 0; i < a.heads; ++i)
+        for (int j = 0; j < b.heads; ++j)
+            if (heads_meet(i, j)) return true;
+    return false;
+}
+
+// An output is the input itself or lies elsewhere.
+int check_output(const RowTensor& out, const RowTensor& in, int rows, int dim, int dtype)
+{
     char msg[96];
-    snprintf(msg, sizeof msg, "%s in place of its input needs the input's strides", name);
+    if (out.p == in.p && (rows < 2 || out.row == in.row) && (in.heads < 2 || out.head == in.head)) return HY_OK;
+    if (out.p == in.p) snprintf(msg, sizeof msg, "%s in place of its input needs the input's strides", out.name);
+    else if (rows_meet(out, in, rows, dim, elem_size(dtype))) snprintf(msg, sizeof msg, "%s must be its input or not overlap it", out.name);
+    else return HY_OK;
+    return fail(HY_ERR_INVALID_ARGUMENT, msg);
+}
+
+// Two that lie apart.
+int check_elsewhere(const RowTensor& out, const RowTensor& other, int rows, int dim, int dtype)
+{
+    if (out.p != other.p && !rows_meet(out, other, rows, dim, elem_size(dtype))) return HY_OK;
+    char msg[96];
+    snprintf(msg, sizeof msg, "%s must not overlap %s", out.name, other.name);
     return fail(HY_ERR_INVALID_ARGUMENT, msg);
 }
 
@@ -102,11 +151,14 @@ int hy_norm_rotate(const hy_rotation* rotation, int rows, int q_heads, int kv_he
     if (!rc) rc = check_rows("k_out", k_out_dev, rows, kv_heads, k_out_row_stride, k_out_head_stride, dtype);
     if (!rc) rc = check_apart("q_out", rows, q_heads, head_dim, q_out_row_stride, q_out_head_stride);
     if (!rc) rc = check_apart("k_out", rows, kv_heads, head_dim, k_out_row_stride, k_out_head_stride);
-    if (!rc) rc = check_output("q_out", q_out_dev, q_out_row_stride, q_out_head_stride, q_dev, q_row_stride, q_head_stride, rows, q_heads);
-    if (!rc) rc = check_output("k_out", k_out_dev, k_out_row_stride, k_out_head_stride, k_dev, k_row_stride, k_head_stride, rows, kv_heads);
+    const RowTensor q{"q", q_dev, q_heads, q_row_stride, q_head_stride}, k{"k", k_dev, kv_heads, k_row_stride, k_head_stride},
+        q_out{"q_out", q_out_dev, q_heads, q_out_row_stride, q_out_head_stride}, k_out{"k_out", k_out_dev, kv_heads, k_out_row_stride, k_out_head_stride};
+    if (!rc) rc = check_output(q_out, q, rows, head_dim, dtype);
+    if (!rc) rc = check_output(k_out, k, rows, head_dim, dtype);
+    if (!rc) rc = check_elsewhere(q_out, k_out, rows, head_dim, dtype);
+    if (!rc) rc = check_elsewhere(q_out, k, rows, head_dim, dtype);
+    if (!rc) rc = check_elsewhere(k_out, q, rows, head_dim, dtype);
     if (rc) return rc;
-    if (q_out_dev == k_out_dev || q_out_dev == k_dev || k_out_dev == q_dev)
-        return fail(HY_ERR_INVALID_ARGUMENT, "q_out and k_out must not overlap, nor each the other's input");
     DeviceGuard guard(device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     RotateArgs a = rotate_args(rotation, rows, q_heads, kv_heads, head_dim);
@@ -144,10 +196,12 @@ int hy_paged_kv_write_rotated(const hy_paged_cache* cache, const hy_paged_batch*
     if (!rc) rc = check_rows("v", v_dev, rows, kv_heads, v_row_stride, v_head_stride, dtype);
     if (!rc) rc = check_rows("q_out", q_out_dev, rows, q_heads, q_out_row_stride, q_out_head_stride, dtype);
     if (!rc) rc = check_apart("q_out", rows, q_heads, cache->head_dim, q_out_row_stride, q_out_head_stride);
-    if (!rc) rc = check_output("q_out", q_out_dev, q_out_row_stride, q_out_head_stride, q_dev, q_row_stride, q_head_stride, rows, q_heads);
+    const RowTensor q{"q", q_dev, q_heads, q_row_stride, q_head_stride}, k{"k", k_dev, kv_heads, k_row_stride, k_head_stride},
+        v{"v", v_dev, kv_heads, v_row_stride, v_head_stride}, q_out{"q_out", q_out_dev, q_heads, q_out_row_stride, q_out_head_stride};
+    if (!rc) rc = check_output(q_out, q, rows, cache->head_dim, dtype);
+    if (!rc) rc = check_elsewhere(q_out, k, rows, cache->head_dim, dtype);
+    if (!rc) rc = check_elsewhere(q_out, v, rows, cache->head_dim, dtype);
     if (rc) return rc;
-    if (q_out_dev == k_dev || q_out_dev == v_dev)
-        return fail(HY_ERR_INVALID_ARGUMENT, "q_out must not overlap k or v");
     DeviceGuard guard(cache->device);
     if (guard.error() != cudaSuccess) return cuda_fail("device", guard.error());
     RotateArgs a = rotate_args(rotation, rows, q_heads, kv_heads, cache->head_dim);

@@ -44,7 +44,8 @@ typedef struct hy_rotation {
  * head_dim (64 or 128) elements of `dtype` (HY_DTYPE_F32 or HY_DTYPE_BF16); every
  * (row, head) starts on 16 bytes. The outputs may be the inputs themselves (the
  * same pointer and strides); otherwise they share no memory with the inputs, with
- * each other or with themselves. status_dev (nullable): as in hy_paged_cache.
+ * each other or with themselves (refused where it shows: rows equally far apart in
+ * both, or one row). status_dev (nullable): as in hy_paged_cache.
  * Limits: heads 1024, rows * heads 2^31. */
 int hy_norm_rotate(const hy_rotation* rotation, int rows, int q_heads, int kv_heads, int head_dim, int dtype,
                    int device, const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, const void* k_dev,

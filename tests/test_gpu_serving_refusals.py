@@ -44,3 +44,28 @@ def test_forward_mode_tangents(mods, pkg):
         got = rotary.norm_rotate(q, k, w, w, cos, sin)   # (a level alone refuses nothing)
     assert all(torch.equal(a, b) for a, b in zip(got, rotary.norm_rotate(q, k, w, w, cos, sin)))
     assert logprobs.token_logprobs(logits, tokens).logprob.shape == (3,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 50, 700])
+def test_outputs_beside_their_inputs_in_one_projection(mods, pkg, rows, dtype):
+    """Interleaved views share no element and are right; those that share some are refused."""
+    _, rotary, _ = mods
+    x = _projection(rows, 13, 64, dtype, rows)
+    cos, sin = _angles(rows, 64)
+    w = torch.rand(64, device="cuda") + 0.5
+    q, k = x[:, :4], x[:, 4:6]
+    want = rotary.norm_rotate(q, k, w, w, cos, sin)
+    held = x.clone()
+    for a, b in ((6, 11), (0, 4), (8, 4), (0, 11)):   # first heads of the outputs
+        x.copy_(held)
+        out = x[:, a:a + 4], x[:, b:b + 2]
+        rotary.norm_rotate(q, k, w, w, cos, sin, out=out)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        rest = [h for h in range(13) if not a <= h < a + 4 and not b <= h < b + 2]
+        assert torch.equal(x[:, rest], held[:, rest])
+    x.copy_(held)
+    for a, b in ((7, 0), (2, 11), (1, 4), (6, 5), (6, 3), (6, 9)):
+        with pytest.raises(pkg.HyError, match="overlap"):
+            rotary.norm_rotate(q, k, w, w, cos, sin, out=(x[:, a:a + 4], x[:, b:b + 2]))
+    assert torch.equal(x, held)

@@ -8,6 +8,7 @@ import torch
 
 import test_paged
 import test_paged_weights
+import test_rotary
 
 
 @pytest.fixture(scope="module")
@@ -160,3 +161,26 @@ def test_forward_mode_tangents(paged, pkg, no_stream):
                 if call is not turn:
                     with pytest.raises(Reached):
                         call(*args)
+
+
+@pytest.mark.parametrize("over", [
+    dict(qo=test_paged.FAKE + 256), dict(qo=test_paged.FAKE + 1024), dict(qo=test_paged.FAKE - 768), dict(qo=test_paged.FAKE + 16),
+    dict(qo=test_paged.FAKE + 1024 * 99 + 768), dict(qo=2 * test_paged.FAKE - 256), dict(qo=2 * test_paged.FAKE + 256),
+    dict(rows=1, qo=test_paged.FAKE + 768, out_strides=(4096, 128)), dict(out_strides=(512, 256), qo=test_paged.FAKE + 256),
+])
+def test_outputs_over_other_rows_of_the_inputs(pkg, over):
+    """Rows of a shared projection: an output that starts some heads or rows further in the same memory."""
+    mods = importlib.import_module("hy_b200.rotary"), importlib.import_module("hy_b200.paged")
+    f = dict(rows=100)
+    f.update(over)
+    for rc in test_rotary._calls(mods, test_rotary._rotation(mods[0], positions_dev=None, table_rows=100), **f):
+        assert rc == 1
+        assert b"overlap" in mods[0]._library().hy_last_error()
+
+
+@pytest.mark.parametrize("ko", [test_paged.FAKE + 512, 2 * test_paged.FAKE + 256, 3 * test_paged.FAKE + 512, 2 * test_paged.FAKE - 1024 * 9])
+def test_keys_over_other_rows(pkg, ko):
+    mods = importlib.import_module("hy_b200.rotary"), importlib.import_module("hy_b200.paged")
+    calls = test_rotary._calls(mods, test_rotary._rotation(mods[0], positions_dev=None, table_rows=100), rows=100, ko=ko)
+    assert next(calls) == 1
+    assert b"overlap" in mods[0]._library().hy_last_error()
