@@ -286,6 +286,8 @@ class PagedKVCache:
         if batch.index != self._index:
             raise HyError(HY_ERR_INVALID_ARGUMENT, "the batch must be on the cache's device")
         w = self._weights(weights)
+        if 0 in lse.stride():   # (expanded: the library takes numbers of their own)
+            lse = lse.contiguous()
         q0, q1, _ = q.stride()
         window, sinks = max(min(window, _INT_MAX), -1), max(min(sinks, _INT_MAX), -1)   # (a C int would wrap)
         rc = self._lib.hy_paged_add_weights(self._ref, batch._ref, rows, heads, dtype, q.data_ptr(), q0, q1,

@@ -176,7 +176,8 @@ typedef struct hy_paged_weights {
  * own positions start anew: theirs are set, others' added to. So one call for
  * every attention call, with its q, lse, scale, window and sinks, keeps the
  * weights. Positions that no row sees stay as they are. Sequences of a call must
- * not share pages (a position's number would be written by both). fp32 throughout
+ * not share pages (a position's number would be written by both). The strides of
+ * lse are as in hy_paged_attention_lse (0 only where there is one entry). fp32 throughout
  * (products as in hy_paged_attention); the same call gives the same bits. */
 int hy_paged_add_weights(const hy_paged_cache* cache, const hy_paged_batch* batch, int rows, int q_heads, int dtype,
                          const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, const float* lse_dev,

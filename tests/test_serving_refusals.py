@@ -184,3 +184,23 @@ def test_keys_over_other_rows(pkg, ko):
     calls = test_rotary._calls(mods, test_rotary._rotation(mods[0], positions_dev=None, table_rows=100), rows=100, ko=ko)
     assert next(calls) == 1
     assert b"overlap" in mods[0]._library().hy_last_error()
+
+
+def test_expanded_logarithms_are_read(paged, no_stream):
+    """add_weights only reads lse: one number for all rows or heads is as good as a number for each."""
+    import ctypes
+    seen = []
+
+    class Library(NoLibrary):
+        def hy_paged_add_weights(self, *args):
+            at, row, head = args[8:11]
+            seen.append([ctypes.c_float.from_address(at + 4 * (i * row + j * head)).value for i in range(3) for j in range(4)])
+            assert row > 0 and head > 0   # (the library takes no others)
+            return 0
+
+    c, q, weights = _cache(paged), torch.zeros(3, 4, 64), torch.zeros(4, 2, 8)
+    c._lib = Library()
+    for lse in (torch.arange(4.0).expand(3, 4), torch.arange(3.0)[:, None].expand(3, 4), torch.tensor(5.0).expand(3, 4),
+                torch.arange(12.0).view(3, 4), torch.arange(12.0).view(4, 3).t()):
+        c.add_weights(_batch(paged), q, lse, 0.1, weights)
+        assert seen[-1] == lse.reshape(-1).tolist()
