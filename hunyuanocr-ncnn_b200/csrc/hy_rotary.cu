@@ -14,7 +14,7 @@ namespace {
 int check_rotation(const hy_rotation* t)
 {
     if (!t) return fail(HY_ERR_INVALID_ARGUMENT, "rotation is null");
-    if (!t->q_weight_dev || !t->k_weight_dev || !t->cos_dev || !t->sin_dev)
+    if (!t->q_weight_dev || !t->k_weight_dev || (t->table_rows != 0 && (!t->cos_dev || !t->sin_dev)))
         return fail(HY_ERR_INVALID_ARGUMENT, "norm weights or angles are null");
     if (!aligned16(t->q_weight_dev) || !aligned16(t->k_weight_dev) || !aligned16(t->cos_dev) || !aligned16(t->sin_dev) ||
         off16(t->table_stride, 4, t->table_rows))

@@ -31,7 +31,7 @@ extern "C" {
 typedef struct hy_rotation {
     const float* q_weight_dev; /* [head_dim] */
     const float* k_weight_dev; /* [head_dim] */
-    const float* cos_dev;
+    const float* cos_dev;      /* (NULL: a table of no rows) */
     const float* sin_dev;
     int table_rows;
     int64_t table_stride;

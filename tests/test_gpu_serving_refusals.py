@@ -69,3 +69,20 @@ def test_outputs_beside_their_inputs_in_one_projection(mods, pkg, rows, dtype):
         with pytest.raises(pkg.HyError, match="overlap"):
             rotary.norm_rotate(q, k, w, w, cos, sin, out=(x[:, a:a + 4], x[:, b:b + 2]))
     assert torch.equal(x, held)
+
+
+def test_a_table_without_rows(mods):
+    """No rows give nothing; rows whose positions lie outside the empty table are NaN, and reported."""
+    paged, rotary, _ = mods
+    x = _projection(3, 6, 64, torch.float32, 1)
+    cos = torch.ones(0, 64, device="cuda")
+    w = torch.ones(64, device="cuda")
+    a, b = rotary.norm_rotate(x[:0, :4], x[:0, 4:], w, w, cos, cos)
+    assert a.shape == (0, 4, 64) and b.shape == (0, 2, 64)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a, b = rotary.norm_rotate(x[:, :4], x[:, 4:], w, w, cos, cos, torch.zeros(3, dtype=torch.int32, device="cuda"), status=status)
+    assert torch.isnan(a).all() and torch.isnan(b).all() and status.item() == 16
+    cache = paged.PagedKVCache.allocate(2, 2, 16, 64, torch.float32)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    batch = paged.PagedBatch(i32(0, 0), i32(0), i32(0)[:, None], 1)
+    assert cache.write_rotated(batch, x[:0, :2], x[:0, 2:4], x[:0, 4:], w, w, cos, cos).shape == (0, 2, 64)

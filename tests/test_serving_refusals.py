@@ -204,3 +204,10 @@ def test_expanded_logarithms_are_read(paged, no_stream):
                 torch.arange(12.0).view(3, 4), torch.arange(12.0).view(4, 3).t()):
         c.add_weights(_batch(paged), q, lse, 0.1, weights)
         assert seen[-1] == lse.reshape(-1).tolist()
+
+
+def test_calls_without_rows_and_angles(pkg):
+    """No rows, and a table of angles of no rows, whose memory is null: nothing to do."""
+    mods = importlib.import_module("hy_b200.rotary"), importlib.import_module("hy_b200.paged")
+    turn = test_rotary._rotation(mods[0], cos_dev=None, sin_dev=None, table_rows=0, table_stride=64, positions_dev=None)
+    assert list(test_rotary._calls(mods, turn, rows=0, q=None, k=None, qo=None, ko=None)) == [0, 0]
