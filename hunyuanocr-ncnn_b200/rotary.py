@@ -79,11 +79,8 @@ def rotation(rows: int, dim: int, index: int, q_weight, k_weight, cos, sin, posi
                 not positions.is_contiguous()):
             _refuse("positions must be a contiguous int32 tensor [rows] on the rows' device")
         where = positions.data_ptr()
-    try:
-        return _pack(q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), shape[0], stride, where, eps,
-                     rotate_first)
-    except (OverflowError, struct.error):
-        _refuse("eps must be finite and not negative in float32, the table must have less than 2^31 rows")
+    return _pack(q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), shape[0], stride, where, eps,
+                 rotate_first)
 
 
 def norm_rotate(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,

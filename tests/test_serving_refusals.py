@@ -211,11 +211,3 @@ def test_calls_without_rows_and_angles(pkg):
     mods = importlib.import_module("hy_b200.rotary"), importlib.import_module("hy_b200.paged")
     turn = test_rotary._rotation(mods[0], cos_dev=None, sin_dev=None, table_rows=0, table_stride=64, positions_dev=None)
     assert list(test_rotary._calls(mods, turn, rows=0, q=None, k=None, qo=None, ko=None)) == [0, 0]
-
-
-@pytest.mark.parametrize("eps", [1e39, -1e39, 2.0 ** 128])
-def test_an_eps_past_fp32(pkg, eps):
-    rotary = importlib.import_module("hy_b200.rotary")
-    w, table, pos = torch.ones(64), torch.ones(5, 64), torch.zeros(1, dtype=torch.int32)
-    with pytest.raises(pkg.HyError, match="eps"):
-        rotary.rotation(1, 64, -1, w, w, table, table, pos, eps, True)
