@@ -15,8 +15,10 @@
 // ahead and across rows (with loads into registers, one step ahead, too little was in flight). A row
 // is split over the warps of a CTA, and over several CTAs, only while there are too
 // few rows to fill the GPU. 20011 bf16 rows of 36 heads of 64: 38 us, 5.0 TB/s (62 us with loads into registers);
-// 38.6k bf16 rows of 32 heads of 128, k and v into E4M3 pages: 131 us, 4.4 TB/s, bound by instructions (59% of the issue
-// slots; with five CTAs per SM instead of four the registers spill: 150 us); one fp32 row: 1.7 us.
+// 38.6k bf16 rows of 32 heads of 128, k and v into E4M3 pages: 131 us, 4.4 TB/s. What bounds that one is a warp's chain of
+// shared-memory loads, two reductions over a head's lanes, divide, quantise and store, with too few warps to hide it: four
+// CTAs of four per SM (122 registers; shared memory allows no more either), 59% of the issue slots, and of a warp's time
+// hardly any waits for memory. With five CTAs the registers spill: 150 us. One fp32 row: 1.7 us.
 #pragma once
 
 #include "hy_paged_attn.cuh"
